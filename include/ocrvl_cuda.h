@@ -17,7 +17,8 @@
  *   - Tensor types: 0 = F32, 1000 = Q8_ROW, 1001 = Q4_ROW, 1002 = Q6_ROW
  *     (internal/gguf/gguf.go:19-22).  Quantized tensors are passed exactly
  *     as stored in the repo's GGUF files: rows f32 scales, then rows packed
- *     rows (internal/gguf/gguf.go:435-569).
+ *     rows (internal/gguf/gguf.go:435-569).  The paged-cache operators also
+ *     take 1 = F16 and 30 = BF16 caches (GGUF's own numbers).
  */
 #ifndef OCRVL_CUDA_H
 #define OCRVL_CUDA_H
@@ -36,6 +37,8 @@ extern "C" {
 #define OCRVL_E_TIMEOUT (-4)  /* a bounded device-side wait gave up */
 
 #define OCRVL_F32 0
+#define OCRVL_F16 1
+#define OCRVL_BF16 30
 #define OCRVL_Q8_ROW 1000
 #define OCRVL_Q4_ROW 1001
 #define OCRVL_Q6_ROW 1002
@@ -278,6 +281,119 @@ int ocrvl_op_sample(int m, int vocab, const float *logits, double temperature, i
 
 /* out = RMSNorm(x, w, eps) for m vectors of n (tensor.RMSNorm). */
 int ocrvl_op_rmsnorm(int n, int m, const float *x, const float *w, float eps, float *out, void *stream);
+
+/* ---- paged-cache operators ---------------------------------------------
+ * Drafted tokens verified over a paged cache, and the cache cut to a budget.
+ * No reference counterpart (the reference decodes one token a step and keeps
+ * every position).  All pointers are device pointers except the descriptor;
+ * calls are asynchronous on `stream`, allocate nothing and read lengths on
+ * the device, so they can be captured in a CUDA graph.
+ *
+ * The cache: pages of page_size positions.  Element (position t, kv head h,
+ * dim d) of sequence b, layer l lies at
+ *   table[b * table_stride + t / page_size] * page_stride + l * layer_stride
+ *     + h * head_stride + (t % page_size) * token_stride + d
+ * of k and of v (strides in elements).  A table entry outside 0..num_pages-1
+ * is an unmapped page: its positions are not attended, and nothing is written
+ * there.  A length counts as at most max_pages * page_size, a negative one
+ * as 0.  The engine's own pool has this form (ocrvl_seq_kv_view). */
+typedef struct ocrvl_kv_cache {
+  int32_t type;         /* OCRVL_F32, OCRVL_F16 or OCRVL_BF16 */
+  int32_t head_dim;     /* 64 or 128, contiguous */
+  int32_t num_kv_heads;
+  int32_t num_layers;
+  int32_t page_size;    /* positions a page: a power of two, at least 16 */
+  int32_t num_pages;    /* pages that k and v hold */
+  int32_t batch;        /* rows of the table */
+  int32_t max_pages;    /* entries a row */
+  int64_t page_stride, layer_stride, head_stride, token_stride; /* elements; multiples of 16 bytes */
+  int64_t table_stride; /* entries */
+  void *k, *v;          /* 16-byte aligned */
+  const int32_t *table;
+} ocrvl_kv_cache;
+
+/* The cache of an engine sequence as a descriptor of one table row: every
+ * layer, pages of 16 positions, f32.  The table holds the pages of the
+ * positions the sequence has (ocrvl_seq_len); order work on it against the
+ * model's stream. */
+int ocrvl_seq_kv_view(ocrvl_seq *s, ocrvl_kv_cache *out);
+
+/* Drops all positions from n on (0 <= n <= length), as after an in-place
+ * ocrvl_op_kv_compact or when drafted positions are taken back; pages that
+ * hold none of the rest return to the pool.  The next step appends at
+ * position n; its rotary position is (n, n, n) unless pos_thw says otherwise,
+ * which it has to after an eviction. */
+int ocrvl_seq_truncate(ocrvl_seq *s, int n);
+
+/* Attention of drafted tokens over a cache and over one another.
+ * Sequence b drafted the tokens indptr[b] .. indptr[b+1]-1 of the flat
+ * token axis (at most max_draft <= 64 of them; more are not computed); q, k, v
+ * and out are [n_tokens][heads][head_dim] of the cache's type with a stride
+ * in elements between tokens (k and v: num_kv_heads).  Token i of the
+ * sequence attends every cached position below lens[b] and the sequence's
+ * drafted tokens j whose bit j of mask[token] is set (its own among them only
+ * if set).  heads is a multiple of num_kv_heads, at most 16 times it.
+ *   out = softmax(scale q . k) v,  lse (may be NULL) = log of the sum of
+ *   exp(scale q . k), [n_tokens][heads] f32
+ * A token that attends nothing gets out = 0 and lse = -inf.  Sums, softmax
+ * statistics and the output are held in 32 bits; for the 16-bit types the
+ * softmax weights are rounded to the type for the product with v.  What lies in
+ * masked places (NaN and infinities too) does not reach the output.
+ * work: ocrvl_op_tree_attn_workspace bytes, 16-byte aligned; its contents
+ * need no preparation and mean nothing afterwards. */
+int ocrvl_op_tree_attn_workspace(const ocrvl_kv_cache *c, int heads, int max_draft, int64_t *bytes);
+int ocrvl_op_tree_attn(const ocrvl_kv_cache *c, int layer, int heads, int n_tokens, int max_draft,
+                       const int32_t *lens, const int32_t *indptr, const int64_t *mask, const void *q,
+                       int64_t q_stride, const void *k, const void *v, int64_t kv_stride, float scale, void *out,
+                       int64_t out_stride, float *lse, void *work, int64_t work_bytes, void *stream);
+
+/* The attention weight that cached positions got from tokens:
+ *   acc_out[b][h][t] = decay acc[b][h][t] + sum over the counted tokens i of b
+ *     and the query heads of kv head h of exp(scale q . k_t - lse)
+ * for t < lens[b], and 0 for lens[b] <= t < out_width, so that positions
+ * appended later start at 0.  q, indptr, max_draft, lens as
+ * ocrvl_op_tree_attn takes them, lse as it returns it; a token whose lse is
+ * -inf adds nothing.  counted (may be NULL: all): one word a sequence, bit i
+ * counts its token i, e.g. the accepted path.  acc (may be NULL: 0) is
+ * [batch][num_kv_heads] rows of acc_width values acc_stride apart, 0 past
+ * acc_width; acc_out likewise, and may be acc itself with the same stride. */
+int ocrvl_op_attn_mass(const ocrvl_kv_cache *c, int layer, int heads, int n_tokens, int max_draft,
+                       const int32_t *lens, const int32_t *indptr, const int64_t *counted, const void *q,
+                       int64_t q_stride, const float *lse, float scale, float decay, const float *acc, int acc_width,
+                       int64_t acc_stride, float *acc_out, int out_width, int64_t out_stride, void *stream);
+
+/* The positions that a cut to `keep` positions leaves: all when
+ * lens[b] <= keep, else the first `sinks`, the last `recent`
+ * (sinks + recent <= keep) and of those between the ones with the largest
+ * sums, the lower position first among equals (NaN counts as the lowest).
+ * acc: rows [num_layers * batch * num_kv_heads] of acc_width sums acc_stride
+ * apart, layer outermost; lens: [batch], at most acc_width counts.
+ * idx: [rows][keep] positions in rising order, -1 past the count; sums (may be
+ * NULL): [rows][keep] their sums, 0 past the count; new_lens (may be NULL):
+ * [batch], min(lens, keep).  The outputs overlap none of the inputs. */
+int ocrvl_op_kv_select(int num_layers, int batch, int num_kv_heads, const float *acc, int acc_width,
+                       int64_t acc_stride, const int32_t *lens, int keep, int sinks, int recent, int32_t *idx,
+                       float *sums, int32_t *new_lens, void *stream);
+
+/* Moves the kept positions of every layer and kv head together: position j
+ * of `to` becomes position idx[layer][b][h][j] of `from`, for j up to the
+ * first negative index or `keep`.  `to` is `from` itself (same pool, same
+ * table: in place; idx is then strictly rising), or a cache of the same shape whose
+ * pages that table rows name share nothing with from's. */
+int ocrvl_op_kv_compact(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const int32_t *idx, int keep,
+                        void *stream);
+
+/* Writes tokens behind the cache: for i < n_path[b] (at most max_path),
+ * position lens[b] + i of every layer becomes token indptr[b] + path[b][i];
+ * path NULL: token indptr[b] + i, for all of the sequence's tokens.  k and v are
+ * [num_layers][n_tokens][num_kv_heads][head_dim] with kv_stride elements
+ * between tokens and kv_layer_stride between layers.  Rows that name no
+ * token of the sequence, positions past the table and unmapped pages are
+ * skipped.  new_lens[b] = lens[b] + the count, at most max_pages *
+ * page_size; it must not be lens itself. */
+int ocrvl_op_kv_append(const ocrvl_kv_cache *c, int n_tokens, const int32_t *lens, const int32_t *indptr,
+                       const int32_t *path, const int32_t *n_path, int max_path, const void *k, const void *v,
+                       int64_t kv_stride, int64_t kv_layer_stride, int32_t *new_lens, void *stream);
 
 #ifdef __cplusplus
 }

@@ -44,6 +44,29 @@ class ModelDesc(C.Structure):
     ]
 
 
+class KVCache(C.Structure):
+    """ocrvl_kv_cache: a paged cache's addressing."""
+
+    _fields_ = [
+        ("type", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("num_layers", C.c_int32),
+        ("page_size", C.c_int32),
+        ("num_pages", C.c_int32),
+        ("batch", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("page_stride", C.c_int64),
+        ("layer_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("token_stride", C.c_int64),
+        ("table_stride", C.c_int64),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("table", C.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); the exported symbol set of include/ocrvl_cuda.h
 P, I, I64, F = C.c_void_p, C.c_int, C.c_int64, C.c_float
 SIGNATURES = {
@@ -80,6 +103,14 @@ SIGNATURES = {
     "ocrvl_op_argmax_noalloc": (I, [I, I, I, P, P, P, I, P, P, P]),
     "ocrvl_op_sample": (I, [I, I, P, C.c_double, I, P, P, P, P, P, P]),
     "ocrvl_op_rmsnorm": (I, [I, I, P, P, F, P, P]),
+    "ocrvl_seq_kv_view": (I, [P, C.POINTER(KVCache)]),
+    "ocrvl_seq_truncate": (I, [P, I]),
+    "ocrvl_op_tree_attn_workspace": (I, [C.POINTER(KVCache), I, I, C.POINTER(I64)]),
+    "ocrvl_op_tree_attn": (I, [C.POINTER(KVCache), I, I, I, I, P, P, P, P, I64, P, P, I64, F, P, I64, P, P, I64, P]),
+    "ocrvl_op_attn_mass": (I, [C.POINTER(KVCache), I, I, I, I, P, P, P, P, I64, P, F, F, P, I, I64, P, I, I64, P]),
+    "ocrvl_op_kv_select": (I, [I, I, I, P, I, I64, P, I, I, I, P, P, P, P]),
+    "ocrvl_op_kv_compact": (I, [C.POINTER(KVCache), C.POINTER(KVCache), P, I, P]),
+    "ocrvl_op_kv_append": (I, [C.POINTER(KVCache), I, P, P, P, P, I, P, P, I64, I64, P, P]),
 }
 
 

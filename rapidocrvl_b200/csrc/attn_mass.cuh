@@ -1,0 +1,214 @@
+// The attention weight that cached positions got from a set of tokens
+// (ocrvl_op_attn_mass):
+//   acc'[t] = decay acc[t] + sum over rows of 2^(scale log2(e) q . k_t - lse log2(e))
+// with the rows' lse known, so one pass over K does: no maximum, no second
+// pass.  Every position belongs to one warp, which adds its rows' weights in
+// a fixed order: no atomics, the same sums every time.
+//
+// A block takes a run of tiles of 128 positions (16 a warp) of one
+// (sequence, kv head) after another; query fragments of up to kRowTiles x 16
+// rows lie in shared memory, more rows take further passes over the run's K.
+#pragma once
+#include "paged.cuh"
+
+namespace ocrvl {
+namespace paged {
+
+constexpr int kMassWarps = 8;
+constexpr int kMassThreads = kMassWarps * 32;
+
+struct MassArgs {
+  Cache c;
+  Seqs s;
+  int kv_heads, group;
+  const void *q;
+  long long q_stride;
+  const long long *counted;
+  const float *lse;
+  float scale, decay;  // scale * log2(e)
+  const float *acc;
+  float *out;
+  long long acc_stride, out_stride;
+  int acc_width, out_width;
+};
+
+// A sequence's tiles and what one costs: K's load and the rows' products.
+struct MassShare {
+  int first, count, len, tiles, cost;
+
+  __device__ MassShare(const MassArgs &a, int b) {
+    count = a.s.tokens(b, &first);
+    len = min(a.s.len(b), a.out_width);
+    tiles = (len + kMassWarps * kChunk - 1) / (kMassWarps * kChunk);
+    cost = 1 + (count * a.group + 15) / 16;
+  }
+  __device__ long long total(int kv_heads) const { return (long long)kv_heads * tiles * cost; }
+};
+
+template <typename T, int D>
+struct MassShape {
+  using L = Tile<T, D>;
+  static constexpr int kUnits = L::kBytes >= 8192 ? 3 : L::kBytes >= 4096 ? 4 : 6;
+  static constexpr int kRing = kMassWarps * kUnits * L::kBytes;
+  static constexpr int kRowTiles = L::f32 ? (D == 128 ? 2 : 8) : 16;
+  static constexpr int kSmem = kRing + kRowTiles * L::kQBytes + kRowTiles * 16 * 4 + 64;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
+  using S = MassShape<T, D>;
+  using L = Tile<T, D>;
+  constexpr int NU = S::kUnits;
+  extern __shared__ __align__(128) char sm[];
+  char *ring = sm, *q_sm = sm + S::kRing;
+  float *shift = (float *)(q_sm + S::kRowTiles * L::kQBytes);  // lse log2(e), +inf for rows that do not count
+  long long *plan = (long long *)(shift + S::kRowTiles * 16);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2;
+
+  // where this block's share of the cost starts: a sequence, the cost below it
+  if (warp == 0) {
+    long long all = 0;
+    for (int b = lane; b < a.s.batch; b += 32) all += MassShare(a, b).total(a.kv_heads);
+    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+    const long long lo = all * blockIdx.x / gridDim.x;
+    if (lane == 0) plan[0] = all, plan[1] = a.s.batch, plan[2] = all;
+    __syncwarp();
+    long long below = 0;
+    for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
+      const long long mine = b0 + lane < a.s.batch ? MassShare(a, b0 + lane).total(a.kv_heads) : 0;
+      long long upto = mine;
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long x = __shfl_up_sync(~0u, upto, d);
+        if (lane >= d) upto += x;
+      }
+      const unsigned hit = __ballot_sync(~0u, below + upto > lo);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) plan[1] = b0 + lane, plan[2] = below + upto - mine;
+        break;
+      }
+      below += __shfl_sync(~0u, upto, 31);
+    }
+  }
+  __syncthreads();
+  const long long lo = plan[0] * blockIdx.x / gridDim.x, hi = plan[0] * (blockIdx.x + 1) / gridDim.x;
+
+  const uint32_t my_ring = smem_addr(ring) + warp * NU * L::kBytes, q_at = smem_addr(q_sm);
+  long long at = plan[2];  // cost below the current segment
+  for (int b = (int)plan[1]; b < a.s.batch && at < hi; b++) {
+    const MassShare sh(a, b);
+    for (int head = 0; head < a.kv_heads; head++) {
+      // the tiles whose cost starts in this block's share
+      const long long from = max(lo - at, 0ll), to = hi - at;
+      const int t0 = (int)min((long long)sh.tiles, (from + sh.cost - 1) / sh.cost);
+      const int t1 = to <= 0 ? 0 : (int)min((long long)sh.tiles, (to + sh.cost - 1) / sh.cost);
+      at += (long long)sh.tiles * sh.cost;
+      if (t0 >= t1) continue;
+      const int c0 = t0 * kMassWarps + warp, chunks = (sh.len + kChunk - 1) / kChunk;
+      const int c_end = min(t1 * kMassWarps, chunks);
+      const int nk = c0 < c_end ? (c_end - c0 + kMassWarps - 1) / kMassWarps : 0;
+      const int rows = sh.count * a.group, row_tiles = (rows + 15) / 16;
+      const float *acc = a.acc ? a.acc + ((long long)b * a.kv_heads + head) * a.acc_stride : nullptr;
+      float *out = a.out + ((long long)b * a.kv_heads + head) * a.out_stride;
+
+      for (int m0 = 0; m0 == 0 || m0 < row_tiles; m0 += S::kRowTiles) {
+        const int mt = min(S::kRowTiles, row_tiles - m0);
+        int pages = -1;
+        unsigned long long valids = 0;  // 8 bits a unit in flight, the next one lowest
+        auto issue = [&](int k) {
+          if (k < nk) {
+            const int c = c0 + k * kMassWarps, pos = c * kChunk;
+            if ((k & 31) == 0) {
+              const int mine = c + lane * kMassWarps;
+              pages = mine < chunks ? a.c.table[b * a.c.table_stride + ((mine * kChunk) >> a.c.page_shift)] : -1;
+            }
+            const int pg = __shfl_sync(~0u, pages, k & 31);
+            const bool mapped = pg >= 0 && pg < a.c.num_pages;
+            const int valid = mapped ? min(kChunk, sh.len - pos) : 0;
+            valids |= (unsigned long long)valid << (8 * (k % NU));
+            L::template load<false>(my_ring + k % NU * L::kBytes,
+                                    a.c.k + (mapped ? pg : 0) * a.c.page_bytes + head * a.c.head_bytes +
+                                        (long long)(pos & ((1 << a.c.page_shift) - 1)) * a.c.token_bytes,
+                                    a.c.token_bytes, valid, lane);
+          }
+          copy_commit();
+        };
+        __syncthreads();  // the last pass is done with the query rows
+#pragma unroll
+        for (int k = 0; k < NU - 1; k++) issue(k);
+        const unsigned long long on = a.counted ? (unsigned long long)a.counted[b] : ~0ull;
+        auto counts = [&](int r) { return r < rows && (on >> (r / a.group) & 1); };
+        for (int m = 0; m < mt; m++)
+          L::query(q_at + m * L::kQBytes, tid, kMassThreads, [&](int r) -> const T * {
+            const int x = (m0 + m) * 16 + r;
+            return counts(x) ? (const T *)a.q + (sh.first + x / a.group) * a.q_stride +
+                                   (long long)(head * a.group + x % a.group) * D
+                             : nullptr;
+          });
+        for (int r = tid; r < mt * 16; r += kMassThreads) {
+          const int x = m0 * 16 + r;
+          float l = INFINITY;
+          if (counts(x)) {
+            l = a.lse[(long long)(sh.first + x / a.group) * a.kv_heads * a.group + head * a.group + x % a.group] * kLog2e;
+            if (l == -INFINITY) l = INFINITY;  // attended nothing
+          }
+          shift[r] = l;
+        }
+        __syncthreads();
+        for (int k = 0; k < nk; k++) {
+          copy_wait<NU - 2>();
+          __syncwarp();
+          const int valid = (int)(valids >> (8 * (k % NU))) & 31;
+          valids &= ~(0xffull << (8 * (k % NU)));
+          issue(k + NU - 1);
+          // what the sums were, while the products run: lane j < 16 has position j
+          const int pos = (c0 + k * kMassWarps) * kChunk + lane;
+          float old = 0.f;
+          if (lane < kChunk && pos < sh.len) {
+            if (m0)
+              old = out[pos];
+            else if (acc && pos < a.acc_width)
+              old = a.decay * acc[pos];
+          }
+          float w[2][2] = {};  // positions 8 n + 2 t + e
+          typename L::KFrag f;
+#pragma unroll
+          for (int blk = 0; blk < D / 16; blk++) L::k_load(f, blk, my_ring + k % NU * L::kBytes, lane);
+          for (int m = 0; m < mt; m++) {
+            float s[2][4] = {}, c[2][4] = {};
+#pragma unroll
+            for (int blk = 0; blk < D / 16; blk++) L::k_product(s, c, q_at + m * L::kQBytes, f, blk, lane);
+            const float l0 = shift[m * 16 + g], l1 = shift[m * 16 + 8 + g];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+              for (int e = 0; e < 2; e++)
+                w[n][e] += exp2_(fmaf(s[n][e] + c[n][e], a.scale, -l0)) + exp2_(fmaf(s[n][2 + e] + c[n][2 + e], a.scale, -l1));
+          }
+#pragma unroll
+          for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) w[n][e] += __shfl_xor_sync(~0u, w[n][e], d);
+          // lane j takes position j's sum from the lane that holds it
+          const int j = lane & 15, src = (j & 7) >> 1;
+          const float w00 = __shfl_sync(~0u, w[0][0], src), w01 = __shfl_sync(~0u, w[0][1], src);
+          const float w10 = __shfl_sync(~0u, w[1][0], src), w11 = __shfl_sync(~0u, w[1][1], src);
+          float mine = j & 8 ? (j & 1 ? w11 : w10) : (j & 1 ? w01 : w00);
+          if (j >= valid) mine = 0.f;
+          if (lane < kChunk && pos < sh.len) out[pos] = old + mine;
+        }
+        copy_wait<0>();
+      }
+    }
+  }
+  // 0 past the lengths: each row by the blocks that share its remainder
+  const int all_rows = a.s.batch * a.kv_heads, share = max(1, (int)gridDim.x / all_rows);
+  for (int i = blockIdx.x; i < all_rows * share; i += gridDim.x) {
+    const int r = i % all_rows, p = i / all_rows, len = min(a.s.len(r / a.kv_heads), a.out_width);
+    for (int x = len + p * kMassThreads + tid; x < a.out_width; x += share * kMassThreads) a.out[r * a.out_stride + x] = 0.f;
+  }
+}
+
+}  // namespace paged
+}  // namespace ocrvl

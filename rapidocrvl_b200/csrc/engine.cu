@@ -19,6 +19,7 @@
 #include <cuda.h>
 
 #include "../../include/ocrvl_cuda.h"
+#include "capi.h"
 #include "decoder.cuh"
 #include "batched.cuh"
 #include "sample.cuh"
@@ -50,6 +51,14 @@ int packed_row_bytes(int type, int cols) {
 }
 
 }  // namespace
+
+int ocrvl::api_fail(int code, const char *msg) noexcept {
+  try {
+    g_err = msg;
+  } catch (...) {  // no memory for the text: the code alone
+  }
+  return code;
+}
 
 // ---------------------------------------------------------------------------
 // Kernels
@@ -1243,6 +1252,47 @@ void ocrvl_seq_free(ocrvl_seq *s) {
 }
 
 int ocrvl_seq_len(const ocrvl_seq *s) { return s ? s->len : OCRVL_E_INVALID; }
+
+int ocrvl_seq_kv_view(ocrvl_seq *s, ocrvl_kv_cache *out) {
+  if (!s || !out) return fail(OCRVL_E_INVALID, "null argument");
+  ocrvl_model *m = s->m;
+  std::lock_guard<std::mutex> lk(m->mu);
+  const ocrvl_model_desc &d = m->desc;
+  // [page][layer][kv head][K, V][16][head_dim]
+  ocrvl_kv_cache c{};
+  c.type = OCRVL_F32;
+  c.head_dim = d.head_dim;
+  c.num_kv_heads = d.num_kv_heads;
+  c.num_layers = d.num_layers;
+  c.page_size = kPageTokens;
+  c.num_pages = m->num_pages;
+  c.batch = 1;
+  c.max_pages = (s->max_tokens + kPageTokens - 1) / kPageTokens;
+  c.token_stride = d.head_dim;
+  c.head_stride = 2ll * kPageTokens * d.head_dim;
+  c.layer_stride = c.head_stride * d.num_kv_heads;
+  c.page_stride = m->page_floats;
+  c.table_stride = c.max_pages;
+  c.k = m->kv_pool;
+  c.v = m->kv_pool + (size_t)kPageTokens * d.head_dim;
+  c.table = s->bt_d;
+  *out = c;
+  return OCRVL_OK;
+}
+
+int ocrvl_seq_truncate(ocrvl_seq *s, int n) {
+  if (!s) return fail(OCRVL_E_INVALID, "null seq");
+  ocrvl_model *m = s->m;
+  std::lock_guard<std::mutex> lk(m->mu);
+  if (n < 0 || n > s->len) return fail(OCRVL_E_INVALID, "n outside 0..length");
+  const size_t keep = (size_t)(n + kPageTokens - 1) / kPageTokens;
+  while (s->pages.size() > keep) {
+    m->free_pages.push_back(s->pages.back());
+    s->pages.pop_back();
+  }
+  s->len = n;
+  return OCRVL_OK;
+}
 
 int ocrvl_seq_import_kv(ocrvl_seq *s, int n, const float *k, const float *v) {
   if (!s) return fail(OCRVL_E_INVALID, "null seq");

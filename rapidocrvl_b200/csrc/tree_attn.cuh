@@ -1,0 +1,465 @@
+// Attention of drafted tokens over a paged cache and over one another
+// (ocrvl_op_tree_attn).
+//
+// For one kv head the rows are the sequence's drafted tokens times the query
+// heads that share it.  A block takes 16 MT rows against a run of positions; its
+// eight warps stream 16-position chunks of K and V of their own through private
+// rings of shared memory (no block barrier on the way), each with the running
+// maximum m, sum l and weighted values o of its own positions:
+//   m' = max(m, max s),  a = 2^(m - m'),  p = 2^(s - m'),
+//   l' = a l + sum p,    o' = a o + p v        (s = scale log2(e) q . k)
+// and are joined at the run's end: o = sum_w 2^(m_w - M) o_w, l likewise.
+//
+// Work is split by tiles of 128 positions over a persistent grid in equal
+// runs, whatever the lengths are: a block's run may cover several
+// (sequence, kv head, row block) segments and a segment several blocks.  A
+// segment within one block is written at once, else its parts go to the
+// workspace and k_tree_combine joins them.
+#pragma once
+#include "paged.cuh"
+
+namespace ocrvl {
+namespace paged {
+
+constexpr int kTreeWarps = 8;
+constexpr int kTreeThreads = kTreeWarps * 32;
+constexpr int kTileChunks = kTreeWarps;  // chunks a tile: one a warp
+
+struct TreeArgs {
+  Cache c;
+  Seqs s;
+  int kv_heads, group;  // group: query heads a kv head
+  const void *q, *dk, *dv;
+  void *out;
+  long long q_stride, kv_stride, out_stride;  // elements
+  const long long *mask;
+  float scale;    // scale * log2(e)
+  float *lse;
+  float *part;    // [2 grid][rows][D]
+  float *part_ml; // [2 grid][rows][2]
+};
+
+struct Segments {  // a sequence's share of the tiles
+  int first, count, len, chunks_c, chunks, tiles, blocks;
+
+  __device__ Segments(const TreeArgs &a, int b, int rows) {
+    count = a.s.tokens(b, &first);
+    len = a.s.len(b);
+    chunks_c = (len + kChunk - 1) / kChunk;
+    chunks = chunks_c + (count + kChunk - 1) / kChunk;
+    tiles = (chunks + kTileChunks - 1) / kTileChunks;
+    blocks = (count * a.group + rows - 1) / rows;
+  }
+  __device__ long long total(int kv_heads) const { return (long long)kv_heads * blocks * tiles; }
+};
+
+// Tiles of the sequences below b, and of all, by one warp.
+__device__ __forceinline__ void count_tiles(const TreeArgs &a, int rows, int b, int lane, long long *below, long long *all) {
+  long long lo = 0, sum = 0;
+  for (int i = lane; i < a.s.batch; i += 32) {
+    const long long n = Segments(a, i, rows).total(a.kv_heads);
+    sum += n;
+    if (i < b) lo += n;
+  }
+  for (int d = 16; d; d >>= 1) {
+    sum += __shfl_xor_sync(~0u, sum, d);
+    lo += __shfl_xor_sync(~0u, lo, d);
+  }
+  *below = lo;
+  *all = sum;
+}
+
+// First tile of block c of n.
+__device__ __forceinline__ long long run_start(long long all, int c, int n) { return all * c / n; }
+
+// Sets non-finite values to 0: in the matrix product 0 * NaN would reach rows
+// that do not see the draft they belong to.  The rows that see it get them
+// added apart.
+template <typename T, int D>
+__device__ __noinline__ void drop_nonfinite(uint32_t v, int lane) {
+  using L = Tile<T, D>;
+  for (int i = lane; i < kChunk * L::kPieces; i += 32) {
+    const uint32_t at = v + i * 16;
+    uint32_t x[4];
+    lds4u(x, at);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if constexpr (sizeof(T) == 4) {
+        if ((x[j] & 0x7f800000u) == 0x7f800000u) x[j] = 0u;
+      } else {
+        constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+        if ((x[j] & e) == e) x[j] &= 0xffff0000u;
+        if ((x[j] >> 16 & e) == e) x[j] &= 0xffffu;
+      }
+    }
+    sts4u(at, x[0], x[1], x[2], x[3]);
+  }
+  __syncwarp();
+}
+
+template <typename T, int D>
+__device__ __forceinline__ bool any_nonfinite(uint32_t v, int lane) {
+  using L = Tile<T, D>;
+  bool bad = false;
+  for (int i = lane; i < kChunk * L::kPieces; i += 32) {
+    uint32_t x[4];
+    lds4u(x, v + i * 16);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if constexpr (sizeof(T) == 4) {
+        bad |= (x[j] & 0x7f800000u) == 0x7f800000u;
+      } else {
+        constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+        bad |= (x[j] & e) == e || (x[j] >> 16 & e) == e;
+      }
+    }
+  }
+  return __any_sync(~0u, bad);
+}
+
+template <typename T, int D, int MT>
+struct TreeShape {
+  using L = Tile<T, D>;
+  static constexpr int kRows = 16 * MT;
+  // 16-bit types at 16 rows: two blocks an SM; else one
+  static constexpr int kBlocks = sizeof(T) == 2 && MT == 1 ? 2 : 1;
+  // chunks of K or V in a warp's ring: about 192 KB an SM
+  static constexpr int kUnits = L::kBytes * kBlocks >= 8192 ? 3 : 6;
+  static constexpr int kRing = kTreeWarps * kUnits * L::kBytes;
+  static constexpr int kPitch = D + 4;  // floats a row of the join: rows start 4 banks apart
+  static constexpr int kJoin = kTreeWarps * kRows * kPitch * 4;
+  static constexpr int kQ = MT * L::kQBytes;
+  static constexpr int kSmem = kQ + (kRing > kJoin ? kRing : kJoin) + kTreeWarps * kRows * 8 + kRows * 8 + 64 +
+                               kTreeWarps * 8 * 4;
+};
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) k_tree_attn(const TreeArgs a) {
+  using S = TreeShape<T, D, MT>;
+  using L = Tile<T, D>;
+  constexpr int ROWS = S::kRows, NU = S::kUnits;
+  extern __shared__ __align__(128) char sm[];
+  char *q_sm = sm, *ring = sm + S::kQ;
+  char *p = ring + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
+  float *ml = (float *)p;  // [warp][row][m, l]
+  p += kTreeWarps * ROWS * 8;
+  unsigned long long *seen = (unsigned long long *)p;  // [row]
+  p += ROWS * 8;
+  long long *plan = (long long *)p;  // all tiles; where this block starts: b, kv head, row block, tile
+  p += 64;
+  int *there = (int *)p;  // [warp][unit]: positions of the chunk that exist
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+
+  // where this block's run starts
+  if (warp == 0) {
+    long long below, all;
+    count_tiles(a, ROWS, 0, lane, &below, &all);
+    const int n = (int)min((long long)gridDim.x, all);
+    if (lane == 0) plan[0] = all, plan[1] = a.s.batch;
+    __syncwarp();
+    if (blockIdx.x < n) {
+      const long long w0 = run_start(all, blockIdx.x, n);
+      long long at = 0;
+      for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
+        const int b = b0 + lane;
+        const long long mine = b < a.s.batch ? Segments(a, b, ROWS).total(a.kv_heads) : 0;
+        long long upto = mine;
+        for (int d = 1; d < 32; d <<= 1) {
+          const long long x = __shfl_up_sync(~0u, upto, d);
+          if (lane >= d) upto += x;
+        }
+        const unsigned hit = __ballot_sync(~0u, at + upto > w0);
+        if (hit) {
+          if (lane == __ffs(hit) - 1) {
+            const Segments g_(a, b, ROWS);
+            const long long in = w0 - (at + upto - mine);
+            plan[1] = b;
+            plan[2] = in / g_.tiles / g_.blocks;
+            plan[3] = in / g_.tiles % g_.blocks;
+            plan[4] = in % g_.tiles;
+          }
+          break;
+        }
+        at += __shfl_sync(~0u, upto, 31);
+      }
+    }
+  }
+  pdl_launch();
+  __syncthreads();
+  const long long all = plan[0];
+  const int grid = (int)min((long long)gridDim.x, all);
+  if ((int)blockIdx.x >= grid) return;
+  long long left = run_start(all, blockIdx.x + 1, grid) - run_start(all, blockIdx.x, grid);
+  int b = (int)plan[1], head = (int)plan[2], rb = (int)plan[3], t0 = (int)plan[4];
+
+  const uint32_t my_ring = smem_addr(ring) + warp * NU * L::kBytes, q_at = smem_addr(q_sm);
+  int *my_there = there + warp * NU;
+
+  for (int piece = 0; left > 0 && b < a.s.batch; piece++) {
+    const Segments sg(a, b, ROWS);
+    if (sg.blocks == 0) {  // no drafted tokens
+      b++, piece--;
+      continue;
+    }
+    const int t1 = (int)min((long long)sg.tiles, t0 + left);
+    const int rows = min(ROWS, sg.count * a.group - rb * ROWS);
+    // this warp's chunks: c0, c0 + 8, ...
+    const int c0 = t0 * kTileChunks + warp;
+    const int c_end = min(t1 * kTileChunks, sg.chunks);
+    const int nk = c0 < c_end ? (c_end - c0 + kTileChunks - 1) / kTileChunks : 0;
+
+    int pages = -1;  // lane i: the page of the chunk 32 j + i
+    auto issue = [&](int u) {
+      if (u < 2 * nk) {
+        const int k = u >> 1, c = c0 + k * kTileChunks, slot = u % NU;
+        const uint32_t to = my_ring + slot * L::kBytes;
+        const char *src;
+        long long row_bytes;
+        int valid;
+        if (!(u & 1) && (k & 31) == 0) {
+          const int mine = c + lane * kTileChunks;
+          const int pg = mine < sg.chunks_c ? (mine * kChunk) >> a.c.page_shift : -1;
+          pages = pg >= 0 ? a.c.table[b * a.c.table_stride + pg] : -1;
+        }
+        if (c < sg.chunks_c) {
+          const int pos = c * kChunk, pg = __shfl_sync(~0u, pages, k & 31);
+          const bool mapped = pg >= 0 && pg < a.c.num_pages;
+          valid = mapped ? min(kChunk, sg.len - pos) : 0;
+          row_bytes = a.c.token_bytes;
+          src = (u & 1 ? a.c.v : a.c.k) + (mapped ? pg : 0) * a.c.page_bytes + head * a.c.head_bytes +
+                (long long)(pos & ((1 << a.c.page_shift) - 1)) * a.c.token_bytes;
+        } else {
+          const int j = (c - sg.chunks_c) * kChunk;
+          valid = min(kChunk, sg.count - j);
+          row_bytes = a.kv_stride * (long long)sizeof(T);
+          src = (const char *)((const T *)(u & 1 ? a.dv : a.dk) + (sg.first + j) * a.kv_stride + (long long)head * D);
+        }
+        if (u & 1)
+          L::template load<true>(to, src, row_bytes, valid, lane);
+        else
+          L::template load<false>(to, src, row_bytes, valid, lane);
+        if (lane == 0) my_there[slot] = valid;
+      }
+      copy_commit();
+    };
+#pragma unroll
+    for (int u = 0; u < NU - 1; u++) issue(u);
+
+    // the query rows and the drafts that each sees
+    for (int m = 0; m < MT; m++)
+      L::query(q_at + m * L::kQBytes, tid, kTreeThreads, [&](int r) -> const T * {
+        const int row = m * 16 + r, x = rb * ROWS + row;
+        return row < rows ? (const T *)a.q + (sg.first + x / a.group) * a.q_stride +
+                                (long long)(head * a.group + x % a.group) * D
+                          : nullptr;
+      });
+    for (int r = tid; r < ROWS; r += kTreeThreads)
+      seen[r] = r < rows ? (unsigned long long)a.mask[sg.first + (rb * ROWS + r) / a.group] : 0ull;
+    __syncthreads();
+
+    float o[MT][D / 8][4] = {}, mx[MT][2], sum[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; m++) mx[m][0] = mx[m][1] = -INFINITY, sum[m][0] = sum[m][1] = 0.f;
+
+    for (int k = 0; k < nk; k++) {
+      const int c = c0 + k * kTileChunks, u = 2 * k;
+      copy_wait<NU - 2>();
+      __syncwarp();
+      issue(u + NU - 1);
+      float s[MT][2][4];
+      L::template scores<MT>(s, q_at, my_ring + (u % NU) * L::kBytes, lane);
+      const int valid = my_there[u % NU];
+      const bool draft = c >= sg.chunks_c;
+      const int j0 = (c - sg.chunks_c) * kChunk;
+      float alpha[MT][2];
+      bool rescale = false;
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {  // rows g and g + 8
+          float x[4] = {s[m][0][2 * h], s[m][0][2 * h + 1], s[m][1][2 * h], s[m][1][2 * h + 1]};
+          unsigned ok = 0;
+#pragma unroll
+          for (int i = 0; i < 4; i++) ok |= ((i >> 1) * 8 + 2 * t + (i & 1) < valid ? 1u : 0u) << i;
+          if (draft) {
+            const unsigned w = (unsigned)(seen[m * 16 + 8 * h + g] >> j0);
+            ok &= (w >> (2 * t) & 3u) | (w >> (8 + 2 * t) & 3u) << 2;
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (ok >> i & 1) top = fmaxf(top, x[i] * a.scale);
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+          const float now = fmaxf(mx[m][h], top), ref = now == -INFINITY ? 0.f : now;
+          alpha[m][h] = exp2_(mx[m][h] - ref);
+          rescale |= alpha[m][h] != 1.f;
+          mx[m][h] = now;
+          float add = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            x[i] = ok >> i & 1 ? exp2_(fmaf(x[i], a.scale, -ref)) : 0.f;
+            add += x[i];
+          }
+          sum[m][h] = fmaf(sum[m][h], alpha[m][h], add);
+          s[m][0][2 * h] = x[0], s[m][0][2 * h + 1] = x[1], s[m][1][2 * h] = x[2], s[m][1][2 * h + 1] = x[3];
+        }
+      rescale = __any_sync(~0u, rescale);
+      copy_wait<NU - 2>();
+      __syncwarp();
+      issue(u + NU);
+      const uint32_t v = my_ring + ((u + 1) % NU) * L::kBytes;
+      bool bad = false;
+      if (draft) {
+        bad = any_nonfinite<T, D>(v, lane);
+        if (bad) drop_nonfinite<T, D>(v, lane);
+      }
+      L::template values<MT>(o, s, alpha, rescale, v, lane);
+      if (bad) {
+        for (int j = 0; j < valid; j++) {
+          const T *row = (const T *)a.dv + (sg.first + j0 + j) * a.kv_stride + (long long)head * D;
+#pragma unroll
+          for (int m = 0; m < MT; m++) {
+            const int from = (lane & ~3) | ((j & 7) >> 1);
+            float w[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const float x0 = j & 1 ? s[m][0][2 * h + 1] : s[m][0][2 * h], x1 = j & 1 ? s[m][1][2 * h + 1] : s[m][1][2 * h];
+              w[h] = __shfl_sync(~0u, j >> 3 ? x1 : x0, from);
+            }
+            const bool see0 = seen[m * 16 + g] >> (j0 + j) & 1, see1 = seen[m * 16 + 8 + g] >> (j0 + j) & 1;
+#pragma unroll
+            for (int nt = 0; nt < D / 8; nt++)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const float x = to_f(row[L::out_dim(nt, e, t)]);
+                if (!isfinite(x)) {
+                  if (see0) o[m][nt][e] += w[0] * x;
+                  if (see1) o[m][nt][e + 2] += w[1] * x;
+                }
+              }
+          }
+        }
+      }
+    }
+    copy_wait<0>();
+    __syncthreads();  // every warp is done with the ring: it takes the parts
+
+    float *join = (float *)ring;
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float l = sum[m][h];
+        l += __shfl_xor_sync(~0u, l, 1);
+        l += __shfl_xor_sync(~0u, l, 2);
+        const int row = m * 16 + 8 * h + g;
+        if (t == 0) ml[(warp * ROWS + row) * 2] = mx[m][h], ml[(warp * ROWS + row) * 2 + 1] = l;
+        float *to = join + (warp * ROWS + row) * S::kPitch;
+        if constexpr (L::f32) {
+#pragma unroll
+          for (int blk = 0; blk < D / 32; blk++) {
+            auto &x = o[m];
+            *(float4 *)(to + blk * 32 + 8 * t) = make_float4(x[blk * 4][2 * h], x[blk * 4 + 1][2 * h], x[blk * 4 + 2][2 * h], x[blk * 4 + 3][2 * h]);
+            *(float4 *)(to + blk * 32 + 8 * t + 4) = make_float4(x[blk * 4][2 * h + 1], x[blk * 4 + 1][2 * h + 1], x[blk * 4 + 2][2 * h + 1], x[blk * 4 + 3][2 * h + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int nt = 0; nt < D / 8; nt++) *(float2 *)(to + nt * 8 + 2 * t) = make_float2(o[m][nt][2 * h], o[m][nt][2 * h + 1]);
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == sg.tiles;
+    const long long slot = 2 * (long long)blockIdx.x + (piece ? 1 : 0);
+    for (int i = tid; i < rows * (D / 4); i += kTreeThreads) {
+      const int row = i / (D / 4), d = i % (D / 4) * 4;
+      float top = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; w++) top = fmaxf(top, ml[(w * ROWS + row) * 2]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kTreeWarps; w++) {
+        const float f = exp2_(ml[(w * ROWS + row) * 2] - ref);
+        l = fmaf(f, ml[(w * ROWS + row) * 2 + 1], l);
+        const float4 y = *(const float4 *)(join + (w * ROWS + row) * S::kPitch + d);
+        x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+      }
+      if (whole) {
+        const int r = rb * ROWS + row, tok = sg.first + r / a.group, hd = head * a.group + r % a.group;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        store4((T *)a.out + tok * a.out_stride + (long long)hd * D + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        if (d == 0 && a.lse) a.lse[(long long)tok * a.kv_heads * a.group + hd] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+      } else {
+        *(float4 *)(a.part + (slot * ROWS + row) * D + d) = x;
+        if (d == 0) *(float2 *)(a.part_ml + (slot * ROWS + row) * 2) = make_float2(top, l);
+      }
+    }
+    left -= t1 - t0;
+    t0 = 0;
+    if (++rb == sg.blocks) rb = 0, head++;
+    if (head == a.kv_heads) head = 0, b++;
+    __syncthreads();  // the ring and the query rows are free again
+  }
+}
+
+// Joins the parts of the segments that several blocks share: one block a
+// (row, segment), its four warps over the parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) k_tree_combine(const TreeArgs a, int rows_a_block, int main_grid) {
+  __shared__ float o_sm[4][D], ml_sm[4][2];
+  __shared__ long long plan[2];
+  const int b = blockIdx.z, head = blockIdx.y % a.kv_heads, rb = blockIdx.y / a.kv_heads, row = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Segments sg(a, b, rows_a_block);
+  const int r = rb * rows_a_block + row;
+  if (warp == 0) {
+    long long below, all;
+    count_tiles(a, rows_a_block, b, lane, &below, &all);
+    if (lane == 0) plan[0] = below, plan[1] = all;
+  }
+  pdl_wait();  // on every path: this grid's end is to mean the main one's too
+  if (r >= sg.count * a.group) return;
+  __syncthreads();
+  const long long all = plan[1], s0 = plan[0] + (long long)(head * sg.blocks + rb) * sg.tiles, s1 = s0 + sg.tiles;
+  const int grid = (int)min((long long)main_grid, all);
+  const int first = (int)(((s0 + 1) * grid - 1) / all), last = (int)((s1 * grid - 1) / all);
+  if (first == last) return;  // written already
+  constexpr int V = D / 32;
+  float top = -INFINITY, l = 0.f, x[V] = {};
+  for (int c = first + warp; c <= last; c += 4) {
+    const long long slot = 2ll * c + (run_start(all, c, grid) >= s0 ? 0 : 1);
+    const float2 p = *(const float2 *)(a.part_ml + (slot * rows_a_block + row) * 2);
+    const float now = fmaxf(top, p.x), ref = now == -INFINITY ? 0.f : now;
+    const float f0 = exp2_(top - ref), f1 = exp2_(p.x - ref);
+    top = now;
+    l = fmaf(l, f0, f1 * p.y);
+    const float *from = a.part + (slot * rows_a_block + row) * D + lane * V;
+#pragma unroll
+    for (int i = 0; i < V; i++) x[i] = fmaf(x[i], f0, f1 * from[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++) o_sm[warp][lane * V + i] = x[i];
+  if (lane == 0) ml_sm[warp][0] = top, ml_sm[warp][1] = l;
+  __syncthreads();
+  if (tid < D / 4) {
+    float m = -INFINITY, sum = 0.f;
+    for (int w = 0; w < 4; w++) m = fmaxf(m, ml_sm[w][0]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < 4; w++) {
+      const float f = exp2_(ml_sm[w][0] - ref);
+      sum = fmaf(f, ml_sm[w][1], sum);
+      const float4 z = *(const float4 *)&o_sm[w][tid * 4];
+      y.x = fmaf(f, z.x, y.x), y.y = fmaf(f, z.y, y.y), y.z = fmaf(f, z.z, y.z), y.w = fmaf(f, z.w, y.w);
+    }
+    const int tok = sg.first + r / a.group, hd = head * a.group + r % a.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    store4((T *)a.out + tok * a.out_stride + (long long)hd * D + tid * 4, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+    if (tid == 0 && a.lse) a.lse[(long long)tok * a.kv_heads * a.group + hd] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+  }
+}
+
+}  // namespace paged
+}  // namespace ocrvl
