@@ -148,11 +148,28 @@ int64_t tree_work_bytes(int sms, int dim) { return (int64_t)sms * 2 * 2 * 32 * (
 template <typename T, int D, int MT>
 int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stream) {
   using S = TreeShape<T, D, MT>;
+  const int blocks = (rows_max + S::kRows - 1) / S::kRows;
+  const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
+  if (segments > 1 << 24) return invalid("too many sequences and kv heads");
+  // A cluster a segment where a block then has at most kFew tiles of the longest cache
+  // and all clusters run at once: saves the second launch.
+  constexpr int kFew = 4;
+  const int tiles = (a.s.capacity + 64 + kChunk * kTileChunks - 1) / (kChunk * kTileChunks);
+  auto one = [&](auto kernel, int cs) {
+    return launch("tree attention", kernel, dim3((unsigned)(segments * cs)), kTreeThreads, S::kSmem, stream, false, cs, a, blocks);
+  };
+  const int room = sms * S::kBlocks;
+  if (tiles <= kFew && (segments >= room || tiles <= 2)) return one(k_tree_attn<T, D, MT, 1>, 1);
+  if (tiles <= 4 * kFew && segments * 4 <= room) {
+    if (tiles > 4 && segments * 8 <= room) return one(k_tree_attn<T, D, MT, 8>, 8);
+    return one(k_tree_attn<T, D, MT, 4>, 4);
+  }
+  if (tiles <= 8 * kFew && segments * 8 <= room) return one(k_tree_attn<T, D, MT, 8>, 8);
+
   const int grid = sms * S::kBlocks;
   a.part = (float *)work;
   a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
-  if (int rc = launch("tree attention", k_tree_attn<T, D, MT>, dim3(grid), kTreeThreads, S::kSmem, stream, false, 1, a)) return rc;
-  const int blocks = (rows_max + S::kRows - 1) / S::kRows;
+  if (int rc = launch("tree attention", k_tree_attn<T, D, MT, 0>, dim3(grid), kTreeThreads, S::kSmem, stream, false, 1, a, blocks)) return rc;
   if ((long long)blocks * a.kv_heads > 65535) return invalid("too many kv heads");
   return launch("tree attention (join)", k_tree_combine<T, D>, dim3(rows_max < S::kRows ? rows_max : S::kRows, blocks * a.kv_heads, a.s.batch), 128, 0,
                 stream, true, 1, a, S::kRows, grid);

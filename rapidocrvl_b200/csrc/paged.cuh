@@ -67,8 +67,7 @@ __device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
 }
 
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -77,15 +76,13 @@ template <typename T>
 __device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma_16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma_16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -222,13 +219,14 @@ struct Tile {
         uint32_t h[4], l[4];
         lds4u(h, at + step * 512);
         lds4u(l, at + 1024 + step * 512);
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-          const uint32_t *kh = f.hi[blk] + n * 4 + 2 * step, *kl = f.lo[blk] + n * 4 + 2 * step;
-          mma_tf32(s[n], h, kh[0], kh[1]);
-          mma_tf32(c[n], h, kl[0], kl[1]);
-          mma_tf32(c[n], l, kh[0], kh[1]);
-        }
+        // neighbours use different accumulators: a chain of its own takes 11.5 ns a link
+        const uint32_t *kh = f.hi[blk] + 2 * step, *kl = f.lo[blk] + 2 * step;
+        mma_tf32(c[0], h, kl[0], kl[1]);
+        mma_tf32(c[1], h, kl[4], kl[5]);
+        mma_tf32(s[0], h, kh[0], kh[1]);
+        mma_tf32(s[1], h, kh[4], kh[5]);
+        mma_tf32(c[0], l, kh[0], kh[1]);
+        mma_tf32(c[1], l, kh[4], kh[5]);
       }
     } else {
       uint32_t x[4];
@@ -301,23 +299,28 @@ struct Tile {
             split(x.z, vh[n][j][2], vl[n][j][2]), split(x.w, vh[n][j][3], vl[n][j][3]);
           }
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int m = 0; m < MT; m++) {
+          float a[4][4] = {};
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) mma_tf32(a[i], ph[m][n], vl[n][0][i], vl[n][1][i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) mma_tf32(a[i], pl[m][n], vh[n][0][i], vh[n][1][i]);
+          }
+#pragma unroll
+          for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) mma_tf32(a[i], ph[m][n], vh[n][0][i], vh[n][1][i]);
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            float a[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-              mma_tf32(a, ph[m][n], vl[n][0][i], vl[n][1][i]);
-              mma_tf32(a, pl[m][n], vh[n][0][i], vh[n][1][i]);
-            }
-#pragma unroll
-            for (int n = 0; n < 2; n++) mma_tf32(a, ph[m][n], vh[n][0][i], vh[n][1][i]);
             float(&to)[4] = o[m][blk * 4 + i];
-            to[0] = fmaf(to[0], alpha[m][0], a[0]);
-            to[1] = fmaf(to[1], alpha[m][0], a[1]);
-            to[2] = fmaf(to[2], alpha[m][1], a[2]);
-            to[3] = fmaf(to[3], alpha[m][1], a[3]);
+            to[0] = fmaf(to[0], alpha[m][0], a[i][0]);
+            to[1] = fmaf(to[1], alpha[m][0], a[i][1]);
+            to[2] = fmaf(to[2], alpha[m][1], a[i][2]);
+            to[3] = fmaf(to[3], alpha[m][1], a[i][3]);
           }
+        }
       }
     } else {
       if (rescale) {

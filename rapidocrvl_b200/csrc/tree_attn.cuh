@@ -10,12 +10,19 @@
 //   l' = a l + sum p,    o' = a o + p v        (s = scale log2(e) q . k)
 // and are joined at the run's end: o = sum_w 2^(m_w - M) o_w, l likewise.
 //
-// Work is split by tiles of 128 positions over a persistent grid in equal
-// runs, whatever the lengths are: a block's run may cover several
-// (sequence, kv head, row block) segments and a segment several blocks.  A
-// segment within one block is written at once, else its parts go to the
-// workspace and k_tree_combine joins them.
+// A (sequence, kv head, row block) is a segment.  Two ways to share them out:
+//   CS = 0  tiles of 128 positions over a persistent grid in equal runs,
+//           whatever the lengths are: a run may cover several segments and a
+//           segment several runs.  A segment within one run is written at
+//           once, else its parts go to the workspace and k_tree_combine joins
+//           them.  The first chunks of a run's next segment are fetched
+//           before the warps join, so the memory does not idle.
+//   CS > 0  a cluster of CS blocks a segment, joined over distributed shared
+//           memory: one launch, no workspace, no search for the run's start.
+//           For calls whose segments and lengths are few.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "paged.cuh"
 
 namespace ocrvl {
@@ -24,6 +31,9 @@ namespace paged {
 constexpr int kTreeWarps = 8;
 constexpr int kTreeThreads = kTreeWarps * 32;
 constexpr int kTileChunks = kTreeWarps;  // chunks a tile: one a warp
+// Cost of a tile, and of starting a segment (filling the rings, joining the
+// warps takes about as long as a tile), in the split of runs.
+constexpr int kTileCost = 1, kSegmentCost = 1;
 
 struct TreeArgs {
   Cache c;
@@ -39,9 +49,10 @@ struct TreeArgs {
   float *part_ml; // [2 grid][rows][2]
 };
 
-struct Segments {  // a sequence's share of the tiles
+struct Segments {  // what a sequence's segments have in common
   int first, count, len, chunks_c, chunks, tiles, blocks;
 
+  __device__ Segments() {}
   __device__ Segments(const TreeArgs &a, int b, int rows) {
     count = a.s.tokens(b, &first);
     len = a.s.len(b);
@@ -50,11 +61,12 @@ struct Segments {  // a sequence's share of the tiles
     tiles = (chunks + kTileChunks - 1) / kTileChunks;
     blocks = (count * a.group + rows - 1) / rows;
   }
-  __device__ long long total(int kv_heads) const { return (long long)kv_heads * blocks * tiles; }
+  __device__ int cost() const { return kSegmentCost + kTileCost * tiles; }
+  __device__ long long total(int kv_heads) const { return (long long)kv_heads * blocks * cost(); }
 };
 
-// Tiles of the sequences below b, and of all, by one warp.
-__device__ __forceinline__ void count_tiles(const TreeArgs &a, int rows, int b, int lane, long long *below, long long *all) {
+// Cost of the sequences below b, and of all, by one warp.
+__device__ __forceinline__ void count_cost(const TreeArgs &a, int rows, int b, int lane, long long *below, long long *all) {
   long long lo = 0, sum = 0;
   for (int i = lane; i < a.s.batch; i += 32) {
     const long long n = Segments(a, i, rows).total(a.kv_heads);
@@ -69,8 +81,13 @@ __device__ __forceinline__ void count_tiles(const TreeArgs &a, int rows, int b, 
   *all = sum;
 }
 
-// First tile of block c of n.
+// Run c of n covers the costs from run_start(c) to run_start(c + 1) and takes
+// the tiles that start there; a segment's tiles start behind its own cost.
 __device__ __forceinline__ long long run_start(long long all, int c, int n) { return all * c / n; }
+__device__ __forceinline__ int tiles_below(long long x, long long segment, int tiles) {
+  const long long t = (x - segment - kSegmentCost + kTileCost - 1) / kTileCost;
+  return x <= segment + kSegmentCost ? 0 : (int)min(t, (long long)tiles);
+}
 
 // Sets non-finite values to 0: in the matrix product 0 * NaN would reach rows
 // that do not see the draft they belong to.  The rows that see it get them
@@ -125,152 +142,207 @@ struct TreeShape {
   static constexpr int kBlocks = sizeof(T) == 2 && MT == 1 ? 2 : 1;
   // chunks of K or V in a warp's ring: about 192 KB an SM
   static constexpr int kUnits = L::kBytes * kBlocks >= 8192 ? 3 : 6;
-  static constexpr int kRing = kTreeWarps * kUnits * L::kBytes;
-  static constexpr int kPitch = D + 4;  // floats a row of the join: rows start 4 banks apart
-  static constexpr int kJoin = kTreeWarps * kRows * kPitch * 4;
+  static constexpr int kSlot = kTreeWarps * L::kBytes;  // one unit of every warp
+  // the join of 16 rows of eight warps in f32 lies over the last slots, so the
+  // others can be filled meanwhile
+  static constexpr int kJoinSlots = 4 / (int)sizeof(T);
+  static constexpr int kEarly = kUnits - kJoinSlots;
   static constexpr int kQ = MT * L::kQBytes;
-  static constexpr int kSmem = kQ + (kRing > kJoin ? kRing : kJoin) + kTreeWarps * kRows * 8 + kRows * 8 + 64 +
-                               kTreeWarps * 8 * 4;
+  static constexpr int kSmem = kQ + kUnits * kSlot + kTreeWarps * kRows * 8 + kRows * 8 + 64 + kTreeWarps * 8 * 4 + kRows * 8;
+  static_assert(kTreeWarps * 16 * D * 4 == kJoinSlots * kSlot && kEarly >= 1 && kEarly <= kUnits - 1, "");
 };
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) k_tree_attn(const TreeArgs a) {
+// A warp's part in a run of one segment's positions.
+struct Piece {
+  Segments sg;
+  int b, head, rb, t0, t1;  // tiles
+  int c0, step, nk;         // chunks c0, c0 + step, ...: nk of them
+  __device__ void chunks_of(int warp, int stride) {
+    c0 = t0 * kTileChunks + warp, step = stride;
+    const int end = min(t1 * kTileChunks, sg.chunks);
+    nk = c0 < end ? (end - c0 + step - 1) / step : 0;
+  }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const TreeArgs &a, const Segments &sg, int head, int r, int d, float4 x, float top, float l) {
+  const int tok = sg.first + r / a.group, hd = head * a.group + r % a.group;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  store4((T *)a.out + tok * a.out_stride + (long long)hd * D + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+  if (d == 0 && a.lse) a.lse[(long long)tok * a.kv_heads * a.group + hd] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+}
+
+template <typename T, int D, int MT, int CS>
+__global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) k_tree_attn(const TreeArgs a, int row_blocks) {
   using S = TreeShape<T, D, MT>;
   using L = Tile<T, D>;
   constexpr int ROWS = S::kRows, NU = S::kUnits;
+  namespace cg = cooperative_groups;
   extern __shared__ __align__(128) char sm[];
   char *q_sm = sm, *ring = sm + S::kQ;
-  char *p = ring + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
+  char *p = ring + NU * S::kSlot;
   float *ml = (float *)p;  // [warp][row][m, l]
   p += kTreeWarps * ROWS * 8;
   unsigned long long *seen = (unsigned long long *)p;  // [row]
   p += ROWS * 8;
-  long long *plan = (long long *)p;  // all tiles; where this block starts: b, kv head, row block, tile
+  long long *plan = (long long *)p;  // the cost of all; where this block's run starts: a sequence, the cost below it
   p += 64;
   int *there = (int *)p;  // [warp][unit]: positions of the chunk that exist
+  p += kTreeWarps * 8 * 4;
+  float *part_ml = (float *)p;  // CS > 1: [row][m, l] of this block
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-  // where this block's run starts
-  if (warp == 0) {
-    long long below, all;
-    count_tiles(a, ROWS, 0, lane, &below, &all);
-    const int n = (int)min((long long)gridDim.x, all);
-    if (lane == 0) plan[0] = all, plan[1] = a.s.batch;
-    __syncwarp();
-    if (blockIdx.x < n) {
-      const long long w0 = run_start(all, blockIdx.x, n);
-      long long at = 0;
-      for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
-        const int b = b0 + lane;
-        const long long mine = b < a.s.batch ? Segments(a, b, ROWS).total(a.kv_heads) : 0;
-        long long upto = mine;
-        for (int d = 1; d < 32; d <<= 1) {
-          const long long x = __shfl_up_sync(~0u, upto, d);
-          if (lane >= d) upto += x;
-        }
-        const unsigned hit = __ballot_sync(~0u, at + upto > w0);
-        if (hit) {
-          if (lane == __ffs(hit) - 1) {
-            const Segments g_(a, b, ROWS);
-            const long long in = w0 - (at + upto - mine);
-            plan[1] = b;
-            plan[2] = in / g_.tiles / g_.blocks;
-            plan[3] = in / g_.tiles % g_.blocks;
-            plan[4] = in % g_.tiles;
+  Piece cur;
+  long long at = 0, hi = 0;  // cost at which the current segment starts; the run's end
+  bool more = true;
+  if constexpr (CS == 0) {
+    if (warp == 0) {
+      long long below, all;
+      count_cost(a, ROWS, 0, lane, &below, &all);
+      const int n = (int)min((long long)gridDim.x, all);
+      if (lane == 0) plan[0] = all, plan[1] = a.s.batch;
+      __syncwarp();
+      if (blockIdx.x < n) {
+        const long long lo = run_start(all, blockIdx.x, n);
+        long long sum = 0;
+        for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
+          const int b = b0 + lane;
+          const long long mine = b < a.s.batch ? Segments(a, b, ROWS).total(a.kv_heads) : 0;
+          long long upto = mine;
+          for (int d = 1; d < 32; d <<= 1) {
+            const long long x = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += x;
           }
-          break;
+          const unsigned hit = __ballot_sync(~0u, sum + upto > lo);
+          if (hit) {
+            if (lane == __ffs(hit) - 1) plan[1] = b, plan[2] = sum + upto - mine;
+            break;
+          }
+          sum += __shfl_sync(~0u, upto, 31);
         }
-        at += __shfl_sync(~0u, upto, 31);
       }
     }
+    pdl_launch();
+    __syncthreads();
+    const long long all = plan[0];
+    const int n = (int)min((long long)gridDim.x, all);
+    cur.b = (int)plan[1];
+    if ((int)blockIdx.x >= n || cur.b >= a.s.batch) return;
+    const long long lo = run_start(all, blockIdx.x, n);
+    hi = run_start(all, blockIdx.x + 1, n);
+    cur.sg = Segments(a, cur.b, ROWS);
+    const int i = (int)((lo - plan[2]) / cur.sg.cost());
+    at = plan[2] + (long long)i * cur.sg.cost();
+    cur.head = i / cur.sg.blocks, cur.rb = i % cur.sg.blocks;
+    cur.t0 = tiles_below(lo, at, cur.sg.tiles);
+    cur.t1 = tiles_below(hi, at, cur.sg.tiles);
+    cur.chunks_of(warp, kTileChunks);
+  } else {
+    const int seg = blockIdx.x / CS;
+    cur.rb = seg % row_blocks, cur.head = seg / row_blocks % a.kv_heads, cur.b = seg / row_blocks / a.kv_heads;
+    cur.sg = Segments(a, cur.b, ROWS);
+    if (cur.rb >= cur.sg.blocks) return;  // the whole cluster alike
+    cur.t0 = blockIdx.x % CS, cur.t1 = cur.sg.tiles;
+    cur.chunks_of(warp, kTileChunks * CS);
   }
-  pdl_launch();
-  __syncthreads();
-  const long long all = plan[0];
-  const int grid = (int)min((long long)gridDim.x, all);
-  if ((int)blockIdx.x >= grid) return;
-  long long left = run_start(all, blockIdx.x + 1, grid) - run_start(all, blockIdx.x, grid);
-  int b = (int)plan[1], head = (int)plan[2], rb = (int)plan[3], t0 = (int)plan[4];
-
-  const uint32_t my_ring = smem_addr(ring) + warp * NU * L::kBytes, q_at = smem_addr(q_sm);
-  int *my_there = there + warp * NU;
-
-  for (int piece = 0; left > 0 && b < a.s.batch; piece++) {
-    const Segments sg(a, b, ROWS);
-    if (sg.blocks == 0) {  // no drafted tokens
-      b++, piece--;
-      continue;
-    }
-    const int t1 = (int)min((long long)sg.tiles, t0 + left);
-    const int rows = min(ROWS, sg.count * a.group - rb * ROWS);
-    // this warp's chunks: c0, c0 + 8, ...
-    const int c0 = t0 * kTileChunks + warp;
-    const int c_end = min(t1 * kTileChunks, sg.chunks);
-    const int nk = c0 < c_end ? (c_end - c0 + kTileChunks - 1) / kTileChunks : 0;
-
-    int pages = -1;  // lane i: the page of the chunk 32 j + i
-    auto issue = [&](int u) {
-      if (u < 2 * nk) {
-        const int k = u >> 1, c = c0 + k * kTileChunks, slot = u % NU;
-        const uint32_t to = my_ring + slot * L::kBytes;
-        const char *src;
-        long long row_bytes;
-        int valid;
-        if (!(u & 1) && (k & 31) == 0) {
-          const int mine = c + lane * kTileChunks;
-          const int pg = mine < sg.chunks_c ? (mine * kChunk) >> a.c.page_shift : -1;
-          pages = pg >= 0 ? a.c.table[b * a.c.table_stride + pg] : -1;
+  // the run's next piece that has tiles
+  auto next = [&](Piece &x) {
+    while (true) {
+      at += x.sg.cost();
+      if (at >= hi) return false;
+      if (++x.rb == x.sg.blocks) {
+        x.rb = 0;
+        if (++x.head == a.kv_heads) {
+          x.head = 0;
+          do {
+            if (++x.b >= a.s.batch) return false;
+            x.sg = Segments(a, x.b, ROWS);
+          } while (x.sg.blocks == 0);
         }
-        if (c < sg.chunks_c) {
-          const int pos = c * kChunk, pg = __shfl_sync(~0u, pages, k & 31);
-          const bool mapped = pg >= 0 && pg < a.c.num_pages;
-          valid = mapped ? min(kChunk, sg.len - pos) : 0;
-          row_bytes = a.c.token_bytes;
-          src = (u & 1 ? a.c.v : a.c.k) + (mapped ? pg : 0) * a.c.page_bytes + head * a.c.head_bytes +
-                (long long)(pos & ((1 << a.c.page_shift) - 1)) * a.c.token_bytes;
-        } else {
-          const int j = (c - sg.chunks_c) * kChunk;
-          valid = min(kChunk, sg.count - j);
-          row_bytes = a.kv_stride * (long long)sizeof(T);
-          src = (const char *)((const T *)(u & 1 ? a.dv : a.dk) + (sg.first + j) * a.kv_stride + (long long)head * D);
-        }
-        if (u & 1)
-          L::template load<true>(to, src, row_bytes, valid, lane);
-        else
-          L::template load<false>(to, src, row_bytes, valid, lane);
-        if (lane == 0) my_there[slot] = valid;
       }
-      copy_commit();
-    };
-#pragma unroll
-    for (int u = 0; u < NU - 1; u++) issue(u);
+      x.t0 = 0;
+      x.t1 = tiles_below(hi, at, x.sg.tiles);
+      x.chunks_of(warp, kTileChunks);
+      if (x.t1 > 0) return true;
+    }
+  };
+  if (CS == 0 && cur.t0 >= cur.t1) {
+    if (!next(cur)) return;
+  }
 
-    // the query rows and the drafts that each sees
+  const uint32_t my_ring = smem_addr(ring) + warp * L::kBytes, q_at = smem_addr(q_sm);
+  int *my_there = there + warp * NU;
+  int pages = -1;  // lane i: the page of the chunk 32 j + i
+  auto issue = [&](const Piece &x, int u) {
+    if (u < 2 * x.nk) {
+      const int k = u >> 1, c = x.c0 + k * x.step, slot = u % NU;
+      const uint32_t to = my_ring + slot * S::kSlot;
+      const char *src;
+      long long row_bytes;
+      int valid;
+      if (!(u & 1) && (k & 31) == 0) {
+        const int mine = c + lane * x.step;
+        const int pg = mine < x.sg.chunks_c ? (mine * kChunk) >> a.c.page_shift : -1;
+        pages = pg >= 0 ? a.c.table[x.b * a.c.table_stride + pg] : -1;
+      }
+      if (c < x.sg.chunks_c) {
+        const int pos = c * kChunk, pg = __shfl_sync(~0u, pages, k & 31);
+        const bool mapped = pg >= 0 && pg < a.c.num_pages;
+        valid = mapped ? min(kChunk, x.sg.len - pos) : 0;
+        row_bytes = a.c.token_bytes;
+        src = (u & 1 ? a.c.v : a.c.k) + (mapped ? pg : 0) * a.c.page_bytes + x.head * a.c.head_bytes +
+              (long long)(pos & ((1 << a.c.page_shift) - 1)) * a.c.token_bytes;
+      } else {
+        const int j = (c - x.sg.chunks_c) * kChunk;
+        valid = min(kChunk, x.sg.count - j);
+        row_bytes = a.kv_stride * (long long)sizeof(T);
+        src = (const char *)((const T *)(u & 1 ? a.dv : a.dk) + (x.sg.first + j) * a.kv_stride + (long long)x.head * D);
+      }
+      if (u & 1)
+        L::template load<true>(to, src, row_bytes, valid, lane);
+      else
+        L::template load<false>(to, src, row_bytes, valid, lane);
+      if (lane == 0) my_there[slot] = valid;
+    }
+    copy_commit();
+  };
+  // the query rows of a piece and the drafts that each sees
+  auto load_query = [&](const Piece &x) {
+    const int rows = min(ROWS, x.sg.count * a.group - x.rb * ROWS);
     for (int m = 0; m < MT; m++)
       L::query(q_at + m * L::kQBytes, tid, kTreeThreads, [&](int r) -> const T * {
-        const int row = m * 16 + r, x = rb * ROWS + row;
-        return row < rows ? (const T *)a.q + (sg.first + x / a.group) * a.q_stride +
-                                (long long)(head * a.group + x % a.group) * D
+        const int row = m * 16 + r, i = x.rb * ROWS + row;
+        return row < rows ? (const T *)a.q + (x.sg.first + i / a.group) * a.q_stride +
+                                (long long)(x.head * a.group + i % a.group) * D
                           : nullptr;
       });
     for (int r = tid; r < ROWS; r += kTreeThreads)
-      seen[r] = r < rows ? (unsigned long long)a.mask[sg.first + (rb * ROWS + r) / a.group] : 0ull;
-    __syncthreads();
+      seen[r] = r < rows ? (unsigned long long)a.mask[x.sg.first + (x.rb * ROWS + r) / a.group] : 0ull;
+  };
+
+#pragma unroll
+  for (int u = 0; u < S::kEarly; u++) issue(cur, u);
+  load_query(cur);
+  __syncthreads();
+
+  for (int piece = 0; more; piece++) {
+#pragma unroll
+    for (int u = S::kEarly; u < NU - 1; u++) issue(cur, u);
 
     float o[MT][D / 8][4] = {}, mx[MT][2], sum[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; m++) mx[m][0] = mx[m][1] = -INFINITY, sum[m][0] = sum[m][1] = 0.f;
 
-    for (int k = 0; k < nk; k++) {
-      const int c = c0 + k * kTileChunks, u = 2 * k;
+    for (int k = 0; k < cur.nk; k++) {
+      const int c = cur.c0 + k * cur.step, u = 2 * k;
       copy_wait<NU - 2>();
       __syncwarp();
-      issue(u + NU - 1);
+      issue(cur, u + NU - 1);
       float s[MT][2][4];
-      L::template scores<MT>(s, q_at, my_ring + (u % NU) * L::kBytes, lane);
+      L::template scores<MT>(s, q_at, my_ring + (u % NU) * S::kSlot, lane);
       const int valid = my_there[u % NU];
-      const bool draft = c >= sg.chunks_c;
-      const int j0 = (c - sg.chunks_c) * kChunk;
+      const bool draft = c >= cur.sg.chunks_c;
+      const int j0 = (c - cur.sg.chunks_c) * kChunk;
       float alpha[MT][2];
       bool rescale = false;
 #pragma unroll
@@ -307,8 +379,8 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) 
       rescale = __any_sync(~0u, rescale);
       copy_wait<NU - 2>();
       __syncwarp();
-      issue(u + NU);
-      const uint32_t v = my_ring + ((u + 1) % NU) * L::kBytes;
+      issue(cur, u + NU);
+      const uint32_t v = my_ring + ((u + 1) % NU) * S::kSlot;
       bool bad = false;
       if (draft) {
         bad = any_nonfinite<T, D>(v, lane);
@@ -317,7 +389,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) 
       L::template values<MT>(o, s, alpha, rescale, v, lane);
       if (bad) {
         for (int j = 0; j < valid; j++) {
-          const T *row = (const T *)a.dv + (sg.first + j0 + j) * a.kv_stride + (long long)head * D;
+          const T *row = (const T *)a.dv + (cur.sg.first + j0 + j) * a.kv_stride + (long long)cur.head * D;
 #pragma unroll
           for (int m = 0; m < MT; m++) {
             const int from = (lane & ~3) | ((j & 7) >> 1);
@@ -342,65 +414,101 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) 
         }
       }
     }
-    copy_wait<0>();
-    __syncthreads();  // every warp is done with the ring: it takes the parts
-
-    float *join = (float *)ring;
+    // the next piece's first chunks are on their way while this one is joined
+    const Piece done = cur;
+    if constexpr (CS == 0) {
+      more = next(cur);
+      if (more) {
+#pragma unroll
+        for (int u = 0; u < S::kEarly; u++) issue(cur, u);
+      }
+    } else {
+      more = false;
+    }
+    const int rows = min(ROWS, done.sg.count * a.group - done.rb * ROWS);
+    const bool whole = CS == 0 ? done.t0 == 0 && done.t1 == done.sg.tiles : CS == 1;
+    const long long slot = 2 * (long long)blockIdx.x + (piece ? 1 : 0);
+    float *join = (float *)(ring + S::kEarly * S::kSlot);
+    float *part = CS > 1 ? (float *)ring : a.part + slot * ROWS * D;
+    float *to_ml = CS > 1 ? part_ml : a.part_ml + slot * ROWS * 2;
+    // 16 bytes d of row r: exchanged so that a warp's stores hit different banks
+    auto piece_of = [](int r, int d) { return L::f32 ? d ^ (r & 1) : d ^ ((r & 3) << 1); };
 #pragma unroll
     for (int m = 0; m < MT; m++) {
+      __syncthreads();  // every warp is done with what the join lies over
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         float l = sum[m][h];
         l += __shfl_xor_sync(~0u, l, 1);
         l += __shfl_xor_sync(~0u, l, 2);
-        const int row = m * 16 + 8 * h + g;
-        if (t == 0) ml[(warp * ROWS + row) * 2] = mx[m][h], ml[(warp * ROWS + row) * 2 + 1] = l;
-        float *to = join + (warp * ROWS + row) * S::kPitch;
+        const int r = 8 * h + g;
+        if (t == 0) ml[(warp * ROWS + m * 16 + r) * 2] = mx[m][h], ml[(warp * ROWS + m * 16 + r) * 2 + 1] = l;
+        float4 *to = (float4 *)join + (warp * 16 + r) * (D / 4);
+        auto &x = o[m];
         if constexpr (L::f32) {
 #pragma unroll
           for (int blk = 0; blk < D / 32; blk++) {
-            auto &x = o[m];
-            *(float4 *)(to + blk * 32 + 8 * t) = make_float4(x[blk * 4][2 * h], x[blk * 4 + 1][2 * h], x[blk * 4 + 2][2 * h], x[blk * 4 + 3][2 * h]);
-            *(float4 *)(to + blk * 32 + 8 * t + 4) = make_float4(x[blk * 4][2 * h + 1], x[blk * 4 + 1][2 * h + 1], x[blk * 4 + 2][2 * h + 1], x[blk * 4 + 3][2 * h + 1]);
+            to[piece_of(r, blk * 8 + 2 * t)] = make_float4(x[blk * 4][2 * h], x[blk * 4 + 1][2 * h], x[blk * 4 + 2][2 * h], x[blk * 4 + 3][2 * h]);
+            to[piece_of(r, blk * 8 + 2 * t + 1)] = make_float4(x[blk * 4][2 * h + 1], x[blk * 4 + 1][2 * h + 1], x[blk * 4 + 2][2 * h + 1], x[blk * 4 + 3][2 * h + 1]);
           }
         } else {
 #pragma unroll
-          for (int nt = 0; nt < D / 8; nt++) *(float2 *)(to + nt * 8 + 2 * t) = make_float2(o[m][nt][2 * h], o[m][nt][2 * h + 1]);
+          for (int nt = 0; nt < D / 8; nt++)
+            ((float2 *)(to + piece_of(r, nt * 2 + (t >> 1))))[t & 1] = make_float2(x[nt][2 * h], x[nt][2 * h + 1]);
+        }
+      }
+      if (m == MT - 1 && more) load_query(cur);
+      __syncthreads();
+      for (int i = tid; i < min(16, rows - m * 16) * (D / 4); i += kTreeThreads) {
+        const int r = i / (D / 4), d = i % (D / 4), row = m * 16 + r;
+        float top = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kTreeWarps; w++) top = fmaxf(top, ml[(w * ROWS + row) * 2]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kTreeWarps; w++) {
+          const float f = exp2_(ml[(w * ROWS + row) * 2] - ref);
+          l = fmaf(f, ml[(w * ROWS + row) * 2 + 1], l);
+          const float4 y = ((const float4 *)join)[(w * 16 + r) * (D / 4) + piece_of(r, d)];
+          x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+        }
+        if (whole) {
+          write_row<T, D>(a, done.sg, done.head, done.rb * ROWS + row, d * 4, x, top, l);
+        } else {
+          *(float4 *)(part + row * D + d * 4) = x;
+          if (d == 0) *(float2 *)(to_ml + row * 2) = make_float2(top, l);
         }
       }
     }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == sg.tiles;
-    const long long slot = 2 * (long long)blockIdx.x + (piece ? 1 : 0);
-    for (int i = tid; i < rows * (D / 4); i += kTreeThreads) {
-      const int row = i / (D / 4), d = i % (D / 4) * 4;
-      float top = -INFINITY, l = 0.f;
+    if constexpr (CS > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      for (int i = (int)cluster.block_rank() * kTreeThreads + tid; i < rows * (D / 4); i += CS * kTreeThreads) {
+        const int row = i / (D / 4), d = i % (D / 4);
+        float2 w[CS];
+        float4 y[CS];
 #pragma unroll
-      for (int w = 0; w < kTreeWarps; w++) top = fmaxf(top, ml[(w * ROWS + row) * 2]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < CS; r++) {
+          w[r] = *(const float2 *)(cluster.map_shared_rank(part_ml, r) + row * 2);
+          y[r] = *(const float4 *)(cluster.map_shared_rank(part, r) + row * D + d * 4);
+        }
+        float top = -INFINITY, l = 0.f;
 #pragma unroll
-      for (int w = 0; w < kTreeWarps; w++) {
-        const float f = exp2_(ml[(w * ROWS + row) * 2] - ref);
-        l = fmaf(f, ml[(w * ROWS + row) * 2 + 1], l);
-        const float4 y = *(const float4 *)(join + (w * ROWS + row) * S::kPitch + d);
-        x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+        for (int r = 0; r < CS; r++) top = fmaxf(top, w[r].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < CS; r++) {
+          const float f = exp2_(w[r].x - ref);
+          l = fmaf(f, w[r].y, l);
+          x.x = fmaf(f, y[r].x, x.x), x.y = fmaf(f, y[r].y, x.y), x.z = fmaf(f, y[r].z, x.z), x.w = fmaf(f, y[r].w, x.w);
+        }
+        write_row<T, D>(a, cur.sg, cur.head, cur.rb * ROWS + row, d * 4, x, top, l);
       }
-      if (whole) {
-        const int r = rb * ROWS + row, tok = sg.first + r / a.group, hd = head * a.group + r % a.group;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        store4((T *)a.out + tok * a.out_stride + (long long)hd * D + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-        if (d == 0 && a.lse) a.lse[(long long)tok * a.kv_heads * a.group + hd] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
-      } else {
-        *(float4 *)(a.part + (slot * ROWS + row) * D + d) = x;
-        if (d == 0) *(float2 *)(a.part_ml + (slot * ROWS + row) * 2) = make_float2(top, l);
-      }
+      cluster.sync();  // no block ends while another reads its part
     }
-    left -= t1 - t0;
-    t0 = 0;
-    if (++rb == sg.blocks) rb = 0, head++;
-    if (head == a.kv_heads) head = 0, b++;
-    __syncthreads();  // the ring and the query rows are free again
+    __syncthreads();  // the join is read, the query rows are there
   }
 }
 
@@ -416,20 +524,23 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeArgs a, int rows
   const int r = rb * rows_a_block + row;
   if (warp == 0) {
     long long below, all;
-    count_tiles(a, rows_a_block, b, lane, &below, &all);
+    count_cost(a, rows_a_block, b, lane, &below, &all);
     if (lane == 0) plan[0] = below, plan[1] = all;
   }
   pdl_wait();  // on every path: this grid's end is to mean the main one's too
   if (r >= sg.count * a.group) return;
   __syncthreads();
-  const long long all = plan[1], s0 = plan[0] + (long long)(head * sg.blocks + rb) * sg.tiles, s1 = s0 + sg.tiles;
+  const long long all = plan[1], at = plan[0] + (long long)(head * sg.blocks + rb) * sg.cost();
+  const long long tile0 = at + kSegmentCost, tile1 = tile0 + (long long)(sg.tiles - 1) * kTileCost;  // where they start
   const int grid = (int)min((long long)main_grid, all);
-  const int first = (int)(((s0 + 1) * grid - 1) / all), last = (int)((s1 * grid - 1) / all);
+  const int first = (int)(((tile0 + 1) * grid - 1) / all), last = (int)(((tile1 + 1) * grid - 1) / all);
   if (first == last) return;  // written already
   constexpr int V = D / 32;
   float top = -INFINITY, l = 0.f, x[V] = {};
   for (int c = first + warp; c <= last; c += 4) {
-    const long long slot = 2ll * c + (run_start(all, c, grid) >= s0 ? 0 : 1);
+    const long long lo = run_start(all, c, grid);
+    if (tiles_below(lo, at, sg.tiles) == tiles_below(run_start(all, c + 1, grid), at, sg.tiles)) continue;
+    const long long slot = 2ll * c + (lo <= at - kTileCost ? 1 : 0);  // the run's first piece or, behind another segment's, its last
     const float2 p = *(const float2 *)(a.part_ml + (slot * rows_a_block + row) * 2);
     const float now = fmaxf(top, p.x), ref = now == -INFINITY ? 0.f : now;
     const float f0 = exp2_(top - ref), f1 = exp2_(p.x - ref);
@@ -454,10 +565,7 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeArgs a, int rows
       const float4 z = *(const float4 *)&o_sm[w][tid * 4];
       y.x = fmaf(f, z.x, y.x), y.y = fmaf(f, z.y, y.y), y.z = fmaf(f, z.z, y.z), y.w = fmaf(f, z.w, y.w);
     }
-    const int tok = sg.first + r / a.group, hd = head * a.group + r % a.group;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    store4((T *)a.out + tok * a.out_stride + (long long)hd * D + tid * 4, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
-    if (tid == 0 && a.lse) a.lse[(long long)tok * a.kv_heads * a.group + hd] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    write_row<T, D>(a, sg, head, r, tid * 4, y, m, sum);
   }
 }
 
