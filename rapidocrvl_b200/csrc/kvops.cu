@@ -166,12 +166,13 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   }
   if (tiles <= 8 * kFew && segments * 8 <= room) return one(k_tree_attn<T, D, MT, 8>, 8);
 
-  const int grid = sms * S::kBlocks;
+  const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
   a.part = (float *)work;
   a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
   if (int rc = launch("tree attention", k_tree_attn<T, D, MT, 0>, dim3(grid), kTreeThreads, S::kSmem, stream, false, 1, a, blocks)) return rc;
   if ((long long)blocks * a.kv_heads > 65535) return invalid("too many kv heads");
-  return launch("tree attention (join)", k_tree_combine<T, D>, dim3(rows_max < S::kRows ? rows_max : S::kRows, blocks * a.kv_heads, a.s.batch), 128, 0,
+  return launch("tree attention (join)", k_tree_combine<T, D>, dim3(rows_max < S::kRows ? rows_max : S::kRows, blocks * a.kv_heads, a.s.batch),
+                kCombineWarps * 32, 0,
                 stream, true, 1, a, S::kRows, grid);
 }
 

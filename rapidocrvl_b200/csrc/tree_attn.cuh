@@ -512,11 +512,17 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) 
   }
 }
 
-// Joins the parts of the segments that several blocks share: one block a
-// (row, segment), its four warps over the parts.
+// Joins the parts of the segments that several runs share: one block a
+// (row, segment).  All parts' maxima are read first, so the sums over the
+// parts are independent loads; eight warps take turns at the parts.
+constexpr int kCombineWarps = 8;
+constexpr int kMaxRuns = 512;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) k_tree_combine(const TreeArgs a, int rows_a_block, int main_grid) {
-  __shared__ float o_sm[4][D], ml_sm[4][2];
+__global__ void __launch_bounds__(kCombineWarps * 32) k_tree_combine(const TreeArgs a, int rows_a_block, int main_grid) {
+  __shared__ __align__(16) float o_sm[kCombineWarps][D];
+  __shared__ float f_sm[kMaxRuns], red[2][kCombineWarps];
+  __shared__ int slot_sm[kMaxRuns];  // of run first + i, or -1
   __shared__ long long plan[2];
   const int b = blockIdx.z, head = blockIdx.y % a.kv_heads, rb = blockIdx.y / a.kv_heads, row = blockIdx.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -535,37 +541,71 @@ __global__ void __launch_bounds__(128) k_tree_combine(const TreeArgs a, int rows
   const int grid = (int)min((long long)main_grid, all);
   const int first = (int)(((tile0 + 1) * grid - 1) / all), last = (int)(((tile1 + 1) * grid - 1) / all);
   if (first == last) return;  // written already
-  constexpr int V = D / 32;
-  float top = -INFINITY, l = 0.f, x[V] = {};
-  for (int c = first + warp; c <= last; c += 4) {
-    const long long lo = run_start(all, c, grid);
-    if (tiles_below(lo, at, sg.tiles) == tiles_below(run_start(all, c + 1, grid), at, sg.tiles)) continue;
-    const long long slot = 2ll * c + (lo <= at - kTileCost ? 1 : 0);  // the run's first piece or, behind another segment's, its last
-    const float2 p = *(const float2 *)(a.part_ml + (slot * rows_a_block + row) * 2);
-    const float now = fmaxf(top, p.x), ref = now == -INFINITY ? 0.f : now;
-    const float f0 = exp2_(top - ref), f1 = exp2_(p.x - ref);
-    top = now;
-    l = fmaf(l, f0, f1 * p.y);
-    const float *from = a.part + (slot * rows_a_block + row) * D + lane * V;
+  const int n = last - first + 1;
+  float top = -INFINITY, l = 0.f;
+  float2 p[kMaxRuns / (kCombineWarps * 32)];
 #pragma unroll
-    for (int i = 0; i < V; i++) x[i] = fmaf(x[i], f0, f1 * from[i]);
+  for (int j = 0; j < kMaxRuns / (kCombineWarps * 32); j++) {
+    const int i = j * kCombineWarps * 32 + tid, c = first + i;
+    p[j] = make_float2(-INFINITY, 0.f);
+    if (i < n) {
+      const long long lo = run_start(all, c, grid);
+      int slot = -1;
+      if (tiles_below(lo, at, sg.tiles) < tiles_below(run_start(all, c + 1, grid), at, sg.tiles))
+        slot = 2 * c + (lo <= at - kTileCost ? 1 : 0);  // the run's first piece or, behind another segment's, its last
+      if (slot >= 0) p[j] = *(const float2 *)(a.part_ml + ((long long)slot * rows_a_block + row) * 2);
+      slot_sm[i] = slot;
+      top = fmaxf(top, p[j].x);
+    }
+  }
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+  if (lane == 0) red[0][warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; w++) top = fmaxf(top, red[0][w]);
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int j = 0; j < kMaxRuns / (kCombineWarps * 32); j++) {
+    const int i = j * kCombineWarps * 32 + tid;
+    if (i < n) {
+      const float f = exp2_(p[j].x - ref);
+      f_sm[i] = f;
+      l = fmaf(f, p[j].y, l);
+    }
+  }
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; w++) l += red[1][w];
+  constexpr int V = D / 32;
+  float x[V] = {};
+#pragma unroll 4
+  for (int i = warp; i < n; i += kCombineWarps) {
+    const int slot = slot_sm[i];
+    if (slot < 0) continue;
+    const float f = f_sm[i];
+    const float *from = a.part + ((long long)slot * rows_a_block + row) * D + lane * V;
+    float y[V];
+    if constexpr (V == 4)
+      *(float4 *)y = *(const float4 *)from;
+    else
+      *(float2 *)y = *(const float2 *)from;
+#pragma unroll
+    for (int j = 0; j < V; j++) x[j] = fmaf(f, y[j], x[j]);
   }
 #pragma unroll
-  for (int i = 0; i < V; i++) o_sm[warp][lane * V + i] = x[i];
-  if (lane == 0) ml_sm[warp][0] = top, ml_sm[warp][1] = l;
+  for (int j = 0; j < V; j++) o_sm[warp][lane * V + j] = x[j];
   __syncthreads();
   if (tid < D / 4) {
-    float m = -INFINITY, sum = 0.f;
-    for (int w = 0; w < 4; w++) m = fmaxf(m, ml_sm[w][0]);
-    const float ref = m == -INFINITY ? 0.f : m;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < 4; w++) {
-      const float f = exp2_(ml_sm[w][0] - ref);
-      sum = fmaf(f, ml_sm[w][1], sum);
+#pragma unroll
+    for (int w = 0; w < kCombineWarps; w++) {
       const float4 z = *(const float4 *)&o_sm[w][tid * 4];
-      y.x = fmaf(f, z.x, y.x), y.y = fmaf(f, z.y, y.y), y.z = fmaf(f, z.z, y.z), y.w = fmaf(f, z.w, y.w);
+      y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
     }
-    write_row<T, D>(a, sg, head, r, tid * 4, y, m, sum);
+    write_row<T, D>(a, sg, head, r, tid * 4, y, top, l);
   }
 }
 
