@@ -6,8 +6,9 @@
 // a fixed order: no atomics, the same sums every time.
 //
 // A block takes a run of tiles of 128 positions (16 a warp) of one
-// (sequence, kv head) after another; query fragments of up to kRowTiles x 16
-// rows lie in shared memory, more rows take further passes over the run's K.
+// (sequence, kv head) after another; query fragments of up to kRowTiles x 8
+// rows lie in shared memory (of 8 rows, in registers), more rows take further
+// passes over the run's K.
 #pragma once
 #include "paged.cuh"
 
@@ -40,30 +41,30 @@ struct MassShare {
     count = a.s.tokens(b, &first);
     len = min(a.s.len(b), a.out_width);
     tiles = (len + kMassWarps * kChunk - 1) / (kMassWarps * kChunk);
-    cost = 1 + (count * a.group + 15) / 16;
+    cost = 1 + (count * a.group + 7) / 8;
   }
   __device__ long long total(int kv_heads) const { return (long long)kv_heads * tiles * cost; }
 };
 
-template <typename T, int D>
+template <typename T, int D, bool THIN>
 struct MassShape {
   using L = Tile<T, D>;
   static constexpr int kUnits = L::kBytes >= 8192 ? 3 : L::kBytes >= 4096 ? 4 : 6;
   static constexpr int kRing = kMassWarps * kUnits * L::kBytes;
-  static constexpr int kRowTiles = L::f32 ? (D == 128 ? 2 : 8) : 16;
-  static constexpr int kSmem = kRing + kRowTiles * L::kQBytes + kRowTiles * 16 * 4 + 64;
+  static constexpr int kRowTiles = THIN ? 1 : L::f32 ? (D == 128 ? 4 : 16) : 32;
+  static constexpr int kSmem = kRing + kRowTiles * L::kQBytes + kRowTiles * 8 * 4 + 64;
 };
 
-template <typename T, int D>
+template <typename T, int D, bool THIN>
 __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
-  using S = MassShape<T, D>;
+  using S = MassShape<T, D, THIN>;
   using L = Tile<T, D>;
   constexpr int NU = S::kUnits;
   extern __shared__ __align__(128) char sm[];
   char *ring = sm, *q_sm = sm + S::kRing;
   float *shift = (float *)(q_sm + S::kRowTiles * L::kQBytes);  // lse log2(e), +inf for rows that do not count
-  long long *plan = (long long *)(shift + S::kRowTiles * 16);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2;
+  long long *plan = (long long *)(shift + S::kRowTiles * 8);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane & 3;
 
   // where this block's share of the cost starts: a sequence, the cost below it
   if (warp == 0) {
@@ -106,7 +107,7 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
       const int c0 = t0 * kMassWarps + warp, chunks = (sh.len + kChunk - 1) / kChunk;
       const int c_end = min(t1 * kMassWarps, chunks);
       const int nk = c0 < c_end ? (c_end - c0 + kMassWarps - 1) / kMassWarps : 0;
-      const int rows = sh.count * a.group, row_tiles = (rows + 15) / 16;
+      const int rows = sh.count * a.group, row_tiles = (rows + 7) / 8;
       const float *acc = a.acc ? a.acc + ((long long)b * a.kv_heads + head) * a.acc_stride : nullptr;
       float *out = a.out + ((long long)b * a.kv_heads + head) * a.out_stride;
 
@@ -139,13 +140,13 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
         auto counts = [&](int r) { return r < rows && (on >> (r / a.group) & 1); };
         for (int m = 0; m < mt; m++)
           L::query(q_at + m * L::kQBytes, tid, kMassThreads, [&](int r) -> const T * {
-            const int x = (m0 + m) * 16 + r;
+            const int x = (m0 + m) * 8 + r;
             return counts(x) ? (const T *)a.q + (sh.first + x / a.group) * a.q_stride +
                                    (long long)(head * a.group + x % a.group) * D
                              : nullptr;
           });
-        for (int r = tid; r < mt * 16; r += kMassThreads) {
-          const int x = m0 * 16 + r;
+        for (int r = tid; r < mt * 8; r += kMassThreads) {
+          const int x = m0 * 8 + r;
           float l = INFINITY;
           if (counts(x)) {
             l = a.lse[(long long)(sh.first + x / a.group) * a.kv_heads * a.group + head * a.group + x % a.group] * kLog2e;
@@ -154,6 +155,15 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
           shift[r] = l;
         }
         __syncthreads();
+        uint32_t qr[THIN ? L::kTiles : 1][L::kQRegs];
+        float l0 = INFINITY, l1 = INFINITY;
+        if constexpr (THIN) {
+          if (mt > 0) {
+#pragma unroll
+            for (int blk = 0; blk < L::kTiles; blk++) L::q_load(qr[blk], q_at, blk, lane);
+            l0 = shift[2 * t], l1 = shift[2 * t + 1];
+          }
+        }
         for (int k = 0; k < nk; k++) {
           copy_wait<NU - 2>();
           __syncwarp();
@@ -169,32 +179,50 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
             else if (acc && pos < a.acc_width)
               old = a.decay * acc[pos];
           }
-          float w[2][2] = {};  // positions 8 n + 2 t + e
-          typename L::KFrag f;
+          const uint32_t k_at = my_ring + k % NU * L::kBytes;
+          float w[2] = {0.f, 0.f};  // positions g and g + 8
+          auto add = [&](const float(&s)[4], const float(&c)[2][4]) {
+            float y[4];
 #pragma unroll
-          for (int blk = 0; blk < D / 16; blk++) L::k_load(f, blk, my_ring + k % NU * L::kBytes, lane);
-          for (int m = 0; m < mt; m++) {
-            float s[2][4] = {}, c[2][4] = {};
+            for (int e = 0; e < 4; e++) y[e] = L::f32 ? s[e] + (c[0][e] + c[1][e]) : s[e];
+            w[0] += exp2_(fmaf(y[0], a.scale, -l0)) + exp2_(fmaf(y[1], a.scale, -l1));
+            w[1] += exp2_(fmaf(y[2], a.scale, -l0)) + exp2_(fmaf(y[3], a.scale, -l1));
+          };
+          if constexpr (THIN) {
+            if (mt > 0) {
+              float s[4] = {}, c[2][4] = {};
 #pragma unroll
-            for (int blk = 0; blk < D / 16; blk++) L::k_product(s, c, q_at + m * L::kQBytes, f, blk, lane);
-            const float l0 = shift[m * 16 + g], l1 = shift[m * 16 + 8 + g];
+              for (int blk = 0; blk < L::kTiles; blk++) {
+                typename L::KFrag f;
+                L::k_load(f, blk, k_at, lane);
+                L::k_product(s, c, qr[blk], f);
+              }
+              add(s, c);
+            }
+          } else {
+            typename L::KFrag f[L::kTiles];
 #pragma unroll
-            for (int n = 0; n < 2; n++)
+            for (int blk = 0; blk < L::kTiles; blk++) L::k_load(f[blk], blk, k_at, lane);
+            for (int m = 0; m < mt; m++) {
+              float s[4] = {}, c[2][4] = {};
 #pragma unroll
-              for (int e = 0; e < 2; e++)
-                w[n][e] += exp2_(fmaf(s[n][e] + c[n][e], a.scale, -l0)) + exp2_(fmaf(s[n][2 + e] + c[n][2 + e], a.scale, -l1));
+              for (int blk = 0; blk < L::kTiles; blk++) {
+                uint32_t x[L::kQRegs];
+                L::q_load(x, q_at + m * L::kQBytes, blk, lane);
+                L::k_product(s, c, x, f[blk]);
+              }
+              l0 = shift[m * 8 + 2 * t], l1 = shift[m * 8 + 2 * t + 1];
+              add(s, c);
+            }
           }
 #pragma unroll
           for (int n = 0; n < 2; n++)
 #pragma unroll
-            for (int e = 0; e < 2; e++)
-#pragma unroll
-              for (int d = 4; d < 32; d <<= 1) w[n][e] += __shfl_xor_sync(~0u, w[n][e], d);
+            for (int d = 1; d < 4; d <<= 1) w[n] += __shfl_xor_sync(~0u, w[n], d);
           // lane j takes position j's sum from the lane that holds it
-          const int j = lane & 15, src = (j & 7) >> 1;
-          const float w00 = __shfl_sync(~0u, w[0][0], src), w01 = __shfl_sync(~0u, w[0][1], src);
-          const float w10 = __shfl_sync(~0u, w[1][0], src), w11 = __shfl_sync(~0u, w[1][1], src);
-          float mine = j & 8 ? (j & 1 ? w11 : w10) : (j & 1 ? w01 : w00);
+          const int j = lane & 15;
+          const float w0 = __shfl_sync(~0u, w[0], (j & 7) * 4), w1 = __shfl_sync(~0u, w[1], (j & 7) * 4);
+          float mine = j & 8 ? w1 : w0;
           if (j >= valid) mine = 0.f;
           if (lane < kChunk && pos < sh.len) out[pos] = old + mine;
         }

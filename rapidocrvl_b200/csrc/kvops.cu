@@ -140,14 +140,12 @@ int check_tokens(const ocrvl_kv_cache *c, int layer, int heads, int n_tokens, in
 
 // ---- tree attention ----------------------------------------------------------
 
-int rows_a_block(int rows) { return rows <= 16 ? 16 : 32; }
-
 // Parts in the workspace: two a block of the widest grid.
 int64_t tree_work_bytes(int sms, int dim) { return (int64_t)sms * 2 * 2 * 32 * (dim + 2) * 4; }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int NT>
 int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stream) {
-  using S = TreeShape<T, D, MT>;
+  using S = TreeShape<T, D, NT>;
   const int blocks = (rows_max + S::kRows - 1) / S::kRows;
   const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
   if (segments > 1 << 24) return invalid("too many sequences and kv heads");
@@ -159,34 +157,42 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
     return launch("tree attention", kernel, dim3((unsigned)(segments * cs)), kTreeThreads, S::kSmem, stream, false, cs, a, blocks);
   };
   const int room = sms * S::kBlocks;
-  if (tiles <= kFew && (segments >= room || tiles <= 2)) return one(k_tree_attn<T, D, MT, 1>, 1);
+  if (tiles <= kFew && (segments >= room || tiles <= 2)) return one(k_tree_attn<T, D, NT, 1>, 1);
   if (tiles <= 4 * kFew && segments * 4 <= room) {
-    if (tiles > 4 && segments * 8 <= room) return one(k_tree_attn<T, D, MT, 8>, 8);
-    return one(k_tree_attn<T, D, MT, 4>, 4);
+    if (tiles > 4 && segments * 8 <= room) return one(k_tree_attn<T, D, NT, 8>, 8);
+    return one(k_tree_attn<T, D, NT, 4>, 4);
   }
-  if (tiles <= 8 * kFew && segments * 8 <= room) return one(k_tree_attn<T, D, MT, 8>, 8);
+  if (tiles <= 8 * kFew && segments * 8 <= room) return one(k_tree_attn<T, D, NT, 8>, 8);
 
   const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
   a.part = (float *)work;
   a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
-  if (int rc = launch("tree attention", k_tree_attn<T, D, MT, 0>, dim3(grid), kTreeThreads, S::kSmem, stream, false, 1, a, blocks)) return rc;
+  if (int rc = launch("tree attention", k_tree_attn<T, D, NT, 0>, dim3(grid), kTreeThreads, S::kSmem, stream, false, 1, a, blocks)) return rc;
   if ((long long)blocks * a.kv_heads > 65535) return invalid("too many kv heads");
   return launch("tree attention (join)", k_tree_combine<T, D>, dim3(rows_max < S::kRows ? rows_max : S::kRows, blocks * a.kv_heads, a.s.batch),
                 kCombineWarps * 32, 0,
                 stream, true, 1, a, S::kRows, grid);
 }
 
+// Rows a block: 8 where that is all there are, 16, or 32 (the accumulators' limit).
+template <typename T, int D>
+int launch_tree_rows(const TreeArgs &a, int sms, int rows_max, char *work, cudaStream_t stream) {
+  if (rows_max <= 8) return launch_tree<T, D, 1>(a, sms, rows_max, work, stream);
+  if (rows_max <= 16) return launch_tree<T, D, 2>(a, sms, rows_max, work, stream);
+  return launch_tree<T, D, 4>(a, sms, rows_max, work, stream);
+}
+
 template <typename T>
 int launch_tree_dim(const TreeArgs &a, int dim, int sms, int rows_max, char *work, cudaStream_t stream) {
-  const bool thin = rows_a_block(rows_max) == 16;
-  if (dim == 128)
-    return thin ? launch_tree<T, 128, 1>(a, sms, rows_max, work, stream) : launch_tree<T, 128, 2>(a, sms, rows_max, work, stream);
-  return thin ? launch_tree<T, 64, 1>(a, sms, rows_max, work, stream) : launch_tree<T, 64, 2>(a, sms, rows_max, work, stream);
+  return dim == 128 ? launch_tree_rows<T, 128>(a, sms, rows_max, work, stream) : launch_tree_rows<T, 64>(a, sms, rows_max, work, stream);
 }
 
 template <typename T, int D>
 int launch_mass(const MassArgs &a, int sms, cudaStream_t stream) {
-  return launch("attention mass", k_attn_mass<T, D>, dim3(sms), kMassThreads, MassShape<T, D>::kSmem, stream, false, 1, a);
+  // eight rows (one token of up to eight heads, say): their fragments stay in registers
+  if (a.s.max_draft * a.group <= 8)
+    return launch("attention mass", k_attn_mass<T, D, true>, dim3(sms), kMassThreads, MassShape<T, D, true>::kSmem, stream, false, 1, a);
+  return launch("attention mass", k_attn_mass<T, D, false>, dim3(sms), kMassThreads, MassShape<T, D, false>::kSmem, stream, false, 1, a);
 }
 
 template <int CS>

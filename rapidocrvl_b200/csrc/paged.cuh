@@ -119,17 +119,35 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
   return *reinterpret_cast<uint32_t *>(&h);
 }
 
-// What a type's chunk of 16 rows x D looks like in shared memory and how the
-// matrix instructions read it.  Rows are stored whole; the 16-byte pieces of a
-// row are exchanged by a rule on the row so that the fragment loads of a warp
-// hit 32 different banks.
+// 8 x 8 16-bit values, a row g and two columns 2 t, 2 t + 1 a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// The same for 32-bit values: a, b in columns 2 t, 2 t + 1 become those of rows 2 t, 2 t + 1.
+__device__ __forceinline__ void transpose8(float a, float b, float &x, float &y) {
+  const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
+  const uint32_t lo = transpose8(__byte_perm(u, v, 0x5410)), hi = transpose8(__byte_perm(u, v, 0x7632));
+  x = __uint_as_float(__byte_perm(lo, hi, 0x5410));
+  y = __uint_as_float(__byte_perm(lo, hi, 0x7632));
+}
+
+// What a type's chunk of 16 positions x D looks like in shared memory and how
+// the matrix instructions read it.  The positions are the 16 rows of the
+// instruction and the query rows its 8 columns, so 8 rows (one token of eight
+// heads) fill it: s' = K q' and o' = V' p'.  Rows of K and V are stored
+// whole; the 16-byte pieces of a row are exchanged by a rule on the row so that the
+// fragment loads of a warp hit 32 different banks.
 template <typename T, int D>
 struct Tile {
   static constexpr bool f32 = sizeof(T) == 4;
   static constexpr int kRowBytes = D * (int)sizeof(T);
   static constexpr int kBytes = kChunk * kRowBytes;
   static constexpr int kPieces = kRowBytes / 16;
-  static constexpr int kQBytes = f32 ? 16 * D * 8 : 16 * D * 2;  // query fragments of 16 rows
+  static constexpr int kQBytes = f32 ? 8 * D * 8 : 8 * D * 2;  // fragments of 8 query rows
+  static constexpr int kQRegs = f32 ? 8 : 2;                   // of them, a lane's registers for 16 dims
+  static constexpr int kTiles = D / 16;                        // output tiles of 16 dims
 
   static __device__ __forceinline__ int k_piece(int row, int piece) {
     return f32 ? piece ^ ((row & 1) << 2) : piece ^ (row & 7);
@@ -153,205 +171,188 @@ struct Tile {
     }
   }
 
-  // Writes the query fragments of 16 rows; row(r) gives row r's address or
+  // Writes the fragments of 8 query rows; row(r) gives row r's address or
   // NULL (a zero row).  Called by a whole block of `threads`.
-  //   f32: per 16 dims, four float4 a lane: high parts of rows g and g + 8,
-  //   then the low parts, dims 4t .. 4t+3 (the contraction takes the dims in
-  //   the order that lets K be read 16 bytes at a time).
-  //   16 bits: per 16 dims, the four registers of the m16k16 fragment.
+  //   f32: per 16 dims, two float4 a lane, the high and the low parts of row
+  //   g's dims 4t .. 4t+3 (the contraction takes the dims in the order that
+  //   lets K be read 16 bytes at a time).
+  //   16 bits: per 16 dims, two registers a lane: row g's dims 2t, 2t+1 and 2t+8, 2t+9.
   template <typename Row>
   static __device__ __forceinline__ void query(uint32_t dst, int tid, int threads, Row row) {
-    constexpr int kItems = (D / 16) * 32;
+    constexpr int kItems = (f32 ? D / 16 : D / 32) * 32;
     for (int i = tid; i < kItems; i += threads) {
       const int lane = i & 31, blk = i >> 5, g = lane >> 2, t = lane & 3;
-      const T *a = row(g), *b = row(g + 8);
+      const T *a = row(g);
       if constexpr (f32) {
-        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 x = a ? *reinterpret_cast<const float4 *>(a + blk * 16 + t * 4) : z;
-        const float4 y = b ? *reinterpret_cast<const float4 *>(b + blk * 16 + t * 4) : z;
-        uint32_t h[8], l[8];
+        const float4 x = a ? *reinterpret_cast<const float4 *>(a + blk * 16 + t * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        uint32_t h[4], l[4];
         split(x.x, h[0], l[0]), split(x.y, h[1], l[1]), split(x.z, h[2], l[2]), split(x.w, h[3], l[3]);
-        split(y.x, h[4], l[4]), split(y.y, h[5], l[5]), split(y.z, h[6], l[6]), split(y.w, h[7], l[7]);
-        const uint32_t to = dst + blk * 2048 + lane * 16;
-        // the fragment's order: (g, k), (g+8, k), (g, k+4), (g+8, k+4)
-        sts4u(to, h[0], h[4], h[1], h[5]);
-        sts4u(to + 512, h[2], h[6], h[3], h[7]);
-        sts4u(to + 1024, l[0], l[4], l[1], l[5]);
-        sts4u(to + 1536, l[2], l[6], l[3], l[7]);
+        sts4u(dst + blk * 1024 + lane * 16, h[0], h[1], h[2], h[3]);
+        sts4u(dst + blk * 1024 + 512 + lane * 16, l[0], l[1], l[2], l[3]);
       } else {
-        const uint32_t *p = reinterpret_cast<const uint32_t *>(a), *q = reinterpret_cast<const uint32_t *>(b);
-        const int c = blk * 8 + t;  // pairs of dims
-        sts4u(dst + blk * 512 + lane * 16, p ? p[c] : 0u, q ? q[c] : 0u, p ? p[c + 4] : 0u, q ? q[c + 4] : 0u);
+        const uint32_t *p = reinterpret_cast<const uint32_t *>(a) + blk * 16 + t;  // pairs of dims
+        sts4u(dst + blk * 512 + lane * 16, a ? p[0] : 0u, a ? p[4] : 0u, a ? p[8] : 0u, a ? p[12] : 0u);
       }
     }
   }
+  // A lane's registers of the fragments for dims 16 blk .. + 15.
+  static __device__ __forceinline__ void q_load(uint32_t (&r)[kQRegs], uint32_t q, int blk, int lane) {
+    if constexpr (f32) {
+      uint32_t h[4], l[4];
+      lds4u(h, q + blk * 1024 + lane * 16);
+      lds4u(l, q + blk * 1024 + 512 + lane * 16);
+#pragma unroll
+      for (int i = 0; i < 4; i++) r[i] = h[i], r[4 + i] = l[i];
+    } else {
+      asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(q + (blk >> 1) * 512 + lane * 16 + (blk & 1) * 8));
+    }
+  }
 
-  // The chunk's K as matrix operands.
+  // K's fragments for dims 16 blk .. + 15.
+  //   f32: [step of 8 dims][register], hi and lo.
   struct KFrag {
-    uint32_t hi[D / 16][f32 ? 8 : 4], lo[f32 ? D / 16 : 1][f32 ? 8 : 1];
+    uint32_t hi[f32 ? 2 : 1][4], lo[f32 ? 2 : 1][4];
   };
   static __device__ __forceinline__ void k_load(KFrag &f, int blk, uint32_t k, int lane) {
     if constexpr (f32) {
       const int g = lane >> 2, t = lane & 3;
-#pragma unroll
-      for (int n = 0; n < 2; n++) {
-        const int row = n * 8 + g;
-        const float4 x = lds4(k + row * kRowBytes + k_piece(row, blk * 4 + t) * 16);
-        uint32_t *h = f.hi[blk] + n * 4, *l = f.lo[blk] + n * 4;
-        split(x.x, h[0], l[0]), split(x.y, h[1], l[1]), split(x.z, h[2], l[2]), split(x.w, h[3], l[3]);
-      }
+      const float4 x = lds4(k + g * kRowBytes + k_piece(g, blk * 4 + t) * 16);
+      const float4 y = lds4(k + (g + 8) * kRowBytes + k_piece(g + 8, blk * 4 + t) * 16);
+      split(x.x, f.hi[0][0], f.lo[0][0]), split(y.x, f.hi[0][1], f.lo[0][1]);
+      split(x.y, f.hi[0][2], f.lo[0][2]), split(y.y, f.hi[0][3], f.lo[0][3]);
+      split(x.z, f.hi[1][0], f.lo[1][0]), split(y.z, f.hi[1][1], f.lo[1][1]);
+      split(x.w, f.hi[1][2], f.lo[1][2]), split(y.w, f.hi[1][3], f.lo[1][3]);
     } else {
-      const int row = (lane >> 4) * 8 + (lane & 7);
-      ldmatrix4(f.hi[blk], k + row * kRowBytes + k_piece(row, blk * 2 + ((lane >> 3) & 1)) * 16);
+      const int row = lane & 15;
+      ldmatrix4(f.hi[0], k + row * kRowBytes + k_piece(row, blk * 2 + (lane >> 4)) * 16);
     }
   }
 
-  // s[n][.] (with c[n][.] for f32) += 16 rows' dims 16 blk .. + 15 times the
-  // chunk's 16 positions: the accumulator layout of m16n8 (rows g and g + 8,
-  // positions 8 n + 2 t and + 1).  f32 is three tf32 products,
-  // hi hi + hi lo + lo hi, the small ones summed apart in c.
-  static __device__ __forceinline__ void k_product(float (&s)[2][4], float (&c)[2][4], uint32_t q, const KFrag &f, int blk,
-                                                   int lane) {
+  // s (with c for f32) += the chunk's 16 positions' dims 16 blk .. + 15 times
+  // 8 rows': elements 0, 1 are position g and rows 2 t, 2 t + 1; elements 2, 3
+  // position g + 8.  f32 is three tf32 products, hi hi + hi lo + lo hi, the
+  // small ones summed apart in c.
+  static __device__ __forceinline__ void k_product(float (&s)[4], float (&c)[2][4], const uint32_t (&q)[kQRegs], const KFrag &f) {
     if constexpr (f32) {
-      const uint32_t at = q + blk * 2048 + lane * 16;
 #pragma unroll
-      for (int step = 0; step < 2; step++) {
-        uint32_t h[4], l[4];
-        lds4u(h, at + step * 512);
-        lds4u(l, at + 1024 + step * 512);
-        // neighbours use different accumulators: a chain of its own takes 11.5 ns a link
-        const uint32_t *kh = f.hi[blk] + 2 * step, *kl = f.lo[blk] + 2 * step;
-        mma_tf32(c[0], h, kl[0], kl[1]);
-        mma_tf32(c[1], h, kl[4], kl[5]);
-        mma_tf32(s[0], h, kh[0], kh[1]);
-        mma_tf32(s[1], h, kh[4], kh[5]);
-        mma_tf32(c[0], l, kh[0], kh[1]);
-        mma_tf32(c[1], l, kh[4], kh[5]);
+      for (int i = 0; i < 2; i++) {
+        mma_tf32(c[0], f.lo[i], q[2 * i], q[2 * i + 1]);
+        mma_tf32(c[1], f.hi[i], q[4 + 2 * i], q[5 + 2 * i]);
+        mma_tf32(s, f.hi[i], q[2 * i], q[2 * i + 1]);
       }
     } else {
-      uint32_t x[4];
-      lds4u(x, q + blk * 512 + lane * 16);
-      mma_16<T>(s[0], x, f.hi[blk][0], f.hi[blk][1]);
-      mma_16<T>(s[1], x, f.hi[blk][2], f.hi[blk][3]);
+      mma_16<T>(s, f.hi[0], q[0], q[1]);
     }
   }
 
-  // s[mt] = q . k of MT x 16 rows.
-  template <int MT>
-  static __device__ __forceinline__ void scores(float (&s)[MT][2][4], uint32_t q, uint32_t k, int lane) {
-    float c[MT][2][4];
+  // s[n] of NT x 8 rows.  The fragments of the rows come from registers
+  // (qr, NT = 1) or from shared memory.
+  template <int NT, bool REGS>
+  static __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&qr)[REGS ? kTiles : 1][kQRegs], uint32_t q, uint32_t k,
+                                                int lane) {
+    static_assert(!REGS || NT == 1, "");
+    float c[NT][2][4];
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) s[m][i >> 2][i & 3] = c[m][i >> 2][i & 3] = 0.f;
-    KFrag f;
+      for (int e = 0; e < 4; e++) s[n][e] = c[n][0][e] = c[n][1][e] = 0.f;
 #pragma unroll
-    for (int blk = 0; blk < D / 16; blk++) {
+    for (int blk = 0; blk < kTiles; blk++) {
+      KFrag f;
       k_load(f, blk, k, lane);
 #pragma unroll
-      for (int m = 0; m < MT; m++) k_product(s[m], c[m], q + m * kQBytes, f, blk, lane);
+      for (int n = 0; n < NT; n++) {
+        if constexpr (REGS) {
+          k_product(s[n], c[n], qr[blk], f);
+        } else {
+          uint32_t x[kQRegs];
+          q_load(x, q + n * kQBytes, blk, lane);
+          k_product(s[n], c[n], x, f);
+        }
+      }
     }
     if constexpr (f32) {
 #pragma unroll
-      for (int m = 0; m < MT; m++)
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) s[m][i >> 2][i & 3] += c[m][i >> 2][i & 3];
+        for (int e = 0; e < 4; e++) s[n][e] += c[n][0][e] + c[n][1][e];
     }
   }
 
-  // The dim that accumulator element e (0, 1 of row g; 2, 3 of row g + 8) of
-  // output tile nt holds.
-  static __device__ __forceinline__ int out_dim(int nt, int e, int t) {
-    return f32 ? (nt >> 2) * 32 + 8 * t + (e & 1) * 4 + (nt & 3) : nt * 8 + 2 * t + (e & 1);
+  // The dim that element e of output tile i holds (elements 0, 2 are of row
+  // 2 t, elements 1, 3 of row 2 t + 1).
+  static __device__ __forceinline__ int out_dim(int i, int e, int g) {
+    return f32 ? (i >> 1) * 32 + 4 * g + (i & 1) * 2 + (e >> 1) : i * 16 + g + (e >> 1) * 8;
   }
 
-  // o = o * alpha + p v over the chunk's 16 positions; p in the layout of
-  // scores().  alpha[mt][0], [1]: of rows g and g + 8; rescale: whether any
-  // alpha of the warp is not 1.
+  // o += v' p' over the chunk's 16 positions; p in the layout of scores().
   // f32: the chunk's product is summed apart and added in one rounded
-  // multiply-add, since the matrix instruction's own sums are cut, not
-  // rounded, which over thousands of chunks would add up.
-  template <int MT>
-  static __device__ __forceinline__ void values(float (&o)[MT][D / 8][4], const float (&p)[MT][2][4],
-                                                const float (&alpha)[MT][2], bool rescale, uint32_t v, int lane) {
+  // addition, since the matrix instruction's own sums are cut, not rounded,
+  // which over thousands of chunks would add up.
+  template <int NT>
+  static __device__ __forceinline__ void values(float (&o)[kTiles][NT][4], const float (&p)[NT][4], uint32_t v, int lane) {
     const int g = lane >> 2, t = lane & 3;
     if constexpr (f32) {
-      uint32_t ph[MT][2][4], pl[MT][2][4];
+      uint32_t ph[NT][2][2], pl[NT][2][2];  // [positions 8 j ..][2t, 2t+1] of row g
 #pragma unroll
-      for (int m = 0; m < MT; m++)
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-          split(p[m][n][0], ph[m][n][0], pl[m][n][0]);  // (g, position 2t)
-          split(p[m][n][2], ph[m][n][1], pl[m][n][1]);  // (g+8, 2t)
-          split(p[m][n][1], ph[m][n][2], pl[m][n][2]);  // (g, 2t+1)
-          split(p[m][n][3], ph[m][n][3], pl[m][n][3]);  // (g+8, 2t+1)
+        for (int j = 0; j < 2; j++) {
+          float x, y;
+          transpose8(p[n][2 * j], p[n][2 * j + 1], x, y);
+          split(x, ph[n][j][0], pl[n][j][0]), split(y, ph[n][j][1], pl[n][j][1]);
         }
 #pragma unroll
       for (int blk = 0; blk < D / 32; blk++) {
-        uint32_t vh[2][2][4], vl[2][2][4];  // [positions 8n ..][2t, 2t+1][dim 4g + i]
+        uint32_t vh[2][2][4], vl[2][2][4];  // [tile][positions 8 j ..]
 #pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            const int row = n * 8 + 2 * t + j;
-            const float4 x = lds4(v + row * kRowBytes + v_piece(row, blk * 8 + g) * 16);
-            split(x.x, vh[n][j][0], vl[n][j][0]), split(x.y, vh[n][j][1], vl[n][j][1]);
-            split(x.z, vh[n][j][2], vl[n][j][2]), split(x.w, vh[n][j][3], vl[n][j][3]);
-          }
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-          float a[4][4] = {};
-#pragma unroll
-          for (int n = 0; n < 2; n++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) mma_tf32(a[i], ph[m][n], vl[n][0][i], vl[n][1][i]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) mma_tf32(a[i], pl[m][n], vh[n][0][i], vh[n][1][i]);
-          }
-#pragma unroll
-          for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) mma_tf32(a[i], ph[m][n], vh[n][0][i], vh[n][1][i]);
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            float(&to)[4] = o[m][blk * 4 + i];
-            to[0] = fmaf(to[0], alpha[m][0], a[i][0]);
-            to[1] = fmaf(to[1], alpha[m][0], a[i][1]);
-            to[2] = fmaf(to[2], alpha[m][1], a[i][2]);
-            to[3] = fmaf(to[3], alpha[m][1], a[i][3]);
-          }
+        for (int j = 0; j < 2; j++) {
+          const int row = j * 8 + 2 * t;
+          const float4 x = lds4(v + row * kRowBytes + v_piece(row, blk * 8 + g) * 16);
+          const float4 y = lds4(v + (row + 1) * kRowBytes + v_piece(row + 1, blk * 8 + g) * 16);
+          split(x.x, vh[0][j][0], vl[0][j][0]), split(x.y, vh[0][j][1], vl[0][j][1]);
+          split(y.x, vh[0][j][2], vl[0][j][2]), split(y.y, vh[0][j][3], vl[0][j][3]);
+          split(x.z, vh[1][j][0], vl[1][j][0]), split(x.w, vh[1][j][1], vl[1][j][1]);
+          split(y.z, vh[1][j][2], vl[1][j][2]), split(y.w, vh[1][j][3], vl[1][j][3]);
         }
+        float a[NT][2][4] = {};
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) mma_tf32(a[n][i], vl[i][j], ph[n][j][0], ph[n][j][1]);
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) mma_tf32(a[n][i], vh[i][j], pl[n][j][0], pl[n][j][1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) mma_tf32(a[n][i], vh[i][j], ph[n][j][0], ph[n][j][1]);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[2 * blk + i][n][e] += a[n][i][e];
       }
     } else {
-      if (rescale) {
+      uint32_t b[NT][2];
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int nt = 0; nt < D / 8; nt++) {
-            o[m][nt][0] *= alpha[m][0];
-            o[m][nt][1] *= alpha[m][0];
-            o[m][nt][2] *= alpha[m][1];
-            o[m][nt][3] *= alpha[m][1];
-          }
-      }
-      uint32_t a[MT][4];
+        for (int j = 0; j < 2; j++) b[n][j] = transpose8(pack2(p[n][2 * j], p[n][2 * j + 1], T()));
+      const int row = (lane & 7) + (lane >> 4) * 8;
 #pragma unroll
-      for (int m = 0; m < MT; m++) {
-        a[m][0] = pack2(p[m][0][0], p[m][0][1], T());
-        a[m][1] = pack2(p[m][0][2], p[m][0][3], T());
-        a[m][2] = pack2(p[m][1][0], p[m][1][1], T());
-        a[m][3] = pack2(p[m][1][2], p[m][1][3], T());
-      }
-      const int row = lane & 15;
+      for (int i = 0; i < kTiles; i++) {
+        uint32_t a[4];
+        ldmatrix4_t(a, v + row * kRowBytes + v_piece(row, i * 2 + ((lane >> 3) & 1)) * 16);
 #pragma unroll
-      for (int c = 0; c < D / 16; c++) {
-        uint32_t b[4];
-        ldmatrix4_t(b, v + row * kRowBytes + v_piece(row, c * 2 + (lane >> 4)) * 16);
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-          mma_16<T>(o[m][2 * c], a[m], b[0], b[1]);
-          mma_16<T>(o[m][2 * c + 1], a[m], b[2], b[3]);
-        }
+        for (int n = 0; n < NT; n++) mma_16<T>(o[i][n], a, b[n][0], b[n][1]);
       }
     }
   }

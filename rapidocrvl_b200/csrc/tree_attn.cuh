@@ -2,13 +2,16 @@
 // (ocrvl_op_tree_attn).
 //
 // For one kv head the rows are the sequence's drafted tokens times the query
-// heads that share it.  A block takes 16 MT rows against a run of positions; its
+// heads that share it.  A block takes 8 NT rows against a run of positions; its
 // eight warps stream 16-position chunks of K and V of their own through private
-// rings of shared memory (no block barrier on the way), each with the running
-// maximum m, sum l and weighted values o of its own positions:
-//   m' = max(m, max s),  a = 2^(m - m'),  p = 2^(s - m'),
-//   l' = a l + sum p,    o' = a o + p v        (s = scale log2(e) q . k)
-// and are joined at the run's end: o = sum_w 2^(m_w - M) o_w, l likewise.
+// rings of shared memory (no block barrier on the way), each with a reference m,
+// the sum l and the weighted values o of its own positions:
+//   p = 2^(s - m),  l' = l + sum p,  o' = o + p v      (s = scale log2(e) q . k)
+// m follows the running maximum, but only once a score passes it by kSlack:
+//   m' = max(m, max s),  l and o times 2^(m - m')
+// so most chunks need no maximum over lanes and no rescaling, and p stays below
+// 2^kSlack.  At the run's end the warps are joined: o = sum_w 2^(m_w - M) o_w,
+// l likewise.
 //
 // A (sequence, kv head, row block) is a segment.  Two ways to share them out:
 //   CS = 0  tiles of 128 positions over a persistent grid in equal runs,
@@ -34,6 +37,7 @@ constexpr int kTileChunks = kTreeWarps;  // chunks a tile: one a warp
 // Cost of a tile, and of starting a segment (filling the rings, joining the
 // warps takes about as long as a tile), in the split of runs.
 constexpr int kTileCost = 1, kSegmentCost = 1;
+constexpr float kSlack = 8.f;  // p at most 256: far from f16's largest
 
 struct TreeArgs {
   Cache c;
@@ -134,22 +138,24 @@ __device__ __forceinline__ bool any_nonfinite(uint32_t v, int lane) {
   return __any_sync(~0u, bad);
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int NT>
 struct TreeShape {
   using L = Tile<T, D>;
-  static constexpr int kRows = 16 * MT;
-  // 16-bit types at 16 rows: two blocks an SM; else one
-  static constexpr int kBlocks = sizeof(T) == 2 && MT == 1 ? 2 : 1;
+  static constexpr int kRows = 8 * NT;
+  // 16-bit types at up to 16 rows: two blocks an SM; else one
+  static constexpr int kBlocks = sizeof(T) == 2 && NT <= 2 ? 2 : 1;
   // chunks of K or V in a warp's ring: about 192 KB an SM
   static constexpr int kUnits = L::kBytes * kBlocks >= 8192 ? 3 : 6;
   static constexpr int kSlot = kTreeWarps * L::kBytes;  // one unit of every warp
-  // the join of 16 rows of eight warps in f32 lies over the last slots, so the
-  // others can be filled meanwhile
-  static constexpr int kJoinSlots = 4 / (int)sizeof(T);
-  static constexpr int kEarly = kUnits - kJoinSlots;
-  static constexpr int kQ = MT * L::kQBytes;
+  // the join of 8 or 16 rows of eight warps in f32 lies over the last slots, so
+  // the others can be filled meanwhile
+  static constexpr int kJoinRows = NT == 1 ? 8 : 16;
+  static constexpr int kJoinSlots = (kTreeWarps * kJoinRows * D * 4 + kSlot - 1) / kSlot;
+  static constexpr int kEarly = kUnits - kJoinSlots < kUnits - 1 ? kUnits - kJoinSlots : kUnits - 1;
+  static constexpr int kQ = NT * L::kQBytes;
+  static constexpr bool kQInRegs = NT == 1;
   static constexpr int kSmem = kQ + kUnits * kSlot + kTreeWarps * kRows * 8 + kRows * 8 + 64 + kTreeWarps * 8 * 4 + kRows * 8;
-  static_assert(kTreeWarps * 16 * D * 4 == kJoinSlots * kSlot && kEarly >= 1 && kEarly <= kUnits - 1, "");
+  static_assert(kEarly >= 1, "");
 };
 
 // A warp's part in a run of one segment's positions.
@@ -172,9 +178,9 @@ __device__ __forceinline__ void write_row(const TreeArgs &a, const Segments &sg,
   if (d == 0 && a.lse) a.lse[(long long)tok * a.kv_heads * a.group + hd] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
 }
 
-template <typename T, int D, int MT, int CS>
-__global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) k_tree_attn(const TreeArgs a, int row_blocks) {
-  using S = TreeShape<T, D, MT>;
+template <typename T, int D, int NT, int CS>
+__global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) k_tree_attn(const TreeArgs a, int row_blocks) {
+  using S = TreeShape<T, D, NT>;
   using L = Tile<T, D>;
   constexpr int ROWS = S::kRows, NU = S::kUnits;
   namespace cg = cooperative_groups;
@@ -309,9 +315,9 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) 
   // the query rows of a piece and the drafts that each sees
   auto load_query = [&](const Piece &x) {
     const int rows = min(ROWS, x.sg.count * a.group - x.rb * ROWS);
-    for (int m = 0; m < MT; m++)
-      L::query(q_at + m * L::kQBytes, tid, kTreeThreads, [&](int r) -> const T * {
-        const int row = m * 16 + r, i = x.rb * ROWS + row;
+    for (int n = 0; n < NT; n++)
+      L::query(q_at + n * L::kQBytes, tid, kTreeThreads, [&](int r) -> const T * {
+        const int row = n * 8 + r, i = x.rb * ROWS + row;
         return row < rows ? (const T *)a.q + (x.sg.first + i / a.group) * a.q_stride +
                                 (long long)(x.head * a.group + i % a.group) * D
                           : nullptr;
@@ -329,54 +335,68 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) 
 #pragma unroll
     for (int u = S::kEarly; u < NU - 1; u++) issue(cur, u);
 
-    float o[MT][D / 8][4] = {}, mx[MT][2], sum[MT][2];
+    uint32_t qr[S::kQInRegs ? L::kTiles : 1][L::kQRegs];
+    if constexpr (S::kQInRegs) {
 #pragma unroll
-    for (int m = 0; m < MT; m++) mx[m][0] = mx[m][1] = -INFINITY, sum[m][0] = sum[m][1] = 0.f;
+      for (int blk = 0; blk < L::kTiles; blk++) L::q_load(qr[blk], q_at, blk, lane);
+    }
+    float o[L::kTiles][NT][4] = {}, ref[NT][2], sum[NT][2];  // of rows 8 n + 2 t and + 1
+#pragma unroll
+    for (int n = 0; n < NT; n++) ref[n][0] = ref[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.f;
 
     for (int k = 0; k < cur.nk; k++) {
       const int c = cur.c0 + k * cur.step, u = 2 * k;
       copy_wait<NU - 2>();
       __syncwarp();
       issue(cur, u + NU - 1);
-      float s[MT][2][4];
-      L::template scores<MT>(s, q_at, my_ring + (u % NU) * S::kSlot, lane);
+      float s[NT][4];
+      L::template scores<NT, S::kQInRegs>(s, qr, q_at, my_ring + (u % NU) * S::kSlot, lane);
       const int valid = my_there[u % NU];
       const bool draft = c >= cur.sg.chunks_c;
       const int j0 = (c - cur.sg.chunks_c) * kChunk;
-      float alpha[MT][2];
-      bool rescale = false;
+      // scores in units of log2; -inf where there is nothing to see
+      bool above = false;
 #pragma unroll
-      for (int m = 0; m < MT; m++)
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {  // rows g and g + 8
-          float x[4] = {s[m][0][2 * h], s[m][0][2 * h + 1], s[m][1][2 * h], s[m][1][2 * h + 1]};
-          unsigned ok = 0;
+        for (int e = 0; e < 4; e++) s[n][e] *= a.scale;
+      if (draft || valid < kChunk) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) ok |= ((i >> 1) * 8 + 2 * t + (i & 1) < valid ? 1u : 0u) << i;
-          if (draft) {
-            const unsigned w = (unsigned)(seen[m * 16 + 8 * h + g] >> j0);
-            ok &= (w >> (2 * t) & 3u) | (w >> (8 + 2 * t) & 3u) << 2;
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int j = g + (e >> 1) * 8;
+            if (j >= valid || (draft && !(seen[n * 8 + 2 * t + (e & 1)] >> (j0 + j) & 1))) s[n][e] = -INFINITY;
           }
-          float top = -INFINITY;
+      }
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (ok >> i & 1) top = fmaxf(top, x[i] * a.scale);
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-          const float now = fmaxf(mx[m][h], top), ref = now == -INFINITY ? 0.f : now;
-          alpha[m][h] = exp2_(mx[m][h] - ref);
-          rescale |= alpha[m][h] != 1.f;
-          mx[m][h] = now;
-          float add = 0.f;
+      for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            x[i] = ok >> i & 1 ? exp2_(fmaf(x[i], a.scale, -ref)) : 0.f;
-            add += x[i];
+        for (int e = 0; e < 4; e++) above |= s[n][e] > ref[n][e & 1] + kSlack;
+      if (__any_sync(~0u, above)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float top = fmaxf(s[n][h], s[n][2 + h]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            const float now = fmaxf(ref[n][h], top);
+            const float alpha = now == -INFINITY ? 1.f : exp2_(ref[n][h] - now);
+            ref[n][h] = now;
+            sum[n][h] *= alpha;
+#pragma unroll
+            for (int i = 0; i < L::kTiles; i++) o[i][n][h] *= alpha, o[i][n][2 + h] *= alpha;
           }
-          sum[m][h] = fmaf(sum[m][h], alpha[m][h], add);
-          s[m][0][2 * h] = x[0], s[m][0][2 * h + 1] = x[1], s[m][1][2 * h] = x[2], s[m][1][2 * h + 1] = x[3];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float m = ref[n][h] == -INFINITY ? 0.f : ref[n][h];
+          s[n][h] = exp2_(s[n][h] - m), s[n][2 + h] = exp2_(s[n][2 + h] - m);
+          sum[n][h] += s[n][h] + s[n][2 + h];
         }
-      rescale = __any_sync(~0u, rescale);
       copy_wait<NU - 2>();
       __syncwarp();
       issue(cur, u + NU);
@@ -386,31 +406,24 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) 
         bad = any_nonfinite<T, D>(v, lane);
         if (bad) drop_nonfinite<T, D>(v, lane);
       }
-      L::template values<MT>(o, s, alpha, rescale, v, lane);
+      L::template values<NT>(o, s, v, lane);
       if (bad) {
         for (int j = 0; j < valid; j++) {
           const T *row = (const T *)a.dv + (cur.sg.first + j0 + j) * a.kv_stride + (long long)cur.head * D;
 #pragma unroll
-          for (int m = 0; m < MT; m++) {
-            const int from = (lane & ~3) | ((j & 7) >> 1);
-            float w[2];
+          for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-              const float x0 = j & 1 ? s[m][0][2 * h + 1] : s[m][0][2 * h], x1 = j & 1 ? s[m][1][2 * h + 1] : s[m][1][2 * h];
-              w[h] = __shfl_sync(~0u, j >> 3 ? x1 : x0, from);
-            }
-            const bool see0 = seen[m * 16 + g] >> (j0 + j) & 1, see1 = seen[m * 16 + 8 + g] >> (j0 + j) & 1;
+              const float w = __shfl_sync(~0u, j >> 3 ? s[n][2 + h] : s[n][h], (j & 7) * 4 + t);
+              const bool see = seen[n * 8 + 2 * t + h] >> (j0 + j) & 1;
 #pragma unroll
-            for (int nt = 0; nt < D / 8; nt++)
+              for (int i = 0; i < L::kTiles; i++)
 #pragma unroll
-              for (int e = 0; e < 2; e++) {
-                const float x = to_f(row[L::out_dim(nt, e, t)]);
-                if (!isfinite(x)) {
-                  if (see0) o[m][nt][e] += w[0] * x;
-                  if (see1) o[m][nt][e + 2] += w[1] * x;
+                for (int e = 0; e < 2; e++) {
+                  const float x = to_f(row[L::out_dim(i, 2 * e, g)]);
+                  if (!isfinite(x) && see) o[i][n][2 * e + h] += w * x;
                 }
-              }
-          }
+            }
         }
       }
     }
@@ -431,46 +444,47 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, MT>::kBlocks)) 
     float *join = (float *)(ring + S::kEarly * S::kSlot);
     float *part = CS > 1 ? (float *)ring : a.part + slot * ROWS * D;
     float *to_ml = CS > 1 ? part_ml : a.part_ml + slot * ROWS * 2;
-    // 16 bytes d of row r: exchanged so that a warp's stores hit different banks
-    auto piece_of = [](int r, int d) { return L::f32 ? d ^ (r & 1) : d ^ ((r & 3) << 1); };
+    // dim d of row r: exchanged so that a warp's stores hit different banks
+    auto dim_of = [](int r, int d) { return d ^ (((r >> 1) & 3) << 3); };
+    constexpr int JR = S::kJoinRows;
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
+    for (int m = 0; m < ROWS / JR; m++) {
       __syncthreads();  // every warp is done with what the join lies over
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        float l = sum[m][h];
-        l += __shfl_xor_sync(~0u, l, 1);
-        l += __shfl_xor_sync(~0u, l, 2);
-        const int r = 8 * h + g;
-        if (t == 0) ml[(warp * ROWS + m * 16 + r) * 2] = mx[m][h], ml[(warp * ROWS + m * 16 + r) * 2 + 1] = l;
-        float4 *to = (float4 *)join + (warp * 16 + r) * (D / 4);
-        auto &x = o[m];
-        if constexpr (L::f32) {
+      for (int n = m * (JR / 8); n < (m + 1) * (JR / 8); n++)
 #pragma unroll
-          for (int blk = 0; blk < D / 32; blk++) {
-            to[piece_of(r, blk * 8 + 2 * t)] = make_float4(x[blk * 4][2 * h], x[blk * 4 + 1][2 * h], x[blk * 4 + 2][2 * h], x[blk * 4 + 3][2 * h]);
-            to[piece_of(r, blk * 8 + 2 * t + 1)] = make_float4(x[blk * 4][2 * h + 1], x[blk * 4 + 1][2 * h + 1], x[blk * 4 + 2][2 * h + 1], x[blk * 4 + 3][2 * h + 1]);
+        for (int h = 0; h < 2; h++) {
+          float l = sum[n][h];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(~0u, l, d);
+          const int row = n * 8 + 2 * t + h, r = row - m * JR;
+          if (g == 0) ml[(warp * ROWS + row) * 2] = ref[n][h], ml[(warp * ROWS + row) * 2 + 1] = l;
+          float *to = join + (warp * JR + r) * D;
+          if constexpr (L::f32) {
+#pragma unroll
+            for (int blk = 0; blk < D / 32; blk++)
+              *(float4 *)(to + dim_of(r, blk * 32 + 4 * g)) =
+                  make_float4(o[2 * blk][n][h], o[2 * blk][n][2 + h], o[2 * blk + 1][n][h], o[2 * blk + 1][n][2 + h]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < L::kTiles; i++)
+              to[dim_of(r, i * 16 + g)] = o[i][n][h], to[dim_of(r, i * 16 + 8 + g)] = o[i][n][2 + h];
           }
-        } else {
-#pragma unroll
-          for (int nt = 0; nt < D / 8; nt++)
-            ((float2 *)(to + piece_of(r, nt * 2 + (t >> 1))))[t & 1] = make_float2(x[nt][2 * h], x[nt][2 * h + 1]);
         }
-      }
-      if (m == MT - 1 && more) load_query(cur);
+      if (m == ROWS / JR - 1 && more) load_query(cur);
       __syncthreads();
-      for (int i = tid; i < min(16, rows - m * 16) * (D / 4); i += kTreeThreads) {
-        const int r = i / (D / 4), d = i % (D / 4), row = m * 16 + r;
+      for (int i = tid; i < min(JR, rows - m * JR) * (D / 4); i += kTreeThreads) {
+        const int r = i / (D / 4), d = i % (D / 4), row = m * JR + r;
         float top = -INFINITY, l = 0.f;
 #pragma unroll
         for (int w = 0; w < kTreeWarps; w++) top = fmaxf(top, ml[(w * ROWS + row) * 2]);
-        const float ref = top == -INFINITY ? 0.f : top;
+        const float base = top == -INFINITY ? 0.f : top;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kTreeWarps; w++) {
-          const float f = exp2_(ml[(w * ROWS + row) * 2] - ref);
+          const float f = exp2_(ml[(w * ROWS + row) * 2] - base);
           l = fmaf(f, ml[(w * ROWS + row) * 2 + 1], l);
-          const float4 y = ((const float4 *)join)[(w * 16 + r) * (D / 4) + piece_of(r, d)];
+          const float4 y = *(const float4 *)(join + (w * JR + r) * D + dim_of(r, d * 4));
           x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
         }
         if (whole) {
