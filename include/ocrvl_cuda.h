@@ -383,6 +383,12 @@ int ocrvl_op_kv_select(int num_layers, int batch, int num_kv_heads, const float 
 int ocrvl_op_kv_compact(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const int32_t *idx, int keep,
                         void *stream);
 
+/* ocrvl_op_kv_select on every layer of `from`, then ocrvl_op_kv_compact with
+ * its idx (which may not be NULL), as one call. */
+int ocrvl_op_kv_evict(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const float *acc, int acc_width,
+                      int64_t acc_stride, const int32_t *lens, int keep, int sinks, int recent, int32_t *idx,
+                      float *sums, int32_t *new_lens, void *stream);
+
 /* Writes tokens behind the cache: for i < n_path[b] (at most max_path),
  * position lens[b] + i of every layer becomes token indptr[b] + path[b][i];
  * path NULL: token indptr[b] + i, for all of the sequence's tokens.  k and v are

@@ -110,6 +110,7 @@ SIGNATURES = {
     "ocrvl_op_attn_mass": (I, [C.POINTER(KVCache), I, I, I, I, P, P, P, P, I64, P, F, F, P, I, I64, P, I, I64, P]),
     "ocrvl_op_kv_select": (I, [I, I, I, P, I, I64, P, I, I, I, P, P, P, P]),
     "ocrvl_op_kv_compact": (I, [C.POINTER(KVCache), C.POINTER(KVCache), P, I, P]),
+    "ocrvl_op_kv_evict": (I, [C.POINTER(KVCache), C.POINTER(KVCache), P, I, I64, P, I, I, I, P, P, P, P]),
     "ocrvl_op_kv_append": (I, [C.POINTER(KVCache), I, P, P, P, P, I, P, P, I64, I64, P, P]),
 }
 

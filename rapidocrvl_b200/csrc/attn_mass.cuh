@@ -33,15 +33,16 @@ struct MassArgs {
   int acc_width, out_width;
 };
 
-// A sequence's tiles and what one costs: K's load and the rows' products.
+// A sequence's tiles and what one costs: K's load (about what `load` tiles of
+// 8 rows take) and the rows' products.
 struct MassShare {
   int first, count, len, tiles, cost;
 
-  __device__ MassShare(const MassArgs &a, int b) {
+  __device__ MassShare(const MassArgs &a, int b, int load) {
     count = a.s.tokens(b, &first);
     len = min(a.s.len(b), a.out_width);
     tiles = (len + kMassWarps * kChunk - 1) / (kMassWarps * kChunk);
-    cost = 1 + (count * a.group + 7) / 8;
+    cost = load + (count * a.group + 7) / 8;
   }
   __device__ long long total(int kv_heads) const { return (long long)kv_heads * tiles * cost; }
 };
@@ -52,6 +53,7 @@ struct MassShape {
   static constexpr int kUnits = L::kBytes >= 8192 ? 3 : L::kBytes >= 4096 ? 4 : 6;
   static constexpr int kRing = kMassWarps * kUnits * L::kBytes;
   static constexpr int kRowTiles = THIN ? 1 : L::f32 ? (D == 128 ? 4 : 16) : 32;
+  static constexpr int kLoad = L::f32 ? 4 : 12;
   static constexpr int kSmem = kRing + kRowTiles * L::kQBytes + kRowTiles * 8 * 4 + 64;
 };
 
@@ -69,14 +71,14 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
   // where this block's share of the cost starts: a sequence, the cost below it
   if (warp == 0) {
     long long all = 0;
-    for (int b = lane; b < a.s.batch; b += 32) all += MassShare(a, b).total(a.kv_heads);
+    for (int b = lane; b < a.s.batch; b += 32) all += MassShare(a, b, S::kLoad).total(a.kv_heads);
     for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
     const long long lo = all * blockIdx.x / gridDim.x;
     if (lane == 0) plan[0] = all, plan[1] = a.s.batch, plan[2] = all;
     __syncwarp();
     long long below = 0;
     for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
-      const long long mine = b0 + lane < a.s.batch ? MassShare(a, b0 + lane).total(a.kv_heads) : 0;
+      const long long mine = b0 + lane < a.s.batch ? MassShare(a, b0 + lane, S::kLoad).total(a.kv_heads) : 0;
       long long upto = mine;
       for (int d = 1; d < 32; d <<= 1) {
         const long long x = __shfl_up_sync(~0u, upto, d);
@@ -96,7 +98,7 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
   const uint32_t my_ring = smem_addr(ring) + warp * NU * L::kBytes, q_at = smem_addr(q_sm);
   long long at = plan[2];  // cost below the current segment
   for (int b = (int)plan[1]; b < a.s.batch && at < hi; b++) {
-    const MassShare sh(a, b);
+    const MassShare sh(a, b, S::kLoad);
     for (int head = 0; head < a.kv_heads; head++) {
       // the tiles whose cost starts in this block's share
       const long long from = max(lo - at, 0ll), to = hi - at;
@@ -112,7 +114,7 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
       float *out = a.out + ((long long)b * a.kv_heads + head) * a.out_stride;
 
       for (int m0 = 0; m0 == 0 || m0 < row_tiles; m0 += S::kRowTiles) {
-        const int mt = min(S::kRowTiles, row_tiles - m0);
+        const int mt = min(S::kRowTiles, (row_tiles - m0 + 3) / 4 * 4);  // rows past the last do not count
         int pages = -1;
         unsigned long long valids = 0;  // 8 bits a unit in flight, the next one lowest
         auto issue = [&](int k) {
@@ -203,16 +205,23 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
             typename L::KFrag f[L::kTiles];
 #pragma unroll
             for (int blk = 0; blk < L::kTiles; blk++) L::k_load(f[blk], blk, k_at, lane);
-            for (int m = 0; m < mt; m++) {
-              float s[4] = {}, c[2][4] = {};
+            // several tiles of rows at once: a chain of products of its own takes 11.5 ns a link
+            constexpr int AT = L::f32 ? 2 : 4;
+            for (int m = 0; m < mt; m += AT) {
+              float s[AT][4] = {}, c[AT][2][4] = {};
 #pragma unroll
-              for (int blk = 0; blk < L::kTiles; blk++) {
-                uint32_t x[L::kQRegs];
-                L::q_load(x, q_at + m * L::kQBytes, blk, lane);
-                L::k_product(s, c, x, f[blk]);
+              for (int blk = 0; blk < L::kTiles; blk++)
+#pragma unroll
+                for (int i = 0; i < AT; i++) {
+                  uint32_t x[L::kQRegs];
+                  L::q_load(x, q_at + (m + i) * L::kQBytes, blk, lane);
+                  L::k_product(s[i], c[i], x, f[blk]);
+                }
+#pragma unroll
+              for (int i = 0; i < AT; i++) {
+                l0 = shift[(m + i) * 8 + 2 * t], l1 = shift[(m + i) * 8 + 2 * t + 1];
+                add(s[i], c[i]);
               }
-              l0 = shift[m * 8 + 2 * t], l1 = shift[m * 8 + 2 * t + 1];
-              add(s, c);
             }
           }
 #pragma unroll

@@ -11,9 +11,9 @@ namespace paged {
 
 // ---- select ---------------------------------------------------------------
 
-constexpr int kSelThreads = 1024;
 constexpr int kSelBins = 2048;
-constexpr int kSelStage = 48 * 1024;  // sums a block holds in shared memory
+constexpr int kSelList = 256;  // keys that are ranked directly
+constexpr int kSelStage = 48 * 1024;  // keys a block holds in shared memory: a multiple of its threads times four
 
 struct SelectArgs {
   const float *acc;
@@ -25,26 +25,37 @@ struct SelectArgs {
   int *new_lens;
 };
 
-// A float's bits in an order that unsigned integers have; NaN lowest, -0 = 0.
+// A float's bits in an order that unsigned integers have, NaN lowest, -0 = 0,
+// all of them between kNever (not a position) and kAlways (kept whatever its sum).
+constexpr uint32_t kNever = 0u, kAlways = ~0u;
 __device__ __forceinline__ uint32_t order_key(float x) {
-  if (x != x) return 0u;
+  if (x != x) return 1u;
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One cluster of CS blocks a row, each with a contiguous slice of it.  The
-// need-th largest key of the middle is found 11, 11 and 10 bits at a time from
-// histograms that the blocks add up over distributed shared memory; then each
-// block writes what it keeps, in order, behind what the blocks before it keep.
-template <int CS, bool STAGED>
-__global__ void __launch_bounds__(kSelThreads) k_kv_select(const SelectArgs a) {
+// One cluster of CS blocks a row, each with a contiguous slice of it, each
+// warp with a contiguous part of the slice.  The need-th largest key of the
+// middle is found from histograms of 2048 equal bins, first over the range
+// from the smallest to the largest key, then over the bin that holds it, until a
+// bin is one key, or holds so few that they are listed and ranked directly; the
+// cluster's blocks add their filled bins to the first one's over distributed
+// shared memory, which searches.
+// Sums span many powers of two, so the range fills the bins evenly where the
+// leading bits of the keys would send most of a warp's additions to one
+// address.  Then each warp writes what it keeps, in order, behind what those
+// before it keep.  Bound by latencies: the loads of a step go out together, and
+// a round of the search takes 1 to 2 us.
+template <int CS, bool STAGED, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_kv_select(const SelectArgs a) {
   namespace cg = cooperative_groups;
+  constexpr int WARPS = THREADS / 32, OWN = kSelBins / THREADS;  // bins a thread looks after
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ __align__(16) uint32_t keys[];  // STAGED: the slice's keys
-  __shared__ uint32_t hist[kSelBins];
-  __shared__ uint32_t warp_n[32];
-  __shared__ uint32_t found[2];
-  __shared__ uint32_t part[2];  // how many of the slice are above the threshold (or always kept), and at it
+  __shared__ uint32_t hist[kSelBins], total[CS > 1 ? kSelBins : 1];
+  __shared__ uint32_t warp_n[WARPS], warp_m[WARPS];
+  __shared__ uint32_t found[3], list[kSelList], list_n;
+  __shared__ uint32_t range[2], part[2];  // read by the cluster
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = CS == 1 ? 0 : (int)cluster.block_rank();
   const int row = blockIdx.x / CS, b = row / a.kv_heads % a.batch;
@@ -54,136 +65,228 @@ __global__ void __launch_bounds__(kSelThreads) k_kv_select(const SelectArgs a) {
   int *idx = a.idx + (long long)row * a.keep;
   float *sums = a.sums ? a.sums + (long long)row * a.keep : nullptr;
   if (a.new_lens && row < a.batch * a.kv_heads && row % a.kv_heads == 0 && rank == 0 && tid == 0) a.new_lens[b] = held;
-  for (int j = held + rank * kSelThreads + tid; j < a.keep; j += CS * kSelThreads) {
+  for (int j = held + rank * THREADS + tid; j < a.keep; j += CS * THREADS) {
     idx[j] = -1;
     if (sums) sums[j] = 0.f;
   }
   if (n <= a.keep) {
-    for (int j = rank * kSelThreads + tid; j < n; j += CS * kSelThreads) {
+    for (int j = rank * THREADS + tid; j < n; j += CS * THREADS) {
       idx[j] = j;
       if (sums) sums[j] = acc[j];
     }
     return;  // the whole cluster alike
   }
-  // the middle and the slice of all positions
+  // the middle, the block's slice of all positions and the warp's part of it,
+  // in steps of 128
   const int mid0 = a.sinks, mid1 = n - a.recent;
-  const uint32_t need0 = a.keep - a.sinks - a.recent;
-  const int slice = (n + CS - 1) / CS, s0 = min(n, rank * slice), s1 = min(n, s0 + slice);
-  if (STAGED) {
-    for (int i = s0 + tid; i < s1; i += kSelThreads) keys[i - s0] = order_key(acc[i]);
-    __syncthreads();
-  }
-  auto key = [&](int i) { return STAGED ? keys[i - s0] : order_key(acc[i]); };
-  const int m0 = max(s0, mid0), m1 = min(s1, mid1);
+  const int slice = ((n + CS - 1) / CS + 3) & ~3, s0 = min(n, rank * slice), s1 = min(n, s0 + slice);
+  const int steps = (slice + THREADS * 4 - 1) / (THREADS * 4), w0 = s0 + warp * steps * 128;
+  auto sum_of = [&](int i) { return i < s1 ? __ldg(acc + i) : 0.f; };
+  auto key_of = [&](int i, float x) { return i >= s1 ? kNever : i < mid0 || i >= mid1 ? kAlways : order_key(x); };
+  // the keys of positions i .. i + 3
+  auto key4 = [&](int i) {
+    if constexpr (STAGED)
+      return *reinterpret_cast<const uint4 *>(keys + (i - s0));
+    const float x[4] = {sum_of(i), sum_of(i + 1), sum_of(i + 2), sum_of(i + 3)};
+    return make_uint4(key_of(i, x[0]), key_of(i + 1, x[1]), key_of(i + 2, x[2]), key_of(i + 3, x[3]));
+  };
 
-  uint32_t prefix = 0, need = need0;
-#pragma unroll
-  for (int pass = 0; pass < 3; pass++) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = m0 + tid; i < m1; i += kSelThreads) {
-      const uint32_t k = key(i);
-      if (pass == 0 || k >> (shift + bits) == prefix) atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
-    }
-    uint32_t c[2];
-    if (CS > 1) {
-      cluster.sync();
-      c[0] = c[1] = 0;
-      for (int r = 0; r < CS; r++) {
-        const uint32_t *h = cluster.map_shared_rank(hist, r);
-        c[0] += h[2 * tid], c[1] += h[2 * tid + 1];
+  uint32_t low = ~0u, high = 0u;
+  if (STAGED) {  // all of the warp's sums on their way at once, then turned into keys where they lie
+    const uint32_t at = smem_addr(keys);
+    if (((uintptr_t)(acc + s0) & 15) == 0) {
+      for (int j = 0; j < steps; j++) {
+        const int i = w0 + j * 128 + lane * 4, n4 = min(4, max(0, s1 - i));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + (i - s0) * 4), "l"(n4 ? acc + i : acc), "r"(n4 * 4) : "memory");
       }
-      cluster.sync();  // nobody reads this histogram any more
     } else {
-      __syncthreads();
-      c[0] = hist[2 * tid], c[1] = hist[2 * tid + 1];
-    }
-    // how many lie above this thread's two bins
-    uint32_t mine = c[0] + c[1], above = mine;
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t x = __shfl_down_sync(~0u, above, d);
-      if (lane + d < 32) above += x;
-    }
-    if (lane == 0) warp_n[warp] = above;
-    __syncthreads();
-    if (tid < 32) {
-      uint32_t x = warp_n[lane], y = x;
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t z = __shfl_down_sync(~0u, y, d);
-        if (lane + d < 32) y += z;
+      for (int j = 0; j < steps * 4; j++) {
+        const int i = w0 + j * 32 + lane;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(at + (i - s0) * 4), "l"(i < s1 ? acc + i : acc), "r"(i < s1 ? 4 : 0) : "memory");
       }
-      warp_n[lane] = y - x;  // of the warps above
     }
-    __syncthreads();
-    above += warp_n[warp] - mine;
-    if (above < need && above + mine >= need) {  // exactly one thread, if need > 0
-      const bool upper = above + c[1] >= need;
-      found[0] = 2 * tid + (upper ? 1 : 0);
-      found[1] = need - above - (upper ? 0 : c[1]);
-    }
-    __syncthreads();
-    if (need > 0) prefix = prefix << bits | found[0], need = found[1];
-    __syncthreads();
+    copy_commit();
+    copy_wait<0>();
+    __syncwarp();
   }
-  // kept: always kept ones, keys above prefix, and the first `need` at it
-  const bool any = need0 > 0;
-  auto above_it = [&](int i) { return i < mid0 || i >= mid1 || (any && key(i) > prefix); };
-  auto at_it = [&](int i) { return any && i >= mid0 && i < mid1 && key(i) == prefix; };
-  uint32_t n_above = 0, n_at = 0, base_above = 0, base_at = 0;
+  for (int j = 0; j < steps; j++) {
+    const int i = w0 + j * 128 + lane * 4;
+    uint4 k;
+    if constexpr (STAGED) {
+      const float4 x = *reinterpret_cast<const float4 *>(keys + (i - s0));
+      k = make_uint4(key_of(i, x.x), key_of(i + 1, x.y), key_of(i + 2, x.z), key_of(i + 3, x.w));
+      *reinterpret_cast<uint4 *>(keys + (i - s0)) = k;
+    } else {
+      k = key4(i);
+    }
+    auto widen = [&](uint32_t x) {
+      if (x != kNever && x != kAlways) low = min(low, x), high = max(high, x);
+    };
+    widen(k.x), widen(k.y), widen(k.z), widen(k.w);
+  }
+  low = __reduce_min_sync(~0u, low), high = __reduce_max_sync(~0u, high);
+  if (lane == 0) warp_n[warp] = low, warp_m[warp] = high;
+  if (tid == 0) list_n = 0;
+  for (int i = tid; i < kSelBins; i += THREADS) {
+    hist[i] = 0;
+    if (CS > 1) total[i] = 0;
+  }
+  __syncthreads();
+  low = __reduce_min_sync(~0u, lane < WARPS ? warp_n[lane] : ~0u), high = __reduce_max_sync(~0u, lane < WARPS ? warp_m[lane] : 0u);
   if (CS > 1) {
-    for (int i = s0 + tid; i < s1; i += kSelThreads) n_above += above_it(i), n_at += at_it(i);
-    for (int d = 16; d; d >>= 1) n_above += __shfl_xor_sync(~0u, n_above, d), n_at += __shfl_xor_sync(~0u, n_at, d);
-    if (tid < 2) part[tid] = 0;
-    __syncthreads();
-    if (lane == 0) atomicAdd(&part[0], n_above), atomicAdd(&part[1], n_at);
+    if (tid == 0) range[0] = low, range[1] = high;
+    cluster.sync();
+    for (int r = 0; r < CS; r++) {
+      const uint32_t *p = cluster.map_shared_rank(range, r);
+      low = min(low, p[0]), high = max(high, p[1]);
+    }
+  }
+
+  uint32_t need = a.keep - a.sinks - a.recent, base = kAlways - 1;
+  if (need > 0) {
+    uint32_t span = high - low;  // the key is in base .. base + span
+    base = low;
+    while (true) {
+      const int shift = max(0, 32 - __clz(span) - 11);  // span >> shift < 2048
+      for (int j = 0; j < steps; j++) {
+        const uint4 k = key4(w0 + j * 128 + lane * 4);
+        if (k.x - base <= span) atomicAdd(&hist[(k.x - base) >> shift], 1u);
+        if (k.y - base <= span) atomicAdd(&hist[(k.y - base) >> shift], 1u);
+        if (k.z - base <= span) atomicAdd(&hist[(k.z - base) >> shift], 1u);
+        if (k.w - base <= span) atomicAdd(&hist[(k.w - base) >> shift], 1u);
+      }
+      __syncthreads();
+      uint32_t c[OWN], mine = 0;
+#pragma unroll
+      for (int j = 0; j < OWN; j++) c[j] = hist[OWN * tid + j], hist[OWN * tid + j] = 0;
+      if (CS > 1) {
+        uint32_t *first = cluster.map_shared_rank(total, 0);
+#pragma unroll
+        for (int j = 0; j < OWN; j++)
+          if (c[j]) atomicAdd(first + OWN * tid + j, c[j]);
+        cluster.sync();
+      }
+      if (rank == 0) {
+        if (CS > 1) {
+#pragma unroll
+          for (int j = 0; j < OWN; j++) c[j] = total[OWN * tid + j], total[OWN * tid + j] = 0;
+        }
+        // how many lie above this thread's bins
+#pragma unroll
+        for (int j = 0; j < OWN; j++) mine += c[j];
+        uint32_t above = mine;
+        for (int d = 1; d < 32; d <<= 1) {
+          const uint32_t x = __shfl_down_sync(~0u, above, d);
+          if (lane + d < 32) above += x;
+        }
+        if (lane == 0) warp_n[warp] = above;
+        above -= mine;
+        __syncthreads();
+        above += __reduce_add_sync(~0u, lane > warp && lane < WARPS ? warp_n[lane] : 0u);
+        if (above < need && above + mine >= need) {  // exactly one thread
+          uint32_t over = above;
+#pragma unroll
+          for (int j = OWN - 1; j >= 0; j--) {
+            if (over < need && over + c[j] >= need) {
+              for (int r = 0; r < CS; r++) {
+                uint32_t *to = CS > 1 ? cluster.map_shared_rank(found, r) : found;
+                to[0] = OWN * tid + j, to[1] = need - over, to[2] = c[j];
+              }
+            }
+            over += c[j];
+          }
+        }
+      }
+      if (CS > 1)
+        cluster.sync();
+      else
+        __syncthreads();
+      base += found[0] << shift, need = found[1];
+      if (shift == 0) break;
+      span = (1u << shift) - 1;
+      const uint32_t count = found[2];
+      if (count > kSelList) continue;
+      uint32_t *to = CS > 1 ? cluster.map_shared_rank(list, 0) : list, *to_n = CS > 1 ? cluster.map_shared_rank(&list_n, 0) : &list_n;
+      for (int j = 0; j < steps; j++) {
+        const uint4 k = key4(w0 + j * 128 + lane * 4);
+        if (k.x - base <= span) to[atomicAdd(to_n, 1u)] = k.x;
+        if (k.y - base <= span) to[atomicAdd(to_n, 1u)] = k.y;
+        if (k.z - base <= span) to[atomicAdd(to_n, 1u)] = k.z;
+        if (k.w - base <= span) to[atomicAdd(to_n, 1u)] = k.w;
+      }
+      if (CS > 1)
+        cluster.sync();
+      else
+        __syncthreads();
+      if (rank == 0 && tid < count) {
+        const uint32_t k = list[tid];
+        uint32_t over = 0, same = 0;
+        for (uint32_t i = 0; i < count; i++) over += list[i] > k, same += list[i] == k;
+        if (over < need && over + same >= need) {  // the same values from every thread that has this key
+          for (int r = 0; r < CS; r++) {
+            uint32_t *f = CS > 1 ? cluster.map_shared_rank(found, r) : found;
+            f[0] = k, f[1] = need - over;
+          }
+        }
+      }
+      if (CS > 1)
+        cluster.sync();
+      else
+        __syncthreads();
+      base = found[0], need = found[1];
+      break;
+    }
+  }
+  // kept: keys above base, and the first `need` equal to it
+  uint32_t n_above = 0, n_at = 0;
+  for (int j = 0; j < steps; j++) {
+    const uint4 k = key4(w0 + j * 128 + lane * 4);
+    n_above += (k.x > base) + (k.y > base) + (k.z > base) + (k.w > base);
+    n_at += (k.x == base) + (k.y == base) + (k.z == base) + (k.w == base);
+  }
+  n_above = __reduce_add_sync(~0u, n_above), n_at = __reduce_add_sync(~0u, n_at);
+  __syncthreads();
+  if (lane == 0) warp_n[warp] = n_above, warp_m[warp] = n_at;
+  __syncthreads();
+  const uint32_t x = lane < WARPS ? warp_n[lane] : 0u, y = lane < WARPS ? warp_m[lane] : 0u;
+  uint32_t before = __reduce_add_sync(~0u, lane < warp ? x : 0u), at = __reduce_add_sync(~0u, lane < warp ? y : 0u);
+  if (CS > 1) {
+    const uint32_t all_x = __reduce_add_sync(~0u, x), all_y = __reduce_add_sync(~0u, y);
+    if (tid == 0) part[0] = all_x, part[1] = all_y;
     cluster.sync();
     for (int r = 0; r < rank; r++) {
       const uint32_t *p = cluster.map_shared_rank(part, r);
-      base_above += p[0], base_at += p[1];
+      before += p[0], at += p[1];
     }
     cluster.sync();  // before any block of the cluster may end
   }
-  // in order, 4 positions a thread, 4096 a step: 16 bits hold each count of a step
-  for (int i0 = s0; i0 < s1; i0 += 4 * kSelThreads) {
-    uint32_t up = 0, at = 0;
-    const int i1 = i0 + 4 * tid;
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (i1 + e < s1) up |= (uint32_t)above_it(i1 + e) << e, at |= (uint32_t)at_it(i1 + e) << e;
-    const uint32_t mine = __popc(up) | __popc(at) << 16;
-    uint32_t upto = mine;
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t x = __shfl_up_sync(~0u, upto, d);
-      if (lane >= d) upto += x;
-    }
-    __syncthreads();
-    if (lane == 31) warp_n[warp] = upto;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    {
-      const uint32_t x = warp_n[lane];
-      uint32_t y = x;
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t z = __shfl_up_sync(~0u, y, d);
-        if (lane >= d) y += z;
-      }
-      before = __shfl_sync(~0u, y - x, warp);
-      all = __shfl_sync(~0u, y, 31);
-    }
-    before += upto - mine;
-    uint32_t na = base_above + (before & 0xffff), nt = base_at + (before >> 16);
+  // the sum behind a key: from the key itself, unless that says too little
+  auto sum_behind = [&](uint32_t k, int i) {
+    if (k == kAlways || k == 1u || k == 0x80000000u) return __ldg(acc + i);
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+  };
+  const unsigned lower = (1u << lane) - 1;
+  for (int j = 0; j < steps; j++) {
+    const int i = w0 + j * 128 + lane * 4;
+    const uint4 k4 = key4(i);
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+    uint32_t nu = before, nq = at;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const bool u = up >> e & 1, q = at >> e & 1;
-      if (u || (q && nt < need)) {
-        const uint32_t j = na + min(nt, need);
-        idx[j] = i1 + e;
-        if (sums) sums[j] = acc[i1 + e];
-      }
-      na += u, nt += q;
+      const unsigned us = __ballot_sync(~0u, k[e] > base), qs = __ballot_sync(~0u, k[e] == base);
+      nu += __popc(us & lower), nq += __popc(qs & lower);
+      before += __popc(us), at += __popc(qs);
     }
-    base_above += all & 0xffff, base_at += all >> 16;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const bool u = k[e] > base, q = k[e] == base;
+      if (u || (q && nq < need)) {
+        const uint32_t to = nu + min(nq, need);
+        idx[to] = i + e;
+        if (sums) sums[to] = sum_behind(k[e], i + e);
+      }
+      nu += u, nq += q;
+    }
   }
 }
 
@@ -208,9 +311,11 @@ __device__ __forceinline__ long long row_at(const int *table, long long table_st
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 64;  // rows a block moves at a time
+constexpr int kMoveRows = 32;  // rows a block moves at a time
 
-// To other pages: blocks of 64 rows of K and V, in any order.
+// To other pages: blocks of 32 rows of K and V of ROW bytes, in any order.  A
+// thread's loads are all on their way before its first store.
+template <int ROW>
 __global__ void __launch_bounds__(kMoveThreads) k_kv_compact(const CompactArgs a) {
   __shared__ long long from[kMoveRows], to[kMoveRows];
   const int j0 = blockIdx.y * kMoveRows, row = blockIdx.x;  // row: (layer, sequence, kv head)
@@ -224,14 +329,19 @@ __global__ void __launch_bounds__(kMoveThreads) k_kv_compact(const CompactArgs a
     to[threadIdx.x] = y;
   }
   __syncthreads();
-  const long long s = layer * a.src_layer + head * a.src_head, d = layer * a.dst_layer + head * a.dst_head;
-  const int pieces = a.row_bytes / 16;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < 2 * kMoveRows * pieces; i += kMoveThreads) {
-    const int p = i % pieces, r = i / pieces % kMoveRows, v = i / pieces / kMoveRows;
-    if (from[r] >= 0)
-      *(uint4 *)((v ? a.dst_v : a.dst_k) + d + to[r] + p * 16) =
-          __ldg((const uint4 *)((v ? a.src_v : a.src_k) + s + from[r] + p * 16));
+  constexpr int PIECES = ROW / 16, LANES = kMoveThreads / PIECES, STEPS = kMoveRows / LANES;  // rows at a time, and how often
+  const int p = threadIdx.x % PIECES, r0 = threadIdx.x / PIECES;
+  const long long s = layer * a.src_layer + head * a.src_head + p * 16, d = layer * a.dst_layer + head * a.dst_head + p * 16;
+  uint4 k[STEPS], v[STEPS];
+#pragma unroll
+  for (int i = 0; i < STEPS; i++) {
+    const long long x = from[r0 + i * LANES];
+    if (x >= 0) k[i] = __ldg((const uint4 *)(a.src_k + s + x)), v[i] = __ldg((const uint4 *)(a.src_v + s + x));
+  }
+#pragma unroll
+  for (int i = 0; i < STEPS; i++) {
+    const long long y = to[r0 + i * LANES];
+    if (from[r0 + i * LANES] >= 0) *(uint4 *)(a.dst_k + d + y) = k[i], *(uint4 *)(a.dst_v + d + y) = v[i];
   }
 }
 
@@ -244,7 +354,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_kv_compact_in_place(const Comp
   const int head = row % a.kv_heads, b = row / a.kv_heads % a.batch, layer = row / a.kv_heads / a.batch;
   char *base = (v ? a.dst_v : a.dst_k) + layer * a.dst_layer + head * a.dst_head + column;
   pdl_wait();
-  for (int j0 = 0; j0 < a.keep; j0 += kMoveRows) {
+  for (int j0 = 0; j0 < a.keep; j0 += kMoveThreads / 4) {
     const int j = j0 + threadIdx.x / 4, pos = j < a.keep ? a.idx[(long long)row * a.keep + j] : -1;
     long long x = -1, y = -1;
     if (pos > j) {

@@ -89,13 +89,18 @@ int sm_count(int *out) {
   return OCRVL_OK;
 }
 
+// Blocks that run at once in clusters of up to eight, one an SM: clusters lie within
+// one of the GPU's partitions, so some SMs stay over (15 clusters of eight
+// were resident on 148 SMs).
+int cluster_room(int sms) { return sms * 4 / 5; }
+
 // Launches with `smem` bytes of dynamic shared memory; dependent: may start
 // before the kernel launched just before it on the stream ends (both wait for
 // it with griddepcontrol).
 template <typename... Params, typename... Args>
 int launch(const char *name, void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, bool dependent,
            int cluster, Args... args) {
-  if (smem > 48 * 1024) {
+  if (smem > 24 * 1024) {  // with a kernel's static share possibly past the 48 KB that need no leave
     cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_fail(name, e);
   }
@@ -156,13 +161,13 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   auto one = [&](auto kernel, int cs) {
     return launch("tree attention", kernel, dim3((unsigned)(segments * cs)), kTreeThreads, S::kSmem, stream, false, cs, a, blocks);
   };
-  const int room = sms * S::kBlocks;
+  const int room = sms * S::kBlocks, clustered = cluster_room(sms) * S::kBlocks;
   if (tiles <= kFew && (segments >= room || tiles <= 2)) return one(k_tree_attn<T, D, NT, 1>, 1);
-  if (tiles <= 4 * kFew && segments * 4 <= room) {
-    if (tiles > 4 && segments * 8 <= room) return one(k_tree_attn<T, D, NT, 8>, 8);
+  if (tiles <= 4 * kFew && segments * 4 <= clustered) {
+    if (tiles > 4 && segments * 8 <= clustered) return one(k_tree_attn<T, D, NT, 8>, 8);
     return one(k_tree_attn<T, D, NT, 4>, 4);
   }
-  if (tiles <= 8 * kFew && segments * 8 <= room) return one(k_tree_attn<T, D, NT, 8>, 8);
+  if (tiles <= 8 * kFew && segments * 8 <= clustered) return one(k_tree_attn<T, D, NT, 8>, 8);
 
   const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
   a.part = (float *)work;
@@ -195,11 +200,58 @@ int launch_mass(const MassArgs &a, int sms, cudaStream_t stream) {
   return launch("attention mass", k_attn_mass<T, D, false>, dim3(sms), kMassThreads, MassShape<T, D, false>::kSmem, stream, false, 1, a);
 }
 
-template <int CS>
-int launch_select(const SelectArgs &a, int rows, int stage, cudaStream_t stream) {
+template <int CS, int THREADS>
+int launch_select(const SelectArgs &a, int rows, cudaStream_t stream) {
   const dim3 grid((unsigned)(rows * CS));
-  return stage ? launch("select", k_kv_select<CS, true>, grid, kSelThreads, stage, stream, false, CS, a)
-               : launch("select", k_kv_select<CS, false>, grid, kSelThreads, 0, stream, false, CS, a);
+  const long long step = THREADS * 4, n = (((a.width + CS - 1) / CS + 3) / 4 * 4 + step - 1) / step * step;
+  return n <= kSelStage ? launch("select", k_kv_select<CS, true, THREADS>, grid, THREADS, (int)n * 4, stream, false, CS, a)
+                        : launch("select", k_kv_select<CS, false, THREADS>, grid, THREADS, 0, stream, false, CS, a);
+}
+
+int check_move(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const int32_t *idx, int keep) {
+  if (int rc = check_cache(from)) return rc;
+  if (int rc = check_cache(to)) return rc;
+  if (from->type != to->type || from->head_dim != to->head_dim || from->num_kv_heads != to->num_kv_heads ||
+      from->num_layers != to->num_layers || from->batch != to->batch)
+    return invalid("the caches must have the same type, head_dim, heads, layers and batch");
+  if (keep < 1 || keep > 65535 * kMoveRows) return invalid("keep must be 1..2,097,120");
+  if (!idx) return invalid("null argument");
+  if ((long long)from->num_layers * from->batch * from->num_kv_heads > 1 << 24) return invalid("too many rows");
+  return OCRVL_OK;
+}
+
+// dependent: right behind the kernel that writes idx
+int compact(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const int32_t *idx, int keep, cudaStream_t st, bool dependent) {
+  if (int rc = check_move(from, to, idx, keep)) return rc;
+  const long long rows = (long long)from->num_layers * from->batch * from->num_kv_heads;
+  const long long es = elem_bytes(from->type);
+  CompactArgs a;
+  a.src_k = (const char *)from->k, a.src_v = (const char *)from->v;
+  a.dst_k = (char *)to->k, a.dst_v = (char *)to->v;
+  a.src_table = from->table, a.dst_table = to->table, a.idx = idx;
+  a.src_page = from->page_stride * es, a.dst_page = to->page_stride * es;
+  a.src_layer = from->layer_stride * es, a.dst_layer = to->layer_stride * es;
+  a.src_head = from->head_stride * es, a.dst_head = to->head_stride * es;
+  a.src_table_stride = from->table_stride, a.dst_table_stride = to->table_stride;
+  a.src_token = (int)(from->token_stride * es), a.dst_token = (int)(to->token_stride * es);
+  a.src_shift = log2i(from->page_size), a.dst_shift = log2i(to->page_size);
+  a.src_pages = from->num_pages, a.dst_pages = to->num_pages;
+  a.src_max = from->max_pages, a.dst_max = to->max_pages;
+  a.layers = from->num_layers, a.batch = from->batch, a.kv_heads = from->num_kv_heads, a.keep = keep;
+  a.row_bytes = (int)(from->head_dim * es);
+  if (from->k == to->k || from->v == to->v) {
+    if (from->table == to->table) {
+      if (from->v != to->v || from->k != to->k || a.src_page != a.dst_page || a.src_layer != a.dst_layer ||
+          a.src_head != a.dst_head || a.src_token != a.dst_token || a.src_shift != a.dst_shift ||
+          a.src_table_stride != a.dst_table_stride)
+        return invalid("in place, both descriptors must be the same");
+      return launch("compact in place", k_kv_compact_in_place, dim3((unsigned)rows, a.row_bytes / 64, 2), kMoveThreads, 0, st,
+                    dependent, 1, a);
+    }
+  }
+  const int blocks = (keep + kMoveRows - 1) / kMoveRows;
+  auto kernel = a.row_bytes == 512 ? k_kv_compact<512> : a.row_bytes == 256 ? k_kv_compact<256> : k_kv_compact<128>;
+  return launch("compact", kernel, dim3((unsigned)rows, blocks), kMoveThreads, 0, st, dependent, 1, a);
 }
 
 }  // namespace
@@ -289,57 +341,31 @@ int ocrvl_op_kv_select(int num_layers, int batch, int num_kv_heads, const float 
   if (!acc || !lens || !idx) return invalid("null argument");
   if (new_lens == lens) return invalid("new_lens must not be lens");
   SelectArgs a{acc, acc_stride, lens, batch, num_kv_heads, acc_width, keep, sinks, recent, idx, sums, new_lens};
-  // blocks a row: enough to hold the row's keys, where that is possible
   cudaStream_t st = (cudaStream_t)stream;
-  auto stage = [&](int cs) {
-    const long long n = (acc_width + cs - 1) / cs;
-    return n <= kSelStage ? (int)n * 4 : 0;
-  };
-  if (acc_width <= kSelStage) return launch_select<1>(a, (int)rows, stage(1), st);
-  if (acc_width <= 2 * kSelStage) return launch_select<2>(a, (int)rows, stage(2), st);
-  if (acc_width <= 4 * kSelStage) return launch_select<4>(a, (int)rows, stage(4), st);
-  return launch_select<8>(a, (int)rows, stage(8), st);
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  // Blocks a row: enough to hold the row's keys where that is possible, and more
+  // while they all run at once (two an SM) and have 4096 sums each.
+  int cs = 1;
+  while (cs < 8 && ((acc_width + cs - 1) / cs > kSelStage || (rows * cs * 2 <= 2 * cluster_room(sms) && acc_width / cs > 4096))) cs *= 2;
+  if (cs == 2) return launch_select<2, 512>(a, (int)rows, st);
+  if (cs == 4) return launch_select<4, 512>(a, (int)rows, st);
+  if (cs == 8) return launch_select<8, 512>(a, (int)rows, st);
+  return acc_width <= 2048 ? launch_select<1, 256>(a, (int)rows, st) : launch_select<1, 512>(a, (int)rows, st);
 }
 
 int ocrvl_op_kv_compact(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const int32_t *idx, int keep, void *stream) {
-  if (int rc = check_cache(from)) return rc;
-  if (int rc = check_cache(to)) return rc;
-  if (from->type != to->type || from->head_dim != to->head_dim || from->num_kv_heads != to->num_kv_heads ||
-      from->num_layers != to->num_layers || from->batch != to->batch)
-    return invalid("the caches must have the same type, head_dim, heads, layers and batch");
-  if (keep < 1 || keep > 0x40000000) return invalid("keep must be positive");
-  if (!idx) return invalid("null argument");
-  const long long rows = (long long)from->num_layers * from->batch * from->num_kv_heads;
-  if (rows > 1 << 24) return invalid("too many rows");
-  const long long es = elem_bytes(from->type);
-  CompactArgs a;
-  a.src_k = (const char *)from->k, a.src_v = (const char *)from->v;
-  a.dst_k = (char *)to->k, a.dst_v = (char *)to->v;
-  a.src_table = from->table, a.dst_table = to->table, a.idx = idx;
-  a.src_page = from->page_stride * es, a.dst_page = to->page_stride * es;
-  a.src_layer = from->layer_stride * es, a.dst_layer = to->layer_stride * es;
-  a.src_head = from->head_stride * es, a.dst_head = to->head_stride * es;
-  a.src_table_stride = from->table_stride, a.dst_table_stride = to->table_stride;
-  a.src_token = (int)(from->token_stride * es), a.dst_token = (int)(to->token_stride * es);
-  a.src_shift = log2i(from->page_size), a.dst_shift = log2i(to->page_size);
-  a.src_pages = from->num_pages, a.dst_pages = to->num_pages;
-  a.src_max = from->max_pages, a.dst_max = to->max_pages;
-  a.layers = from->num_layers, a.batch = from->batch, a.kv_heads = from->num_kv_heads, a.keep = keep;
-  a.row_bytes = (int)(from->head_dim * es);
-  cudaStream_t st = (cudaStream_t)stream;
-  if (from->k == to->k || from->v == to->v) {
-    if (from->table == to->table) {
-      if (from->v != to->v || from->k != to->k || a.src_page != a.dst_page || a.src_layer != a.dst_layer ||
-          a.src_head != a.dst_head || a.src_token != a.dst_token || a.src_shift != a.dst_shift ||
-          a.src_table_stride != a.dst_table_stride)
-        return invalid("in place, both descriptors must be the same");
-      return launch("compact in place", k_kv_compact_in_place, dim3((unsigned)rows, a.row_bytes / 64, 2), kMoveThreads, 0, st,
-                    false, 1, a);
-    }
-  }
-  const int blocks = (keep + kMoveRows - 1) / kMoveRows;
-  if (blocks > 65535) return invalid("keep is too large");
-  return launch("compact", k_kv_compact, dim3((unsigned)rows, blocks), kMoveThreads, 0, st, false, 1, a);
+  return compact(from, to, idx, keep, (cudaStream_t)stream, false);
+}
+
+int ocrvl_op_kv_evict(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const float *acc, int acc_width, int64_t acc_stride,
+                      const int32_t *lens, int keep, int sinks, int recent, int32_t *idx, float *sums, int32_t *new_lens,
+                      void *stream) {
+  if (int rc = check_move(from, to, idx, keep)) return rc;
+  if (int rc = ocrvl_op_kv_select(from->num_layers, from->batch, from->num_kv_heads, acc, acc_width, acc_stride, lens, keep, sinks,
+                                  recent, idx, sums, new_lens, stream))
+    return rc;
+  return compact(from, to, idx, keep, (cudaStream_t)stream, true);
 }
 
 int ocrvl_op_kv_append(const ocrvl_kv_cache *c, int n_tokens, const int32_t *lens, const int32_t *indptr, const int32_t *path,

@@ -192,25 +192,30 @@ PyObject *attention_mass(PyObject *const *a) {
   return THPVariable_Wrap(out);
 }
 
-void select_into(const Cache &c, PyObject *const *a, at::Tensor *idx, at::Tensor *sums, at::Tensor *new_lens, void *stream) {
+// The shared part of select and evict: to is NULL for select.
+PyObject *choose(const Cache &c, const ocrvl_kv_cache *to, PyObject *const *a) {
   const at::Tensor &acc = tensor(a[2], "acc");
-  const int64_t stride = c.rows(acc, "acc", true), keep = std::max(small(a[4], "keep"), 0);
+  const int64_t stride = c.rows(acc, "acc", true);
+  const int keep = small(a[4], "keep"), sinks = small(a[5], "sinks"), recent = small(a[6], "recent");
   const int32_t *lens = c.ints(a[3], "lens", c.c->batch);
-  *idx = at::empty({c.c->num_layers, c.c->batch, c.c->num_kv_heads, keep}, c.options(at::kInt));
-  *sums = at::empty({c.c->num_layers, c.c->batch, c.c->num_kv_heads, keep}, c.options(at::kFloat));
-  *new_lens = at::empty({c.c->batch}, c.options(at::kInt));
-  ok(ocrvl_op_kv_select(c.c->num_layers, c.c->batch, c.c->num_kv_heads, (const float *)acc.data_ptr(), narrow(acc.size(3), "acc"),
-                        stride, lens, small(a[4], "keep"), small(a[5], "sinks"), small(a[6], "recent"), (int32_t *)idx->data_ptr(),
-                        (float *)sums->data_ptr(), (int32_t *)new_lens->data_ptr(), stream));
+  const float *from = (const float *)acc.data_ptr();
+  const int width = narrow(acc.size(3), "acc");
+  void *stream = c.stream();
+  const int64_t shape[4] = {c.c->num_layers, c.c->batch, c.c->num_kv_heads, std::max(keep, 0)};
+  const at::Tensor idx = at::empty(shape, c.options(at::kInt)), sums = at::empty(shape, c.options(at::kFloat));
+  const at::Tensor new_lens = at::empty({c.c->batch}, c.options(at::kInt));
+  int32_t *i = (int32_t *)idx.data_ptr(), *l = (int32_t *)new_lens.data_ptr();
+  float *s = (float *)sums.data_ptr();
+  ok(to ? ocrvl_op_kv_evict(c.c, to, from, width, stride, lens, keep, sinks, recent, i, s, l, stream)
+        : ocrvl_op_kv_select(c.c->num_layers, c.c->batch, c.c->num_kv_heads, from, width, stride, lens, keep, sinks, recent, i, s, l, stream));
+  return pack({idx, sums, new_lens});
 }
 
 // (cache, device, acc, lens, keep, sinks, recent)
-PyObject *select(PyObject *const *a) {
-  const Cache c(a[0], a[1]);
-  at::Tensor idx, sums, new_lens;
-  select_into(c, a, &idx, &sums, &new_lens, c.stream());
-  return pack({idx, sums, new_lens});
-}
+PyObject *select(PyObject *const *a) { return choose(Cache(a[0], a[1]), nullptr, a); }
+
+// (cache, device, acc, lens, keep, sinks, recent, into)
+PyObject *evict(PyObject *const *a) { return choose(Cache(a[0], a[1]), Cache(a[7], a[1]).c, a); }
 
 // (cache, device, idx, into)
 PyObject *compact(PyObject *const *a) {
@@ -220,16 +225,6 @@ PyObject *compact(PyObject *const *a) {
     throw Wrong{"idx must be [layers, batch, kv heads, keep] of the cache's shape"};
   ok(ocrvl_op_kv_compact(c.c, to.c, (const int32_t *)c.flat(idx, "idx", at::kInt, idx.numel()), narrow(idx.size(3), "keep"), c.stream()));
   Py_RETURN_NONE;
-}
-
-// (cache, device, acc, lens, keep, sinks, recent, into)
-PyObject *evict(PyObject *const *a) {
-  const Cache c(a[0], a[1]), to(a[7], a[1]);
-  at::Tensor idx, sums, new_lens;
-  void *stream = c.stream();
-  select_into(c, a, &idx, &sums, &new_lens, stream);
-  ok(ocrvl_op_kv_compact(c.c, to.c, (const int32_t *)idx.data_ptr(), (int)idx.size(3), stream));
-  return pack({idx, sums, new_lens});
 }
 
 // (cache, device, k, v, lens, indptr, path, n_path)

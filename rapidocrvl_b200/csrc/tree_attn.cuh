@@ -85,9 +85,25 @@ __device__ __forceinline__ void count_cost(const TreeArgs &a, int rows, int b, i
   *all = sum;
 }
 
-// Run c of n covers the costs from run_start(c) to run_start(c + 1) and takes
-// the tiles that start there; a segment's tiles start behind its own cost.
-__device__ __forceinline__ long long run_start(long long all, int c, int n) { return all * c / n; }
+// Run c of n covers the costs from start(c) to start(c + 1) and takes the tiles
+// that start there; a segment's tiles start behind its own cost.
+struct Runs {
+  long long all, each;
+  int n, rest;  // the first `rest` runs are one longer than `each`
+
+  static __device__ long long over(long long x, long long d) {  // 32-bit division where that is enough
+    return (x | d) >> 32 ? x / d : (long long)((unsigned)x / (unsigned)d);
+  }
+  __device__ Runs(long long all_, int grid) : all(all_) {
+    n = (int)min((long long)grid, all);
+    each = n ? over(all, n) : 0, rest = n ? (int)(all - each * n) : 0;
+  }
+  __device__ long long start(int c) const { return c * each + min(c, rest); }
+  __device__ int of(long long x) const {  // the run that covers cost x
+    const long long longer = rest * (each + 1);
+    return x < longer ? (int)over(x, each + 1) : rest + (int)over(x - longer, each);
+  }
+};
 __device__ __forceinline__ int tiles_below(long long x, long long segment, int tiles) {
   const long long t = (x - segment - kSegmentCost + kTileCost - 1) / kTileCost;
   return x <= segment + kSegmentCost ? 0 : (int)min(t, (long long)tiles);
@@ -205,11 +221,11 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
     if (warp == 0) {
       long long below, all;
       count_cost(a, ROWS, 0, lane, &below, &all);
-      const int n = (int)min((long long)gridDim.x, all);
+      const Runs runs(all, gridDim.x);
       if (lane == 0) plan[0] = all, plan[1] = a.s.batch;
       __syncwarp();
-      if (blockIdx.x < n) {
-        const long long lo = run_start(all, blockIdx.x, n);
+      if (blockIdx.x < runs.n) {
+        const long long lo = runs.start(blockIdx.x);
         long long sum = 0;
         for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
           const int b = b0 + lane;
@@ -230,12 +246,11 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
     }
     pdl_launch();
     __syncthreads();
-    const long long all = plan[0];
-    const int n = (int)min((long long)gridDim.x, all);
+    const Runs runs(plan[0], gridDim.x);
     cur.b = (int)plan[1];
-    if ((int)blockIdx.x >= n || cur.b >= a.s.batch) return;
-    const long long lo = run_start(all, blockIdx.x, n);
-    hi = run_start(all, blockIdx.x + 1, n);
+    if ((int)blockIdx.x >= runs.n || cur.b >= a.s.batch) return;
+    const long long lo = runs.start(blockIdx.x);
+    hi = runs.start(blockIdx.x + 1);
     cur.sg = Segments(a, cur.b, ROWS);
     const int i = (int)((lo - plan[2]) / cur.sg.cost());
     at = plan[2] + (long long)i * cur.sg.cost();
@@ -550,10 +565,10 @@ __global__ void __launch_bounds__(kCombineWarps * 32) k_tree_combine(const TreeA
   pdl_wait();  // on every path: this grid's end is to mean the main one's too
   if (r >= sg.count * a.group) return;
   __syncthreads();
-  const long long all = plan[1], at = plan[0] + (long long)(head * sg.blocks + rb) * sg.cost();
+  const Runs runs(plan[1], main_grid);
+  const long long at = plan[0] + (long long)(head * sg.blocks + rb) * sg.cost();
   const long long tile0 = at + kSegmentCost, tile1 = tile0 + (long long)(sg.tiles - 1) * kTileCost;  // where they start
-  const int grid = (int)min((long long)main_grid, all);
-  const int first = (int)(((tile0 + 1) * grid - 1) / all), last = (int)(((tile1 + 1) * grid - 1) / all);
+  const int first = runs.of(tile0), last = runs.of(tile1);
   if (first == last) return;  // written already
   const int n = last - first + 1;
   float top = -INFINITY, l = 0.f;
@@ -563,9 +578,9 @@ __global__ void __launch_bounds__(kCombineWarps * 32) k_tree_combine(const TreeA
     const int i = j * kCombineWarps * 32 + tid, c = first + i;
     p[j] = make_float2(-INFINITY, 0.f);
     if (i < n) {
-      const long long lo = run_start(all, c, grid);
+      const long long lo = runs.start(c);
       int slot = -1;
-      if (tiles_below(lo, at, sg.tiles) < tiles_below(run_start(all, c + 1, grid), at, sg.tiles))
+      if (tiles_below(lo, at, sg.tiles) < tiles_below(runs.start(c + 1), at, sg.tiles))
         slot = 2 * c + (lo <= at - kTileCost ? 1 : 0);  // the run's first piece or, behind another segment's, its last
       if (slot >= 0) p[j] = *(const float2 *)(a.part_ml + ((long long)slot * rows_a_block + row) * 2);
       slot_sm[i] = slot;
