@@ -8,6 +8,7 @@
 #include "capi.h"
 #include "kv_move.cuh"
 #include "tree_attn.cuh"
+#include "tree_mma.cuh"
 
 using namespace ocrvl;
 using namespace ocrvl::paged;
@@ -145,8 +146,33 @@ int check_tokens(const ocrvl_kv_cache *c, int layer, int heads, int n_tokens, in
 
 // ---- tree attention ----------------------------------------------------------
 
-// Parts in the workspace: two a block of the widest grid.
-int64_t tree_work_bytes(int sms, int dim) { return (int64_t)sms * 2 * 2 * 32 * (dim + 2) * 4; }
+// 16-bit types take the fifth generation's products where a kv head has more
+// rows than one block of the other kernel's narrow forms.
+bool tree_mma(int type, int rows) { return type != OCRVL_F32 && rows > 16; }
+
+// Parts in the workspace: two a block.
+int64_t tree_work_bytes(int type, int sms, int dim, int rows) {
+  const int64_t parts = 2ll * sms * (tree_mma(type, rows) ? (rows > 128 ? 256 : 128) : 2 * 32);
+  return parts * (dim + 2) * 4;
+}
+
+template <typename T, int D, bool WIDE>
+int launch_tree_mma(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stream) {
+  using S = MmaShape<D, WIDE>;
+  const int blocks = (rows_max + S::kRows - 1) / S::kRows;
+  const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
+  if (segments > 1 << 24 || (long long)blocks * a.kv_heads > 65535) return invalid("too many sequences and kv heads");
+  // a block a segment where that is short: saves the second launch
+  const int tiles = (a.s.capacity + 64 + kChunk * kTileChunks - 1) / (kChunk * kTileChunks);
+  if (tiles <= 8)
+    return launch("tree attention", k_tree_mma<T, D, WIDE, false>, dim3((unsigned)segments), kMmaThreads, S::kSmem, stream, false, 1, a, blocks);
+  const int grid = sms < kMaxRuns ? sms : kMaxRuns;
+  a.part = (float *)work;
+  a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
+  if (int rc = launch("tree attention", k_tree_mma<T, D, WIDE, true>, dim3(grid), kMmaThreads, S::kSmem, stream, false, 1, a, blocks)) return rc;
+  return launch("tree attention (join)", k_tree_combine<T, D>, dim3(rows_max < S::kRows ? rows_max : S::kRows, blocks * a.kv_heads, a.s.batch),
+                kCombineWarps * 32, 0, stream, true, 1, a, S::kRows, grid);
+}
 
 template <typename T, int D, int NT>
 int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stream) {
@@ -179,12 +205,16 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
                 stream, true, 1, a, S::kRows, grid);
 }
 
-// Rows a block: 8 where that is all there are, 16, or 32 (the accumulators' limit).
+// Rows a block: 8 where that is all there are, 16, or 32 (the accumulators' limit; f32).
 template <typename T, int D>
 int launch_tree_rows(const TreeArgs &a, int sms, int rows_max, char *work, cudaStream_t stream) {
   if (rows_max <= 8) return launch_tree<T, D, 1>(a, sms, rows_max, work, stream);
   if (rows_max <= 16) return launch_tree<T, D, 2>(a, sms, rows_max, work, stream);
-  return launch_tree<T, D, 4>(a, sms, rows_max, work, stream);
+  if constexpr (sizeof(T) == 4)
+    return launch_tree<T, D, 4>(a, sms, rows_max, work, stream);
+  else
+    return rows_max <= 128 ? launch_tree_mma<T, D, false>(a, sms, rows_max, work, stream)
+                           : launch_tree_mma<T, D, true>(a, sms, rows_max, work, stream);
 }
 
 template <typename T>
@@ -261,10 +291,10 @@ extern "C" {
 int ocrvl_op_tree_attn_workspace(const ocrvl_kv_cache *c, int heads, int max_draft, int64_t *bytes) {
   if (!bytes) return invalid("null argument");
   if (int rc = check_cache(c)) return rc;
-  (void)heads, (void)max_draft;
+  if (heads < 1 || heads % c->num_kv_heads || max_draft < 1 || max_draft > 64) return invalid("heads must be a multiple of num_kv_heads, max_draft 1..64");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  *bytes = tree_work_bytes(sms, c->head_dim);
+  *bytes = tree_work_bytes(c->type, sms, c->head_dim, heads / c->num_kv_heads * max_draft);
   return OCRVL_OK;
 }
 
@@ -278,11 +308,12 @@ int ocrvl_op_tree_attn(const ocrvl_kv_cache *c, int layer, int heads, int n_toke
   if (!mask || !k || !v || !out || !work) return invalid("null argument");
   if (!aligned16(k) || !aligned16(v) || kv_stride * es % 16 || kv_stride < (int64_t)c->num_kv_heads * D)
     return invalid("k and v must be 16-byte aligned rows of num_kv_heads * head_dim elements");
+  if (kv_stride * es > 0x7fffffff) return invalid("kv_stride is too large");
   if (!aligned16(out) || out_stride * es % 16 || out_stride < (int64_t)heads * D)
     return invalid("out must be 16-byte aligned rows of heads * head_dim elements");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  if (!aligned16(work) || work_bytes < tree_work_bytes(sms, D)) return invalid("work is too small or not 16-byte aligned");
+  if (!aligned16(work) || work_bytes < tree_work_bytes(c->type, sms, D, heads / c->num_kv_heads * max_draft)) return invalid("work is too small or not 16-byte aligned");
   TreeArgs a;
   a.c = layer_of(c, layer);
   a.s = Seqs{lens, indptr, c->batch, n_tokens, max_draft, c->max_pages * c->page_size};

@@ -154,14 +154,15 @@ PyObject *tree_attention(PyObject *const *a) {
   const int32_t *lens = c.ints(a[5], "lens", c.c->batch), *indptr = c.ints(a[6], "indptr", c.c->batch + 1);
   const void *mask = c.flat(tensor(a[7], "mask"), "mask", at::kLong, n);
   void *stream = c.stream();
+  const int max_draft = draft_of(a[9], n);
   int64_t bytes = 0;
-  ok(ocrvl_op_tree_attn_workspace(c.c, narrow(heads, "heads"), 1, &bytes));
+  ok(ocrvl_op_tree_attn_workspace(c.c, narrow(heads, "heads"), max_draft, &bytes));
   const at::Tensor out = none(a[11]) ? at::empty({n, heads, c.c->head_dim}, c.options(c.dtype)) : tensor(a[11], "out");
   const int64_t out_stride = c.tokens(out, "out", heads);
   if (out.size(0) != n) throw Wrong{"out must have q's shape"};
   const at::Tensor lse = none(a[12]) ? at::empty({n, heads}, c.options(at::kFloat)) : tensor(a[12], "lse");
   const at::Tensor work = none(a[13]) ? at::empty({bytes}, c.options(at::kByte)) : tensor(a[13], "work");
-  ok(ocrvl_op_tree_attn(c.c, small(a[8], "layer"), narrow(heads, "heads"), narrow(n, "tokens"), draft_of(a[9], n), lens, indptr,
+  ok(ocrvl_op_tree_attn(c.c, small(a[8], "layer"), narrow(heads, "heads"), narrow(n, "tokens"), max_draft, lens, indptr,
                         (const int64_t *)mask, q.data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), kv_stride, scale_of(a[10], c),
                         out.data_ptr(), out_stride, (float *)c.flat(lse, "lse", at::kFloat, n * heads),
                         c.flat(work, "work", at::kByte, work.numel()), work.numel(), stream));

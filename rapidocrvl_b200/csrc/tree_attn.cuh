@@ -109,6 +109,81 @@ __device__ __forceinline__ int tiles_below(long long x, long long segment, int t
   return x <= segment + kSegmentCost ? 0 : (int)min(t, (long long)tiles);
 }
 
+// A part of a segment's positions: tiles t0 .. t1 - 1.
+struct Piece {
+  Segments sg;
+  int b, head, rb, t0, t1;
+};
+
+// The runs of CS = 0: finds where this block's starts (one warp searches; plan: three
+// words of shared memory), then steps through its pieces.
+struct Walk {
+  long long at, hi;  // cost at which the current segment starts; the run's end
+
+  // False where the run is empty.  Called by the whole block.
+  __device__ __forceinline__ bool start(const TreeArgs &a, int rows, long long *plan, int warp, int lane, Piece &x) {
+    if (warp == 0) {
+      long long below, all;
+      count_cost(a, rows, 0, lane, &below, &all);
+      const Runs runs(all, gridDim.x);
+      if (lane == 0) plan[0] = all, plan[1] = a.s.batch;
+      __syncwarp();
+      if (blockIdx.x < runs.n) {
+        const long long lo = runs.start(blockIdx.x);
+        long long sum = 0;
+        for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
+          const int b = b0 + lane;
+          const long long mine = b < a.s.batch ? Segments(a, b, rows).total(a.kv_heads) : 0;
+          long long upto = mine;
+          for (int d = 1; d < 32; d <<= 1) {
+            const long long y = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += y;
+          }
+          const unsigned hit = __ballot_sync(~0u, sum + upto > lo);
+          if (hit) {
+            if (lane == __ffs(hit) - 1) plan[1] = b, plan[2] = sum + upto - mine;
+            break;
+          }
+          sum += __shfl_sync(~0u, upto, 31);
+        }
+      }
+    }
+    __syncthreads();
+    const Runs runs(plan[0], gridDim.x);
+    x.b = (int)plan[1];
+    if ((int)blockIdx.x >= runs.n || x.b >= a.s.batch) return false;
+    const long long lo = runs.start(blockIdx.x);
+    hi = runs.start(blockIdx.x + 1);
+    x.sg = Segments(a, x.b, rows);
+    const int i = (int)Runs::over(lo - plan[2], x.sg.cost());
+    at = plan[2] + (long long)i * x.sg.cost();
+    x.head = i / x.sg.blocks, x.rb = i % x.sg.blocks;
+    x.t0 = tiles_below(lo, at, x.sg.tiles);
+    x.t1 = tiles_below(hi, at, x.sg.tiles);
+    return x.t0 < x.t1 || next(a, rows, x);
+  }
+  // The run's next piece that has tiles.
+  __device__ __forceinline__ bool next(const TreeArgs &a, int rows, Piece &x) {
+    while (true) {
+      at += x.sg.cost();
+      if (at >= hi) return false;
+      if (++x.rb == x.sg.blocks) {
+        x.rb = 0;
+        if (++x.head == a.kv_heads) {
+          x.head = 0;
+          do {
+            if (++x.b >= a.s.batch) return false;
+            x.sg = Segments(a, x.b, rows);
+          } while (x.sg.blocks == 0);
+        }
+      }
+      x.t0 = 0;
+      x.t1 = tiles_below(hi, at, x.sg.tiles);
+      if (x.t1 > 0) return true;
+    }
+  }
+};
+
 // Sets non-finite values to 0: in the matrix product 0 * NaN would reach rows
 // that do not see the draft they belong to.  The rows that see it get them
 // added apart.
@@ -174,11 +249,9 @@ struct TreeShape {
   static_assert(kEarly >= 1, "");
 };
 
-// A warp's part in a run of one segment's positions.
-struct Piece {
-  Segments sg;
-  int b, head, rb, t0, t1;  // tiles
-  int c0, step, nk;         // chunks c0, c0 + step, ...: nk of them
+// A warp's part of a piece.
+struct WarpPiece : Piece {
+  int c0, step, nk;  // chunks c0, c0 + step, ...: nk of them
   __device__ void chunks_of(int warp, int stride) {
     c0 = t0 * kTileChunks + warp, step = stride;
     const int end = min(t1 * kTileChunks, sg.chunks);
@@ -214,49 +287,13 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
   float *part_ml = (float *)p;  // CS > 1: [row][m, l] of this block
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-  Piece cur;
-  long long at = 0, hi = 0;  // cost at which the current segment starts; the run's end
+  WarpPiece cur;
+  Walk walk;
   bool more = true;
   if constexpr (CS == 0) {
-    if (warp == 0) {
-      long long below, all;
-      count_cost(a, ROWS, 0, lane, &below, &all);
-      const Runs runs(all, gridDim.x);
-      if (lane == 0) plan[0] = all, plan[1] = a.s.batch;
-      __syncwarp();
-      if (blockIdx.x < runs.n) {
-        const long long lo = runs.start(blockIdx.x);
-        long long sum = 0;
-        for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
-          const int b = b0 + lane;
-          const long long mine = b < a.s.batch ? Segments(a, b, ROWS).total(a.kv_heads) : 0;
-          long long upto = mine;
-          for (int d = 1; d < 32; d <<= 1) {
-            const long long x = __shfl_up_sync(~0u, upto, d);
-            if (lane >= d) upto += x;
-          }
-          const unsigned hit = __ballot_sync(~0u, sum + upto > lo);
-          if (hit) {
-            if (lane == __ffs(hit) - 1) plan[1] = b, plan[2] = sum + upto - mine;
-            break;
-          }
-          sum += __shfl_sync(~0u, upto, 31);
-        }
-      }
-    }
+    const bool any = walk.start(a, ROWS, plan, warp, lane, cur);
     pdl_launch();
-    __syncthreads();
-    const Runs runs(plan[0], gridDim.x);
-    cur.b = (int)plan[1];
-    if ((int)blockIdx.x >= runs.n || cur.b >= a.s.batch) return;
-    const long long lo = runs.start(blockIdx.x);
-    hi = runs.start(blockIdx.x + 1);
-    cur.sg = Segments(a, cur.b, ROWS);
-    const int i = (int)((lo - plan[2]) / cur.sg.cost());
-    at = plan[2] + (long long)i * cur.sg.cost();
-    cur.head = i / cur.sg.blocks, cur.rb = i % cur.sg.blocks;
-    cur.t0 = tiles_below(lo, at, cur.sg.tiles);
-    cur.t1 = tiles_below(hi, at, cur.sg.tiles);
+    if (!any) return;
     cur.chunks_of(warp, kTileChunks);
   } else {
     const int seg = blockIdx.x / CS;
@@ -266,35 +303,11 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
     cur.t0 = blockIdx.x % CS, cur.t1 = cur.sg.tiles;
     cur.chunks_of(warp, kTileChunks * CS);
   }
-  // the run's next piece that has tiles
-  auto next = [&](Piece &x) {
-    while (true) {
-      at += x.sg.cost();
-      if (at >= hi) return false;
-      if (++x.rb == x.sg.blocks) {
-        x.rb = 0;
-        if (++x.head == a.kv_heads) {
-          x.head = 0;
-          do {
-            if (++x.b >= a.s.batch) return false;
-            x.sg = Segments(a, x.b, ROWS);
-          } while (x.sg.blocks == 0);
-        }
-      }
-      x.t0 = 0;
-      x.t1 = tiles_below(hi, at, x.sg.tiles);
-      x.chunks_of(warp, kTileChunks);
-      if (x.t1 > 0) return true;
-    }
-  };
-  if (CS == 0 && cur.t0 >= cur.t1) {
-    if (!next(cur)) return;
-  }
 
   const uint32_t my_ring = smem_addr(ring) + warp * L::kBytes, q_at = smem_addr(q_sm);
   int *my_there = there + warp * NU;
   int pages = -1;  // lane i: the page of the chunk 32 j + i
-  auto issue = [&](const Piece &x, int u) {
+  auto issue = [&](const WarpPiece &x, int u) {
     if (u < 2 * x.nk) {
       const int k = u >> 1, c = x.c0 + k * x.step, slot = u % NU;
       const uint32_t to = my_ring + slot * S::kSlot;
@@ -328,7 +341,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
     copy_commit();
   };
   // the query rows of a piece and the drafts that each sees
-  auto load_query = [&](const Piece &x) {
+  auto load_query = [&](const WarpPiece &x) {
     const int rows = min(ROWS, x.sg.count * a.group - x.rb * ROWS);
     for (int n = 0; n < NT; n++)
       L::query(q_at + n * L::kQBytes, tid, kTreeThreads, [&](int r) -> const T * {
@@ -443,10 +456,11 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
       }
     }
     // the next piece's first chunks are on their way while this one is joined
-    const Piece done = cur;
+    const WarpPiece done = cur;
     if constexpr (CS == 0) {
-      more = next(cur);
+      more = walk.next(a, ROWS, cur);
       if (more) {
+        cur.chunks_of(warp, kTileChunks);
 #pragma unroll
         for (int u = 0; u < S::kEarly; u++) issue(cur, u);
       }

@@ -78,10 +78,10 @@ class PagedCache:
         self._set(d)
         return self
 
-    def work_bytes(self) -> int:
-        """Bytes of workspace a ``tree_attention`` call takes."""
+    def work_bytes(self, heads: int, max_draft: int = 64) -> int:
+        """Bytes of workspace a ``tree_attention`` call with that many query heads takes."""
         n = C.c_int64()
-        _lib.check(_lib.load().ocrvl_op_tree_attn_workspace(C.byref(self.desc), self.kv_heads, 1, C.byref(n)))
+        _lib.check(_lib.load().ocrvl_op_tree_attn_workspace(C.byref(self.desc), heads, max_draft, C.byref(n)))
         return n.value
 
 
@@ -98,7 +98,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Pag
     sequence's token j, its own included only if set (-1: all).  ``max_draft``
     bounds the tokens of a sequence (64 at most, which is the default; more
     are not computed and their outputs not written).  ``work``: a uint8 tensor
-    of ``cache.work_bytes()``, else one is taken from torch's allocator.
+    of ``cache.work_bytes(heads, max_draft)``, else one is taken from torch's allocator.
 
     Returns (out, lse): out like q, lse [tokens, heads] f32.  A token that
     attends nothing gets 0 and -inf."""
