@@ -313,7 +313,7 @@ int ocrvl_op_tree_attn(const ocrvl_kv_cache *c, int layer, int heads, int n_toke
     return invalid("out must be 16-byte aligned rows of heads * head_dim elements");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  if (!aligned16(work) || work_bytes < tree_work_bytes(c->type, sms, D, heads / c->num_kv_heads * max_draft)) return invalid("work is too small or not 16-byte aligned");
+  if (((uintptr_t)work & 127) || work_bytes < tree_work_bytes(c->type, sms, D, heads / c->num_kv_heads * max_draft)) return invalid("work is too small or not 128-byte aligned");
   TreeArgs a;
   a.c = layer_of(c, layer);
   a.s = Seqs{lens, indptr, c->batch, n_tokens, max_draft, c->max_pages * c->page_size};
@@ -324,6 +324,7 @@ int ocrvl_op_tree_attn(const ocrvl_kv_cache *c, int layer, int heads, int n_toke
   a.mask = (const long long *)mask;
   a.scale = scale * kLog2e;
   a.lse = lse;
+  a.start_cost = tree_mma(c->type, max_draft * a.group) ? 3 : 1;
   const int rows_max = max_draft * a.group;
   cudaStream_t st = (cudaStream_t)stream;
   if (c->type == OCRVL_F32) return launch_tree_dim<float>(a, D, sms, rows_max, (char *)work, st);

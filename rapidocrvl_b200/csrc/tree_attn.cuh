@@ -34,9 +34,6 @@ namespace paged {
 constexpr int kTreeWarps = 8;
 constexpr int kTreeThreads = kTreeWarps * 32;
 constexpr int kTileChunks = kTreeWarps;  // chunks a tile: one a warp
-// Cost of a tile, and of starting a segment (filling the rings, joining the
-// warps takes about as long as a tile), in the split of runs.
-constexpr int kTileCost = 1, kSegmentCost = 1;
 constexpr float kSlack = 8.f;  // p at most 256: far from f16's largest
 
 struct TreeArgs {
@@ -51,10 +48,11 @@ struct TreeArgs {
   float *lse;
   float *part;    // [2 grid][rows][D]
   float *part_ml; // [2 grid][rows][2]
+  int start_cost; // of a segment's start (filling the rings, joining the warps), in tiles, in the split of runs
 };
 
 struct Segments {  // what a sequence's segments have in common
-  int first, count, len, chunks_c, chunks, tiles, blocks;
+  int first, count, len, chunks_c, chunks, tiles, blocks, start;
 
   __device__ Segments() {}
   __device__ Segments(const TreeArgs &a, int b, int rows) {
@@ -64,8 +62,11 @@ struct Segments {  // what a sequence's segments have in common
     chunks = chunks_c + (count + kChunk - 1) / kChunk;
     tiles = (chunks + kTileChunks - 1) / kTileChunks;
     blocks = (count * a.group + rows - 1) / rows;
+    start = a.start_cost;
   }
-  __device__ int cost() const { return kSegmentCost + kTileCost * tiles; }
+  __device__ int cost() const { return start + tiles; }
+  // Its tiles that start below cost x, if the segment starts at `at`: behind its own cost.
+  __device__ int tiles_below(long long x, long long at) const { return (int)max(0ll, min(x - at - start, (long long)tiles)); }
   __device__ long long total(int kv_heads) const { return (long long)kv_heads * blocks * cost(); }
 };
 
@@ -86,7 +87,7 @@ __device__ __forceinline__ void count_cost(const TreeArgs &a, int rows, int b, i
 }
 
 // Run c of n covers the costs from start(c) to start(c + 1) and takes the tiles
-// that start there; a segment's tiles start behind its own cost.
+// that start there.
 struct Runs {
   long long all, each;
   int n, rest;  // the first `rest` runs are one longer than `each`
@@ -104,11 +105,6 @@ struct Runs {
     return x < longer ? (int)over(x, each + 1) : rest + (int)over(x - longer, each);
   }
 };
-__device__ __forceinline__ int tiles_below(long long x, long long segment, int tiles) {
-  const long long t = (x - segment - kSegmentCost + kTileCost - 1) / kTileCost;
-  return x <= segment + kSegmentCost ? 0 : (int)min(t, (long long)tiles);
-}
-
 // A part of a segment's positions: tiles t0 .. t1 - 1.
 struct Piece {
   Segments sg;
@@ -158,8 +154,8 @@ struct Walk {
     const int i = (int)Runs::over(lo - plan[2], x.sg.cost());
     at = plan[2] + (long long)i * x.sg.cost();
     x.head = i / x.sg.blocks, x.rb = i % x.sg.blocks;
-    x.t0 = tiles_below(lo, at, x.sg.tiles);
-    x.t1 = tiles_below(hi, at, x.sg.tiles);
+    x.t0 = x.sg.tiles_below(lo, at);
+    x.t1 = x.sg.tiles_below(hi, at);
     return x.t0 < x.t1 || next(a, rows, x);
   }
   // The run's next piece that has tiles.
@@ -178,7 +174,7 @@ struct Walk {
         }
       }
       x.t0 = 0;
-      x.t1 = tiles_below(hi, at, x.sg.tiles);
+      x.t1 = x.sg.tiles_below(hi, at);
       if (x.t1 > 0) return true;
     }
   }
@@ -581,7 +577,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) k_tree_combine(const TreeA
   __syncthreads();
   const Runs runs(plan[1], main_grid);
   const long long at = plan[0] + (long long)(head * sg.blocks + rb) * sg.cost();
-  const long long tile0 = at + kSegmentCost, tile1 = tile0 + (long long)(sg.tiles - 1) * kTileCost;  // where they start
+  const long long tile0 = at + sg.start, tile1 = tile0 + sg.tiles - 1;  // where they start
   const int first = runs.of(tile0), last = runs.of(tile1);
   if (first == last) return;  // written already
   const int n = last - first + 1;
@@ -594,8 +590,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32) k_tree_combine(const TreeA
     if (i < n) {
       const long long lo = runs.start(c);
       int slot = -1;
-      if (tiles_below(lo, at, sg.tiles) < tiles_below(runs.start(c + 1), at, sg.tiles))
-        slot = 2 * c + (lo <= at - kTileCost ? 1 : 0);  // the run's first piece or, behind another segment's, its last
+      if (sg.tiles_below(lo, at) < sg.tiles_below(runs.start(c + 1), at))
+        slot = 2 * c + (lo < at ? 1 : 0);  // the run's first piece or, behind another segment's, its last
       if (slot >= 0) p[j] = *(const float2 *)(a.part_ml + ((long long)slot * rows_a_block + row) * 2);
       slot_sm[i] = slot;
       top = fmaxf(top, p[j].x);

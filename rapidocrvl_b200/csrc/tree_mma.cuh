@@ -11,9 +11,9 @@
 // tensor cores busy while the other's softmax runs:
 //   WIDE    up to 256 rows: each stream has 128 of them, both take every tile
 //   narrow  up to 128 rows: both streams have them, and take tiles in turn
-// Warps 0-3 and 4-7 are the streams' softmax (a thread a row), 8 and 9 copy K, V
+// Warps 0-3 and 4-7 are the streams' softmax (a thread a row), 8 to 11 copy K, V
 // and Q (cp.async: pages of 16 positions are too small for tensor copies to
-// pay), warp 10 issues the products.  All waits are bounded: a block that
+// pay), warp 12 issues the products.  All waits are bounded: a block that
 // gives one up writes NaN.
 #pragma once
 #include "tree_attn.cuh"
@@ -21,9 +21,9 @@
 namespace ocrvl {
 namespace paged {
 
-constexpr int kCopyWarps = 2, kCopyThreads = kCopyWarps * 32;
+constexpr int kCopyWarps = 4, kCopyThreads = kCopyWarps * 32;
 constexpr int kMmaWarp = 8 + kCopyWarps;
-constexpr int kMmaThreads = (kMmaWarp + 1) * 32;  // three warps an SM quarter: 168 registers each
+constexpr int kMmaThreads = (kMmaWarp + 1) * 32;
 constexpr int kMmaWaits = 1 << 20;  // polls, of up to some microseconds each, before a wait is given up
 constexpr float kMmaSlack = 8.f;    // as kSlack
 
@@ -56,7 +56,8 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 __device__ __forceinline__ void tc_commit(uint64_t *b) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
 }
-__device__ __forceinline__ void tc_load32(uint32_t addr, uint32_t (&v)[32]) {
+// 32 columns of the warp's lanes; the values are there behind tc_load_wait.
+__device__ __forceinline__ void tc_load32_start(uint32_t addr, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -65,7 +66,36 @@ __device__ __forceinline__ void tc_load32(uint32_t addr, uint32_t (&v)[32]) {
         "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
         "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tc_load_wait(uint32_t (&v)[32]) {  // the operands tie the values' uses to the wait
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]),
+                 "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),
+                 "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28])
+               :
+               : "memory");
+  asm volatile("" : "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
+}
+__device__ __forceinline__ void tc_load32(uint32_t addr, uint32_t (&v)[32]) {
+  tc_load32_start(addr, v);
+  tc_load_wait(v);
+}
+__device__ __forceinline__ void tc_load16(uint32_t addr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_store16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
 }
 __device__ __forceinline__ void tc_store32(uint32_t addr, const uint32_t (&v)[32]) {
   asm volatile(
@@ -79,7 +109,32 @@ __device__ __forceinline__ void tc_store32(uint32_t addr, const uint32_t (&v)[32
 }
 __device__ __forceinline__ void tc_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// A whole sector of 32 bytes: rows lie in threads, so narrower stores would reach
+// L2 as halves of sectors.
+__device__ __forceinline__ void store_sector(float *p, const float *v) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ uint32_t times2(uint32_t two, float x, __half) {
+  __half2 h = __hmul2(*reinterpret_cast<__half2 *>(&two), __float2half2_rn(x));
+  return *reinterpret_cast<uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t times2(uint32_t two, float x, __nv_bfloat16) {
+  __nv_bfloat162 h = __hmul2(*reinterpret_cast<__nv_bfloat162 *>(&two), __float2bfloat162_rn(x));
+  return *reinterpret_cast<uint32_t *>(&h);
+}
+
 // ---- products -----------------------------------------------------------------
+
+// One lane of the converged warp.  Under this predicate the compiler keeps the
+// products' descriptors in uniform registers: 64 cycles a product of N = 128, the
+// tensor cores' own rate, against 80 to 88 behind a test of the lane.
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}\n" : "=r"(p));
+  return p != 0;
+}
 
 // Shared-memory matrix descriptor of rows of 128 bytes, 128-byte swizzle.
 //   K-major (Q, K: a row's 64 dims are contracted): groups of 8 rows 1 KB apart
@@ -137,7 +192,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
   p += 64;
   uint32_t *tmem_at = (uint32_t *)p;
   volatile int *dead = (volatile int *)(p + 4);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < NS; i++) {
@@ -213,62 +268,84 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
             all &= x == 16, poison |= x >> 9 & 1;
             see[c >> 1] = c & 1 ? see[c >> 1] | bits << 16 : bits & 0xffff;
           }
-          uint32_t pk[64];
-          float add, top;
-          auto pass = [&](auto masked) {
+          // 32 columns at a time, the next ones on their way meanwhile; P goes over
+          // columns of S that were read.  The reference starts as the first tile's maximum;
+          // once a score passes it by the slack it rises by a whole power of two, so
+          // what is there already is scaled exactly.
+          uint32_t v[2][32];
+          if (__any_sync(~0u, ref == -INFINITY)) {
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int q = 0; q < 4; q++) {
+              tc_load32(s_at + q * 32, v[0]);
+              const uint32_t m = q < 2 ? (q ? see[1] : see[0]) : q == 2 ? see[2] : see[3];
+#pragma unroll
+              for (int j = 0; j < 32; j++)
+                if (m >> j & 1) top = fmaxf(top, __uint_as_float(v[0][j]) * a.scale);
+            }
+            if (ref == -INFINITY) ref = top;
+          }
+          tc_load32_start(s_at, v[0]);
+          auto tile_pass = [&](auto masked) {
             constexpr bool MASKED = decltype(masked)::value;
-            const float base = ref == -INFINITY ? 0.f : ref;
-            add = 0.f, top = -INFINITY;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-              uint32_t v[32];
-              tc_load32(s_at + q * 32, v);
-              float add1 = 0.f, top1 = -INFINITY;
+              uint32_t(&x)[32] = v[q & 1];
+              tc_load_wait(x);
+              if (q < 3) tc_load32_start(s_at + (q + 1) * 32, v[(q + 1) & 1]);
+              float base = ref == -INFINITY ? 0.f : ref, top = -INFINITY, top1 = -INFINITY;
 #pragma unroll
               for (int j = 0; j < 32; j += 2) {
-                float x = fmaf(__uint_as_float(v[j]), a.scale, -base), y = fmaf(__uint_as_float(v[j + 1]), a.scale, -base);
+                float y = fmaf(__uint_as_float(x[j]), a.scale, -base), z = fmaf(__uint_as_float(x[j + 1]), a.scale, -base);
                 if (MASKED) {
-                  if (!(see[q] >> j & 1)) x = -INFINITY;
-                  if (!(see[q] >> (j + 1) & 1)) y = -INFINITY;
+                  if (!(see[q] >> j & 1)) y = -INFINITY;
+                  if (!(see[q] >> (j + 1) & 1)) z = -INFINITY;
                 }
-                top = fmaxf(top, x), top1 = fmaxf(top1, y);
-                x = exp2_(x), y = exp2_(y);
-                add += x, add1 += y;
-                pk[q * 16 + j / 2] = pack2(x, y, T());
+                top = fmaxf(top, y), top1 = fmaxf(top1, z);
+                x[j] = __float_as_uint(y), x[j + 1] = __float_as_uint(z);
               }
-              add += add1, top = fmaxf(top, top1);
+              top = fmaxf(top, top1);
+              const bool up = top > kMmaSlack;
+              float down = 0.f;
+              if (__any_sync(~0u, up)) {
+                down = up ? ceilf(top) : 0.f;
+                const float alpha = exp2_(-down);
+                ref = up ? base + down : ref;
+                sum *= alpha;
+                for (int c = 0; c < q; c++) {
+                  uint32_t w[16];
+                  tc_load16(s_at + c * 16, w);
+#pragma unroll
+                  for (int j = 0; j < 16; j++) w[j] = times2(w[j], alpha, T());
+                  tc_store16(s_at + c * 16, w);
+                }
+                if (i > 0) {  // S is there, so the products before it are done: O rests
+#pragma unroll 1
+                  for (int c = 0; c < D / 16; c++) {
+                    uint32_t w[16];
+                    tc_load16(o_at + c * 16, w);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
+                    tc_store16(o_at + c * 16, w);
+                  }
+                }
+              }
+              uint32_t p16[16];
+              float add = 0.f, add1 = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                const float y = exp2_(__uint_as_float(x[j]) - down), z = exp2_(__uint_as_float(x[j + 1]) - down);
+                add += y, add1 += z;
+                p16[j / 2] = pack2(y, z, T());
+              }
+              sum += add + add1;
+              tc_store16(s_at + q * 16, p16);
             }
           };
-          for (int again = 0;; again++) {
-            if (all)
-              pass(std::false_type());
-            else
-              pass(std::true_type());
-            // the reference follows the maximum once a score passes it by the slack, or is the first seen
-            const bool up = top > (ref == -INFINITY ? -INFINITY : kMmaSlack);
-            if (again || !__any_sync(~0u, up)) break;
-            const float now = up ? (ref == -INFINITY ? top : ref + top) : ref;
-            const float alpha = ref == now || ref == -INFINITY ? 1.f : exp2_(ref - now);
-            ref = now, sum *= alpha;
-            if (i > 0 && __any_sync(~0u, alpha != 1.f)) {  // S is there, so the products before it are done: O rests
-#pragma unroll
-              for (int q = 0; q < D / 32; q++) {
-                uint32_t v[32];
-                tc_load32(o_at + q * 32, v);
-#pragma unroll
-                for (int j = 0; j < 32; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-                tc_store32(o_at + q * 32, v);
-              }
-            }
-          }
-          sum += add;
-#pragma unroll
-          for (int q = 0; q < 2; q++) {
-            uint32_t v[32];
-#pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = pk[q * 32 + j];
-            tc_store32(s_at + q * 32, v);
-          }
+          if (all)
+            tile_pass(std::false_type());
+          else
+            tile_pass(std::true_type());
           tc_store_wait();
         }
         tc_before();
@@ -337,7 +414,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
             } else {
               float *to = a.part + (slot * S::kRows + row) * D + d0;
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) *(float4 *)(to + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+              for (int j = 0; j < 32; j += 8) store_sector(to + j, o + j);
             }
           }
         }
@@ -357,7 +434,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
     }
   } else if (warp < kMmaWarp) {
     // ---- copies -----------------------------------------------------------------
-    const int w = warp - 8, t = tid - 256;
+    const int w = warp - 8;
     constexpr int CH = kTileChunks / kCopyWarps;  // chunks of a tile that the warp copies
     constexpr int kPieces = D * 2 / 16;   // 16-byte pieces a row
     constexpr int kAtOnce = 32 / kPieces;  // rows a warp copies at once
@@ -448,11 +525,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
         if (i == 0) {  // the query rows, once the piece before has no more use for its own
           ok = __all_sync(~0u, piece == 0 || bar_wait(q_empty, (piece - 1) & 1, dead));
           if (!ok) break;
-          for (int x = t; x < S::kRows * kPieces; x += kCopyThreads) {
-            const int row = x / kPieces, c = x % kPieces, q = cur.rb * S::kRows + row;
-            const T *from = (const T *)a.q;
-            if (row < rows) from += (cur.sg.first + q / a.group) * a.q_stride + (long long)(cur.head * a.group + q % a.group) * D + c * 8;
-            copy16(smem_addr(q_sm) + (row >> 7) * S::kBlock + (c >> 3) * 16384 + (row & 127) * 128 + ((c & 7) ^ (row & 7)) * 16, from, row < rows);
+          constexpr int kMine = S::kRows / kCopyWarps;  // the warp's rows; a lane works out every 32nd's address
+#pragma unroll 1
+          for (int x0 = 0; x0 < kMine; x0 += 32) {
+            const int mine = w * kMine + x0 + lane, q = cur.rb * S::kRows + mine;
+            const char *at = (const char *)((const T *)a.q + (cur.sg.first + q / a.group) * a.q_stride + (long long)(cur.head * a.group + q % a.group) * D);
+            if (mine >= rows) at = nullptr;
+#pragma unroll 8
+            for (int x = 0; x < 32; x += kAtOnce) {
+              const char *from = of(at, x + r0);
+              const int row = w * kMine + x0 + x + r0;
+              copy16(smem_addr(q_sm) + (row >> 7) * S::kBlock + (piece16 >> 3) * 16384 + (row & 127) * 128 + ((piece16 & 7) ^ (row & 7)) * 16,
+                     from ? from + piece16 * 16 : (const char *)a.q, from != nullptr);
+            }
           }
           landed(q_full);
         }
@@ -487,16 +572,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
     }
     copy_commit();
     copy_wait<0>();
-  } else if (lane == 0) {
+  } else {
     // ---- products -----------------------------------------------------------------
-    // the copies were written like plain stores: to be seen by the products, which read
-    // by another proxy, they need a fence behind the wait for them
+    // The whole warp takes every step; one lane issues.
+    // The copies were written like plain stores: to be seen by the products, which read
+    // by another proxy, they need a fence behind the wait for them.
     auto wait_copies = [&](uint64_t *b, uint32_t parity) {
       const bool there = bar_wait(b, parity, dead);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       return there;
     };
     constexpr uint32_t i_s = mma_idesc<T>(128, false), i_o = mma_idesc<T>(D, true);
+    const uint64_t q_desc = mma_desc(smem_addr(q_sm), 16), k_desc = mma_desc(smem_addr(k_sm), 16), v_desc = mma_desc(smem_addr(v_sm), 16384);
     uint32_t p_steps[2] = {0, 0};
     bool ok = true;
     for (int piece = 0; more && ok; piece++) {
@@ -507,37 +594,46 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
       auto score = [&](int s, int i) {
         const uint32_t tile = T0 + (WIDE ? i : 2 * i + s), stage = tile % NS;
         if (!WIDE || s == 0) {
-          if (!wait_copies(&k_full[stage], tile / NS & 1)) return false;
+          if (!__all_sync(~0u, wait_copies(&k_full[stage], tile / NS & 1))) return false;
         }
         tc_after();
-        const uint32_t q = smem_addr(q_sm) + (WIDE ? s * S::kBlock : 0), k = smem_addr(k_sm) + stage * S::kBlock;
+        const uint64_t q = q_desc + (WIDE ? s * S::kBlock : 0) / 16, k = k_desc + stage * (S::kBlock / 16);
+        scored++;
+        if (elected()) {
 #pragma unroll
-        for (int h = 0; h < S::kHalves; h++)
+          for (int h = 0; h < S::kHalves; h++)
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            mma_ss(tmem + s * 128, mma_desc(q + h * 16384 + j * 32, 16), mma_desc(k + h * 16384 + j * 32, 16), i_s, h + j > 0);
-        tc_commit(&s_full[s]);
-        if (!WIDE || s == last_stream) tc_commit(&k_empty[stage]);
-        if (++scored == total) tc_commit(q_empty);
+            for (int j = 0; j < 4; j++)
+              mma_ss(tmem + s * 128, q + (h * 16384 + j * 32) / 16, k + (h * 16384 + j * 32) / 16, i_s, h + j > 0);
+          tc_commit(&s_full[s]);
+          if (!WIDE || s == last_stream) tc_commit(&k_empty[stage]);
+          if (scored == total) tc_commit(q_empty);
+        }
+        __syncwarp();
         return true;
       };
-      ok = wait_copies(q_full, piece & 1);
+      ok = __all_sync(~0u, wait_copies(q_full, piece & 1));
       for (int s = 0; s < 2 && ok; s++)
         if (n_s[s]) ok = score(s, 0);
-      if (ok && piece) ok = bar_wait(o_free, (piece - 1) & 1, dead);
+      if (ok && piece) ok = __all_sync(~0u, bar_wait(o_free, (piece - 1) & 1, dead));
       for (int i = 0; i < n_s[0] && ok; i++)
-        for (int s = 0; s < 2 && ok; s++) {
-          if (i >= n_s[s]) continue;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          if (i >= n_s[s] || !ok) continue;
           const uint32_t tile = T0 + (WIDE ? i : 2 * i + s), stage = tile % NS;
           ok = bar_wait(&p_ready[s], p_steps[s]++ & 1, dead) && wait_copies(&v_full[stage], tile / NS & 1);
-          if (!ok) break;
+          ok = __all_sync(~0u, ok);
+          if (!ok) continue;
           tc_after();
-          const uint32_t v = smem_addr(v_sm) + stage * S::kBlock;
+          const uint64_t v = v_desc + stage * (S::kBlock / 16);
+          if (elected()) {
 #pragma unroll
-          for (int j = 0; j < 8; j++)
-            mma_ts(tmem + 256 + s * 128, tmem + s * 128 + j * 8, mma_desc(v + j * 2048, 16384), i_o, i + j > 0);
-          if (!WIDE || s == last_stream) tc_commit(&v_empty[stage]);
-          if (i == n_s[s] - 1) tc_commit(&o_full[s]);
+            for (int j = 0; j < 8; j++)
+              mma_ts(tmem + 256 + s * 128, tmem + s * 128 + j * 8, v + j * 2048 / 16, i_o, i > 0 || j > 0);
+            if (!WIDE || s == last_stream) tc_commit(&v_empty[stage]);
+            if (i == n_s[s] - 1) tc_commit(&o_full[s]);
+          }
+          __syncwarp();
           if (i + 1 < n_s[s]) ok = score(s, i + 1);
         }
       T0 += n;
