@@ -25,7 +25,7 @@ constexpr int kCopyWarps = 4, kCopyThreads = kCopyWarps * 32;
 constexpr int kMmaWarp = 8 + kCopyWarps;
 constexpr int kMmaThreads = (kMmaWarp + 1) * 32;
 constexpr int kMmaWaits = 1 << 20;  // polls, of up to some microseconds each, before a wait is given up
-constexpr float kMmaSlack = 8.f;    // as kSlack
+constexpr float kMmaMost = 4096.f;   // sum of 32 weights past which the reference rises: far from f16's largest
 
 // ---- barriers and tensor memory ------------------------------------------
 
@@ -179,19 +179,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
   extern __shared__ __align__(1024) char sm_tiles[];  // the swizzle goes by address bits
   char *sm = sm_tiles;
   char *q_sm = sm, *k_sm = sm + S::kQ, *v_sm = k_sm + NS * S::kBlock;
-  char *p = sm + S::kTiles;
-  uint64_t *k_full = (uint64_t *)p, *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
+  // behind the tiles, by falling alignment
+  int *meta = (int *)(sm + S::kTiles);  // [tile % kMeta][chunk]: positions there | draft << 8 | not finite << 9 | first draft << 16
+  float2 *ml = (float2 *)(meta + S::kMeta * 8);  // [stream][row]: reference and sum
+  long long *plan = (long long *)(ml + 2 * 128);
+  uint64_t *k_full = (uint64_t *)(plan + 8), *k_empty = k_full + NS, *v_full = k_empty + NS, *v_empty = v_full + NS;
   uint64_t *s_full = v_empty + NS, *p_ready = s_full + 2, *o_full = p_ready + 2, *meta_full = o_full + 2;
   uint64_t *o_free = meta_full + S::kMeta, *q_full = o_free + 1, *q_empty = q_full + 1;
-  p = (char *)(q_empty + 1);
-  int *meta = (int *)p;  // [tile % kMeta][chunk]: positions there | draft << 8 | not finite << 9 | first draft << 16
-  p += S::kMeta * 8 * 4;
-  float2 *ml = (float2 *)p;  // [stream][row]: reference and sum
-  p += 2 * 128 * 8;
-  long long *plan = (long long *)p;
-  p += 64;
-  uint32_t *tmem_at = (uint32_t *)p;
-  volatile int *dead = (volatile int *)(p + 4);
+  uint32_t *tmem_at = (uint32_t *)(q_empty + 1);
+  volatile int *dead = (volatile int *)(tmem_at + 1);
   const int tid = threadIdx.x, warp = __shfl_sync(~0u, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
@@ -257,90 +253,110 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
         if (!ok) break;
         tc_after();
         if (works) {
-          const int *m = meta + tile % S::kMeta * 8;
-          uint32_t see[4];  // which of the 128 positions the row sees
-          bool all = true;
+          uint32_t v[2][32];
+          tc_load32_start(s_at, v[0]);
+          const int4 *m4 = (const int4 *)(meta + tile % S::kMeta * 8);
+          const int4 ma = m4[0], mb = m4[1];
+          const int m8[8] = {ma.x, ma.y, ma.z, ma.w, mb.x, mb.y, mb.z, mb.w};
+          bool all = true;  // every position is there and seen
 #pragma unroll
-          for (int c = 0; c < 8; c++) {
-            const int x = m[c];
-            uint32_t bits = (1u << (x & 31)) - 1;
-            if (x >> 8 & 1) bits &= (uint32_t)(seen >> (x >> 16));
-            all &= x == 16, poison |= x >> 9 & 1;
-            see[c >> 1] = c & 1 ? see[c >> 1] | bits << 16 : bits & 0xffff;
+          for (int c = 0; c < 8; c++) all &= m8[c] == 16;
+          uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};  // which of the 128 positions the row sees
+          if (!all) {
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+              const int x = m8[c];
+              uint32_t bits = (1u << (x & 31)) - 1;
+              if (x >> 8 & 1) bits &= (uint32_t)(seen >> (x >> 16));
+              poison |= x >> 9 & 1;
+              see[c >> 1] = c & 1 ? (see[c >> 1] & 0xffff) | bits << 16 : bits & 0xffff;
+            }
           }
           // 32 columns at a time, the next ones on their way meanwhile; P goes over
-          // columns of S that were read.  The reference starts as the first tile's maximum;
-          // once a score passes it by the slack it rises by a whole power of two, so
-          // what is there already is scaled exactly.
-          uint32_t v[2][32];
+          // columns of S that were read.  The reference starts as the first tile's maximum
+          // and rises, by a whole power of two so that what is there already is scaled
+          // exactly, only once 32 weights sum to more than kMmaMost: no maximum
+          // stands before the exponentials, which bound this loop (4 lanes a cycle
+          // and SM quarter).
           if (__any_sync(~0u, ref == -INFINITY)) {
+            tc_load_wait(v[0]);
             float top = -INFINITY;
 #pragma unroll 1
-            for (int q = 0; q < 4; q++) {
+            for (int q = 3; q >= 0; q--) {
               tc_load32(s_at + q * 32, v[0]);
               const uint32_t m = q < 2 ? (q ? see[1] : see[0]) : q == 2 ? see[2] : see[3];
 #pragma unroll
               for (int j = 0; j < 32; j++)
                 if (m >> j & 1) top = fmaxf(top, __uint_as_float(v[0][j]) * a.scale);
             }
-            if (ref == -INFINITY) ref = top;
+            if (ref == -INFINITY) ref = top;  // and v[0] holds the first columns again
           }
-          tc_load32_start(s_at, v[0]);
           auto tile_pass = [&](auto masked) {
             constexpr bool MASKED = decltype(masked)::value;
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-              uint32_t(&x)[32] = v[q & 1];
-              tc_load_wait(x);
-              if (q < 3) tc_load32_start(s_at + (q + 1) * 32, v[(q + 1) & 1]);
-              float base = ref == -INFINITY ? 0.f : ref, top = -INFINITY, top1 = -INFINITY;
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                float y = fmaf(__uint_as_float(x[j]), a.scale, -base), z = fmaf(__uint_as_float(x[j + 1]), a.scale, -base);
-                if (MASKED) {
-                  if (!(see[q] >> j & 1)) y = -INFINITY;
-                  if (!(see[q] >> (j + 1) & 1)) z = -INFINITY;
-                }
-                top = fmaxf(top, y), top1 = fmaxf(top1, z);
-                x[j] = __float_as_uint(y), x[j + 1] = __float_as_uint(z);
-              }
-              top = fmaxf(top, top1);
-              const bool up = top > kMmaSlack;
-              float down = 0.f;
-              if (__any_sync(~0u, up)) {
-                down = up ? ceilf(top) : 0.f;
-                const float alpha = exp2_(-down);
-                ref = up ? base + down : ref;
-                sum *= alpha;
-                for (int c = 0; c < q; c++) {
-                  uint32_t w[16];
-                  tc_load16(s_at + c * 16, w);
-#pragma unroll
-                  for (int j = 0; j < 16; j++) w[j] = times2(w[j], alpha, T());
-                  tc_store16(s_at + c * 16, w);
-                }
-                if (i > 0) {  // S is there, so the products before it are done: O rests
 #pragma unroll 1
-                  for (int c = 0; c < D / 16; c++) {
-                    uint32_t w[16];
+            for (int q2 = 0; q2 < 4; q2 += 2)
+#pragma unroll
+              for (int e = 0; e < 2; e++) {
+                const int q = q2 + e;
+                const uint32_t m = e ? (q2 ? see[3] : see[1]) : q2 ? see[2] : see[0];
+                uint32_t(&x)[32] = v[e];
+                tc_load_wait(x);
+                if (q < 3) tc_load32_start(s_at + (q + 1) * 32, v[e ^ 1]);
+                uint32_t p16[16];
+                float add;
+                for (bool again = false;; again = true) {
+                  const float base = ref == -INFINITY ? 0.f : ref;
+                  // the exponentials follow one another without waiting for each other's
+                  // results; what comes before and behind them goes in between
+                  float add0 = 0.f, add1 = 0.f;
+                  auto before = [&](int j) {
+                    float y = fmaf(__uint_as_float(x[j]), a.scale, -base);
+                    if (MASKED && !(m >> j & 1)) y = -INFINITY;
+                    x[j] = __float_as_uint(y);
+                  };
+                  constexpr int AHEAD = 4, BEHIND = 6;
+#pragma unroll
+                  for (int j = 0; j < AHEAD; j++) before(j);
+#pragma unroll
+                  for (int j = 0; j < 32 + BEHIND; j++) {
+                    if (j + AHEAD < 32) before(j + AHEAD);
+                    if (j < 32) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+r"(x[j]));
+                    if (j >= BEHIND && (j - BEHIND) % 2 == 1) {
+                      const int k = j - BEHIND - 1;
+                      const float y = __uint_as_float(x[k]), z = __uint_as_float(x[k + 1]);
+                      add0 += y, add1 += z;
+                      p16[k / 2] = pack2(y, z, T());
+                    }
+                  }
+                  add = add0 + add1;
+                  if (again || !__any_sync(~0u, add > kMmaMost)) break;
+                  tc_load32(s_at + q * 32, x);  // still there
+                  float top = 0.f;
+#pragma unroll
+                  for (int j = 0; j < 32; j++)
+                    if (!MASKED || m >> j & 1) top = fmaxf(top, fmaf(__uint_as_float(x[j]), a.scale, -base));
+                  const float down = add > kMmaMost ? ceilf(top) : 0.f, alpha = exp2_(-down);
+                  ref = down > 0.f ? base + down : ref;
+                  sum *= alpha;
+                  uint32_t w[16];
+#pragma unroll 1
+                  for (int c = 0; c < q; c++) {
+                    tc_load16(s_at + c * 16, w);
+#pragma unroll
+                    for (int k = 0; k < 16; k++) w[k] = times2(w[k], alpha, T());
+                    tc_store16(s_at + c * 16, w);
+                  }
+#pragma unroll 1
+                  for (int c = 0; c < (i > 0 ? D / 16 : 0); c++) {  // S is there, so the products before it are done: O rests
                     tc_load16(o_at + c * 16, w);
 #pragma unroll
-                    for (int j = 0; j < 16; j++) w[j] = __float_as_uint(__uint_as_float(w[j]) * alpha);
+                    for (int k = 0; k < 16; k++) w[k] = __float_as_uint(__uint_as_float(w[k]) * alpha);
                     tc_store16(o_at + c * 16, w);
                   }
                 }
+                sum += add;
+                tc_store16(s_at + q * 16, p16);
               }
-              uint32_t p16[16];
-              float add = 0.f, add1 = 0.f;
-#pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const float y = exp2_(__uint_as_float(x[j]) - down), z = exp2_(__uint_as_float(x[j + 1]) - down);
-                add += y, add1 += z;
-                p16[j / 2] = pack2(y, z, T());
-              }
-              sum += add + add1;
-              tc_store16(s_at + q * 16, p16);
-            }
           };
           if (all)
             tile_pass(std::false_type());
