@@ -150,10 +150,23 @@ int check_tokens(const ocrvl_kv_cache *c, int layer, int heads, int n_tokens, in
 // rows than one block of the other kernel's narrow forms.
 bool tree_mma(int type, int rows) { return type != OCRVL_F32 && rows > 16; }
 
-// Parts in the workspace: two a block.
-int64_t tree_work_bytes(int type, int sms, int dim, int rows) {
-  const int64_t parts = 2ll * sms * (tree_mma(type, rows) ? (rows > 128 ? 256 : 128) : 2 * 32);
-  return parts * (dim + 2) * 4;
+// The workspace: two parts a block, and 16 bytes a segment in front of them.
+int64_t tree_joint_bytes(int batch, int kv_heads, int rows) { return ((int64_t)batch * kv_heads * ((rows + 7) / 8) * 16 + 127) / 128 * 128; }
+int64_t tree_work_bytes(const ocrvl_kv_cache *c, int sms, int rows) {
+  const int64_t parts = 2ll * sms * (tree_mma(c->type, rows) ? (rows > 128 ? 256 : 128) : 2 * 32);
+  return tree_joint_bytes(c->batch, c->num_kv_heads, rows) + parts * (c->head_dim + 2) * 4;
+}
+
+// The join of runs' parts: eight rows a block, or fewer while the blocks would not fill
+// the GPU, down to one (then eight warps share a row's parts).
+template <typename T, int D>
+int launch_combine(const TreeArgs &a, int sms, int rows_max, int rows_a_block, cudaStream_t stream) {
+  const int blocks = (rows_max + rows_a_block - 1) / rows_a_block, rows = rows_max < rows_a_block ? rows_max : rows_a_block;
+  if ((long long)blocks * a.kv_heads > 65535) return invalid("too many kv heads");
+  int group = 8;
+  while (group > 1 && (long long)((rows + group - 1) / group) * blocks * a.kv_heads * a.s.batch < 2 * sms) group /= 2;
+  return launch("tree attention (join)", k_tree_combine<T, D>, dim3((rows + group - 1) / group, blocks * a.kv_heads, a.s.batch),
+                kCombineWarps * 32, 0, stream, true, 1, a, rows_a_block, blocks, group);
 }
 
 template <typename T, int D, bool WIDE>
@@ -161,17 +174,19 @@ int launch_tree_mma(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t 
   using S = MmaShape<D, WIDE>;
   const int blocks = (rows_max + S::kRows - 1) / S::kRows;
   const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
-  if (segments > 1 << 24 || (long long)blocks * a.kv_heads > 65535) return invalid("too many sequences and kv heads");
-  // a block a segment where that is short: saves the second launch
+  if (segments > 1 << 24) return invalid("too many sequences and kv heads");
   const int tiles = (a.s.capacity + 64 + kChunk * kTileChunks - 1) / (kChunk * kTileChunks);
-  if (tiles <= 8)
+  // A block a segment, or runs and their join, by the time each takes in tiles (1.2 us):
+  // a segment's start and end took that of 6, the same and the join in runs that of 18.
+  const long long waves = (segments + sms - 1) / sms;
+  if (waves * (tiles + 6) <= segments * tiles / sms + 18)
     return launch("tree attention", k_tree_mma<T, D, WIDE, false>, dim3((unsigned)segments), kMmaThreads, S::kSmem, stream, false, 1, a, blocks);
   const int grid = sms < kMaxRuns ? sms : kMaxRuns;
-  a.part = (float *)work;
+  a.joint = (int4 *)work;
+  a.part = (float *)(work + tree_joint_bytes(a.s.batch, a.kv_heads, rows_max));
   a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
   if (int rc = launch("tree attention", k_tree_mma<T, D, WIDE, true>, dim3(grid), kMmaThreads, S::kSmem, stream, false, 1, a, blocks)) return rc;
-  return launch("tree attention (join)", k_tree_combine<T, D>, dim3(rows_max < S::kRows ? rows_max : S::kRows, blocks * a.kv_heads, a.s.batch),
-                kCombineWarps * 32, 0, stream, true, 1, a, S::kRows, grid);
+  return launch_combine<T, D>(a, sms, rows_max, S::kRows, stream);
 }
 
 template <typename T, int D, int NT>
@@ -196,13 +211,11 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   if (tiles <= 8 * kFew && segments * 8 <= clustered) return one(k_tree_attn<T, D, NT, 8>, 8);
 
   const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
-  a.part = (float *)work;
+  a.joint = (int4 *)work;
+  a.part = (float *)(work + tree_joint_bytes(a.s.batch, a.kv_heads, rows_max));
   a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
   if (int rc = launch("tree attention", k_tree_attn<T, D, NT, 0>, dim3(grid), kTreeThreads, S::kSmem, stream, false, 1, a, blocks)) return rc;
-  if ((long long)blocks * a.kv_heads > 65535) return invalid("too many kv heads");
-  return launch("tree attention (join)", k_tree_combine<T, D>, dim3(rows_max < S::kRows ? rows_max : S::kRows, blocks * a.kv_heads, a.s.batch),
-                kCombineWarps * 32, 0,
-                stream, true, 1, a, S::kRows, grid);
+  return launch_combine<T, D>(a, sms, rows_max, S::kRows, stream);
 }
 
 // Rows a block: 8 where that is all there are, 16, or 32 (the accumulators' limit; f32).
@@ -294,7 +307,7 @@ int ocrvl_op_tree_attn_workspace(const ocrvl_kv_cache *c, int heads, int max_dra
   if (heads < 1 || heads % c->num_kv_heads || max_draft < 1 || max_draft > 64) return invalid("heads must be a multiple of num_kv_heads, max_draft 1..64");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  *bytes = tree_work_bytes(c->type, sms, c->head_dim, heads / c->num_kv_heads * max_draft);
+  *bytes = tree_work_bytes(c, sms, heads / c->num_kv_heads * max_draft);
   return OCRVL_OK;
 }
 
@@ -313,7 +326,7 @@ int ocrvl_op_tree_attn(const ocrvl_kv_cache *c, int layer, int heads, int n_toke
     return invalid("out must be 16-byte aligned rows of heads * head_dim elements");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  if (((uintptr_t)work & 127) || work_bytes < tree_work_bytes(c->type, sms, D, heads / c->num_kv_heads * max_draft)) return invalid("work is too small or not 128-byte aligned");
+  if (((uintptr_t)work & 127) || work_bytes < tree_work_bytes(c, sms, heads / c->num_kv_heads * max_draft)) return invalid("work is too small or not 128-byte aligned");
   TreeArgs a;
   a.c = layer_of(c, layer);
   a.s = Seqs{lens, indptr, c->batch, n_tokens, max_draft, c->max_pages * c->page_size};

@@ -48,6 +48,7 @@ struct TreeArgs {
   float *lse;
   float *part;    // [2 grid][rows][D]
   float *part_ml; // [2 grid][rows][2]
+  int4 *joint;    // [sequence][kv head][row block] of runs: the first part's slot (-1: the segment is whole), its run, the last run
   int start_cost; // of a segment's start (filling the rings, joining the warps), in tiles, in the split of runs
 };
 
@@ -115,6 +116,7 @@ struct Piece {
 // words of shared memory), then steps through its pieces.
 struct Walk {
   long long at, hi;  // cost at which the current segment starts; the run's end
+  long long all;
 
   // False where the run is empty.  Called by the whole block.
   __device__ __forceinline__ bool start(const TreeArgs &a, int rows, long long *plan, int warp, int lane, Piece &x) {
@@ -145,7 +147,8 @@ struct Walk {
       }
     }
     __syncthreads();
-    const Runs runs(plan[0], gridDim.x);
+    all = plan[0];
+    const Runs runs(all, gridDim.x);
     x.b = (int)plan[1];
     if ((int)blockIdx.x >= runs.n || x.b >= a.s.batch) return false;
     const long long lo = runs.start(blockIdx.x);
@@ -157,6 +160,14 @@ struct Walk {
     x.t0 = x.sg.tiles_below(lo, at);
     x.t1 = x.sg.tiles_below(hi, at);
     return x.t0 < x.t1 || next(a, rows, x);
+  }
+  // Says where the parts of a segment are, if its first one is this piece; by one thread,
+  // while the walk is at the piece.
+  __device__ __forceinline__ void tell(const TreeArgs &a, const Piece &x, int row_blocks, int slot) const {
+    if (x.t0) return;
+    const bool whole = x.t1 == x.sg.tiles;
+    const int last = whole ? 0 : Runs(all, gridDim.x).of(at + x.sg.start + x.sg.tiles - 1);
+    a.joint[((long long)x.b * a.kv_heads + x.head) * row_blocks + x.rb] = make_int4(whole ? -1 : slot, blockIdx.x, last, 0);
   }
   // The run's next piece that has tiles.
   __device__ __forceinline__ bool next(const TreeArgs &a, int rows, Piece &x) {
@@ -454,6 +465,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
     // the next piece's first chunks are on their way while this one is joined
     const WarpPiece done = cur;
     if constexpr (CS == 0) {
+      if (tid == 0) walk.tell(a, cur, row_blocks, 2 * blockIdx.x + (piece ? 1 : 0));
       more = walk.next(a, ROWS, cur);
       if (more) {
         cur.chunks_of(warp, kTileChunks);
@@ -551,100 +563,90 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
   }
 }
 
-// Joins the parts of the segments that several runs share: one block a
-// (row, segment).  All parts' maxima are read first, so the sums over the
-// parts are independent loads; eight warps take turns at the parts.
+// Joins the parts of the segments that several runs share.  A block takes
+// `group` rows of one segment, 8 / group of its warps (at least one) a row.  All
+// parts' maxima are read first, so that the sums over the parts are
+// independent loads.
 constexpr int kCombineWarps = 8;
 constexpr int kMaxRuns = 512;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kCombineWarps * 32) k_tree_combine(const TreeArgs a, int rows_a_block, int main_grid) {
+__global__ void __launch_bounds__(kCombineWarps * 32) k_tree_combine(const TreeArgs a, int rows_a_block, int row_blocks, int group) {
   __shared__ __align__(16) float o_sm[kCombineWarps][D];
-  __shared__ float f_sm[kMaxRuns], red[2][kCombineWarps];
-  __shared__ int slot_sm[kMaxRuns];  // of run first + i, or -1
-  __shared__ long long plan[2];
-  const int b = blockIdx.z, head = blockIdx.y % a.kv_heads, rb = blockIdx.y / a.kv_heads, row = blockIdx.x;
+  __shared__ float f_sm[kCombineWarps][kMaxRuns];
+  const int b = blockIdx.z, head = blockIdx.y % a.kv_heads, rb = blockIdx.y / a.kv_heads;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Segments sg(a, b, rows_a_block);
-  const int r = rb * rows_a_block + row;
-  if (warp == 0) {
-    long long below, all;
-    count_cost(a, rows_a_block, b, lane, &below, &all);
-    if (lane == 0) plan[0] = below, plan[1] = all;
-  }
+  Segments sg;
+  sg.count = a.s.tokens(b, &sg.first);
+  const int rows = min(rows_a_block, sg.count * a.group - rb * rows_a_block), row0 = blockIdx.x * group;
   pdl_wait();  // on every path: this grid's end is to mean the main one's too
-  if (r >= sg.count * a.group) return;
-  __syncthreads();
-  const Runs runs(plan[1], main_grid);
-  const long long at = plan[0] + (long long)(head * sg.blocks + rb) * sg.cost();
-  const long long tile0 = at + sg.start, tile1 = tile0 + sg.tiles - 1;  // where they start
-  const int first = runs.of(tile0), last = runs.of(tile1);
-  if (first == last) return;  // written already
-  const int n = last - first + 1;
-  float top = -INFINITY, l = 0.f;
-  float2 p[kMaxRuns / (kCombineWarps * 32)];
+  if (row0 >= rows) return;
+  const int4 where = a.joint[((long long)b * a.kv_heads + head) * row_blocks + rb];
+  if (where.x < 0) return;  // written already
+  const int n = where.z - where.y + 1;
+  // part i: the first run's piece, then each next run's first
+  auto slot_of = [&](int i) { return (long long)(i ? 2 * (where.y + i) : where.x); };
+  const int share = max(1, kCombineWarps / group);  // warps a row
+  const int mine = warp % share;
+  float *f_mine = f_sm[warp];
+  for (int r0 = 0; r0 < group; r0 += kCombineWarps / share) {
+    const int row = row0 + r0 + warp / share;
+    const bool there = r0 + warp / share < group && row < rows;
+    constexpr int V = D / 32;
+    float top = -INFINITY, l = 0.f, x[V] = {};
+    if (there) {
+      float sums[kMaxRuns / 32];  // of the parts lane, lane + 32, ...
 #pragma unroll
-  for (int j = 0; j < kMaxRuns / (kCombineWarps * 32); j++) {
-    const int i = j * kCombineWarps * 32 + tid, c = first + i;
-    p[j] = make_float2(-INFINITY, 0.f);
-    if (i < n) {
-      const long long lo = runs.start(c);
-      int slot = -1;
-      if (sg.tiles_below(lo, at) < sg.tiles_below(runs.start(c + 1), at))
-        slot = 2 * c + (lo < at ? 1 : 0);  // the run's first piece or, behind another segment's, its last
-      if (slot >= 0) p[j] = *(const float2 *)(a.part_ml + ((long long)slot * rows_a_block + row) * 2);
-      slot_sm[i] = slot;
-      top = fmaxf(top, p[j].x);
-    }
-  }
-  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-  if (lane == 0) red[0][warp] = top;
-  __syncthreads();
+      for (int j = 0; j < kMaxRuns / 32; j++) {
+        const int i = j * 32 + lane;
+        sums[j] = 0.f;
+        if (j * 32 < n && i < n) {
+          const float2 p = *(const float2 *)(a.part_ml + (slot_of(i) * rows_a_block + row) * 2);
+          sums[j] = p.y, f_mine[i] = p.x;
+          top = fmaxf(top, p.x);
+        }
+      }
+      for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+      const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-  for (int w = 0; w < kCombineWarps; w++) top = fmaxf(top, red[0][w]);
-  const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-  for (int j = 0; j < kMaxRuns / (kCombineWarps * 32); j++) {
-    const int i = j * kCombineWarps * 32 + tid;
-    if (i < n) {
-      const float f = exp2_(p[j].x - ref);
-      f_sm[i] = f;
-      l = fmaf(f, p[j].y, l);
-    }
-  }
-  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
-  if (lane == 0) red[1][warp] = l;
-  __syncthreads();
-  l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kCombineWarps; w++) l += red[1][w];
-  constexpr int V = D / 32;
-  float x[V] = {};
+      for (int j = 0; j < kMaxRuns / 32; j++) {
+        const int i = j * 32 + lane;
+        if (j * 32 < n && i < n) {
+          const float f = exp2_(f_mine[i] - ref);
+          f_mine[i] = f;
+          l = fmaf(f, sums[j], l);
+        }
+      }
+      for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(~0u, l, d);
+      __syncwarp();
 #pragma unroll 4
-  for (int i = warp; i < n; i += kCombineWarps) {
-    const int slot = slot_sm[i];
-    if (slot < 0) continue;
-    const float f = f_sm[i];
-    const float *from = a.part + ((long long)slot * rows_a_block + row) * D + lane * V;
-    float y[V];
-    if constexpr (V == 4)
-      *(float4 *)y = *(const float4 *)from;
-    else
-      *(float2 *)y = *(const float2 *)from;
+      for (int i = mine; i < n; i += share) {
+        const float f = f_mine[i];
+        const float *from = a.part + (slot_of(i) * rows_a_block + row) * D + lane * V;
+        float y[V];
+        if constexpr (V == 4)
+          *(float4 *)y = *(const float4 *)from;
+        else
+          *(float2 *)y = *(const float2 *)from;
 #pragma unroll
-    for (int j = 0; j < V; j++) x[j] = fmaf(f, y[j], x[j]);
-  }
+        for (int j = 0; j < V; j++) x[j] = fmaf(f, y[j], x[j]);
+      }
 #pragma unroll
-  for (int j = 0; j < V; j++) o_sm[warp][lane * V + j] = x[j];
-  __syncthreads();
-  if (tid < D / 4) {
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kCombineWarps; w++) {
-      const float4 z = *(const float4 *)&o_sm[w][tid * 4];
-      y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+      for (int j = 0; j < V; j++) o_sm[warp][lane * V + j] = x[j];
     }
-    write_row<T, D>(a, sg, head, r, tid * 4, y, top, l);
+    if (share > 1)
+      __syncthreads();
+    else
+      __syncwarp();
+    if (there && mine == 0 && lane < D / 4) {
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < share; w++) {
+        const float4 z = *(const float4 *)&o_sm[warp + w][lane * 4];
+        y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+      }
+      write_row<T, D>(a, sg, head, rb * rows_a_block + row, lane * 4, y, top, l);
+    }
+    __syncwarp();
   }
 }
 

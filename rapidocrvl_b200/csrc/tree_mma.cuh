@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
       tc_after();
       const bool whole = cur.t0 == 0 && cur.t1 == cur.sg.tiles;
       const long long slot = 2 * (long long)blockIdx.x + (piece ? 1 : 0);
+      if (SPLIT && tid == 0) walk.tell(a, cur, row_blocks, (int)slot);
       const int tok = cur.sg.first + first / a.group, hd = cur.head * a.group + first % a.group;
       float f0 = 1.f, f1 = 0.f, top = ref, l = sum;  // weights of this stream's and the other's O
       if constexpr (!WIDE) {
