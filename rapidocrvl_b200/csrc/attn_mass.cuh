@@ -140,13 +140,11 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
         for (int k = 0; k < NU - 1; k++) issue(k);
         const unsigned long long on = a.counted ? (unsigned long long)a.counted[b] : ~0ull;
         auto counts = [&](int r) { return r < rows && (on >> (r / a.group) & 1); };
-        for (int m = 0; m < mt; m++)
-          L::query(q_at + m * L::kQBytes, tid, kMassThreads, [&](int r) -> const T * {
-            const int x = (m0 + m) * 8 + r;
-            return counts(x) ? (const T *)a.q + (sh.first + x / a.group) * a.q_stride +
-                                   (long long)(head * a.group + x % a.group) * D
-                             : nullptr;
-          });
+        L::query(q_at, mt, tid, kMassThreads, [&](int r) -> const T * {
+          const int x = m0 * 8 + r;
+          return counts(x) ? (const T *)a.q + (sh.first + x / a.group) * a.q_stride + (long long)(head * a.group + x % a.group) * D
+                           : nullptr;
+        });
         for (int r = tid; r < mt * 8; r += kMassThreads) {
           const int x = m0 * 8 + r;
           float l = INFINITY;
@@ -158,6 +156,12 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
         }
         __syncthreads();
         uint32_t qr[THIN ? L::kTiles : 1][L::kQRegs];
+        const float keep = m0 ? 1.f : a.decay;  // further passes add to what the first wrote
+        auto sum_at = [&](int pos) {
+          if (lane >= kChunk || pos >= sh.len) return 0.f;
+          return m0 ? out[pos] : acc && pos < a.acc_width ? acc[pos] : 0.f;
+        };
+        float ahead = nk ? sum_at(c0 * kChunk + lane) : 0.f;
         float l0 = INFINITY, l1 = INFINITY;
         if constexpr (THIN) {
           if (mt > 0) {
@@ -172,15 +176,11 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
           const int valid = (int)(valids >> (8 * (k % NU))) & 31;
           valids &= ~(0xffull << (8 * (k % NU)));
           issue(k + NU - 1);
-          // what the sums were, while the products run: lane j < 16 has position j
+          // lane j < 16 has position j; what the next chunk's sums were is on its way
+          // while this one's products run
           const int pos = (c0 + k * kMassWarps) * kChunk + lane;
-          float old = 0.f;
-          if (lane < kChunk && pos < sh.len) {
-            if (m0)
-              old = out[pos];
-            else if (acc && pos < a.acc_width)
-              old = a.decay * acc[pos];
-          }
+          const float old = ahead;
+          ahead = k + 1 < nk ? sum_at(pos + kMassWarps * kChunk) : 0.f;
           const uint32_t k_at = my_ring + k % NU * L::kBytes;
           float w[2] = {0.f, 0.f};  // positions g and g + 8
           auto add = [&](const float(&s)[4], const float(&c)[2][4]) {
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kMassThreads) k_attn_mass(const MassArgs a) {
           const float w0 = __shfl_sync(~0u, w[0], (j & 7) * 4), w1 = __shfl_sync(~0u, w[1], (j & 7) * 4);
           float mine = j & 8 ? w1 : w0;
           if (j >= valid) mine = 0.f;
-          if (lane < kChunk && pos < sh.len) out[pos] = old + mine;
+          if (lane < kChunk && pos < sh.len) out[pos] = fmaf(keep, old, mine);
         }
         copy_wait<0>();
       }

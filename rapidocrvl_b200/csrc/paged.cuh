@@ -46,6 +46,9 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0)
                : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() {
@@ -162,36 +165,46 @@ struct Tile {
     constexpr int kLanes = kPieces < 32 ? kPieces : 32;  // lanes a row
     constexpr int kRows = 32 / kLanes;                   // rows at a time
     const int piece = lane % kLanes, r0 = lane / kLanes;
+    const char *from = src + r0 * row_bytes + piece * 16;
+    const long long step = kRows * row_bytes;
+    if (valid == kChunk) {
 #pragma unroll
-    for (int i = 0; i < kChunk / kRows; i++) {
-      const int row = i * kRows + r0;
-      const bool there = row < valid;
-      copy16(dst + row * kRowBytes + (V ? v_piece(row, piece) : k_piece(row, piece)) * 16,
-             src + (there ? row * row_bytes + piece * 16 : 0), there);
+      for (int i = 0; i < kChunk / kRows; i++, from += step) {
+        const int row = i * kRows + r0;
+        copy16(dst + row * kRowBytes + (V ? v_piece(row, piece) : k_piece(row, piece)) * 16, from);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kChunk / kRows; i++, from += step) {
+        const int row = i * kRows + r0;
+        copy16(dst + row * kRowBytes + (V ? v_piece(row, piece) : k_piece(row, piece)) * 16, row < valid ? from : src, row < valid);
+      }
     }
   }
 
-  // Writes the fragments of 8 query rows; row(r) gives row r's address or
-  // NULL (a zero row).  Called by a whole block of `threads`.
+  // Writes the fragments of `tiles` x 8 query rows; row(r) gives row r's address
+  // or NULL (a zero row).  Called by a whole block of `threads`.
   //   f32: per 16 dims, two float4 a lane, the high and the low parts of row
   //   g's dims 4t .. 4t+3 (the contraction takes the dims in the order that
   //   lets K be read 16 bytes at a time).
   //   16 bits: per 16 dims, two registers a lane: row g's dims 2t, 2t+1 and 2t+8, 2t+9.
   template <typename Row>
-  static __device__ __forceinline__ void query(uint32_t dst, int tid, int threads, Row row) {
+  static __device__ __forceinline__ void query(uint32_t dst, int tiles, int tid, int threads, Row row) {
     constexpr int kItems = (f32 ? D / 16 : D / 32) * 32;
-    for (int i = tid; i < kItems; i += threads) {
-      const int lane = i & 31, blk = i >> 5, g = lane >> 2, t = lane & 3;
-      const T *a = row(g);
+#pragma unroll 4
+    for (int i = tid; i < tiles * kItems; i += threads) {
+      const int lane = i & 31, blk = i / 32 % (kItems / 32), tile = i / kItems, g = lane >> 2, t = lane & 3;
+      const T *a = row(tile * 8 + g);
+      const uint32_t to = dst + tile * kQBytes + lane * 16;
       if constexpr (f32) {
         const float4 x = a ? *reinterpret_cast<const float4 *>(a + blk * 16 + t * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
         uint32_t h[4], l[4];
         split(x.x, h[0], l[0]), split(x.y, h[1], l[1]), split(x.z, h[2], l[2]), split(x.w, h[3], l[3]);
-        sts4u(dst + blk * 1024 + lane * 16, h[0], h[1], h[2], h[3]);
-        sts4u(dst + blk * 1024 + 512 + lane * 16, l[0], l[1], l[2], l[3]);
+        sts4u(to + blk * 1024, h[0], h[1], h[2], h[3]);
+        sts4u(to + blk * 1024 + 512, l[0], l[1], l[2], l[3]);
       } else {
         const uint32_t *p = reinterpret_cast<const uint32_t *>(a) + blk * 16 + t;  // pairs of dims
-        sts4u(dst + blk * 512 + lane * 16, a ? p[0] : 0u, a ? p[4] : 0u, a ? p[8] : 0u, a ? p[12] : 0u);
+        sts4u(to + blk * 512, a ? p[0] : 0u, a ? p[4] : 0u, a ? p[8] : 0u, a ? p[12] : 0u);
       }
     }
   }

@@ -350,13 +350,11 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
   // the query rows of a piece and the drafts that each sees
   auto load_query = [&](const WarpPiece &x) {
     const int rows = min(ROWS, x.sg.count * a.group - x.rb * ROWS);
-    for (int n = 0; n < NT; n++)
-      L::query(q_at + n * L::kQBytes, tid, kTreeThreads, [&](int r) -> const T * {
-        const int row = n * 8 + r, i = x.rb * ROWS + row;
-        return row < rows ? (const T *)a.q + (x.sg.first + i / a.group) * a.q_stride +
-                                (long long)(x.head * a.group + i % a.group) * D
-                          : nullptr;
-      });
+    L::query(q_at, NT, tid, kTreeThreads, [&](int row) -> const T * {
+      const int i = x.rb * ROWS + row;
+      return row < rows ? (const T *)a.q + (x.sg.first + i / a.group) * a.q_stride + (long long)(x.head * a.group + i % a.group) * D
+                        : nullptr;
+    });
     for (int r = tid; r < ROWS; r += kTreeThreads)
       seen[r] = r < rows ? (unsigned long long)a.mask[x.sg.first + (x.rb * ROWS + r) / a.group] : 0ull;
   };
