@@ -187,6 +187,13 @@ class Sequence_:
     def reset(self) -> None:
         _lib.check(self.rt._L.ocrvl_seq_reset(self._h))
 
+    def truncate(self, n: int) -> None:
+        """Drops all positions from n on (ocrvl_seq_truncate): drafts taken back,
+        or what an eviction (``kvops.evict`` on ``PagedCache.of_sequence``) left
+        over.  After an eviction give ``step`` the positions of further tokens,
+        which go on counting from the old length."""
+        _lib.check(self.rt._L.ocrvl_seq_truncate(self._h, int(n)))
+
     def close(self) -> None:
         # sequences must be released before their model (ocrvl_seq_free
         # touches the model's page pool); Runtime.close frees the live ones
