@@ -146,16 +146,15 @@ int check_tokens(const ocrvl_kv_cache *c, int layer, int heads, int n_tokens, in
 
 // ---- tree attention ----------------------------------------------------------
 
-// 16-bit types take the fifth generation's products where a kv head has more
-// rows than one block of the other kernel's narrow forms.
-bool tree_mma(int type, int rows) { return type != OCRVL_F32 && rows > 16; }
-
 // The workspace: two parts a block, and 16 bytes a segment in front of them.
 int64_t tree_joint_bytes(int batch, int kv_heads, int rows) { return ((int64_t)batch * kv_heads * ((rows + 7) / 8) * 16 + 127) / 128 * 128; }
 int64_t tree_work_bytes(const ocrvl_kv_cache *c, int sms, int rows) {
-  const int64_t parts = 2ll * sms * (tree_mma(c->type, rows) ? (rows > 128 ? 256 : 128) : 2 * 32);
+  const int64_t parts = 2ll * sms * (c->type == OCRVL_F32 || rows <= 16 ? 2 * 32 : rows > 128 ? 256 : 128);
   return tree_joint_bytes(c->batch, c->num_kv_heads, rows) + parts * (c->head_dim + 2) * 4;
 }
+
+// Tiles of the longest cache and of its drafts.
+int tree_tiles(const TreeArgs &a) { return (a.s.capacity + a.s.max_draft + kChunk - 1 + kChunk * kTileChunks - 1) / (kChunk * kTileChunks); }
 
 // The join of runs' parts: eight rows a block, or fewer while the blocks would not fill
 // the GPU, down to one (then eight warps share a row's parts).
@@ -175,13 +174,14 @@ int launch_tree_mma(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t 
   const int blocks = (rows_max + S::kRows - 1) / S::kRows;
   const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
   if (segments > 1 << 24) return invalid("too many sequences and kv heads");
-  const int tiles = (a.s.capacity + 64 + kChunk * kTileChunks - 1) / (kChunk * kTileChunks);
+  const int tiles = tree_tiles(a);
   // A block a segment, or runs and their join, by the time each takes in tiles (1.2 us):
   // a segment's start and end took that of 6, the same and the join in runs that of 18.
   const long long waves = (segments + sms - 1) / sms;
   if (waves * (tiles + 6) <= segments * tiles / sms + 18)
     return launch("tree attention", k_tree_mma<T, D, WIDE, false>, dim3((unsigned)segments), kMmaThreads, S::kSmem, stream, false, 1, a, blocks);
   const int grid = sms < kMaxRuns ? sms : kMaxRuns;
+  a.start_cost = 3;
   a.joint = (int4 *)work;
   a.part = (float *)(work + tree_joint_bytes(a.s.batch, a.kv_heads, rows_max));
   a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
@@ -198,7 +198,7 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   // A cluster a segment where a block then has at most kFew tiles of the longest cache
   // and all clusters run at once: saves the second launch.
   constexpr int kFew = 4;
-  const int tiles = (a.s.capacity + 64 + kChunk * kTileChunks - 1) / (kChunk * kTileChunks);
+  const int tiles = tree_tiles(a);
   auto one = [&](auto kernel, int cs) {
     return launch("tree attention", kernel, dim3((unsigned)(segments * cs)), kTreeThreads, S::kSmem, stream, false, cs, a, blocks);
   };
@@ -211,6 +211,7 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   if (tiles <= 8 * kFew && segments * 8 <= clustered) return one(k_tree_attn<T, D, NT, 8>, 8);
 
   const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
+  a.start_cost = 1;
   a.joint = (int4 *)work;
   a.part = (float *)(work + tree_joint_bytes(a.s.batch, a.kv_heads, rows_max));
   a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
@@ -218,11 +219,16 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   return launch_combine<T, D>(a, sms, rows_max, S::kRows, stream);
 }
 
-// Rows a block: 8 where that is all there are, 16, or 32 (the accumulators' limit; f32).
+// Rows a block.  Eight or sixteen where there are no more, or where the calls'
+// tiles are so few that the GPU is not filled otherwise: a warp's pass over
+// its chunk takes 2 us with 8 f32 rows, 7 with 32 (one sequence of 20 positions
+// and 4 drafts: 6.3 us against 8.3 with 16 and 12.4 with 32).  Else 32 for f32 (the
+// accumulators' limit), and the fifth generation's products for 16 bits.
 template <typename T, int D>
 int launch_tree_rows(const TreeArgs &a, int sms, int rows_max, char *work, cudaStream_t stream) {
-  if (rows_max <= 8) return launch_tree<T, D, 1>(a, sms, rows_max, work, stream);
-  if (rows_max <= 16) return launch_tree<T, D, 2>(a, sms, rows_max, work, stream);
+  auto few = [&](int rows) { return (long long)((rows_max + rows - 1) / rows) * a.kv_heads * a.s.batch * tree_tiles(a) * 2 <= 3 * sms; };
+  if (rows_max <= 8 || few(8)) return launch_tree<T, D, 1>(a, sms, rows_max, work, stream);
+  if (rows_max <= 16 || few(16)) return launch_tree<T, D, 2>(a, sms, rows_max, work, stream);
   if constexpr (sizeof(T) == 4)
     return launch_tree<T, D, 4>(a, sms, rows_max, work, stream);
   else
@@ -337,7 +343,6 @@ int ocrvl_op_tree_attn(const ocrvl_kv_cache *c, int layer, int heads, int n_toke
   a.mask = (const long long *)mask;
   a.scale = scale * kLog2e;
   a.lse = lse;
-  a.start_cost = tree_mma(c->type, max_draft * a.group) ? 3 : 1;
   const int rows_max = max_draft * a.group;
   cudaStream_t st = (cudaStream_t)stream;
   if (c->type == OCRVL_F32) return launch_tree_dim<float>(a, D, sms, rows_max, (char *)work, st);
