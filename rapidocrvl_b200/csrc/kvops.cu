@@ -195,20 +195,18 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   const int blocks = (rows_max + S::kRows - 1) / S::kRows;
   const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
   if (segments > 1 << 24) return invalid("too many sequences and kv heads");
-  // A cluster a segment where a block then has at most kFew tiles of the longest cache
-  // and all clusters run at once: saves the second launch.
+  // A cluster (or, for the shortest, a block) a segment where a block then has at most kFew
+  // tiles of the longest cache and all clusters run at once: saves the second launch.
   constexpr int kFew = 4;
   const int tiles = tree_tiles(a);
   auto one = [&](auto kernel, int cs) {
     return launch("tree attention", kernel, dim3((unsigned)(segments * cs)), kTreeThreads, S::kSmem, stream, false, cs, a, blocks);
   };
-  const int room = sms * S::kBlocks, clustered = cluster_room(sms) * S::kBlocks;
-  if (tiles <= kFew && (segments >= room || tiles <= 2)) return one(k_tree_attn<T, D, NT, 1>, 1);
-  if (tiles <= 4 * kFew && segments * 4 <= clustered) {
-    if (tiles > 4 && segments * 8 <= clustered) return one(k_tree_attn<T, D, NT, 8>, 8);
-    return one(k_tree_attn<T, D, NT, 4>, 4);
-  }
-  if (tiles <= 8 * kFew && segments * 8 <= clustered) return one(k_tree_attn<T, D, NT, 8>, 8);
+  const int clustered = cluster_room(sms) * S::kBlocks;
+  if (tiles > 2 && tiles <= 4 * kFew && segments * 4 <= clustered)
+    return tiles > 4 && segments * 8 <= clustered ? one(k_tree_attn<T, D, NT, 8>, 8) : one(k_tree_attn<T, D, NT, 4>, 4);
+  if (tiles > kFew && tiles <= 8 * kFew && segments * 8 <= clustered) return one(k_tree_attn<T, D, NT, 8>, 8);
+  if (tiles <= kFew) return one(k_tree_attn<T, D, NT, 1>, 1);
 
   const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
   a.start_cost = 1;
@@ -226,7 +224,8 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
 // accumulators' limit), and the fifth generation's products for 16 bits.
 template <typename T, int D>
 int launch_tree_rows(const TreeArgs &a, int sms, int rows_max, char *work, cudaStream_t stream) {
-  auto few = [&](int rows) { return (long long)((rows_max + rows - 1) / rows) * a.kv_heads * a.s.batch * tree_tiles(a) * 2 <= 3 * sms; };
+  const int room = sizeof(T) == 4 ? sms : 2 * sms;  // blocks that run at once
+  auto few = [&](int rows) { return (long long)((rows_max + rows - 1) / rows) * a.kv_heads * a.s.batch * tree_tiles(a) * 2 <= 3 * room; };
   if (rows_max <= 8 || few(8)) return launch_tree<T, D, 1>(a, sms, rows_max, work, stream);
   if (rows_max <= 16 || few(16)) return launch_tree<T, D, 2>(a, sms, rows_max, work, stream);
   if constexpr (sizeof(T) == 4)
