@@ -188,25 +188,36 @@ struct Tile {
   //   g's dims 4t .. 4t+3 (the contraction takes the dims in the order that
   //   lets K be read 16 bytes at a time).
   //   16 bits: per 16 dims, two registers a lane: row g's dims 2t, 2t+1 and 2t+8, 2t+9.
+  static constexpr int kQItems = (f32 ? D / 16 : D / 32) * 32;  // 16-byte items of 8 rows
+  // An item's value, and where it goes.
+  template <typename Row>
+  static __device__ __forceinline__ uint4 q_fetch(int i, Row row) {
+    const int blk = i / 32 % (kQItems / 32), g = (i & 31) >> 2, t = i & 3;
+    const T *a = row(i / kQItems * 8 + g);
+    if constexpr (f32) {
+      return a ? *reinterpret_cast<const uint4 *>(a + blk * 16 + t * 4) : make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      const uint32_t *p = reinterpret_cast<const uint32_t *>(a) + blk * 16 + t;  // pairs of dims
+      return a ? make_uint4(p[0], p[4], p[8], p[12]) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  static __device__ __forceinline__ void q_put(uint32_t dst, int i, uint4 x) {
+    const int blk = i / 32 % (kQItems / 32);
+    const uint32_t to = dst + i / kQItems * kQBytes + (i & 31) * 16;
+    if constexpr (f32) {
+      uint32_t h[4], l[4];
+      split(__uint_as_float(x.x), h[0], l[0]), split(__uint_as_float(x.y), h[1], l[1]);
+      split(__uint_as_float(x.z), h[2], l[2]), split(__uint_as_float(x.w), h[3], l[3]);
+      sts4u(to + blk * 1024, h[0], h[1], h[2], h[3]);
+      sts4u(to + blk * 1024 + 512, l[0], l[1], l[2], l[3]);
+    } else {
+      sts4u(to + blk * 512, x.x, x.y, x.z, x.w);
+    }
+  }
   template <typename Row>
   static __device__ __forceinline__ void query(uint32_t dst, int tiles, int tid, int threads, Row row) {
-    constexpr int kItems = (f32 ? D / 16 : D / 32) * 32;
 #pragma unroll 4
-    for (int i = tid; i < tiles * kItems; i += threads) {
-      const int lane = i & 31, blk = i / 32 % (kItems / 32), tile = i / kItems, g = lane >> 2, t = lane & 3;
-      const T *a = row(tile * 8 + g);
-      const uint32_t to = dst + tile * kQBytes + lane * 16;
-      if constexpr (f32) {
-        const float4 x = a ? *reinterpret_cast<const float4 *>(a + blk * 16 + t * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        uint32_t h[4], l[4];
-        split(x.x, h[0], l[0]), split(x.y, h[1], l[1]), split(x.z, h[2], l[2]), split(x.w, h[3], l[3]);
-        sts4u(to + blk * 1024, h[0], h[1], h[2], h[3]);
-        sts4u(to + blk * 1024 + 512, l[0], l[1], l[2], l[3]);
-      } else {
-        const uint32_t *p = reinterpret_cast<const uint32_t *>(a) + blk * 16 + t;  // pairs of dims
-        sts4u(to + blk * 512, a ? p[0] : 0u, a ? p[4] : 0u, a ? p[8] : 0u, a ? p[12] : 0u);
-      }
-    }
+    for (int i = tid; i < tiles * kQItems; i += threads) q_put(dst, i, q_fetch(i, row));
   }
   // A lane's registers of the fragments for dims 16 blk .. + 15.
   static __device__ __forceinline__ void q_load(uint32_t (&r)[kQRegs], uint32_t q, int blk, int lane) {
