@@ -8,7 +8,7 @@
 // A block takes a run of tiles of 128 positions (16 a warp) of one
 // (sequence, kv head) after another.  The fragments of 8 query rows stay in
 // registers; those of more in shared memory, as many as fit, so more yet take several
-// passes over the block's K.  Where a run has at most four chunks, two or four warps share
+// passes over the block's K (f32 only: 16-bit types have mass_mma.cuh then).  Where a run has at most four chunks, two or four warps share
 // one and its rows.  Calls of few tiles and many rows have a cluster of blocks a run, each with
 // a part of the rows; the parts' sums are added in order over distributed shared memory.
 #pragma once
@@ -51,14 +51,72 @@ struct MassShare {
     cost = load + (count * a.group + 7) / 8;
   }
   __device__ long long total(int kv_heads) const { return (long long)kv_heads * tiles * cost; }
+  // The tiles [t0, t1) of a segment whose cost starts in [lo, hi); at: the cost below
+  // it, then below the next one.
+  __device__ bool tiles_in(long long lo, long long hi, long long &at, int *t0, int *t1) const {
+    const long long from = max(lo - at, 0ll), to = hi - at;
+    *t0 = (int)min((long long)tiles, (from + cost - 1) / cost);
+    *t1 = to <= 0 ? 0 : (int)min((long long)tiles, (to + cost - 1) / cost);
+    at += (long long)tiles * cost;
+    return *t0 < *t1;
+  }
 };
+
+// Where a run's share of the cost starts: plan[0] all of it, [1] the sequence, [2] the cost below it.
+__device__ __forceinline__ void mass_start(const MassArgs &a, int load, int run, int runs, long long *plan, int lane) {
+  long long all = 0;
+  for (int b = lane; b < a.s.batch; b += 32) all += MassShare(a, b, load).total(a.kv_heads);
+  for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
+  const long long lo = all * run / runs;
+  if (lane == 0) plan[0] = all, plan[1] = a.s.batch, plan[2] = all;
+  __syncwarp();
+  long long below = 0;
+  for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
+    const long long mine = b0 + lane < a.s.batch ? MassShare(a, b0 + lane, load).total(a.kv_heads) : 0;
+    long long upto = mine;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long x = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += x;
+    }
+    const unsigned hit = __ballot_sync(~0u, below + upto > lo);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) plan[1] = b0 + lane, plan[2] = below + upto - mine;
+      break;
+    }
+    below += __shfl_sync(~0u, upto, 31);
+  }
+}
+
+// f(share, sequence, head, t0, t1) for the tiles [t0, t1) of every segment whose cost starts in
+// the run's share.
+template <typename F>
+__device__ __forceinline__ void mass_segments(const MassArgs &a, int load, int run, int runs, const long long *plan, F f) {
+  const long long lo = plan[0] * run / runs, hi = plan[0] * (run + 1) / runs;
+  long long at = plan[2];  // cost below the current segment
+  for (int b = (int)plan[1]; b < a.s.batch && at < hi; b++) {
+    const MassShare sh(a, b, load);
+    for (int head = 0; head < a.kv_heads; head++) {
+      int t0, t1;
+      if (sh.tiles_in(lo, hi, at, &t0, &t1)) f(sh, b, head, t0, t1);
+    }
+  }
+}
+
+// 0 past the lengths: each row by the blocks that share its remainder
+__device__ __forceinline__ void mass_rest(const MassArgs &a, int threads) {
+  const int all_rows = a.s.batch * a.kv_heads, share = max(1, (int)gridDim.x / all_rows);
+  for (int i = blockIdx.x; i < all_rows * share; i += gridDim.x) {
+    const int r = i % all_rows, p = i / all_rows, len = min(a.s.len(r / a.kv_heads), a.out_width);
+    for (int x = len + p * threads + threadIdx.x; x < a.out_width; x += share * threads) a.out[r * a.out_stride + x] = 0.f;
+  }
+}
 
 template <typename T, int D, bool THIN>
 struct MassShape {
   using L = Tile<T, D>;
   static constexpr int kUnits = L::kBytes >= 8192 ? (THIN ? 3 : 2) : L::kBytes >= 4096 ? 4 : 6;  // 16 positions each
   static constexpr int kRing = kMassWarps * kUnits * L::kBytes;
-  static constexpr int kItems = L::f32 ? 4 : 8;  // a thread's 16 bytes of half the rows in shared memory
+  static constexpr int kItems = 4;  // a thread's 16 bytes of half the rows in shared memory
   static constexpr int kHalf = THIN ? 1 : kItems * kMassThreads / L::kQItems;  // tiles of 8 rows
   static constexpr int kRowTiles = THIN ? 1 : 2 * kHalf;
   static constexpr int kLoad = L::f32 ? 4 : 12;
@@ -79,45 +137,18 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
   const int runs = gridDim.x / parts, run = blockIdx.x / parts, rank = blockIdx.x % parts;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane & 3;
 
-  // where this block's share of the cost starts: a sequence, the cost below it
-  if (warp == 0) {
-    long long all = 0;
-    for (int b = lane; b < a.s.batch; b += 32) all += MassShare(a, b, S::kLoad).total(a.kv_heads);
-    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(~0u, all, d);
-    const long long lo = all * run / runs;
-    if (lane == 0) plan[0] = all, plan[1] = a.s.batch, plan[2] = all;
-    __syncwarp();
-    long long below = 0;
-    for (int b0 = 0; b0 < a.s.batch; b0 += 32) {
-      const long long mine = b0 + lane < a.s.batch ? MassShare(a, b0 + lane, S::kLoad).total(a.kv_heads) : 0;
-      long long upto = mine;
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(~0u, upto, d);
-        if (lane >= d) upto += x;
-      }
-      const unsigned hit = __ballot_sync(~0u, below + upto > lo);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) plan[1] = b0 + lane, plan[2] = below + upto - mine;
-        break;
-      }
-      below += __shfl_sync(~0u, upto, 31);
-    }
-  }
+  if (warp == 0) mass_start(a, S::kLoad, run, runs, plan, lane);
   __syncthreads();
-  const long long lo = plan[0] * run / runs, hi = plan[0] * (run + 1) / runs;
 
   const uint32_t my_ring = smem_addr(ring) + warp * NU * L::kBytes, q_at = smem_addr(q_sm);
   int flip = 0;
+  const long long lo = plan[0] * run / runs, hi = plan[0] * (run + 1) / runs;
   long long at = plan[2];  // cost below the current segment
   for (int b = (int)plan[1]; b < a.s.batch && at < hi; b++) {
     const MassShare sh(a, b, S::kLoad);
     for (int head = 0; head < a.kv_heads; head++) {
-      // the tiles whose cost starts in this block's share
-      const long long from = max(lo - at, 0ll), to = hi - at;
-      const int t0 = (int)min((long long)sh.tiles, (from + sh.cost - 1) / sh.cost);
-      const int t1 = to <= 0 ? 0 : (int)min((long long)sh.tiles, (to + sh.cost - 1) / sh.cost);
-      at += (long long)sh.tiles * sh.cost;
-      if (t0 >= t1) continue;
+      int t0, t1;
+      if (!sh.tiles_in(lo, hi, at, &t0, &t1)) continue;
       // this block's rows: all, or a part of their tiles of eight
       const int all_tiles = (sh.count * a.group + 7) / 8, r0 = all_tiles * rank / parts * 8;
       const int rows = min(sh.count * a.group, all_tiles * (rank + 1) / parts * 8) - r0, row_tiles = (rows + 7) / 8;
@@ -169,8 +200,8 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
         const float l = a.lse[(long long)(sh.first + x / a.group) * a.kv_heads * a.group + head * a.group + x % a.group] * kLog2e;
         return l == -INFINITY ? INFINITY : l;  // attended nothing
       };
-      // whole groups of four tiles: rows past the last do not count
-      auto tiles_of = [&](int pass) { return max(0, min(S::kRowTiles, (row_tiles - pass * S::kRowTiles + 3) / 4 * 4)); };
+      // whole pairs of tiles: rows past the last do not count
+      auto tiles_of = [&](int pass) { return max(0, min(S::kRowTiles, (row_tiles - pass * S::kRowTiles + 1) / 2 * 2)); };
       if (!THIN || row_tiles) {
         const int tiles = THIN ? 1 : tiles_of(0);
         L::query(q_at, tiles, tid, kMassThreads, query);
@@ -195,9 +226,9 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
         w[0] += exp2_(fmaf(y[0], a.scale, -l0)) + exp2_(fmaf(y[1], a.scale, -l1));
         w[1] += exp2_(fmaf(y[2], a.scale, -l0)) + exp2_(fmaf(y[3], a.scale, -l1));
       };
-      // a chunk's K with the tiles of rows from m on (the warp's share of them, AT at once: a
+      // a chunk's K with the tiles of rows from m on (the warp's share of them, two at once: a
       // chain of products of its own takes 11.5 ns a link)
-      constexpr int AT = L::f32 ? 2 : 4;
+      constexpr int AT = 2;
       auto weigh = [&](const typename L::KFrag(&f)[THIN ? 1 : L::kTiles], int m, int tiles) {
         if constexpr (!THIN) {
           for (m += part * AT; m < tiles; m += share * AT) {
@@ -239,12 +270,12 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
             __syncwarp();
             valid = (int)(valids >> (8 * (item % NU))) & 31;
             valids &= ~(0xffull << (8 * (item % NU)));
-            issue(item + NU - 1);
-            item++;
             // lane j < 16 has position j; what the next chunk's sums were is on its way while
             // this one's products run
             old = ahead;
             ahead = alone && k + 1 < nk ? sum_at(pos + kMassWarps * kChunk) : 0.f;
+            issue(item + NU - 1);
+            item++;
             if constexpr (!THIN) {
 #pragma unroll
               for (int blk = 0; blk < L::kTiles; blk++) L::k_load(f[blk], blk, k_at, lane);
@@ -321,12 +352,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
     }
   }
   if (parts > 1) cg::this_cluster().sync();  // no block ends while another reads its sums
-  // 0 past the lengths: each row by the blocks that share its remainder
-  const int all_rows = a.s.batch * a.kv_heads, share = max(1, (int)gridDim.x / all_rows);
-  for (int i = blockIdx.x; i < all_rows * share; i += gridDim.x) {
-    const int r = i % all_rows, p = i / all_rows, len = min(a.s.len(r / a.kv_heads), a.out_width);
-    for (int x = len + p * kMassThreads + tid; x < a.out_width; x += share * kMassThreads) a.out[r * a.out_stride + x] = 0.f;
-  }
+  mass_rest(a, kMassThreads);
 }
 
 }  // namespace paged
