@@ -9,6 +9,10 @@
 // runs while the last one's weights are summed.  Warps 8 to 11 copy, warp 12 issues.  Bound
 // by the exponentials: 128 rows a tile take 1,024 cycles of an SM's 16 a cycle.  All waits are
 // bounded: what a block gave up is NaN.
+//
+// bf16, 131,072 positions, 64 drafts of 8 heads: 58 us, 590 TFLOP/s (31 us of exponentials; K is
+// read twice); 64 sequences of 4,000, one token: 31 us, 4.2 TB/s; 4 of up to 8,448, 32 drafts:
+// 12.3 us, a launch and the first loads of Q and K.
 #pragma once
 #include "attn_mass.cuh"
 #include "tree_mma.cuh"

@@ -23,6 +23,12 @@
 //   CS > 0  a cluster of CS blocks a segment, joined over distributed shared
 //           memory: one launch, no workspace, no search for the run's start.
 //           For calls whose segments and lengths are few.
+//
+// 64 sequences of up to 4,096 positions, one token, f32: 59.6 us, 4.9 TB/s of K
+// and V, bound by a warp's work on a chunk (the split into pairs of tf32 and three
+// products of each, 1.2 us); 648 positions of one sequence: 9 us, bound by a
+// launch and two loads behind one another; 8 sequences of up to 4,095 with 12 drafts: 37.5 us,
+// bound by the products of three blocks of 32 rows.
 #pragma once
 #include <cooperative_groups.h>
 

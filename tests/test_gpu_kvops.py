@@ -315,6 +315,38 @@ def test_attention_mass_narrow_sums(kvops):
     mass_check(kvops.attention_mass(s.q, lse, s.cache, s.lens, s.indptr, scale=s.scale, out=out), mass_want(s, lse, width=300))
 
 
+@pytest.mark.parametrize("dtype,dim,group", [("bf16", 128, 8), ("f16", 64, 16), ("f32", 128, 8), ("bf16", 128, 1)])
+def test_attention_mass_many_tiles(kvops, dtype, dim, group):
+    """Several tiles and segments a block, some without tokens, and more rows than a block
+    holds at a time."""
+    s = Setup(kvops, dtype, [90000, 33, 700, 12001], [3, 64, 0, 33], 2 * group, 2, dim, 32, seed=23)
+    _, lse = s.run(kvops)
+    width = s.cache.capacity
+    acc = torch.rand(4, 2, width, device="cuda")
+    got = kvops.attention_mass(s.q, lse, s.cache, s.lens, s.indptr, scale=s.scale, acc=acc, decay=0.75)
+    mass_check(got, mass_want(s, lse, None, acc, 0.75, width))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_attention_mass_many_rows_empty_nonfinite_and_unmapped(kvops, dtype):
+    """As above for many rows: tokens that attended nothing or do not count add nothing whatever
+    their queries hold, an unmapped page gets nothing, a key that is not finite reaches its own position alone."""
+    s = Setup(kvops, dtype, [300, 0, 140], [40, 12, 17], seed=24)
+    _, lse = s.run(kvops)
+    lse[5] = -math.inf
+    counted = [(1 << 40) - 1 - (1 << 7), (1 << 12) - 1, 0b1011]
+    width = s.cache.capacity
+    want = mass_want(s, lse, counted, width=width)
+    s.q[7] = math.nan
+    s.cache.table[0, 3] = -1
+    want[0, :, 48:64] = 0
+    s.cache.k[s.cache.table[2, 2], 0, 1, 5] = math.nan
+    got = kvops.attention_mass(s.q, lse, s.cache, s.lens, s.indptr, scale=s.scale, counted=masks(counted))
+    assert bool(got[2, 1, 37].isnan())
+    got[2, 1, 37] = want[2, 1, 37]
+    mass_check(got, want)
+
+
 # -- select, compact, evict ------------------------------------------------------------
 
 def select_want(row, n, keep, sinks, recent):
