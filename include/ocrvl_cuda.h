@@ -339,6 +339,8 @@ int ocrvl_seq_truncate(ocrvl_seq *s, int n);
  * statistics and the output are held in 32 bits; for the 16-bit types the
  * softmax weights are rounded to the type for the product with v.  What lies in
  * masked places (NaN and infinities too) does not reach the output.
+ * Waits within a kernel are bounded: if one ran out, the outputs that depend
+ * on it are NaN (so in ocrvl_op_attn_mass).
  * work: ocrvl_op_tree_attn_workspace bytes, 128-byte aligned; its contents
  * need no preparation and mean nothing afterwards. */
 int ocrvl_op_tree_attn_workspace(const ocrvl_kv_cache *c, int heads, int max_draft, int64_t *bytes);

@@ -392,28 +392,38 @@ struct AppendArgs {
   int layers, batch, kv_heads, n_tokens, max_path, row_bytes;
 };
 
-// A warp an item: one token of one layer, K or V, all heads.  Bound by its stores:
-// 1,241 tokens of 18 bf16 layers take 12.4 us, 3.7 TB/s read and written; 64 sequences' accepted
-// tokens 6.2 us, a launch and three loads behind one another.
+// A warp an item: K and V of one token in up to kAppendLayers layers, all heads: the
+// token's place is looked up once, and the loads of all its layers are on their way
+// before the first store (a layer, K or V an item: 12.4 us for the prompt below, bound by
+// each item's divisions and look-ups).  1,241 tokens of 18 bf16 layers: 8.3 us, 5.5 TB/s
+// read and written; 64 sequences' accepted tokens: 6.2 us, a launch and three loads
+// behind one another.
+constexpr int kAppendLayers = 3;
 __global__ void __launch_bounds__(kMoveThreads) k_kv_append(const AppendArgs a) {
   const int b = blockIdx.y, lane = threadIdx.x & 31;
   const int first = min(max(a.indptr[b], 0), a.n_tokens), count = min(max(a.indptr[b + 1], first), a.n_tokens) - first;
   const int len = min(max(a.lens[b], 0), a.capacity);
   const int n = a.path ? min(max(a.n_path[b], 0), a.max_path) : count;
   if (blockIdx.x == 0 && threadIdx.x == 0) a.new_lens[b] = min(len + n, a.capacity);
-  const int pieces = a.row_bytes / 16 * a.kv_heads;
-  const int items = n * a.layers * 2;
+  const int row_pieces = a.row_bytes / 16, pieces = row_pieces * a.kv_heads;
+  const int groups = (a.layers + kAppendLayers - 1) / kAppendLayers, items = n * groups;
   for (int it = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); it < items; it += gridDim.x * (kMoveThreads / 32)) {
-    const int v = it & 1, layer = (it >> 1) % a.layers, i = (it >> 1) / a.layers;
+    const int i = it / groups, layer0 = it % groups * kAppendLayers;
     const int node = a.path ? a.path[(long long)b * a.max_path + i] : i, pos = len + i;
     if (node < 0 || node >= count) continue;
     const long long at = row_at(a.table, a.table_stride, b, pos, a.shift, a.max_pages, a.num_pages, a.page, a.token);
     if (at < 0) continue;
-    const char *src = (v ? a.src_v : a.src_k) + layer * a.src_layer + (first + node) * a.src_token;
-    char *dst = (v ? a.v : a.k) + at + layer * a.layer;
+    const long long from = layer0 * a.src_layer + (first + node) * a.src_token, to = at + layer0 * a.layer;
     for (int p = lane; p < pieces; p += 32) {
-      const int h = p / (a.row_bytes / 16), o = p % (a.row_bytes / 16);
-      *(uint4 *)(dst + h * a.head + o * 16) = __ldg((const uint4 *)(src + (long long)p * 16));
+      const char *src_k = a.src_k + from + (long long)p * 16, *src_v = a.src_v + from + (long long)p * 16;
+      const long long dst = to + p / row_pieces * a.head + p % row_pieces * 16;
+      uint4 k[kAppendLayers], v[kAppendLayers];
+#pragma unroll
+      for (int l = 0; l < kAppendLayers; l++)
+        if (layer0 + l < a.layers) k[l] = __ldg((const uint4 *)(src_k + l * a.src_layer)), v[l] = __ldg((const uint4 *)(src_v + l * a.src_layer));
+#pragma unroll
+      for (int l = 0; l < kAppendLayers; l++)
+        if (layer0 + l < a.layers) *(uint4 *)(a.k + dst + l * a.layer) = k[l], *(uint4 *)(a.v + dst + l * a.layer) = v[l];
     }
   }
 }

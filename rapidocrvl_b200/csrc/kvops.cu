@@ -481,7 +481,7 @@ int ocrvl_op_kv_append(const ocrvl_kv_cache *c, int n_tokens, const int32_t *len
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   // a warp an item, as many blocks as the longest path can use or the GPU holds
-  const long long items = 2ll * c->num_layers * (path ? max_path : n_tokens);
+  const long long items = (c->num_layers + kAppendLayers - 1) / kAppendLayers * (long long)(path ? max_path : n_tokens);
   const long long blocks = (items + kMoveThreads / 32 - 1) / (kMoveThreads / 32), most = (sms * 16 + c->batch - 1) / c->batch;
   const unsigned gx = (unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most);
   return launch("append", k_kv_append, dim3(gx, c->batch), kMoveThreads, 0, (cudaStream_t)stream, false, 1, a);

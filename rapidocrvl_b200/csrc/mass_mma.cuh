@@ -10,7 +10,7 @@
 // by the exponentials: 128 rows a tile take 1,024 cycles of an SM's 16 a cycle.  All waits are
 // bounded: what a block gave up is NaN.
 //
-// bf16, 131,072 positions, 64 drafts of 8 heads: 58 us, 590 TFLOP/s (31 us of exponentials; K is
+// bf16, 131,072 positions, 64 drafts of 8 heads: 58 us, 590 TFLOP/s (30 us of it exponentials; K is
 // read twice); 64 sequences of 4,000, one token: 31 us, 4.2 TB/s; 4 of up to 8,448, 32 drafts:
 // 12.3 us, a launch and the first loads of Q and K.
 #pragma once

@@ -16,10 +16,11 @@
 // pay), warp 12 issues the products.  All waits are bounded: a block that
 // gives one up writes NaN.
 //
-// 131,071 positions, 64 drafts of 8 heads, bf16: 107 us, 640 TFLOP/s, bound by the
-// exponentials (16 a cycle and SM: 2,048 cycles a tile of 256 rows, of 2,400 that it
-// takes).  8 sequences of up to 8,448, 16 drafts: 29 us, 1.4 TB/s, four tiles a block and
-// half of it the start, the end and the join.
+// 131,071 positions, 64 drafts of 8 heads, bf16: 107 us, 640 TFLOP/s: tensor cores and
+// exponentials (16 a cycle and SM) are each busy for 36 % of it, bound by the chain of a stream
+// (S, its softmax by one warp an SM quarter, P, O) that the other one covers in part.
+// 8 sequences of up to 8,448, 16 drafts: 29 us, 1.4 TB/s, seven tiles a block and half of it
+// the start, the end and the join.  16 of 4,000, 64 drafts, a block a segment of 128 rows: 53 us.
 #pragma once
 #include "tree_attn.cuh"
 
