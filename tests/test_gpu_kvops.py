@@ -144,6 +144,18 @@ def test_tree_attention_many_sequences(kvops):
     s.check(*s.run(kvops))
 
 
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("lens,counts,most", [
+    ([(29 * b) % 110 for b in range(40)], [64] + [1 + b % 3 for b in range(39)], 64),  # two row blocks, more segments than SMs
+    ([(29 * b) % 700 for b in range(8)], [64, 33, 0, 1, 17, 2, 5, 40], 64),  # one wave of segments
+    ([9000, 5], [64, 3], 64),  # runs, two row blocks
+    ([7000, 12, 900], [9, 1, 16], 16),  # runs, one row block
+    ([(29 * b) % 110 for b in range(40)], [1 + b % 9 for b in range(40)], 9)])  # a wave of segments, one row block
+def test_tree_attention_shapes_of_many_rows(kvops, dtype, dim, lens, counts, most):
+    s = Setup(kvops, dtype, lens, counts, dim=dim, seed=len(lens) + most)
+    s.check(*s.run(kvops, max_draft=most))
+
+
 def test_tree_attention_second_layer_and_strides(kvops):
     s = Setup(kvops, "f32", [50, 33], [3, 9], layers=3, seed=8)
     N = s.q.shape[0]
@@ -325,6 +337,15 @@ def test_attention_mass_many_tiles(kvops, dtype, dim, group):
     acc = torch.rand(4, 2, width, device="cuda")
     got = kvops.attention_mass(s.q, lse, s.cache, s.lens, s.indptr, scale=s.scale, acc=acc, decay=0.75)
     mass_check(got, mass_want(s, lse, None, acc, 0.75, width))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_mass_one_token_many_tiles(kvops, dtype):
+    s = Setup(kvops, dtype, [70000, 0, 31], [1, 1, 1], seed=25)
+    _, lse = s.run(kvops, max_draft=1)
+    width = s.cache.capacity
+    got = kvops.attention_mass(s.q, lse, s.cache, s.lens, s.indptr, scale=s.scale, max_draft=1)
+    mass_check(got, mass_want(s, lse, width=width))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
