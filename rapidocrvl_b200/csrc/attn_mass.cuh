@@ -7,10 +7,11 @@
 //
 // A block takes a run of tiles of 128 positions (16 a warp) of one
 // (sequence, kv head) after another.  The fragments of 8 query rows stay in
-// registers; those of more in shared memory, as many as fit, so more yet take several
-// passes over the block's K (f32 only: 16-bit types have mass_mma.cuh then).  Where a run has at most four chunks, two or four warps share
-// one and its rows.  Calls of few tiles and many rows have a cluster of blocks a run, each with
-// a part of the rows; the parts' sums are added in order over distributed shared memory.
+// registers; those of more (f32 only: 16-bit types have mass_mma.cuh then) in shared
+// memory, as many as fit, so more yet take several passes over the block's K.  Where
+// a run has at most four chunks, two or four warps share one and its rows.  Calls
+// of few tiles and many rows have a cluster of blocks a run, each with a part
+// of the rows; the parts' sums are added in order over distributed shared memory.
 //
 // f32, 64 sequences of up to 4,096 positions, one token: 38.9 us, 3.8 TB/s, bound by a warp's
 // work on a chunk (its split into pairs of tf32 and the three products).  131,072 positions, 64 drafts
