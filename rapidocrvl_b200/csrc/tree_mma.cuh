@@ -121,6 +121,17 @@ __device__ __forceinline__ uint32_t times2(uint32_t two, float x, __nv_bfloat16)
   return *reinterpret_cast<uint32_t *>(&h);
 }
 
+// Meets the 256 threads of warps 0 to 7 and says whether x holds for any of them.
+__device__ __forceinline__ bool softmax_any(bool x) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbarrier.cta.red.or.pred.aligned p, 1, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(any)
+      : "r"((uint32_t)x)
+      : "memory");
+  return any != 0;
+}
+
 // ---- products -----------------------------------------------------------------
 
 // One lane of the converged warp.  Under this predicate the compiler keeps the
@@ -377,7 +388,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
       float f0 = 1.f, f1 = 0.f, top = ref, l = sum;  // weights of this stream's and the other's O
       if constexpr (!WIDE) {
         ml[s * 128 + r] = make_float2(ref, sum);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        poison = softmax_any(poison);  // a thread adds up half the dims of both streams' tiles
         const float2 x = ml[r], y = ml[128 + r];
         top = n_1 ? fmaxf(x.x, y.x) : x.x;
         const float base = top == -INFINITY ? 0.f : top;
