@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
                   }
                   add = add0 + add1;
                   if (again || !__any_sync(~0u, add > kMmaMost)) break;
+                  tc_store_wait();  // P's columns and O may have been stored a moment ago: loads are not ordered behind that
                   tc_load32(s_at + q * 32, x);  // still there
                   float top = 0.f;
 #pragma unroll

@@ -29,23 +29,25 @@ def want(s, see_cached=None):
     out, lse = torch.zeros(N, H, D, dtype=torch.float64), torch.full((N, H), -math.inf, dtype=torch.float64)
     top = torch.zeros(N, H, 1, dtype=torch.float64)
     q, k, v = (x.cpu().double() for x in (s.q, s.k, s.v))
-    mask, group = s.mask.cpu(), H // s.kv_heads
+    mask, group = s.mask.tolist(), H // s.kv_heads
     for b, t in enumerate(s.counts):
-        i0 = int(s.indptr[b])
+        if not t:
+            continue
+        at = slice(int(s.indptr[b]), int(s.indptr[b]) + t)
         ck, cv = s.rows(b)
         if see_cached is not None:
             ck, cv = ck[see_cached[b]], cv[see_cached[b]]
-        for i in range(i0, i0 + t):
-            see = [i0 + j for j in range(t) if int(mask[i]) >> j & 1]
-            if not len(ck) and not see:
-                continue
-            keys, values = torch.cat((ck, k[see])), torch.cat((cv, v[see]))  # [n, kv heads, D]
-            x = torch.einsum("ngd,ghd->ghn", keys, q[i].view(s.kv_heads, group, D)) * s.scale
-            lse[i] = torch.logsumexp(x, -1).view(H)
-            w = torch.softmax(x, -1)
-            o = torch.einsum("ghn,ngd->ghd", w, values)
-            out[i] = o.reshape(H, D)
-            top[i] = values.abs().amax((0, 2)).repeat_interleave(group)[:, None]
+        n = len(ck)
+        keys, values = torch.cat((ck, k[at])), torch.cat((cv, v[at]))
+        see = torch.ones(t, n + t, dtype=torch.bool)
+        see[:, n:] = torch.tensor([[bool(m >> j & 1) for j in range(t)] for m in mask[at]])
+        for h in range(H):
+            g = h // group
+            x = (q[at, h] @ keys[:, g].T * s.scale).masked_fill(~see, -math.inf)
+            lse[at, h] = torch.logsumexp(x, 1)
+            w = torch.where(see.any(1)[:, None], torch.softmax(x, 1), torch.zeros_like(x))
+            out[at, h] = w @ values[:, g]
+            top[at, h, 0] = torch.where(see, values[:, g].abs().amax(1)[None], torch.zeros(())).amax(1)
     return out, lse, top
 
 
@@ -97,3 +99,62 @@ def want_nonfinite(s):
             if int(s.mask[j]) >> (i - i0) & 1:
                 out[j, g * group:(g + 1) * group, d] += float(v[i, g, d])
     return out, lse, top
+
+
+# -- the reference's rise, rows and pages with nothing in them --------------------------
+
+# As MANY_ROWS, with several tiles a group of warps.
+MANY_TILES = {
+    "narrow, runs": ([40000, 300], [16, 5], 16),
+    "narrow, whole": ([(137 * b) % 1000 for b in range(40)], [16, 11] + [1 + b % 3 for b in range(38)], 16),
+    "wide, runs": ([20000, 4130], [64, 3], 64),
+    "wide, whole": ([(137 * b) % 1000 for b in range(37)], [64, 40] + [b % 3 for b in range(35)], 64),
+    "few rows": ([2000, 40], [2, 1], 2),
+}
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("f32", 128)])
+@pytest.mark.parametrize("shape", MANY_TILES)
+def test_scores_that_rise_along_the_context(kvops, shape, dtype, dim):
+    """Some rows' scores rise by 16 powers of two every 32 positions of some tiles and by 100 at once
+    further on, others fall alike.  A score of size x is off by its sum's roundings, at most one of 2^-23 for each
+    of eight products of 16 dims: x 2^-20 of a weight."""
+    lens, counts, most = MANY_TILES[shape]
+    s = Setup(kvops, dtype, lens, counts, dim=dim, seed=71)
+    per = 4 * s.scale / math.log(2)  # powers of two a unit of dim 0, whose queries are 4 and -4
+    s.q[:, ::2, 0], s.q[:, 1::2, 0] = 4, -4
+    for b, n in enumerate(lens):
+        t = torch.arange(n)
+        steps = torch.cumsum((t % 32 == 0) & (t // 128 % 7 % 3 == 1) & (t < 2300), 0).clamp(max=12) * 16 + (t >= 700) * 100
+        pages = s.table_h[b, t // s.page].long().cuda()
+        for g in range(2):
+            s.pool[pages, 0, g, 0, (t % s.page).cuda(), 0] = (steps / per).to(s.dtype).cuda()
+    w = want(s)
+    check(s, s.run(kvops, max_draft=most), w, extra=2.0 ** -20 * float(w[1][torch.isfinite(w[1])].abs().max()))
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("shape", MANY_TILES)
+def test_many_rows_with_unmapped_pages_and_nothing_to_see(kvops, shape, dtype, dim):
+    lens, counts, most = MANY_TILES[shape]
+    s = Setup(kvops, dtype, lens, counts, dim=dim, seed=72)
+    table, starts = s.table_h.clone(), s.indptr.tolist()
+    mapped = [torch.ones(n, dtype=torch.bool) for n in lens]
+
+    def unmap(b, page, entry):
+        table[b, page] = entry
+        mapped[b][page * 16:(page + 1) * 16] = False
+
+    for page in list(range(17)) + [20, 23, 40, 55]:  # whole tiles at the start, then single pages
+        if page * 16 < lens[0]:
+            unmap(0, page, -1 if page % 2 else 1 << 30)
+    for page in range(-(-lens[1] // 16)):  # the second sequence has nothing cached
+        unmap(1, page, table.shape[0] * 10000 if page % 3 else -5)
+    bits = s.mask.tolist()
+    for i in range(starts[1], starts[2], 2):  # and half of its tokens do not see themselves either
+        bits[i] = 0
+    for i in range(starts[0], starts[1], 3):
+        bits[i] = 0
+    s.mask = masks(bits)
+    s.cache = kvops.PagedCache(s.pool[:, :, :, 0], s.pool[:, :, :, 1], table.cuda())
+    check(s, s.run(kvops, max_draft=most), want(s, see_cached=mapped))
