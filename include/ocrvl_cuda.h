@@ -314,8 +314,11 @@ typedef struct ocrvl_kv_cache {
 
 /* The cache of an engine sequence as a descriptor of one table row: every
  * layer, pages of 16 positions, f32.  The table holds the pages of the
- * positions the sequence has (ocrvl_seq_len); order work on it against the
- * model's stream. */
+ * positions the sequence has (ocrvl_seq_len), as it grows and shrinks; what is
+ * past them is unmapped.  Order work on it against the model's stream.  For the
+ * operators that read the cache and for an eviction in place: a sequence
+ * grows by ocrvl_step and the loops alone (an append through the view gets no
+ * pages, and the sequence's length does not follow it). */
 int ocrvl_seq_kv_view(ocrvl_seq *s, ocrvl_kv_cache *out);
 
 /* Drops all positions from n on (0 <= n <= length), as after an in-place

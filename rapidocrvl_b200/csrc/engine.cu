@@ -1229,18 +1229,38 @@ int ocrvl_seq_create(ocrvl_model *m, int max_tokens, ocrvl_seq **out) {
     delete s;
     return fail(OCRVL_E_NOMEM, "block table allocation failed");
   }
-  cudaMemset(s->bt_d, 0, (size_t)np * 4);
+  // -1: a position that has no page (the step kernels read the entries of positions 0..len alone)
+  cudaError_t e = cudaMemsetAsync(s->bt_d, 0xff, (size_t)np * 4, m->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(m->stream);
+  if (e != cudaSuccess) {
+    cudaFree(s->bt_d);
+    delete s;
+    return fail(OCRVL_E_CUDA, std::string("block table: ") + cudaGetErrorString(e));
+  }
   *out = s;
+  return OCRVL_OK;
+}
+
+// Gives a sequence's pages from `keep` on back to the pool and unmaps them in
+// its table, which the paged-cache operators read too: a page that was
+// returned may be another sequence's next.  Model lock held.
+static int drop_pages(ocrvl_seq *s, size_t keep) {
+  ocrvl_model *m = s->m;
+  const size_t had = s->pages.size();
+  if (had <= keep) return OCRVL_OK;
+  m->free_pages.insert(m->free_pages.end(), s->pages.begin() + keep, s->pages.end());
+  s->pages.resize(keep);
+  if (int rc = set_device(m)) return rc;
+  CK(cudaMemsetAsync(s->bt_d + keep, 0xff, (had - keep) * 4, m->stream));
+  CK(cudaStreamSynchronize(m->stream));
   return OCRVL_OK;
 }
 
 int ocrvl_seq_reset(ocrvl_seq *s) {
   if (!s) return fail(OCRVL_E_INVALID, "null seq");
   std::lock_guard<std::mutex> lk(s->m->mu);
-  for (int p : s->pages) s->m->free_pages.push_back(p);
-  s->pages.clear();
   s->len = 0;
-  return OCRVL_OK;
+  return drop_pages(s, 0);
 }
 
 void ocrvl_seq_free(ocrvl_seq *s) {
@@ -1285,13 +1305,8 @@ int ocrvl_seq_truncate(ocrvl_seq *s, int n) {
   ocrvl_model *m = s->m;
   std::lock_guard<std::mutex> lk(m->mu);
   if (n < 0 || n > s->len) return fail(OCRVL_E_INVALID, "n outside 0..length");
-  const size_t keep = (size_t)(n + kPageTokens - 1) / kPageTokens;
-  while (s->pages.size() > keep) {
-    m->free_pages.push_back(s->pages.back());
-    s->pages.pop_back();
-  }
   s->len = n;
-  return OCRVL_OK;
+  return drop_pages(s, (size_t)(n + kPageTokens - 1) / kPageTokens);
 }
 
 int ocrvl_seq_import_kv(ocrvl_seq *s, int n, const float *k, const float *v) {
@@ -1326,16 +1341,14 @@ int ocrvl_seq_import_kv(ocrvl_seq *s, int n, const float *k, const float *v) {
     cudaError_t e = cudaMemcpy(m->kv_pool + (size_t)ids[p] * m->page_floats, page.data(), page.size() * 4,
                                cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
-      for (int q : s->pages) m->free_pages.push_back(q);
-      s->pages.clear();
+      drop_pages(s, 0);
       return fail(OCRVL_E_CUDA, std::string("cudaMemcpy: ") + cudaGetErrorString(e));
     }
   }
   if (np > 0) {
     cudaError_t e = cudaMemcpy(s->bt_d, ids.data(), (size_t)np * 4, cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
-      for (int q : s->pages) m->free_pages.push_back(q);
-      s->pages.clear();
+      drop_pages(s, 0);
       return fail(OCRVL_E_CUDA, std::string("cudaMemcpy: ") + cudaGetErrorString(e));
     }
   }
@@ -1365,8 +1378,7 @@ int ocrvl_seq_fill_synthetic(ocrvl_seq *s, int n, uint64_t seed) {
     s->pages.push_back(ids[p]);
   }
   auto undo = [&](cudaError_t e) {
-    for (int q : s->pages) m->free_pages.push_back(q);
-    s->pages.clear();
+    drop_pages(s, 0);
     return fail(OCRVL_E_CUDA, std::string("fill: ") + cudaGetErrorString(e));
   };
   cudaError_t e = cudaMemcpy(s->bt_d, ids.data(), (size_t)np * 4, cudaMemcpyHostToDevice);
