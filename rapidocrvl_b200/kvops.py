@@ -37,8 +37,8 @@ class PagedCache:
     """A paged cache: ``k`` and ``v`` are [pages, layers, kv heads, page_size,
     head_dim] tensors of the same type and strides (views of one pool, for
     instance) and ``table`` [batch, max_pages] int32 names the pages of each
-    sequence in order, an entry outside 0..pages-1 none.  Page sizes are powers
-    of two from 16 on, head_dim is 64 or 128."""
+    sequence in order, an entry outside 0..pages-1 none; its rows may lie apart, but not
+    share memory.  Page sizes are powers of two from 16 on, head_dim is 64 or 128."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor):
         if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.dtype is not v.dtype:
@@ -49,11 +49,13 @@ class PagedCache:
             raise ValueError("head_dim must be contiguous")
         if table.dim() != 2 or table.dtype is not torch.int32 or table.device != k.device or table.stride(1) != 1:
             raise ValueError(f"table must be a [batch, max_pages] int32 tensor on {k.device}")
+        if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+            raise ValueError("the table's rows must not overlap (an expanded row needs a copy: .contiguous())")
         self.k, self.v, self.table = k, v, table
         self.dtype, self.device = k.dtype, k.device
         pages, layers, heads, page, dim = k.shape
         d = _lib.KVCache(_TYPES[k.dtype], dim, heads, layers, page, pages, table.shape[0], table.shape[1], k.stride(0),
-                         k.stride(1), k.stride(2), k.stride(3), max(table.stride(0), table.shape[1]), k.data_ptr(),
+                         k.stride(1), k.stride(2), k.stride(3), table.stride(0) if table.shape[0] > 1 else table.shape[1], k.data_ptr(),
                          v.data_ptr(), table.data_ptr())
         self._set(d)
 

@@ -158,3 +158,24 @@ def test_many_rows_with_unmapped_pages_and_nothing_to_see(kvops, shape, dtype, d
     s.mask = masks(bits)
     s.cache = kvops.PagedCache(s.pool[:, :, :, 0], s.pool[:, :, :, 1], table.cuda())
     check(s, s.run(kvops, max_draft=most), want(s, see_cached=mapped))
+
+
+# -- tables -----------------------------------------------------------------------------
+
+def test_tables_whose_rows_overlap_are_refused(kvops):
+    s = Setup(kvops, "f32", [100, 100], [1, 2], seed=73)
+    k, v, row = s.cache.k, s.cache.v, s.cache.table[:1]
+    for bad in (row.expand(2, -1), torch.as_strided(s.cache.table, (2, 6), (1, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            kvops.PagedCache(k, v, bad)
+    # one row, a copy of it, and rows that lie apart are fine
+    kvops.PagedCache(k, v, row.expand(1, -1))
+    apart = torch.full((2, 2 * row.shape[1]), 1 << 30, dtype=torch.int32, device="cuda")[:, :row.shape[1]]
+    apart.copy_(row.expand(2, -1))
+    same = []
+    for table in (row.expand(2, -1).contiguous(), apart):
+        s.cache = kvops.PagedCache(k, v, table)
+        same.append(s.run(kvops))
+    assert torch.equal(same[0][0], same[1][0]) and torch.equal(same[0][1], same[1][1])
+    s.table_h[1] = s.table_h[0]
+    s.check(*same[0])
