@@ -63,9 +63,12 @@ __device__ __forceinline__ float exp2_(float x) {  // 0 at -inf; relative error 
 
 // ---- fragments ----------------------------------------------------------
 // x = hi + lo with hi the nearest tf32 (11 significant bits); lo keeps the
-// rest, of which the instruction takes 11 bits: 22 bits of x in all.
+// rest, of which the instruction takes 11 bits: 22 bits of x in all.  Past the
+// largest tf32 hi is that one, so that it is never infinite: an infinity or NaN is lo's alone.
 __device__ __forceinline__ void split(float x, uint32_t &hi, uint32_t &lo) {
-  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  float y;  // |x| up to what rounds to the largest tf32, with x's sign
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(__uint_as_float(0x7f7fefffu)));
+  hi = (__float_as_uint(y) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi));
 }
 

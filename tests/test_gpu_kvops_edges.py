@@ -101,6 +101,30 @@ def want_nonfinite(s):
     return out, lse, top
 
 
+@pytest.mark.parametrize("big", [torch.finfo(torch.float32).min, torch.finfo(torch.float32).max, 3.402e38])
+@pytest.mark.parametrize("counts,heads", [([6, 1], 4), ([20, 3], 16), ([64, 3], 16)])  # 8, 16 and 32 rows a block
+def test_f32_drafts_as_large_as_the_type_goes(kvops, counts, heads, big):
+    """Keys and values filled with the type's lowest or largest value, masked."""
+    s = Setup(kvops, "f32", [40, 300], counts, heads=heads, seed=62)
+    s.mask = masks([1 << i | (i > 0) for t in counts for i in range(t)])
+    s.k[3], s.v[3] = big, big  # only token 3 sees it
+    got = s.run(kvops)
+    s.k[3], s.v[3] = 0.5, 0.5
+    rest = [i for i in range(sum(counts)) if i != 3]
+    check(s, [x[rest] for x in got], [x[rest] for x in want(s)])
+
+
+@pytest.mark.parametrize("big", [torch.finfo(torch.float32).min, torch.finfo(torch.float32).max])
+def test_f32_largest_values_seen(kvops, big):
+    s = Setup(kvops, "f32", [0, 20], [2, 1], seed=63)
+    s.mask = masks([1, 3, 1])
+    s.v[0] = big
+    s.k[1] = s.k[0]  # token 1 sees both alike
+    s.v[1, :, 1:] = 0
+    s.pool[s.table_h[1, 0].long(), 0, :, 1, 4] = big / 4
+    check(s, s.run(kvops), want(s))
+
+
 # -- the reference's rise, rows and pages with nothing in them --------------------------
 
 # As MANY_ROWS, with several tiles a group of warps.
