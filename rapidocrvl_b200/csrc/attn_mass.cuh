@@ -199,17 +199,20 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
         const int x = r0 + r;
         return counts(r) ? (const T *)a.q + (sh.first + x / a.group) * a.q_stride + (long long)(head * a.group + x % a.group) * D : nullptr;
       };
-      auto shift_of = [&](int r) {
-        if (!counts(r)) return INFINITY;
+      auto lse_of = [&](int r) {
         const int x = r0 + r;
-        const float l = a.lse[(long long)(sh.first + x / a.group) * a.kv_heads * a.group + head * a.group + x % a.group] * kLog2e;
-        return l == -INFINITY ? INFINITY : l;  // attended nothing
+        return counts(r) ? a.lse[(long long)(sh.first + x / a.group) * a.kv_heads * a.group + head * a.group + x % a.group] : -INFINITY;
+      };
+      auto none = [&](int r) { return lse_of(r) == -INFINITY; };  // attended nothing: adds nothing, whatever its query holds
+      auto shift_of = [&](int r) {
+        const float l = lse_of(r);
+        return l == -INFINITY ? INFINITY : l * kLog2e;
       };
       // whole pairs of tiles: rows past the last do not count
       auto tiles_of = [&](int pass) { return max(0, min(S::kRowTiles, (row_tiles - pass * S::kRowTiles + 1) / 2 * 2)); };
       if (!THIN || row_tiles) {
         const int tiles = THIN ? 1 : tiles_of(0);
-        L::query(q_at, tiles, tid, kMassThreads, query);
+        L::query(q_at, tiles, tid, kMassThreads, query, none);
         for (int r = tid; r < tiles * 8; r += kMassThreads) shift[r] = shift_of(r);
       }
       __syncthreads();
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
               uint4 x[S::kItems];
               float l_next = INFINITY;
 #pragma unroll
-              for (int i = 0; i < S::kItems; i++) x[i] = L::q_fetch(at * L::kQItems + i * kMassThreads + tid, query);
+              for (int i = 0; i < S::kItems; i++) x[i] = L::q_fetch(at * L::kQItems + i * kMassThreads + tid, query, none);
               if (tid < S::kHalf * 8) l_next = shift_of(at * 8 + tid);
               if (k < nk) weigh(f, h * S::kHalf, min(tiles, (h + 1) * S::kHalf));
               __syncthreads();

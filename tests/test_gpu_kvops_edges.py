@@ -125,6 +125,24 @@ def test_f32_largest_values_seen(kvops, big):
     check(s, s.run(kvops), want(s))
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens,counts,heads", [
+    ([300, 20, 90], [2, 1, 2], 4), ([300, 20, 140], [40, 1, 17], 16), ([9000], [64], 32), ([90000], [1], 16)])
+def test_attention_mass_of_tokens_that_attended_nothing(kvops, dtype, lens, counts, heads, bad):
+    """A token, or some of its heads, whose lse is -inf adds nothing whatever its query holds."""
+    s = Setup(kvops, dtype, lens, counts, heads=heads, seed=64)
+    _, lse = s.run(kvops, max_draft=max(counts))
+    none = [0, sum(counts) - 1] if sum(counts) > 1 else []
+    half = heads // 2 + 1
+    lse[none] = -math.inf
+    lse[0, half:] = -math.inf
+    w = mass_want(s, lse, width=s.cache.capacity)
+    s.q[none] = bad
+    s.q[0, half:, 7] = bad
+    mass_check(kvops.attention_mass(s.q, lse, s.cache, s.lens, s.indptr, scale=s.scale, max_draft=max(counts)), w)
+
+
 # -- the reference's rise, rows and pages with nothing in them --------------------------
 
 # As MANY_ROWS, with several tiles a group of warps.
