@@ -160,7 +160,8 @@ int ocrvl_seq_fill_synthetic(ocrvl_seq *s, int n, uint64_t seed);
  * to 8 sequences.
  *   ids       n token ids (embedding rows), or NULL when embeds is given
  *   embeds    n*hidden_size f32 input embeddings, or NULL
- *   pos_thw   n*3 M-RoPE positions, or NULL for (len, len, len)
+ *   pos_thw   n*3 M-RoPE positions, or NULL for the length three times (or what
+ *             ocrvl_seq_set_position said)
  *   need_logits  0: prompt token (K/V only in the last layer), 1: full step
  *   out_ids   n greedy ids (lm_head argmax, ties -> lowest id), may be NULL
  *   out_logits  n*vocab_size f32 logits, may be NULL
@@ -324,9 +325,16 @@ int ocrvl_seq_kv_view(ocrvl_seq *s, ocrvl_kv_cache *out);
 /* Drops all positions from n on (0 <= n <= length), as after an in-place
  * ocrvl_op_kv_compact or when drafted positions are taken back; pages that
  * hold none of the rest return to the pool.  The next step appends at
- * position n; its rotary position is (n, n, n) unless pos_thw says otherwise,
- * which it has to after an eviction. */
+ * position n.  After an eviction ocrvl_seq_set_position has to follow: the keys
+ * that are left have the rotary positions they were written with. */
 int ocrvl_seq_truncate(ocrvl_seq *s, int n);
+
+/* The rotary position of the sequence's next token where none is given (a step
+ * without pos_thw, the device-fed loop): pos, length <= pos < max_position,
+ * and one more for every token after it.  Without this call it is the
+ * length; truncate, which takes tokens back, lowers it by as many; reset and what
+ * replaces the cache set it to the length again. */
+int ocrvl_seq_set_position(ocrvl_seq *s, int pos);
 
 /* Attention of drafted tokens over a cache and over one another.
  * Sequence b drafted the tokens indptr[b] .. indptr[b+1]-1 of the flat

@@ -105,6 +105,7 @@ SIGNATURES = {
     "ocrvl_op_rmsnorm": (I, [I, I, P, P, F, P, P]),
     "ocrvl_seq_kv_view": (I, [P, C.POINTER(KVCache)]),
     "ocrvl_seq_truncate": (I, [P, I]),
+    "ocrvl_seq_set_position": (I, [P, I]),
     "ocrvl_op_tree_attn_workspace": (I, [C.POINTER(KVCache), I, I, C.POINTER(I64)]),
     "ocrvl_op_tree_attn": (I, [C.POINTER(KVCache), I, I, I, I, P, P, P, P, I64, P, P, I64, F, P, I64, P, P, I64, P]),
     "ocrvl_op_attn_mass": (I, [C.POINTER(KVCache), I, I, I, I, P, P, P, P, I64, P, F, F, P, I, I64, P, I, I64, P]),

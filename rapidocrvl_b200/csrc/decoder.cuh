@@ -849,7 +849,7 @@ __device__ void gemv_drain(const Ctx &c) {
 
 // Last block of the lm_head phase: keys -> ids (ties -> lowest id), key and
 // counter reset, and (device-side greedy loop) the next step's parameters:
-// tok = argmax, len + 1, position (len, len, len).
+// tok = argmax, len + 1, position (the same three times) + 1.
 __device__ void argmax_finish(const Ctx &c, int M, int feed) {
   const StepParams &sp = *c.sp;
   StepParams &spw = *c.sp_w;
@@ -867,7 +867,7 @@ __device__ void argmax_finish(const Ctx &c, int M, int feed) {
       int len = sp.seq[m].len + 1;
       spw.seq[m].tok = id;
       spw.seq[m].len = len;
-      spw.seq[m].pos[0] = spw.seq[m].pos[1] = spw.seq[m].pos[2] = len;
+      spw.seq[m].pos[0] = spw.seq[m].pos[1] = spw.seq[m].pos[2] = sp.seq[m].pos[0] + 1;
     }
   }
   __syncthreads();

@@ -660,6 +660,7 @@ struct ocrvl_model {
 struct ocrvl_seq {
   ocrvl_model *m = nullptr;
   int max_tokens = 0, len = 0;
+  int shift = 0;  // of the rotary position against len where none is given (ocrvl_seq_set_position)
   std::vector<int> pages;
   int *bt_d = nullptr;
 };
@@ -1259,7 +1260,7 @@ static int drop_pages(ocrvl_seq *s, size_t keep) {
 int ocrvl_seq_reset(ocrvl_seq *s) {
   if (!s) return fail(OCRVL_E_INVALID, "null seq");
   std::lock_guard<std::mutex> lk(s->m->mu);
-  s->len = 0;
+  s->len = s->shift = 0;
   return drop_pages(s, 0);
 }
 
@@ -1307,6 +1308,14 @@ int ocrvl_seq_truncate(ocrvl_seq *s, int n) {
   if (n < 0 || n > s->len) return fail(OCRVL_E_INVALID, "n outside 0..length");
   s->len = n;
   return drop_pages(s, (size_t)(n + kPageTokens - 1) / kPageTokens);
+}
+
+int ocrvl_seq_set_position(ocrvl_seq *s, int pos) {
+  if (!s) return fail(OCRVL_E_INVALID, "null seq");
+  std::lock_guard<std::mutex> lk(s->m->mu);
+  if (pos < s->len || pos >= s->m->desc.max_position) return fail(OCRVL_E_INVALID, "position outside length..max_position - 1");
+  s->shift = pos - s->len;
+  return OCRVL_OK;
 }
 
 int ocrvl_seq_import_kv(ocrvl_seq *s, int n, const float *k, const float *v) {
@@ -1500,7 +1509,8 @@ int step_group(ocrvl_model *m, ocrvl_seq *const *seqs, int n, const int32_t *ids
   int max_n = 0;
   for (int i = 0; i < n; i++) {
     ocrvl_seq *s = seqs[i];
-    int p[3] = {s->len, s->len, s->len};
+    const int next = s->len + s->shift;
+    int p[3] = {next, next, next};
     if (pos_thw)
       for (int a = 0; a < 3; a++) p[a] = pos_thw[3 * i + a];
     sp.seq[i].tok = ids ? ids[i] : 0;
@@ -1592,7 +1602,7 @@ int step_impl(ocrvl_model *m, ocrvl_seq *const *seqs, int n, const int32_t *ids,
       for (int a = 0; a < 3; a++)
         if (pos_thw[3 * i + a] < 0 || pos_thw[3 * i + a] >= d.max_position)
           return fail(OCRVL_E_INVALID, "position outside RoPE table");
-    if (!pos_thw && s->len >= d.max_position) return fail(OCRVL_E_INVALID, "position outside RoPE table");
+    if (!pos_thw && s->len + s->shift >= d.max_position) return fail(OCRVL_E_INVALID, "position outside RoPE table");
     if (s->len % kPageTokens == 0 && (int)s->pages.size() <= s->len / kPageTokens) new_pages++;
   }
   if (new_pages > m->free_pages.size()) return fail(OCRVL_E_NOMEM, "KV page pool exhausted");
@@ -1662,11 +1672,11 @@ int decode_group(ocrvl_model *m, ocrvl_seq *const *seqs, int n, const int32_t *f
     for (int j = 0; j < i; j++)
       if (seqs[j] == s) return fail(OCRVL_E_INVALID, "sequence repeated in one step");
     if (s->len + steps > s->max_tokens) return fail(OCRVL_E_INVALID, "steps exceed the sequence's max_tokens");
-    if (s->len + steps > d.max_position) return fail(OCRVL_E_INVALID, "positions exceed the RoPE table");
+    if (s->len + s->shift + steps > d.max_position) return fail(OCRVL_E_INVALID, "positions exceed the RoPE table");
     if (first_ids[i] < 0 || first_ids[i] >= d.vocab_size) return fail(OCRVL_E_INVALID, "token id outside vocab");
     sp.seq[i].tok = first_ids[i];
     sp.seq[i].len = s->len;
-    sp.seq[i].pos[0] = sp.seq[i].pos[1] = sp.seq[i].pos[2] = s->len;
+    sp.seq[i].pos[0] = sp.seq[i].pos[1] = sp.seq[i].pos[2] = s->len + s->shift;
     sp.seq[i].need = 1;
     sp.seq[i].bt = s->bt_d;
     max_n = std::max(max_n, s->len + 1);

@@ -190,9 +190,14 @@ class Sequence_:
     def truncate(self, n: int) -> None:
         """Drops all positions from n on (ocrvl_seq_truncate): drafts taken back,
         or what an eviction (``kvops.evict`` on ``PagedCache.of_sequence``) left
-        over.  After an eviction give ``step`` the positions of further tokens,
-        which go on counting from the old length."""
+        over.  After an eviction further tokens go on counting from the old
+        length: say so with :meth:`set_position`, or give ``step`` their positions."""
         _lib.check(self.rt._L.ocrvl_seq_truncate(self._h, int(n)))
+
+    def set_position(self, pos: int) -> None:
+        """The rotary position of the next token where none is given
+        (ocrvl_seq_set_position); those after it count on from there."""
+        _lib.check(self.rt._L.ocrvl_seq_set_position(self._h, int(pos)))
 
     def close(self) -> None:
         # sequences must be released before their model (ocrvl_seq_free

@@ -74,3 +74,54 @@ def test_lengths_past_a_sequences_pages_attend_nothing():
         rt.step([seq], ids=[3 + t], need_logits=False)
     assert abs(float(attend(52)[1].sum() - attend(32)[1].sum())) > 1e-3
     rt.close()
+
+
+@pytest.mark.parametrize("q,n,keep", [("q8", 50, 20), ("q4", 37, 32), ("q6", 90, 33)])
+def test_evicted_sequence_counts_on_without_positions_given(q, n, keep):
+    """Steps without positions and the device-fed loop after evict, truncate
+    and set_position give what steps with explicit positions give."""
+    import torch
+
+    from rapidocrvl_b200 import kvops
+    from rapidocrvl_b200._lib import OcrvlError
+
+    rt, cfg = _runtime(q)
+    seq = _prefill(rt, cfg, n, 3)
+    acc = torch.rand(cfg.num_hidden_layers, 1, cfg.num_key_value_heads, n, generator=torch.Generator().manual_seed(n)).cuda()
+    kvops.evict(kvops.PagedCache.of_sequence(seq), acc, torch.tensor([n], dtype=torch.int32, device="cuda"), keep=keep, sinks=2, recent=5)
+    torch.cuda.synchronize()
+    seq.truncate(keep)
+    seq.set_position(n)
+    ref = rt.new_sequence(n + 80)
+    ref.import_kv(*_cache(seq, cfg))
+    tok, at = 7, n
+    for _ in range(4):  # steps
+        a, la = rt.step([seq], ids=[tok], return_logits=True)
+        b, lb = rt.step([ref], ids=[tok], positions=[(at,) * 3], return_logits=True)
+        assert int(a[0]) == int(b[0]) and np.array_equal(la.view(np.uint32), lb.view(np.uint32))
+        tok, at = int(b[0]), at + 1
+    got, want = rt.decode_device([seq], [tok], 20).ravel().tolist(), []  # the loop
+    first = tok
+    for _ in range(20):
+        tok = int(rt.step([ref], ids=[tok], positions=[(at,) * 3])[0][0])
+        want.append(tok)
+        at += 1
+    assert got == want and _same(_cache(seq, cfg), _cache(ref, cfg))
+    seq.truncate(len(seq) - 6)  # taken back: the positions go back too
+    ref.truncate(len(ref) - 6)
+    (a, la), (b, lb) = rt.step([seq], ids=[first], return_logits=True), rt.step([ref], ids=[first], positions=[(at - 6,) * 3], return_logits=True)
+    assert np.array_equal(la.view(np.uint32), lb.view(np.uint32))
+    for bad in (len(seq) - 1, 2048, -1):
+        with pytest.raises(OcrvlError):
+            seq.set_position(bad)
+    seq.set_position(2048 - 3)
+    with pytest.raises(OcrvlError):
+        rt.decode_device([seq], [first], 4)
+    rt.decode_device([seq], [first], 3)
+    with pytest.raises(OcrvlError):
+        rt.step([seq], ids=[first])
+    seq.reset()
+    ref.reset()
+    (_, la), (_, lb) = rt.step([seq], ids=[5], return_logits=True), rt.step([ref], ids=[5], return_logits=True)
+    assert np.array_equal(la.view(np.uint32), lb.view(np.uint32))
+    rt.close()

@@ -80,3 +80,8 @@ def test_sequence_entries_reject_null():
     L, d = _lib.load(), _lib.KVCache()
     assert L.ocrvl_seq_kv_view(None, C.byref(d)) == _lib.E_INVALID
     assert L.ocrvl_seq_truncate(None, 0) == _lib.E_INVALID
+
+
+def test_set_position_rejects_null():
+    assert _lib.load().ocrvl_seq_set_position(None, 0) == _lib.E_INVALID
+    assert "null" in _lib.last_error()
