@@ -96,20 +96,29 @@ int sm_count(int *out) {
 // were resident on 148 SMs).
 int cluster_room(int sms) { return sms * 4 / 5; }
 
-// Launches with `smem` bytes of dynamic shared memory; dependent: may start
+// Bytes of dynamic shared memory: of this call, and the most that any call of
+// the kernel takes.  The limit that a kernel has leave for is shared by all host threads, so it
+// is always set to the same value.
+struct Smem {
+  int bytes, most;
+  Smem(int all) : bytes(all), most(all) {}
+  Smem(int bytes_, int most_) : bytes(bytes_), most(most_) {}
+};
+
+// Launches with dynamic shared memory; dependent: may start
 // before the kernel launched just before it on the stream ends (both wait for
 // it with griddepcontrol).
 template <typename... Params, typename... Args>
-int launch(const char *name, void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t stream, bool dependent,
+int launch(const char *name, void (*kernel)(Params...), dim3 grid, int threads, Smem smem, cudaStream_t stream, bool dependent,
            int cluster, Args... args) {
-  if (smem > 24 * 1024) {  // with a kernel's static share possibly past the 48 KB that need no leave
-    cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (smem.bytes > 24 * 1024) {  // with a kernel's static share possibly past the 48 KB that need no leave
+    cudaError_t e = cudaFuncSetAttribute((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem.most);
     if (e != cudaSuccess) return cuda_fail(name, e);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = smem.bytes;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
   int n = 0;
@@ -291,7 +300,7 @@ template <int CS, int THREADS>
 int launch_select(const SelectArgs &a, int rows, cudaStream_t stream) {
   const dim3 grid((unsigned)(rows * CS));
   const long long step = THREADS * 4, n = (((a.width + CS - 1) / CS + 3) / 4 * 4 + step - 1) / step * step;
-  return n <= kSelStage ? launch("select", k_kv_select<CS, true, THREADS>, grid, THREADS, (int)n * 4, stream, false, CS, a)
+  return n <= kSelStage ? launch("select", k_kv_select<CS, true, THREADS>, grid, THREADS, Smem((int)n * 4, kSelStage * 4), stream, false, CS, a)
                         : launch("select", k_kv_select<CS, false, THREADS>, grid, THREADS, 0, stream, false, CS, a);
 }
 

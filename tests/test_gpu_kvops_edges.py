@@ -4,6 +4,7 @@ along the context, rows and pages with nothing in them, on every shape of
 kernel.  Setup, types and the tolerances' derivation are test_gpu_kvops.py's;
 what a test adds to them is said there."""
 import math
+import threading
 
 import pytest
 import torch
@@ -221,3 +222,31 @@ def test_tables_whose_rows_overlap_are_refused(kvops):
     assert torch.equal(same[0][0], same[1][0]) and torch.equal(same[0][1], same[1][1])
     s.table_h[1] = s.table_h[0]
     s.check(*same[0])
+
+
+# -- select -----------------------------------------------------------------------------
+
+def test_select_of_several_widths_from_several_threads(kvops):
+    """Calls of the C entry (which takes no lock) on streams of their own, each of another width."""
+    from rapidocrvl_b200 import _lib
+
+    L, said = _lib.load(), []
+
+    def calls(acc, lens, idx, stream):
+        for _ in range(400):
+            if L.ocrvl_op_kv_select(1, 1, 2, acc.data_ptr(), acc.shape[1], acc.shape[1], lens.data_ptr(), 64, 0, 0, idx.data_ptr(), None, None,
+                                    stream.cuda_stream):
+                return said.append((acc.shape[1], _lib.last_error()))
+
+    work = [(torch.stack([torch.randperm(w, device="cuda").float() for _ in range(2)]), torch.tensor([w], dtype=torch.int32, device="cuda"),
+             torch.empty(2, 64, dtype=torch.int32, device="cuda"), torch.cuda.Stream()) for w in (390000, 300000, 200000, 100000)]
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=calls, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not said
+    for acc, _, idx, _ in work:
+        assert torch.equal(idx.long(), acc.topk(64).indices.sort().values)
