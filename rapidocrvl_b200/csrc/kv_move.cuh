@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_kv_select(const Sel
   uint32_t low = ~0u, high = 0u;
   if (STAGED) {  // all of the warp's sums on their way at once, then turned into keys where they lie
     const uint32_t at = smem_addr(keys);
-    if (((uintptr_t)(acc + s0) & 15) == 0) {
+    if (((uintptr_t)acc & 15) == 0) {  // then acc + s0 is too, but where the slice is empty
       for (int j = 0; j < steps; j++) {
         const int i = w0 + j * 128 + lane * 4, n4 = min(4, max(0, s1 - i));
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + (i - s0) * 4), "l"(n4 ? acc + i : acc), "r"(n4 * 4) : "memory");

@@ -9,7 +9,7 @@ import threading
 import pytest
 import torch
 
-from test_gpu_kvops import REL, Setup, kvops, masks, mass_check, mass_want  # noqa: F401 (kvops: the fixture)
+from test_gpu_kvops import REL, Setup, kvops, mass_check, mass_want, masks, select_check  # noqa: F401 (kvops: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -250,3 +250,11 @@ def test_select_of_several_widths_from_several_threads(kvops):
     assert not said
     for acc, _, idx, _ in work:
         assert torch.equal(idx.long(), acc.topk(64).indices.sort().values)
+
+
+@pytest.mark.parametrize("width", [9001, 30003, 300001])  # clusters of several sizes
+def test_select_of_few_positions_in_wide_unaligned_rows(kvops, width):
+    """Most blocks of a row's cluster have nothing to hold, and rows start at each alignment."""
+    acc = torch.rand(2, 8, 1, width, device="cuda", generator=torch.Generator(device="cuda").manual_seed(width))
+    select_check(kvops, acc, [5, 6, 7, 9, 13, 33, 61, 130], 4, 1, 1)
+    select_check(kvops, acc[..., :width - 2], [17, 18, 19, 23, 5, 64, 1, 0], 4, 0, 2)
