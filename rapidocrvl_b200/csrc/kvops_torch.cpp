@@ -4,6 +4,7 @@
 // same checks took 16 to 24 us on the host, more than most single-token calls
 // take on the GPU; this takes a third of that.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -30,9 +31,21 @@ void ok(int rc) {
   if (rc < 0) throw Refused{rc};
 }
 
+// The operators have no backward pass: a result without a gradient is not to be taken for one.
+const at::Tensor &no_gradient(const at::Tensor &t, const char *name) {
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    throw Wrong{std::string(name) + " requires a gradient, which this operator does not have (call it under torch.no_grad())"};
+  return t;
+}
+
 const at::Tensor &tensor(PyObject *o, const char *name) {
   if (!THPVariable_Check(o)) throw Wrong{std::string(name) + " must be a tensor"};
-  return THPVariable_Unpack(o);
+  return no_gradient(THPVariable_Unpack(o), name);
+}
+
+// Tells autograd that a tensor of the caller's was written.
+void wrote(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 bool none(PyObject *o) { return o == Py_None; }
@@ -70,12 +83,22 @@ struct Cache {
   const ocrvl_kv_cache *c;
   int device;
   at::ScalarType dtype;
+  PyObject *pools[2];  // k and v, None where the engine holds them
 
-  // a PagedCache's descriptor (its address) and device
-  Cache(PyObject *at_, PyObject *device_) {
-    c = (const ocrvl_kv_cache *)(uintptr_t)whole(at_, "cache");
-    device = small(device_, "device");
+  // a PagedCache's (address of the descriptor, device, k, v)
+  explicit Cache(PyObject *o) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) throw Wrong{"cache must be a PagedCache"};
+    c = (const ocrvl_kv_cache *)(uintptr_t)whole(PyTuple_GET_ITEM(o, 0), "cache");
+    device = small(PyTuple_GET_ITEM(o, 1), "device");
+    for (int i = 0; i < 2; i++) {
+      pools[i] = PyTuple_GET_ITEM(o, 2 + i);
+      if (!none(pools[i])) tensor(pools[i], i ? "the cache's v" : "the cache's k");
+    }
     dtype = c->type == OCRVL_F32 ? at::kFloat : c->type == OCRVL_F16 ? at::kHalf : at::kBFloat16;
+  }
+  void written() const {
+    for (PyObject *o : pools)
+      if (!none(o)) wrote(THPVariable_Unpack(o));
   }
   std::string where() const { return "cuda:" + std::to_string(device); }
   void on_device(const at::Tensor &t, const char *name) const {
@@ -143,62 +166,64 @@ PyObject *pack(std::initializer_list<at::Tensor> ts) {
   return t;
 }
 
-// (cache, device, q, k, v, lens, indptr, mask, layer, max_draft, scale, out, lse, work)
+// (cache, q, k, v, lens, indptr, mask, layer, max_draft, scale, out, lse, work)
 PyObject *tree_attention(PyObject *const *a) {
-  const Cache c(a[0], a[1]);
-  const at::Tensor &q = tensor(a[2], "q"), &k = tensor(a[3], "k"), &v = tensor(a[4], "v");
+  const Cache c(a[0]);
+  const at::Tensor &q = tensor(a[1], "q"), &k = tensor(a[2], "k"), &v = tensor(a[3], "v");
   const int64_t q_stride = c.tokens(q, "q", 0), kv_stride = c.tokens(k, "k", c.c->num_kv_heads);
   const int64_t n = q.size(0), heads = q.size(1);
   if (c.tokens(v, "v", c.c->num_kv_heads) != kv_stride || k.size(0) != n || v.size(0) != n)
     throw Wrong{"k and v must have q's tokens and the same stride"};
-  const int32_t *lens = c.ints(a[5], "lens", c.c->batch), *indptr = c.ints(a[6], "indptr", c.c->batch + 1);
-  const void *mask = c.flat(tensor(a[7], "mask"), "mask", at::kLong, n);
+  const int32_t *lens = c.ints(a[4], "lens", c.c->batch), *indptr = c.ints(a[5], "indptr", c.c->batch + 1);
+  const void *mask = c.flat(tensor(a[6], "mask"), "mask", at::kLong, n);
   void *stream = c.stream();
-  const int max_draft = draft_of(a[9], n);
+  const int max_draft = draft_of(a[8], n);
   int64_t bytes = 0;
   ok(ocrvl_op_tree_attn_workspace(c.c, narrow(heads, "heads"), max_draft, &bytes));
-  const at::Tensor out = none(a[11]) ? at::empty({n, heads, c.c->head_dim}, c.options(c.dtype)) : tensor(a[11], "out");
+  const at::Tensor out = none(a[10]) ? at::empty({n, heads, c.c->head_dim}, c.options(c.dtype)) : tensor(a[10], "out");
   const int64_t out_stride = c.tokens(out, "out", heads);
   if (out.size(0) != n) throw Wrong{"out must have q's shape"};
-  const at::Tensor lse = none(a[12]) ? at::empty({n, heads}, c.options(at::kFloat)) : tensor(a[12], "lse");
-  const at::Tensor work = none(a[13]) ? at::empty({bytes}, c.options(at::kByte)) : tensor(a[13], "work");
-  ok(ocrvl_op_tree_attn(c.c, small(a[8], "layer"), narrow(heads, "heads"), narrow(n, "tokens"), max_draft, lens, indptr,
-                        (const int64_t *)mask, q.data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), kv_stride, scale_of(a[10], c),
+  const at::Tensor lse = none(a[11]) ? at::empty({n, heads}, c.options(at::kFloat)) : tensor(a[11], "lse");
+  const at::Tensor work = none(a[12]) ? at::empty({bytes}, c.options(at::kByte)) : tensor(a[12], "work");
+  ok(ocrvl_op_tree_attn(c.c, small(a[7], "layer"), narrow(heads, "heads"), narrow(n, "tokens"), max_draft, lens, indptr,
+                        (const int64_t *)mask, q.data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), kv_stride, scale_of(a[9], c),
                         out.data_ptr(), out_stride, (float *)c.flat(lse, "lse", at::kFloat, n * heads),
                         c.flat(work, "work", at::kByte, work.numel()), work.numel(), stream));
+  wrote(out), wrote(lse), wrote(work);
   return pack({out, lse});
 }
 
-// (cache, device, q, lse, lens, indptr, layer, max_draft, scale, counted, acc, decay, out)
+// (cache, q, lse, lens, indptr, layer, max_draft, scale, counted, acc, decay, out)
 PyObject *attention_mass(PyObject *const *a) {
-  const Cache c(a[0], a[1]);
-  const at::Tensor &q = tensor(a[2], "q"), &lse = tensor(a[3], "lse");
+  const Cache c(a[0]);
+  const at::Tensor &q = tensor(a[1], "q"), &lse = tensor(a[2], "lse");
   const int64_t q_stride = c.tokens(q, "q", 0), n = q.size(0), heads = q.size(1);
   const float *lse_at = (const float *)c.flat(lse, "lse", at::kFloat, n * heads);
-  const int32_t *lens = c.ints(a[4], "lens", c.c->batch), *indptr = c.ints(a[5], "indptr", c.c->batch + 1);
-  const int64_t *counted = none(a[9]) ? nullptr : (const int64_t *)c.flat(tensor(a[9], "counted"), "counted", at::kLong, c.c->batch);
+  const int32_t *lens = c.ints(a[3], "lens", c.c->batch), *indptr = c.ints(a[4], "indptr", c.c->batch + 1);
+  const int64_t *counted = none(a[8]) ? nullptr : (const int64_t *)c.flat(tensor(a[8], "counted"), "counted", at::kLong, c.c->batch);
   const float *acc = nullptr;
   int64_t acc_width = 0, acc_stride = 0, width = (int64_t)c.c->max_pages * c.c->page_size;
-  if (!none(a[10])) {
-    const at::Tensor &t = tensor(a[10], "acc");
+  if (!none(a[9])) {
+    const at::Tensor &t = tensor(a[9], "acc");
     acc_stride = c.rows(t, "acc", false);
     acc = (const float *)t.data_ptr(), acc_width = width = t.size(2);
   }
   void *stream = c.stream();
-  const at::Tensor out = none(a[12]) ? at::empty({c.c->batch, c.c->num_kv_heads, width}, c.options(at::kFloat)) : tensor(a[12], "out");
+  const at::Tensor out = none(a[11]) ? at::empty({c.c->batch, c.c->num_kv_heads, width}, c.options(at::kFloat)) : tensor(a[11], "out");
   const int64_t out_stride = c.rows(out, "out", false);
-  ok(ocrvl_op_attn_mass(c.c, small(a[6], "layer"), narrow(heads, "heads"), narrow(n, "tokens"), draft_of(a[7], n), lens, indptr, counted,
-                        q.data_ptr(), q_stride, lse_at, scale_of(a[8], c), real(a[11], "decay"), acc, narrow(acc_width, "acc"),
+  ok(ocrvl_op_attn_mass(c.c, small(a[5], "layer"), narrow(heads, "heads"), narrow(n, "tokens"), draft_of(a[6], n), lens, indptr, counted,
+                        q.data_ptr(), q_stride, lse_at, scale_of(a[7], c), real(a[10], "decay"), acc, narrow(acc_width, "acc"),
                         acc_stride, (float *)out.data_ptr(), narrow(out.size(2), "out"), out_stride, stream));
+  wrote(out);
   return THPVariable_Wrap(out);
 }
 
 // The shared part of select and evict: to is NULL for select.
-PyObject *choose(const Cache &c, const ocrvl_kv_cache *to, PyObject *const *a) {
-  const at::Tensor &acc = tensor(a[2], "acc");
+PyObject *choose(const Cache &c, const Cache *to, PyObject *const *a) {
+  const at::Tensor &acc = tensor(a[1], "acc");
   const int64_t stride = c.rows(acc, "acc", true);
-  const int keep = small(a[4], "keep"), sinks = small(a[5], "sinks"), recent = small(a[6], "recent");
-  const int32_t *lens = c.ints(a[3], "lens", c.c->batch);
+  const int keep = small(a[3], "keep"), sinks = small(a[4], "sinks"), recent = small(a[5], "recent");
+  const int32_t *lens = c.ints(a[2], "lens", c.c->batch);
   const float *from = (const float *)acc.data_ptr();
   const int width = narrow(acc.size(3), "acc");
   void *stream = c.stream();
@@ -207,49 +232,55 @@ PyObject *choose(const Cache &c, const ocrvl_kv_cache *to, PyObject *const *a) {
   const at::Tensor new_lens = at::empty({c.c->batch}, c.options(at::kInt));
   int32_t *i = (int32_t *)idx.data_ptr(), *l = (int32_t *)new_lens.data_ptr();
   float *s = (float *)sums.data_ptr();
-  ok(to ? ocrvl_op_kv_evict(c.c, to, from, width, stride, lens, keep, sinks, recent, i, s, l, stream)
+  ok(to ? ocrvl_op_kv_evict(c.c, to->c, from, width, stride, lens, keep, sinks, recent, i, s, l, stream)
         : ocrvl_op_kv_select(c.c->num_layers, c.c->batch, c.c->num_kv_heads, from, width, stride, lens, keep, sinks, recent, i, s, l, stream));
+  if (to) to->written();
   return pack({idx, sums, new_lens});
 }
 
-// (cache, device, acc, lens, keep, sinks, recent)
-PyObject *select(PyObject *const *a) { return choose(Cache(a[0], a[1]), nullptr, a); }
+// (cache, acc, lens, keep, sinks, recent)
+PyObject *select(PyObject *const *a) { return choose(Cache(a[0]), nullptr, a); }
 
-// (cache, device, acc, lens, keep, sinks, recent, into)
-PyObject *evict(PyObject *const *a) { return choose(Cache(a[0], a[1]), Cache(a[7], a[1]).c, a); }
+// (cache, acc, lens, keep, sinks, recent, into)
+PyObject *evict(PyObject *const *a) {
+  const Cache to(a[6]);
+  return choose(Cache(a[0]), &to, a);
+}
 
-// (cache, device, idx, into)
+// (cache, idx, into)
 PyObject *compact(PyObject *const *a) {
-  const Cache c(a[0], a[1]), to(a[3], a[1]);
-  const at::Tensor &idx = tensor(a[2], "idx");
+  const Cache c(a[0]), to(a[2]);
+  const at::Tensor &idx = tensor(a[1], "idx");
   if (idx.dim() != 4 || idx.size(0) != c.c->num_layers || idx.size(1) != c.c->batch || idx.size(2) != c.c->num_kv_heads)
     throw Wrong{"idx must be [layers, batch, kv heads, keep] of the cache's shape"};
   ok(ocrvl_op_kv_compact(c.c, to.c, (const int32_t *)c.flat(idx, "idx", at::kInt, idx.numel()), narrow(idx.size(3), "keep"), c.stream()));
+  to.written();
   Py_RETURN_NONE;
 }
 
-// (cache, device, k, v, lens, indptr, path, n_path)
+// (cache, k, v, lens, indptr, path, n_path)
 PyObject *append(PyObject *const *a) {
-  const Cache c(a[0], a[1]);
-  const at::Tensor &k = tensor(a[2], "k"), &v = tensor(a[3], "v");
+  const Cache c(a[0]);
+  const at::Tensor &k = tensor(a[1], "k"), &v = tensor(a[2], "v");
   const int64_t stride = c.tokens(k, "k", c.c->num_kv_heads, 4);
   if (c.tokens(v, "v", c.c->num_kv_heads, 4) != stride || v.sizes() != k.sizes() || k.size(0) != c.c->num_layers ||
       (k.size(0) > 1 && v.stride(0) != k.stride(0)))
     throw Wrong{"k and v must be [" + std::to_string(c.c->num_layers) + ", tokens, kv heads, head_dim] of the same strides"};
-  const int32_t *lens = c.ints(a[4], "lens", c.c->batch), *indptr = c.ints(a[5], "indptr", c.c->batch + 1);
+  const int32_t *lens = c.ints(a[3], "lens", c.c->batch), *indptr = c.ints(a[4], "indptr", c.c->batch + 1);
   const int32_t *path = nullptr, *n_path = nullptr;
   int64_t most = 0;
-  if (none(a[6]) != none(a[7])) throw Wrong{"path and n_path go together"};
-  if (!none(a[6])) {
-    const at::Tensor &p = tensor(a[6], "path");
+  if (none(a[5]) != none(a[6])) throw Wrong{"path and n_path go together"};
+  if (!none(a[5])) {
+    const at::Tensor &p = tensor(a[5], "path");
     if (p.dim() != 2 || p.size(0) != c.c->batch) throw Wrong{"path must be [batch, most]"};
     path = (const int32_t *)c.flat(p, "path", at::kInt, p.numel()), most = p.size(1);
-    n_path = c.ints(a[7], "n_path", c.c->batch);
+    n_path = c.ints(a[6], "n_path", c.c->batch);
   }
   void *stream = c.stream();
   const at::Tensor new_lens = at::empty({c.c->batch}, c.options(at::kInt));
   ok(ocrvl_op_kv_append(c.c, narrow(k.size(1), "tokens"), lens, indptr, path, n_path, narrow(most, "path"), k.data_ptr(), v.data_ptr(),
                         stride, k.size(0) > 1 ? k.stride(0) : 0, (int32_t *)new_lens.data_ptr(), stream));
+  c.written();
   return THPVariable_Wrap(new_lens);
 }
 
@@ -273,8 +304,8 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 #define ENTRY(f, n) {#f, (PyCFunction)(void (*)(void))entry<f, n>, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ENTRY(tree_attention, 14), ENTRY(attention_mass, 13), ENTRY(select, 7), ENTRY(compact, 4),
-                         ENTRY(evict, 8),           ENTRY(append, 8),          {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {ENTRY(tree_attention, 13), ENTRY(attention_mass, 12), ENTRY(select, 6), ENTRY(compact, 3),
+                         ENTRY(evict, 7),           ENTRY(append, 7),          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kvops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -14,7 +14,8 @@ All run on the tensors' device and torch's current stream, read lengths on the
 device and wait for nothing, so they can be captured in a CUDA graph.  They call
 the C ABI of include/ocrvl_cuda.h (ocrvl_op_tree_attn and following), whose
 comments say what each computes; a wrong argument raises OcrvlError or
-ValueError before anything runs.
+ValueError before anything runs.  There is no backward pass: a tensor that
+requires a gradient is refused unless gradients are off.
 """
 from __future__ import annotations
 
@@ -61,7 +62,7 @@ class PagedCache:
 
     def _set(self, d) -> None:
         self.desc = d
-        self._at, self._dev = C.addressof(d), self.device.index  # for the native side
+        self._ref = (C.addressof(d), self.device.index, self.k, self.v)  # for the native side
         self.head_dim, self.kv_heads, self.layers, self.batch = d.head_dim, d.num_kv_heads, d.num_layers, d.batch
         self.capacity = d.max_pages * d.page_size
 
@@ -104,7 +105,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Pag
 
     Returns (out, lse): out like q, lse [tokens, heads] f32.  A token that
     attends nothing gets 0 and -inf."""
-    return _kvops.tree_attention(cache._at, cache._dev, q, k, v, lens, indptr, mask, layer, max_draft, scale, out, lse, work)
+    return _kvops.tree_attention(cache._ref, q, k, v, lens, indptr, mask, layer, max_draft, scale, out, lse, work)
 
 
 
@@ -121,7 +122,7 @@ def attention_mass(q: torch.Tensor, lse: torch.Tensor, cache: PagedCache, lens: 
     heads, width] f32, or None for zeros.  Returns the new sums, [batch, kv heads,
     width] (the cache's capacity without acc), 0 past each length; ``out`` may be
     ``acc`` itself."""
-    return _kvops.attention_mass(cache._at, cache._dev, q, lse, lens, indptr, layer, max_draft, scale, counted, acc, decay, out)
+    return _kvops.attention_mass(cache._ref, q, lse, lens, indptr, layer, max_draft, scale, counted, acc, decay, out)
 
 
 
@@ -135,7 +136,7 @@ def select(cache: PagedCache, acc: torch.Tensor, lens: torch.Tensor, *, keep: in
     Returns (idx, sums, new_lens): idx [layers, batch, kv heads, keep] int32 in
     rising order, -1 past the count, with their sums (0 there), and [batch]
     int32."""
-    return _kvops.select(cache._at, cache._dev, acc, lens, keep, sinks, recent)
+    return _kvops.select(cache._ref, acc, lens, keep, sinks, recent)
 
 
 
@@ -151,7 +152,7 @@ def compact(cache: PagedCache, idx: torch.Tensor, *, into: Optional[PagedCache] 
     """Moves the positions that ``idx`` (from :func:`select`) names to the
     front, in place or into the pages of another cache of the same shape
     (which share nothing with this one's)."""
-    _kvops.compact(cache._at, cache._dev, idx, _other(cache, into)._at)
+    _kvops.compact(cache._ref, idx, _other(cache, into)._ref)
 
 
 
@@ -161,7 +162,7 @@ def evict(cache: PagedCache, acc: torch.Tensor, lens: torch.Tensor, *, keep: int
     :func:`compact`) and returns what select does.  Keys keep the rotary
     positions they were written with, so tokens after the cut go on counting
     from the old length: the caller keeps that count."""
-    return _kvops.evict(cache._at, cache._dev, acc, lens, keep, sinks, recent, _other(cache, into)._at)
+    return _kvops.evict(cache._ref, acc, lens, keep, sinks, recent, _other(cache, into)._ref)
 
 
 
@@ -174,4 +175,4 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lens: torch.Tens
     [batch] int32 names the tokens of each sequence to write, in order (the
     accepted path through its tree); without them all are written.  Returns
     the new lengths."""
-    return _kvops.append(cache._at, cache._dev, k, v, lens, indptr, path, n_path)
+    return _kvops.append(cache._ref, k, v, lens, indptr, path, n_path)

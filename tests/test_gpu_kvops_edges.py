@@ -258,3 +258,52 @@ def test_select_of_few_positions_in_wide_unaligned_rows(kvops, width):
     acc = torch.rand(2, 8, 1, width, device="cuda", generator=torch.Generator(device="cuda").manual_seed(width))
     select_check(kvops, acc, [5, 6, 7, 9, 13, 33, 61, 130], 4, 1, 1)
     select_check(kvops, acc[..., :width - 2], [17, 18, 19, 23, 5, 64, 1, 0], 4, 0, 2)
+
+
+# -- autograd ---------------------------------------------------------------------------
+
+def _calls(kvops, s, into):
+    """Every operator on tensors by name."""
+    layers = torch.randn(1, s.q.shape[0], 2, 128, device="cuda")
+    _, lse = s.run(kvops)
+    x = dict(q=s.q, k=s.k, v=s.v, lse=lse, acc=torch.rand(1, 2, s.cache.capacity, device="cuda"), out=torch.empty_like(s.q),
+             new_k=layers, new_v=layers.clone(), idx=torch.arange(8, dtype=torch.int32, device="cuda").expand(1, 1, 2, 8).contiguous())
+    seqs = (s.lens, s.indptr)
+    return x, {
+        "tree_attention": (lambda: kvops.tree_attention(x["q"], x["k"], x["v"], s.cache, *seqs, s.mask, out=x["out"], lse=x["lse"]),
+                           ("q", "k", "v"), ("out", "lse")),
+        "attention_mass": (lambda: kvops.attention_mass(x["q"], x["lse"], s.cache, *seqs, acc=x["acc"], out=x["acc"]), ("q", "lse", "acc"), ("acc",)),
+        "append": (lambda: kvops.append(s.cache, x["new_k"], x["new_v"], *seqs), ("new_k", "new_v"), "cache"),
+        "evict": (lambda: kvops.evict(s.cache, x["acc"][None], s.lens, keep=8, into=into), ("acc",), "into"),
+        "evict in place": (lambda: kvops.evict(s.cache, x["acc"][None], s.lens, keep=8), ("acc",), "cache"),
+        "select": (lambda: kvops.select(s.cache, x["acc"][None], s.lens, keep=8), ("acc",), ()),
+        "compact": (lambda: kvops.compact(s.cache, x["idx"], into=into), (), "into"),
+    }
+
+
+def test_tensors_that_require_a_gradient_are_refused_and_writes_are_counted(kvops):
+    s = Setup(kvops, "f32", [40], [3], seed=81, room=4)
+    pool = torch.zeros(1, 1, 2, 2, 16, 128, device="cuda")
+    into = kvops.PagedCache(pool[:, :, :, 0], pool[:, :, :, 1], torch.zeros(1, 1, dtype=torch.int32, device="cuda"))
+    x, calls = _calls(kvops, s, into)
+    for name, (call, reads, writes) in calls.items():
+        for key in reads:
+            x[key].requires_grad_()
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+            x[key].requires_grad_(False)
+        counted = {"cache": (s.cache.k, s.cache.v), "into": (into.k, into.v)}[writes] if isinstance(writes, str) else [x[w] for w in writes]
+        before = [t._version for t in counted]
+        call()
+        assert all(t._version > b for t, b in zip(counted, before)), name
+        with torch.inference_mode():
+            call()
+    grown = s.pool.clone().requires_grad_()  # a cache that requires one
+    s.cache = kvops.PagedCache(grown[:, :, :, 0], grown[:, :, :, 1], s.cache.table)
+    for call, _, _ in calls.values():
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():
+        s.run(kvops)
+        x["q"].requires_grad_()
+        s.run(kvops)
