@@ -392,7 +392,10 @@ int ocrvl_op_kv_select(int num_layers, int batch, int num_kv_heads, const float 
  * of `to` becomes position idx[layer][b][h][j] of `from`, for j up to the
  * first negative index or `keep`.  `to` is `from` itself (same pool, same
  * table: in place; idx is then strictly rising), or a cache of the same shape whose
- * pages that table rows name share nothing with from's. */
+ * pages that table rows name share nothing with from's, with room for `keep`
+ * positions (or for all that `from` can have).  The pages of the positions named
+ * and of those they move to have to be mapped: a position without a page is
+ * skipped. */
 int ocrvl_op_kv_compact(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const int32_t *idx, int keep,
                         void *stream);
 

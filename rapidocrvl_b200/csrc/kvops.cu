@@ -311,6 +311,8 @@ int check_move(const ocrvl_kv_cache *from, const ocrvl_kv_cache *to, const int32
       from->num_layers != to->num_layers || from->batch != to->batch)
     return invalid("the caches must have the same type, head_dim, heads, layers and batch");
   if (keep < 1 || keep > 65535 * kMoveRows) return invalid("keep must be 1..2,097,120");
+  const long long room = (long long)to->max_pages * to->page_size, held = (long long)from->max_pages * from->page_size;
+  if (keep > room && held > room) return invalid("to has no room for the positions that are kept");
   if (!idx) return invalid("null argument");
   if ((long long)from->num_layers * from->batch * from->num_kv_heads > 1 << 24) return invalid("too many rows");
   return OCRVL_OK;

@@ -151,7 +151,8 @@ def _other(cache: PagedCache, into: Optional[PagedCache]) -> PagedCache:
 def compact(cache: PagedCache, idx: torch.Tensor, *, into: Optional[PagedCache] = None) -> None:
     """Moves the positions that ``idx`` (from :func:`select`) names to the
     front, in place or into the pages of another cache of the same shape
-    (which share nothing with this one's)."""
+    (which share nothing with this one's), with room for them.  All these
+    positions' pages have to be mapped."""
     _kvops.compact(cache._ref, idx, _other(cache, into)._ref)
 
 

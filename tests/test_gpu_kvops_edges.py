@@ -260,6 +260,30 @@ def test_select_of_few_positions_in_wide_unaligned_rows(kvops, width):
     select_check(kvops, acc[..., :width - 2], [17, 18, 19, 23, 5, 64, 1, 0], 4, 0, 2)
 
 
+# -- compact and evict ------------------------------------------------------------------
+
+@pytest.mark.parametrize("keep", [65, 200])
+def test_evict_into_too_little_room_is_refused(kvops, keep):
+    from rapidocrvl_b200._lib import OcrvlError
+
+    s = Setup(kvops, "f32", [200], [0], seed=66)
+    pool = torch.full((4, 1, 2, 2, 16, 128), 9.0, device="cuda")
+    into = kvops.PagedCache(pool[:, :, :, 0], pool[:, :, :, 1], torch.arange(4, dtype=torch.int32, device="cuda")[None])
+    acc = torch.rand(1, 1, 2, 208, device="cuda")
+    with pytest.raises(OcrvlError, match="room"):
+        kvops.evict(s.cache, acc, s.lens, keep=keep, into=into)
+    idx, _, _ = kvops.select(s.cache, acc, s.lens, keep=keep)
+    with pytest.raises(OcrvlError, match="room"):
+        kvops.compact(s.cache, idx, into=into)
+    assert bool((pool == 9).all())
+    _, _, new = kvops.evict(s.cache, acc, s.lens, keep=64, into=into)
+    assert new.tolist() == [64] and not bool((pool == 9).any())
+    # a cache that holds no more than there is room for may be asked to keep any number
+    small = Setup(kvops, "f32", [40], [0], seed=67)
+    _, _, new = kvops.evict(small.cache, acc[..., :48].contiguous(), small.lens, keep=keep, into=into)
+    assert new.tolist() == [40]
+
+
 # -- autograd ---------------------------------------------------------------------------
 
 def _calls(kvops, s, into):

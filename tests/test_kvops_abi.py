@@ -85,3 +85,9 @@ def test_sequence_entries_reject_null():
 def test_set_position_rejects_null():
     assert _lib.load().ocrvl_seq_set_position(None, 0) == _lib.E_INVALID
     assert "null" in _lib.last_error()
+
+
+def test_moves_into_too_little_room_are_refused():
+    small = cache(max_pages=2, table=3 << 20, k=4 << 20, v=(4 << 20) + 8192)
+    rc, said = compact(cache(), small, keep=33)
+    assert rc == _lib.E_INVALID and "room" in said
