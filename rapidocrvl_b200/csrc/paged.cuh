@@ -61,6 +61,14 @@ __device__ __forceinline__ float exp2_(float x) {  // 0 at -inf; relative error 
   return y;
 }
 
+// sum + low += x, without the roundings of sum: over 100,000 positions, each far below the sum so far, those
+// would add up to 1e-4 of it.
+__device__ __forceinline__ void add_exactly(float &sum, float &low, float x) {
+  const float s = sum + x, y = s - sum;
+  low += (sum - (s - y)) + (x - y);
+  sum = s;
+}
+
 // ---- fragments ----------------------------------------------------------
 // x = hi + lo with hi the nearest tf32 (11 significant bits); lo keeps the
 // rest, of which the instruction takes 11 bits: 22 bits of x in all.  Past the

@@ -379,9 +379,9 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
 #pragma unroll
       for (int blk = 0; blk < L::kTiles; blk++) L::q_load(qr[blk], q_at, blk, lane);
     }
-    float o[L::kTiles][NT][4] = {}, ref[NT][2], sum[NT][2];  // of rows 8 n + 2 t and + 1
+    float o[L::kTiles][NT][4] = {}, ref[NT][2], sum[NT][2] = {}, low[NT][2] = {};  // of rows 8 n + 2 t and + 1
 #pragma unroll
-    for (int n = 0; n < NT; n++) ref[n][0] = ref[n][1] = -INFINITY, sum[n][0] = sum[n][1] = 0.f;
+    for (int n = 0; n < NT; n++) ref[n][0] = ref[n][1] = -INFINITY;
 
     for (int k = 0; k < cur.nk; k++) {
       const int c = cur.c0 + k * cur.step, u = 2 * k;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
             const float now = fmaxf(ref[n][h], top);
             const float alpha = now == -INFINITY ? 1.f : exp2_(ref[n][h] - now);
             ref[n][h] = now;
-            sum[n][h] *= alpha;
+            sum[n][h] *= alpha, low[n][h] *= alpha;
 #pragma unroll
             for (int i = 0; i < L::kTiles; i++) o[i][n][h] *= alpha, o[i][n][2 + h] *= alpha;
           }
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
         for (int h = 0; h < 2; h++) {
           const float m = ref[n][h] == -INFINITY ? 0.f : ref[n][h];
           s[n][h] = exp2_(s[n][h] - m), s[n][2 + h] = exp2_(s[n][2 + h] - m);
-          sum[n][h] += s[n][h] + s[n][2 + h];
+          add_exactly(sum[n][h], low[n][h], s[n][h] + s[n][2 + h]);
         }
       copy_wait<NU - 2>();
       __syncwarp();
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
       for (int n = m * (JR / 8); n < (m + 1) * (JR / 8); n++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          float l = sum[n][h];
+          float l = sum[n][h] + low[n][h];
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(~0u, l, d);
           const int row = n * 8 + 2 * t + h, r = row - m * JR;

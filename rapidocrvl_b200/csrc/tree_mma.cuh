@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
       const int row = (WIDE ? s * 128 : 0) + r, first = cur.rb * S::kRows + row;
       const bool works = row - lane < rows;  // the warp has rows
       const unsigned long long seen = row < rows ? (unsigned long long)a.mask[cur.sg.first + first / a.group] : 0ull;
-      float ref = -INFINITY, sum = 0.f;
+      float ref = -INFINITY, sum = 0.f, low = 0.f;
       bool ok = true, poison = false;
       for (int i = 0; i < n_s && ok; i++, steps++) {
         const uint32_t tile = T0 + (WIDE ? i : 2 * i + s);
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
                     if (!MASKED || m >> j & 1) top = fmaxf(top, fmaf(__uint_as_float(x[j]), a.scale, -base));
                   const float down = add > kMmaMost ? ceilf(top) : 0.f, alpha = exp2_(-down);
                   ref = down > 0.f ? base + down : ref;
-                  sum *= alpha;
+                  sum *= alpha, low *= alpha;
                   uint32_t w[16];
 #pragma unroll 1
                   for (int c = 0; c < q; c++) {
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
                     tc_store16(o_at + c * 16, w);
                   }
                 }
-                sum += add;
+                add_exactly(sum, low, add);
                 tc_store16(s_at + q * 16, p16);
               }
           };
@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
         bar_arrive(&p_ready[s]);
       }
       // ---- the piece's end --------------------------------------------------
+      sum += low;
       const int n_0 = tiles_of(0, n, rows), n_1 = tiles_of(1, n, rows);
       ends[0] += n_0 > 0, ends[1] += n_1 > 0;
       if (n_0 && !(WIDE && s == 1)) ok = ok && bar_wait(&o_full[0], (ends[0] - 1) & 1, dead);

@@ -203,6 +203,40 @@ def test_many_rows_with_unmapped_pages_and_nothing_to_see(kvops, shape, dtype, d
     check(s, s.run(kvops, max_draft=most), want(s, see_cached=mapped))
 
 
+def long_tail(kvops, dtype, n, most):
+    """One position far above all others, each of which has 2^-24 to 2^-27 of its weight: together a 400th or a 50th of
+    the sum.  Returns (out, lse) and what they should be."""
+    B, heads, dim, page = 74, 16, 64, 1024
+    pages = n // page
+    g = torch.Generator(device="cuda").manual_seed(65)
+    pool = torch.zeros(128, 1, 2, 2, page, dim, dtype=dtype, device="cuda")
+    pool[:, :, :, 1] = torch.empty(pool[:, :, :, 1].shape, dtype=dtype, device="cuda").uniform_(0.5, 1.0, generator=g)
+    pool[0, 0, :, 0, 0, 0], pool[0, 0, :, 1, 0] = 1.0, 0.0  # the strong position
+    row = torch.arange(pages, dtype=torch.int32)
+    row[128:] = row[128:] % 127 + 1  # long contexts: the pages without it over and over
+    cache = kvops.PagedCache(pool[:, :, :, 0], pool[:, :, :, 1], row.cuda().repeat(B, 1))
+    counts = [most] + [1] * (B - 1)
+    N = sum(counts)
+    q = torch.zeros(N, heads, dim, dtype=dtype, device="cuda")
+    q[:, :, 0] = torch.linspace(16.0, 18.0, heads, device="cuda").to(dtype)
+    kv = torch.zeros(N, 2, dim, dtype=dtype, device="cuda")
+    scale = 25.6 * math.log(2) / 17.0
+    out, lse = kvops.tree_attention(q, kv, kv, cache, torch.full((B,), n, dtype=torch.int32, device="cuda"),
+                                    torch.tensor([0] + [sum(counts[:b + 1]) for b in range(B)], dtype=torch.int32, device="cuda"),
+                                    torch.zeros(N, dtype=torch.int64, device="cuda"), max_draft=most, scale=scale)
+    v = pool[row.cuda().long(), 0, :, 1].double().sum((0, 2)).repeat_interleave(heads // 2, 0)  # [heads, dim]
+    x = q[0, :, 0].double() * scale
+    w = torch.exp(-x)[:, None]
+    return out.double(), lse.double(), v * w / (1 + (n - 1) * w), x + torch.log1p((n - 1) * w[:, 0])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n,most", [(1 << 17, 8), (1 << 20, 1)])  # many rows, eight rows
+def test_long_tails_are_in_the_sum(kvops, n, most, dtype):
+    _, lse, _, want = long_tail(kvops, {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}[dtype], n, most)
+    assert bool(((lse - want).abs() <= 1e-5).all()), float((lse - want).abs().max())
+
+
 # -- tables -----------------------------------------------------------------------------
 
 def test_tables_whose_rows_overlap_are_refused(kvops):
