@@ -8,7 +8,7 @@
 // the sum l and the weighted values o of its own positions:
 //   p = 2^(s - m),  l' = l + sum p,  o' = o + p v      (s = scale log2(e) q . k)
 // m follows the running maximum, but only once a score passes it by kSlack:
-//   m' = max(m, max s),  l and o times 2^(m - m')
+//   m' = max(m, max s),  l and o times 2^(m - m')      (f16: max s - kLift)
 // so most chunks need no maximum over lanes and no rescaling, and p stays below
 // 2^kSlack.  At the run's end the warps are joined: o = sum_w 2^(m_w - M) o_w,
 // l likewise.
@@ -40,7 +40,14 @@ namespace paged {
 constexpr int kTreeWarps = 8;
 constexpr int kTreeThreads = kTreeWarps * 32;
 constexpr int kTileChunks = kTreeWarps;  // chunks a tile: one a warp
-constexpr float kSlack = 8.f;  // p at most 256: far from f16's largest
+// A new reference stands kLift below its largest score, and stays while no score passes it by
+// kSlack.  f16's weights below 2^-24 lose their last bits and those below 2^-25 are 0, which over
+// 100,000 positions under one strong one adds up, so they start as 2^7 and may grow to 2^15, half
+// of f16's largest: what is lost is below 2^-32 of the largest weight.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
+template <typename T>
+constexpr float kSlack = std::is_same<T, __half>::value ? 15.f : 8.f;
 
 struct TreeArgs {
   Cache c;
@@ -411,7 +418,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) above |= s[n][e] > ref[n][e & 1] + kSlack;
+        for (int e = 0; e < 4; e++) above |= s[n][e] > ref[n][e & 1] + kSlack<T>;
       if (__any_sync(~0u, above)) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__(kTreeThreads, (TreeShape<T, D, NT>::kBlocks)) 
             float top = fmaxf(s[n][h], s[n][2 + h]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-            const float now = fmaxf(ref[n][h], top);
+            const float now = fmaxf(ref[n][h], top - kLift<T>);
             const float alpha = now == -INFINITY ? 1.f : exp2_(ref[n][h] - now);
             ref[n][h] = now;
             sum[n][h] *= alpha, low[n][h] *= alpha;

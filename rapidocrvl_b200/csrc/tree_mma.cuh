@@ -31,7 +31,13 @@ constexpr int kCopyWarps = 4, kCopyThreads = kCopyWarps * 32;
 constexpr int kMmaWarp = 8 + kCopyWarps;
 constexpr int kMmaThreads = (kMmaWarp + 1) * 32;
 constexpr int kMmaWaits = 1 << 20;  // polls, of up to some microseconds each, before a wait is given up
-constexpr float kMmaMost = 4096.f;   // sum of 32 weights past which the reference rises: far from f16's largest
+// The reference stands kMmaLift below the largest score when it is set, and rises once 32 weights
+// sum to more than kMmaMost: half of f16's largest for f16, whose small weights need the room
+// (kLift), with as much slack as there is left.
+template <typename T>
+constexpr float kMmaLift = std::is_same<T, __half>::value ? 6.f : 0.f;
+template <typename T>
+constexpr float kMmaMost = std::is_same<T, __half>::value ? 32768.f : 4096.f;
 
 // ---- barriers and tensor memory ------------------------------------------
 
@@ -296,7 +302,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
               for (int j = 0; j < 32; j++)
                 if (m >> j & 1) top = fmaxf(top, __uint_as_float(v[0][j]) * a.scale);
             }
-            if (ref == -INFINITY) ref = top;  // and v[0] holds the first columns again
+            if (ref == -INFINITY) ref = top - kMmaLift<T>;  // and v[0] holds the first columns again
           }
           auto tile_pass = [&](auto masked) {
             constexpr bool MASKED = decltype(masked)::value;
@@ -336,14 +342,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
                     }
                   }
                   add = add0 + add1;
-                  if (again || !__any_sync(~0u, add > kMmaMost)) break;
+                  if (again || !__any_sync(~0u, add > kMmaMost<T>)) break;
                   tc_store_wait();  // P's columns and O may have been stored a moment ago: loads are not ordered behind that
                   tc_load32(s_at + q * 32, x);  // still there
                   float top = 0.f;
 #pragma unroll
                   for (int j = 0; j < 32; j++)
                     if (!MASKED || m >> j & 1) top = fmaxf(top, fmaf(__uint_as_float(x[j]), a.scale, -base));
-                  const float down = add > kMmaMost ? ceilf(top) : 0.f, alpha = exp2_(-down);
+                  const float down = add > kMmaMost<T> ? ceilf(top) - kMmaLift<T> : 0.f, alpha = exp2_(-down);
                   ref = down > 0.f ? base + down : ref;
                   sum *= alpha, low *= alpha;
                   uint32_t w[16];

@@ -237,6 +237,14 @@ def test_long_tails_are_in_the_sum(kvops, n, most, dtype):
     assert bool(((lse - want).abs() <= 1e-5).all()), float((lse - want).abs().max())
 
 
+@pytest.mark.parametrize("n,most", [(1 << 17, 8), (1 << 20, 1)])
+def test_f16_long_tails_keep_their_weight(kvops, n, most):
+    """Weights below f16's smallest numbers reach the values too."""
+    out, _, want, _ = long_tail(kvops, torch.float16, n, most)
+    a, r = REL["f16"]
+    assert bool(((out - want).abs() <= a + r * want).all()), float((out - want).abs().max())
+
+
 # -- tables -----------------------------------------------------------------------------
 
 def test_tables_whose_rows_overlap_are_refused(kvops):
