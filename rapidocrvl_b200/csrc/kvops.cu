@@ -166,12 +166,14 @@ int64_t tree_work_bytes(const ocrvl_kv_cache *c, int sms, int rows) {
 // Tiles of the longest cache and of its drafts.
 int tree_tiles(const TreeArgs &a) { return (a.s.capacity + a.s.max_draft + kChunk - 1 + kChunk * kTileChunks - 1) / (kChunk * kTileChunks); }
 
+// What a call whose runs are joined must keep to, asked before its first launch.
+int check_combine(const TreeArgs &a, int blocks) { return (long long)blocks * a.kv_heads > 65535 ? invalid("too many kv heads") : OCRVL_OK; }
+
 // The join of runs' parts: eight rows a block, or fewer while the blocks would not fill
 // the GPU, down to one (then eight warps share a row's parts).
 template <typename T, int D>
 int launch_combine(const TreeArgs &a, int sms, int rows_max, int rows_a_block, cudaStream_t stream) {
   const int blocks = (rows_max + rows_a_block - 1) / rows_a_block, rows = rows_max < rows_a_block ? rows_max : rows_a_block;
-  if ((long long)blocks * a.kv_heads > 65535) return invalid("too many kv heads");
   int group = 8;
   while (group > 1 && (long long)((rows + group - 1) / group) * blocks * a.kv_heads * a.s.batch < 2 * sms) group /= 2;
   return launch("tree attention (join)", k_tree_combine<T, D>, dim3((rows + group - 1) / group, blocks * a.kv_heads, a.s.batch),
@@ -188,6 +190,7 @@ int launch_tree_mma(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t 
   if constexpr (!SPLIT) {
     return launch("tree attention", k_tree_mma<T, D, WIDE, false>, dim3((unsigned)segments), kMmaThreads, S::kSmem, stream, false, 1, a, blocks);
   } else {
+    if (int rc = check_combine(a, blocks)) return rc;
     const int grid = sms < kMaxRuns ? sms : kMaxRuns;
     a.start_cost = 3;
     a.joint = (int4 *)work;
@@ -239,6 +242,7 @@ int launch_tree(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   if (tiles > kFew && tiles <= 8 * kFew && segments * 8 <= clustered) return one(k_tree_attn<T, D, NT, 8>, 8);
   if (tiles <= kFew) return one(k_tree_attn<T, D, NT, 1>, 1);
 
+  if (int rc = check_combine(a, blocks)) return rc;
   const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
   a.start_cost = 1;
   a.joint = (int4 *)work;

@@ -373,3 +373,21 @@ def test_tensors_that_require_a_gradient_are_refused_and_writes_are_counted(kvop
         s.run(kvops)
         x["q"].requires_grad_()
         s.run(kvops)
+
+
+# -- refusals ---------------------------------------------------------------------------
+
+def test_too_many_kv_heads_are_refused_before_anything_runs(kvops):
+    from rapidocrvl_b200._lib import OcrvlError
+
+    heads = 70000
+    pool = torch.zeros(1, 1, heads, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros(1, 320, dtype=torch.int32, device="cuda")  # long enough to be split and joined
+    cache = kvops.PagedCache(pool[:, :, :, 0], pool[:, :, :, 1], table)
+    q = torch.zeros(1, heads, 64, dtype=torch.bfloat16, device="cuda")
+    out, lse = torch.full_like(q, 7.0), torch.full((1, heads), 7.0, device="cuda")
+    ints = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([5000], [0, 1])]
+    with pytest.raises(OcrvlError, match="heads"):
+        kvops.tree_attention(q, q, q, cache, *ints, torch.ones(1, dtype=torch.int64, device="cuda"), out=out, lse=lse)
+    torch.cuda.synchronize()
+    assert bool((out == 7).all()) and bool((lse == 7).all())
