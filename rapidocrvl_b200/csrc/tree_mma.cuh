@@ -385,7 +385,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
       sum += low;
       const int n_0 = tiles_of(0, n, rows), n_1 = tiles_of(1, n, rows);
       ends[0] += n_0 > 0, ends[1] += n_1 > 0;
-      if (n_0 && !(WIDE && s == 1)) ok = ok && bar_wait(&o_full[0], (ends[0] - 1) & 1, dead);
+      // A stream without tiles waits for the other's end: were it to arrive at o_free for pieces ahead, the
+      // phase would end while the other still reads its O.
+      if (n_0 && !(WIDE && s == 1 && n_1)) ok = ok && bar_wait(&o_full[0], (ends[0] - 1) & 1, dead);
       if (n_1 && !(WIDE && s == 0)) ok = ok && bar_wait(&o_full[1], (ends[1] - 1) & 1, dead);
       ok = __all_sync(~0u, ok);
       tc_after();

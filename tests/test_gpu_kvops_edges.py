@@ -245,6 +245,22 @@ def test_f16_long_tails_keep_their_weight(kvops, n, most):
     assert bool(((out - want).abs() <= a + r * want).all()), float((out - want).abs().max())
 
 
+# -- calls with fewer drafts than max_draft ------------------------------------------------
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("lens,counts,heads,kv_heads,most", [
+    ([16779, 9000, 16779, 300, 12000], [17, 9, 17, 1, 3], 32, 8, 64),  # up to 68 rows where 256 may come
+    ([32344, 0, 20000, 5], [1, 1, 1, 1], 32, 8, 64),
+    ([3000 + 77 * b for b in range(16)], [1 + b % 2 for b in range(16)], 16, 2, 64),
+    ([8000, 8000, 8000], [64, 1, 40], 16, 2, 64),  # blocks of 256 rows, of few, of 256 and 64
+    ([(613 * b) % 2500 for b in range(50)], [b % 3 for b in range(50)], 16, 2, None)])  # the default: the call's tokens
+def test_fewer_drafts_than_the_call_may_have(kvops, lens, counts, heads, kv_heads, most, dtype, dim):
+    s = Setup(kvops, dtype, lens, counts, heads, kv_heads, dim, seed=91)
+    wanted = want(s)
+    for _ in range(3):
+        check(s, s.run(kvops, max_draft=most), wanted)
+
+
 # -- tables -----------------------------------------------------------------------------
 
 def test_tables_whose_rows_overlap_are_refused(kvops):
