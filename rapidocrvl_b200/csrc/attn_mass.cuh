@@ -199,20 +199,17 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
         const int x = r0 + r;
         return counts(r) ? (const T *)a.q + (sh.first + x / a.group) * a.q_stride + (long long)(head * a.group + x % a.group) * D : nullptr;
       };
-      auto lse_of = [&](int r) {
-        const int x = r0 + r;
-        return counts(r) ? a.lse[(long long)(sh.first + x / a.group) * a.kv_heads * a.group + head * a.group + x % a.group] : -INFINITY;
-      };
-      auto none = [&](int r) { return lse_of(r) == -INFINITY; };  // attended nothing: adds nothing, whatever its query holds
       auto shift_of = [&](int r) {
-        const float l = lse_of(r);
-        return l == -INFINITY ? INFINITY : l * kLog2e;
+        if (!counts(r)) return INFINITY;
+        const int x = r0 + r;
+        const float l = a.lse[(long long)(sh.first + x / a.group) * a.kv_heads * a.group + head * a.group + x % a.group] * kLog2e;
+        return l == -INFINITY ? INFINITY : l;  // attended nothing
       };
       // whole pairs of tiles: rows past the last do not count
       auto tiles_of = [&](int pass) { return max(0, min(S::kRowTiles, (row_tiles - pass * S::kRowTiles + 1) / 2 * 2)); };
       if (!THIN || row_tiles) {
         const int tiles = THIN ? 1 : tiles_of(0);
-        L::query(q_at, tiles, tid, kMassThreads, query, none);
+        L::query(q_at, tiles, tid, kMassThreads, query);
         for (int r = tid; r < tiles * 8; r += kMassThreads) shift[r] = shift_of(r);
       }
       __syncthreads();
@@ -231,8 +228,10 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
         float y[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) y[e] = L::f32 ? s[e] + (c[0][e] + c[1][e]) : s[e];
-        w[0] += exp2_(fmaf(y[0], a.scale, -l0)) + exp2_(fmaf(y[1], a.scale, -l1));
-        w[1] += exp2_(fmaf(y[2], a.scale, -l0)) + exp2_(fmaf(y[3], a.scale, -l1));
+        // a row that does not count adds nothing, whatever its query and the key hold
+        auto weight = [&](float x, float l) { return l == INFINITY ? 0.f : exp2_(fmaf(x, a.scale, -l)); };
+        w[0] += weight(y[0], l0) + weight(y[1], l1);
+        w[1] += weight(y[2], l0) + weight(y[3], l1);
       };
       // a chunk's K with the tiles of rows from m on (the warp's share of them, two at once: a
       // chain of products of its own takes 11.5 ns a link)
@@ -311,7 +310,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_attn_mass(const MassArgs a,
               uint4 x[S::kItems];
               float l_next = INFINITY;
 #pragma unroll
-              for (int i = 0; i < S::kItems; i++) x[i] = L::q_fetch(at * L::kQItems + i * kMassThreads + tid, query, none);
+              for (int i = 0; i < S::kItems; i++) x[i] = L::q_fetch(at * L::kQItems + i * kMassThreads + tid, query);
               if (tid < S::kHalf * 8) l_next = shift_of(at * 8 + tid);
               if (k < nk) weigh(f, h * S::kHalf, min(tiles, (h + 1) * S::kHalf));
               __syncthreads();

@@ -117,10 +117,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_mass_mma(const MassArgs a) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4) {
               const float4 y = l4[j / 4];
-              sum0 += exp2_(fmaf(__uint_as_float(x[j]), a.scale, -y.x));
-              sum1 += exp2_(fmaf(__uint_as_float(x[j + 1]), a.scale, -y.y));
-              sum0 += exp2_(fmaf(__uint_as_float(x[j + 2]), a.scale, -y.z));
-              sum1 += exp2_(fmaf(__uint_as_float(x[j + 3]), a.scale, -y.w));
+              // a row that does not count adds nothing, whatever its query and the key hold
+              auto weight = [&](uint32_t s, float l) { return exp2_(l == INFINITY ? -INFINITY : fmaf(__uint_as_float(s), a.scale, -l)); };
+              sum0 += weight(x[j], y.x), sum1 += weight(x[j + 1], y.y);
+              sum0 += weight(x[j + 2], y.z), sum1 += weight(x[j + 3], y.w);
             }
           };
 #pragma unroll 1
@@ -164,17 +164,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_mass_mma(const MassArgs a) {
       if (rows <= 0) return true;
       bool ok = true;
       const int chunks = (sh.len + kChunk - 1) / kChunk, n = t1 - t0;
-      constexpr int kMine = S::kRows / kCopyWarps;  // the warp's rows; a lane works out every 32nd's address
-      // their lse, -inf where they do not count; what attended nothing adds nothing, whatever its query holds
-      const unsigned long long on = a.counted ? (unsigned long long)a.counted[b] : ~0ull;
-      float lse[kMine / 32];
-#pragma unroll
-      for (int x = 0; x < kMine / 32; x++) {
-        const int mine = w * kMine + x * 32 + lane, q = r0 + mine;
-        lse[x] = -INFINITY;
-        if (mine < rows && on >> (q / a.group) & 1)
-          lse[x] = __ldg(a.lse + (long long)(sh.first + q / a.group) * a.kv_heads * a.group + head * a.group + q % a.group);
-      }
       int pages = -1;  // lane i: the page of the warp's i-th chunk from the last look on
       for (int i = 0; i < n && ok; i++, tile++) {
         const uint32_t stage = tile % NS, use = tile / NS;
@@ -206,12 +195,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_mass_mma(const MassArgs a) {
         if (i == 0) {  // the rows, once the piece before has no more use for its own
           ok = __all_sync(~0u, piece == 0 || bar_wait(q_empty, (piece - 1) & 1, dead));
           if (!ok) break;
-#pragma unroll
+          const unsigned long long on = a.counted ? (unsigned long long)a.counted[b] : ~0ull;
+          constexpr int kMine = S::kRows / kCopyWarps;  // the warp's rows; a lane works out every 32nd's address
+#pragma unroll 1
           for (int x0 = 0; x0 < kMine; x0 += 32) {
             if (w * kMine + x0 >= rows) break;  // whole groups of 32
             const int mine = w * kMine + x0 + lane, q = r0 + mine;
             const char *at = nullptr;
-            if (lse[x0 / 32] != -INFINITY)
+            if (mine < rows && on >> (q / a.group) & 1)
               at = (const char *)((const T *)a.q + (sh.first + q / a.group) * a.q_stride + (long long)(head * a.group + q % a.group) * D);
 #pragma unroll 8
             for (int x = 0; x < 32; x += kAtOnce) {

@@ -194,29 +194,23 @@ struct Tile {
   }
 
   // Writes the fragments of `tiles` x 8 query rows; row(r) gives row r's address
-  // or NULL (a zero row), and drop(r) makes one zero whose values were read (so
-  // that the two need not wait for one another).  Called by a whole block of `threads`.
+  // or NULL (a zero row).  Called by a whole block of `threads`.
   //   f32: per 16 dims, two float4 a lane, the high and the low parts of row
   //   g's dims 4t .. 4t+3 (the contraction takes the dims in the order that
   //   lets K be read 16 bytes at a time).
   //   16 bits: per 16 dims, two registers a lane: row g's dims 2t, 2t+1 and 2t+8, 2t+9.
   static constexpr int kQItems = (f32 ? D / 16 : D / 32) * 32;  // 16-byte items of 8 rows
-  struct NoDrop {
-    __device__ bool operator()(int) const { return false; }
-  };
   // An item's value, and where it goes.
-  template <typename Row, typename Drop = NoDrop>
-  static __device__ __forceinline__ uint4 q_fetch(int i, Row row, Drop drop = Drop()) {
-    const int blk = i / 32 % (kQItems / 32), r = i / kQItems * 8 + ((i & 31) >> 2), t = i & 3;
-    const T *a = row(r);
-    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+  template <typename Row>
+  static __device__ __forceinline__ uint4 q_fetch(int i, Row row) {
+    const int blk = i / 32 % (kQItems / 32), g = (i & 31) >> 2, t = i & 3;
+    const T *a = row(i / kQItems * 8 + g);
     if constexpr (f32) {
-      if (a) x = *reinterpret_cast<const uint4 *>(a + blk * 16 + t * 4);
+      return a ? *reinterpret_cast<const uint4 *>(a + blk * 16 + t * 4) : make_uint4(0u, 0u, 0u, 0u);
     } else {
       const uint32_t *p = reinterpret_cast<const uint32_t *>(a) + blk * 16 + t;  // pairs of dims
-      if (a) x = make_uint4(p[0], p[4], p[8], p[12]);
+      return a ? make_uint4(p[0], p[4], p[8], p[12]) : make_uint4(0u, 0u, 0u, 0u);
     }
-    return drop(r) ? make_uint4(0u, 0u, 0u, 0u) : x;
   }
   static __device__ __forceinline__ void q_put(uint32_t dst, int i, uint4 x) {
     const int blk = i / 32 % (kQItems / 32);
@@ -231,10 +225,10 @@ struct Tile {
       sts4u(to + blk * 512, x.x, x.y, x.z, x.w);
     }
   }
-  template <typename Row, typename Drop = NoDrop>
-  static __device__ __forceinline__ void query(uint32_t dst, int tiles, int tid, int threads, Row row, Drop drop = Drop()) {
+  template <typename Row>
+  static __device__ __forceinline__ void query(uint32_t dst, int tiles, int tid, int threads, Row row) {
 #pragma unroll 4
-    for (int i = tid; i < tiles * kQItems; i += threads) q_put(dst, i, q_fetch(i, row, drop));
+    for (int i = tid; i < tiles * kQItems; i += threads) q_put(dst, i, q_fetch(i, row));
   }
   // A lane's registers of the fragments for dims 16 blk .. + 15.
   static __device__ __forceinline__ void q_load(uint32_t (&r)[kQRegs], uint32_t q, int blk, int lane) {

@@ -144,6 +144,23 @@ def test_attention_mass_of_tokens_that_attended_nothing(kvops, dtype, lens, coun
     mass_check(kvops.attention_mass(s.q, lse, s.cache, s.lens, s.indptr, scale=s.scale, max_draft=max(counts)), w)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,counts,heads", [([300, 20], [1, 1], 4), ([300, 140], [40, 3], 16)])
+def test_attention_mass_of_infinite_keys(kvops, dtype, lens, counts, heads):
+    """A key with an infinity counts with the rows that count: one whose score is -inf weighs nothing."""
+    s = Setup(kvops, dtype, lens, counts, heads=heads, seed=68)
+    _, lse = s.run(kvops)
+    s.q[..., 3] = s.q[..., 3].abs() + 0.5
+    s.cache.k[s.cache.table[0, 2], 0, 1, 5, 3] = -math.inf  # position 37: every score is -inf
+    s.cache.k[s.cache.table[1, 0], 0, 0, 2, 3] = math.inf   # every score is inf
+    got = kvops.attention_mass(s.q, lse, s.cache, s.lens, s.indptr, scale=s.scale, counted=masks([1, 1]))
+    w = mass_want(s, lse, [1, 1], width=s.cache.capacity)
+    assert float(got[0, 1, 37]) == 0 and float(w[0, 1, 37]) == 0
+    assert float(got[1, 0, 2]) == math.inf
+    got[1, 0, 2] = w[1, 0, 2] = 0
+    mass_check(got, w)
+
+
 # -- the reference's rise, rows and pages with nothing in them --------------------------
 
 # As MANY_ROWS, with several tiles a group of warps.
