@@ -348,8 +348,12 @@ int ocrvl_seq_set_position(ocrvl_seq *s, int pos);
  *   exp(scale q . k), [n_tokens][heads] f32
  * A token that attends nothing gets out = 0 and lse = -inf.  Sums, softmax
  * statistics and the output are held in 32 bits; for the 16-bit types the
- * softmax weights are rounded to the type for the product with v.  What lies in
- * masked places (NaN and infinities too) does not reach the output.
+ * softmax weights are rounded to the type for the product with v, for f32 products
+ * keep 22 bits of each factor.  What lies in masked places (NaN, infinities and
+ * the type's largest values too) does not reach the output; a value that is seen may
+ * overflow its sum from 2^-12 of bf16's and 2^-8 of f32's largest on.  max_draft
+ * and the table's width (not the lengths, which the host does not know) choose the
+ * kernel: as small as the caller's bounds are is fastest.
  * Waits within a kernel are bounded: if one ran out, the outputs that depend
  * on it are NaN (so in ocrvl_op_attn_mass).
  * work: ocrvl_op_tree_attn_workspace bytes, 128-byte aligned; its contents
@@ -366,7 +370,8 @@ int ocrvl_op_tree_attn(const ocrvl_kv_cache *c, int layer, int heads, int n_toke
  * for t < lens[b], and 0 for lens[b] <= t < out_width, so that positions
  * appended later start at 0.  q, indptr, max_draft, lens as
  * ocrvl_op_tree_attn takes them, lse as it returns it; a token whose lse is
- * -inf adds nothing.  counted (may be NULL: all): one word a sequence, bit i
+ * -inf adds nothing, whatever its q holds.  What a key holds reaches the sums of its own
+ * position alone.  counted (may be NULL: all): one word a sequence, bit i
  * counts its token i, e.g. the accepted path.  acc (may be NULL: 0) is
  * [batch][num_kv_heads] rows of acc_width values acc_stride apart, 0 past
  * acc_width; acc_out likewise, and may be acc itself with the same stride. */

@@ -13,9 +13,9 @@
 // of few tiles and many rows have a cluster of blocks a run, each with a part
 // of the rows; the parts' sums are added in order over distributed shared memory.
 //
-// f32, 64 sequences of up to 4,096 positions, one token: 38.9 us, 3.8 TB/s, bound by a warp's
+// f32, 64 sequences of up to 4,096 positions, one token: 40.2 us, 3.7 TB/s, bound by a warp's
 // work on a chunk (its split into pairs of tf32 and the three products).  131,072 positions, 64 drafts
-// of 8 heads: 558 us, 62 TFLOP/s or 185 of products, of 276 that the instruction gives.
+// of 8 heads: 580 us, 59 TFLOP/s or 178 of products, of 276 that the instruction gives.
 #pragma once
 #include <cooperative_groups.h>
 

@@ -279,7 +279,7 @@ int launch_mass(const MassArgs &a, int sms, cudaStream_t stream) {
   const int width = a.out_width < a.s.capacity ? a.out_width : a.s.capacity, row_tiles = (a.s.max_draft * a.group + 7) / 8;
   const long long tiles = (long long)a.s.batch * a.kv_heads * ((width + kMassWarps * kChunk - 1) / (kMassWarps * kChunk));
   // Up to eight rows (one token of up to eight heads, say) stay in registers.  More of 16 bits go
-  // to the fifth generation's products (4 sequences of 8,448, 32 drafts: 18.5 us here, 12.3 there),
+  // to the fifth generation's products (4 sequences of 8,448, 32 drafts: 18.5 us here, 12.7 there),
   // and so do eight where the blocks have many tiles each (bf16, 64 of 4,000: 40 and 31
   // us, one of 131,072: 18.7 and 16.6; but 16 of 2,000: 10.4 and 11.0, one of 700: 6.5 and 8.2).
   if constexpr (sizeof(T) == 2) {
@@ -291,7 +291,7 @@ int launch_mass(const MassArgs &a, int sms, cudaStream_t stream) {
       return launch("attention mass", k_attn_mass<T, D, true>, dim3(sms), kMassThreads, MassShape<T, D, true>::kSmem, stream, false, 1, a, 1);
     // A cluster a run, each block with a part of the rows, while all the call's tiles of 128
     // positions are in one wave of blocks and a part has about four tiles of eight rows: one
-    // sequence of 700, 64 drafts: 68 us alone, 41, 25 and 20.5 in clusters of 2, 4 and 8; of
+    // sequence of 700, 64 drafts: 68 us alone, 41, 25 and 20.8 in clusters of 2, 4 and 8; of
     // 3000: 68 and 41, but 54 in 4, now two waves; 5 drafts: 13.5 and 12.3.
     int parts = 1;
     while (parts < 8 && tiles * parts * 2 <= (parts == 1 ? sms : cluster_room(sms)) && row_tiles + 3 >= parts * 2 * 4) parts *= 2;

@@ -10,9 +10,9 @@
 // by the exponentials: 128 rows a tile take 1,024 cycles of an SM's 16 a cycle.  All waits are
 // bounded: what a block gave up is NaN.
 //
-// bf16, 131,072 positions, 64 drafts of 8 heads: 58 us, 590 TFLOP/s (30 us of it exponentials; K is
+// bf16, 131,072 positions, 64 drafts of 8 heads: 62 us, 550 TFLOP/s (30 us of it exponentials; K is
 // read twice); 64 sequences of 4,000, one token: 31 us, 4.2 TB/s; 4 of up to 8,448, 32 drafts:
-// 12.3 us, a launch and the first loads of Q and K.
+// 12.7 us, a launch and the first loads of Q and K.
 #pragma once
 #include "attn_mass.cuh"
 #include "tree_mma.cuh"

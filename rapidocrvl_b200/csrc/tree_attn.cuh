@@ -10,7 +10,8 @@
 // m follows the running maximum, but only once a score passes it by kSlack:
 //   m' = max(m, max s),  l and o times 2^(m - m')      (f16: max s - kLift)
 // so most chunks need no maximum over lanes and no rescaling, and p stays below
-// 2^kSlack.  At the run's end the warps are joined: o = sum_w 2^(m_w - M) o_w,
+// 2^kSlack; a value within that factor of the type's largest (f32 and bf16) may
+// overflow its sum.  At the run's end the warps are joined: o = sum_w 2^(m_w - M) o_w,
 // l likewise.
 //
 // A (sequence, kv head, row block) is a segment.  Two ways to share them out:
@@ -24,11 +25,12 @@
 //           memory: one launch, no workspace, no search for the run's start.
 //           For calls whose segments and lengths are few.
 //
-// 64 sequences of up to 4,096 positions, one token, f32: 59.6 us, 4.9 TB/s of K
+// 64 sequences of up to 4,096 positions, one token, f32: 60.3 us, 4.8 TB/s of K
 // and V, bound by a warp's work on a chunk (the split into pairs of tf32 and three
-// products of each, 1.2 us); 648 positions of one sequence: 9 us, bound by a
-// launch and two loads behind one another; 8 sequences of up to 4,095 with 12 drafts: 37.5 us,
-// bound by the products of three blocks of 32 rows.
+// products of each, 1.2 us), bf16 39.0; 648 positions of one sequence: 9 us, bound by a
+// launch and two loads behind one another; 8 sequences of up to 4,095 with 12 drafts: 41.4 us,
+// 16 of 3,000 with 64 549, bound by the products of blocks of 32 rows, each of which reads
+// and splits K and V again.
 #pragma once
 #include <cooperative_groups.h>
 

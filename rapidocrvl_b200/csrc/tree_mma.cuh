@@ -16,10 +16,10 @@
 // pay), warp 12 issues the products.  All waits are bounded: a block that
 // gives one up writes NaN.
 //
-// 131,071 positions, 64 drafts of 8 heads, bf16: 107 us, 640 TFLOP/s: tensor cores and
-// exponentials (16 a cycle and SM) are each busy for 36 % of it, bound by the chain of a stream
+// 131,071 positions, 64 drafts of 8 heads, bf16: 109 us, 630 TFLOP/s: tensor cores and
+// exponentials (16 a cycle and SM) are each busy for 35 % of it, bound by the chain of a stream
 // (S, its softmax by one warp an SM quarter, P, O) that the other one covers in part.
-// 8 sequences of up to 8,448, 16 drafts: 29 us, 1.4 TB/s, seven tiles a block and half of it
+// 8 sequences of up to 8,448, 16 drafts: 29 us, 1.3 TB/s, four tiles a block: most of it is
 // the start, the end and the join.  16 of 4,000, 64 drafts, a block a segment of 128 rows: 53 us.
 #pragma once
 #include "tree_attn.cuh"
@@ -140,9 +140,8 @@ __device__ __forceinline__ bool softmax_any(bool x) {
 
 // ---- products -----------------------------------------------------------------
 
-// One lane of the converged warp.  Under this predicate the compiler keeps the
-// products' descriptors in uniform registers: 64 cycles a product of N = 128, the
-// tensor cores' own rate, against 80 to 88 behind a test of the lane.
+// One lane of the converged warp.  Behind this predicate a product of N = 128 was measured at 64
+// cycles, the tensor cores' own rate, against 80 to 88 behind a test of the lane.
 __device__ __forceinline__ bool elected() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}\n" : "=r"(p));

@@ -99,8 +99,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Pag
     int32 bounds each sequence's tokens, ``lens`` [batch] int32 are the cached
     lengths.  ``mask`` [tokens] int64: bit j lets the token attend its
     sequence's token j, its own included only if set (-1: all).  ``max_draft``
-    bounds the tokens of a sequence (64 at most, which is the default; more
-    are not computed and their outputs not written).  ``work``: a uint8 tensor
+    bounds the tokens of a sequence (64 at most; the default is the call's tokens, up to
+    64; more are not computed and their outputs not written): name the smallest that
+    holds, kernels are chosen by it.  ``work``: a uint8 tensor
     of ``cache.work_bytes(heads, max_draft)``, else one is taken from torch's allocator.
 
     Returns (out, lse): out like q, lse [tokens, heads] f32.  A token that
@@ -131,7 +132,8 @@ def select(cache: PagedCache, acc: torch.Tensor, lens: torch.Tensor, *, keep: in
     """The positions that a cut to ``keep`` leaves of each layer, sequence and
     kv head: all where the length is at most ``keep``, else the first ``sinks``,
     the last ``recent`` and of the others those with the largest sums, the lower
-    position first among equals.  ``acc`` [layers, batch, kv heads, width] f32.
+    position first among equals.  ``acc`` [layers, batch, kv heads, width] f32; of a
+    length above the width the first ``width`` positions count.
 
     Returns (idx, sums, new_lens): idx [layers, batch, kv heads, keep] int32 in
     rising order, -1 past the count, with their sums (0 there), and [batch]
