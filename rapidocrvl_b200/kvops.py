@@ -69,8 +69,9 @@ class PagedCache:
     @classmethod
     def of_sequence(cls, seq) -> "PagedCache":
         """The cache of an engine sequence (``Runtime.new_sequence``): f32,
-        every layer, one table row.  It stays valid while the sequence lives;
-        order work on it against ``Runtime.stream_handle`` (the engine's calls
+        every layer, one table row.  It stays valid while the sequence lives, its
+        table follows the sequence, and positions past it are unmapped (``append`` is for
+        caches of the caller's own); order work on it against ``Runtime.stream_handle`` (the engine's calls
         wait for their own work before they return)."""
         self = cls.__new__(cls)
         d = _lib.KVCache()
