@@ -359,6 +359,30 @@ def test_evict_into_too_little_room_is_refused(kvops, keep):
     assert new.tolist() == [40]
 
 
+# -- large pools --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_pages_past_32_bits(kvops, dtype):
+    """Pages that lie 5 GB behind the start of the pool."""
+    s = Setup(kvops, dtype, [700, 3000, 33], [16, 1, 40], heads=8, kv_heads=2, seed=95, room=64, junk=2.0)
+    pages, far = s.pool.shape[0], -(-(5 << 30) // s.pool[0].nbytes)
+    big = torch.empty((far + pages,) + s.pool.shape[1:], dtype=s.dtype, device="cuda")
+    big[far:] = s.pool
+    moved = torch.where(s.table_h >= 0, s.table_h + far, s.table_h)
+    cache = kvops.PagedCache(big[:, :, :, 0], big[:, :, :, 1], moved.cuda())
+    near = s.cache, s.pool
+    results = []
+    for c, pool in (near, (cache, big[far:])):
+        s.cache = c
+        out, lse = s.run(kvops)
+        mass = kvops.attention_mass(s.q, lse, c, s.lens, s.indptr, scale=s.scale)
+        new = kvops.append(c, s.k[None], s.v[None], s.lens, s.indptr)
+        kept = kvops.evict(c, mass[None], s.lens, keep=100, sinks=2, recent=5)
+        results.append((out, lse, mass, new, *kept, pool))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 # -- autograd ---------------------------------------------------------------------------
 
 def _calls(kvops, s, into):
