@@ -422,6 +422,84 @@ int ocrvl_op_kv_append(const ocrvl_kv_cache *c, int n_tokens, const int32_t *len
                        const int32_t *path, const int32_t *n_path, int max_path, const void *k, const void *v,
                        int64_t kv_stride, int64_t kv_layer_stride, int32_t *new_lens, void *stream);
 
+/* ---- packed cache ---------------------------------------------------------
+ * A paged cache that holds K and V in 4 bits, 4.5 with its scales, and what a
+ * step of a host that keeps one calls (no reference counterpart).  Pointers,
+ * streams and lengths as above: nothing is allocated or waited for.
+ *
+ * 32 consecutive dims of a position's key (or value) share a scale s, each is
+ * c s with a whole number c of -7 .. 7:
+ *   s = max |x| / 7 to the nearest number of five significant bits (of two the even
+ *       one); 0 where that is below 2^-126; NaN where the 32 are not all finite
+ *   c = x / s to the nearest whole number (of two the even one); 0 where s is 0 or NaN
+ * so an error is at most s / 2 and every c s is exactly a bf16 number.
+ * Position t, kv head h of sequence b, layer l has its D / 2 bytes of codes at
+ *   page * page_stride + l * layer_stride + h * head_stride + (t % page_size) * D / 2
+ * of k and of v, and its D / 32 scales (bf16) at
+ *   page * scale_page_stride + l * scale_layer_stride + h * scale_head_stride
+ *     + (t % page_size) * D / 32
+ * of k_scale and v_scale, where page = table[b * table_stride + t / page_size].
+ * c + 8 of dim d is nibble d % 4 (the lowest first) of the row's 16-bit word
+ * (d / 4 % 8) (D / 32) + d / 32, so that all groups' dims for a lane of the matrix
+ * instructions lie together.  Scales of more than five bits are rounded in products. */
+typedef struct ocrvl_packed_cache {
+  int32_t head_dim;     /* 64 or 128 */
+  int32_t num_kv_heads;
+  int32_t num_layers;
+  int32_t page_size;    /* positions a page: a power of two, at least 16 */
+  int32_t num_pages;
+  int32_t batch;        /* rows of the table */
+  int32_t max_pages;    /* entries a row */
+  int32_t reserved;     /* 0 */
+  int64_t page_stride, layer_stride, head_stride;                   /* bytes; multiples of 16 */
+  int64_t scale_page_stride, scale_layer_stride, scale_head_stride; /* scales; multiples of 8 */
+  int64_t table_stride; /* entries */
+  void *k, *v, *k_scale, *v_scale; /* 16-byte aligned */
+  const int32_t *table;
+} ocrvl_packed_cache;
+
+/* ocrvl_op_kv_append into a packed cache: the tokens are quantised as they are
+ * written.  type: of k and v (OCRVL_F32, OCRVL_F16 or OCRVL_BF16). */
+int ocrvl_op_packed_append(const ocrvl_packed_cache *c, int type, int n_tokens, const int32_t *lens, const int32_t *indptr,
+                           const int32_t *path, const int32_t *n_path, int max_path, const void *k, const void *v,
+                           int64_t kv_stride, int64_t kv_layer_stride, int32_t *new_lens, void *stream);
+
+/* Reads positions back, all layers: position lens[b] + i becomes token
+ * indptr[b] + i of k and v ([num_layers][n_tokens][num_kv_heads][head_dim] of `type`,
+ * strides as in append), for all of the sequence's tokens: what an append of the same lens and
+ * indptr wrote.  c s is rounded once for f16 and not at all for the others.  A position without
+ * a page, or past the table, reads as 0; tokens of no sequence are left as they were. */
+int ocrvl_op_packed_read(const ocrvl_packed_cache *c, int type, int n_tokens, const int32_t *lens, const int32_t *indptr,
+                         void *k, void *v, int64_t kv_stride, int64_t kv_layer_stride, void *stream);
+
+/* Rotary positions.  Pair p < pairs is dims p and p + pairs, or 2 p and 2 p + 1
+ * (neighbours); its angle is freq[p] times the token's position on axis[p].
+ * Dims behind 2 pairs are not rotated. */
+typedef struct ocrvl_rotary {
+  int32_t head_dim;   /* a multiple of 8, at most 256 */
+  int32_t pairs;      /* a multiple of 4, at most head_dim / 2 */
+  int32_t num_axes;   /* of a token's position: 1 to 8 */
+  int32_t neighbours; /* 0 or 1 */
+  double freq[128];   /* radians a position */
+  uint8_t axis[128];
+} ocrvl_rotary;
+
+/* Queries and keys of new tokens, normed (where there is a weight) and rotated
+ * (buildMRoPETable and the rotation of a step, internal/model/model.go:7318-7357, for
+ * any number of tokens, axes and head sizes):
+ *   y = x / sqrt(mean x^2 + eps) * weight over a head's dims, then for each pair
+ *   (u, v) -> (u cos - v sin, v cos + u sin)
+ * q and k are [n_tokens][heads][head_dim] with a stride in elements between tokens
+ * (a multiple of 16 bytes; 16-byte aligned), and so are q_out and k_out, which are q and k
+ * themselves or share nothing with either.  k may be NULL.  pos: num_axes int32 a token,
+ * pos_stride entries apart.  q_weight, k_weight: [head_dim] of weight_type (OCRVL_F32 or
+ * `type`; 16-byte aligned), both or (k NULL) the first, or NULL: no norm.
+ * Angles are worked out in 64 bits, the rest in 32, each value is rounded once. */
+int ocrvl_op_rotate(const ocrvl_rotary *r, int type, int n_tokens, const int32_t *pos, int64_t pos_stride, int heads,
+                    const void *q, int64_t q_stride, void *q_out, int64_t q_out_stride, int kv_heads, const void *k,
+                    int64_t k_stride, void *k_out, int64_t k_out_stride, int weight_type, const void *q_weight,
+                    const void *k_weight, float eps, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

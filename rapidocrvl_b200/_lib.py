@@ -67,6 +67,30 @@ class KVCache(C.Structure):
     ]
 
 
+class PackedCache(C.Structure):
+    """ocrvl_packed_cache: a 4-bit paged cache's addressing."""
+
+    _fields_ = [
+        *((n, C.c_int32) for n in ("head_dim", "num_kv_heads", "num_layers", "page_size", "num_pages", "batch", "max_pages", "reserved")),
+        *((n, C.c_int64) for n in ("page_stride", "layer_stride", "head_stride", "scale_page_stride", "scale_layer_stride",
+                                   "scale_head_stride", "table_stride")),
+        *((n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "table")),
+    ]
+
+
+class Rotary(C.Structure):
+    """ocrvl_rotary: which dims turn by which position, and how fast."""
+
+    _fields_ = [
+        ("head_dim", C.c_int32),
+        ("pairs", C.c_int32),
+        ("num_axes", C.c_int32),
+        ("neighbours", C.c_int32),
+        ("freq", C.c_double * 128),
+        ("axis", C.c_uint8 * 128),
+    ]
+
+
 # name -> (restype, argtypes); the exported symbol set of include/ocrvl_cuda.h
 P, I, I64, F = C.c_void_p, C.c_int, C.c_int64, C.c_float
 SIGNATURES = {
@@ -113,6 +137,9 @@ SIGNATURES = {
     "ocrvl_op_kv_compact": (I, [C.POINTER(KVCache), C.POINTER(KVCache), P, I, P]),
     "ocrvl_op_kv_evict": (I, [C.POINTER(KVCache), C.POINTER(KVCache), P, I, I64, P, I, I, I, P, P, P, P]),
     "ocrvl_op_kv_append": (I, [C.POINTER(KVCache), I, P, P, P, P, I, P, P, I64, I64, P, P]),
+    "ocrvl_op_packed_append": (I, [C.POINTER(PackedCache), I, I, P, P, P, P, I, P, P, I64, I64, P, P]),
+    "ocrvl_op_packed_read": (I, [C.POINTER(PackedCache), I, I, P, P, P, P, I64, I64, P]),
+    "ocrvl_op_rotate": (I, [C.POINTER(Rotary), I, I, P, I64, I, P, I64, P, I64, I, P, I64, P, I64, I, P, P, F, P]),
 }
 
 

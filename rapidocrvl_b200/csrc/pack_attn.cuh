@@ -1,0 +1,697 @@
+// Attention of drafted tokens over a packed cache and over one another
+// (ocrvl_op_packed_attn where a kv head has few rows, and for f32 with any number).
+//
+// The mathematics, segments and runs are tree_attn.cuh's; only the cache is read in another way.
+// The 16 positions of a chunk are the rows of the matrix instruction, 8 query rows its
+// columns.  Codes become 16-bit numbers in registers: a nibble at the top of the mantissa of 16
+// is 16 + (c + 8), so
+//   K   q . (16 + c + 8) - 24 sum q, the sum as the accumulator's first value, a group of 32 dims at a time, then
+//       times the group's scale in 32 bits (f32: the 24 taken off the codes, so that nothing cancels)
+//   V   (24 + c) s - 24 s in one fused step, exact: c s and 24 s are bf16 numbers
+// f32 queries and weights are three bf16 parts (all 24 bits), so their products with codes are
+// exact and only sums are rounded.  A lane finds all that it needs of a row in one piece: of K, dims
+// 32 j + 8 t .. + 7 of each group j, of V, dims 32 j + 4 g .. + 3 (g = lane / 4, t = lane % 4).  The chunk's
+// positions are the instruction's rows in the order 0 1 4 5 8 9 12 13, 2 3 6 7 10 11 14 15, so that a
+// lane's four positions of V, and their scales, are neighbours.
+#pragma once
+#include "packed.cuh"
+#include "tree_attn.cuh"
+
+namespace ocrvl {
+namespace paged {
+
+template <typename T>
+using Product = std::conditional_t<std::is_same<T, __half>::value, __half, __nv_bfloat16>;  // the products' type
+
+// Nibble i of both halfwords as 16 + nibble, two numbers of B.
+template <typename B>
+__device__ __forceinline__ uint32_t lifted(uint32_t x, int i) {
+  if constexpr (std::is_same<B, __half>::value)
+    return ((i < 2 ? x << (6 - 4 * i) : x >> (4 * i - 6)) & 0x03c003c0u) | 0x4c004c00u;
+  else
+    return ((i < 1 ? x << 3 : x >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
+}
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
+  return *reinterpret_cast<uint32_t *>(&r);
+}
+template <typename B>
+struct Two;
+template <>
+struct Two<__half> {
+  using V = __half2;
+};
+template <>
+struct Two<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+};
+template <typename B>
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+  using V = typename Two<B>::V;
+  V r = __hfma2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b), *reinterpret_cast<V *>(&c));
+  return *reinterpret_cast<uint32_t *>(&r);
+}
+template <typename B>
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  using V = typename Two<B>::V;
+  V r = __hmul2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b));
+  return *reinterpret_cast<uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+__device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, int high) { return high ? high_halves(a, b) : low_halves(a, b); }
+
+// x as three bf16 numbers, in the upper halves: exact (8 bits each, cut, so that none is rounded up to
+// infinity); what is not finite is the last one's alone, so that it meets nothing but another's first part.
+__device__ __forceinline__ void split3(float x, uint32_t (&p)[3]) {
+  const uint32_t hi = __float_as_uint(x) & 0xffff0000u;
+  const float r = x - __uint_as_float(hi);
+  const uint32_t mid = __float_as_uint(r) & 0xffff0000u;
+  const bool finite = (hi & 0x7f800000u) != 0x7f800000u;
+  p[0] = finite ? hi : 0u, p[1] = finite ? mid : 0u;
+  p[2] = finite ? __float_as_uint(r - __uint_as_float(mid)) : __float_as_uint(x) | ((__float_as_uint(x) & 0x7fffffu) ? 0x400000u : 0u);
+}
+
+template <typename T, int D>
+struct PackTile {
+  using B = Product<T>;
+  static constexpr bool f32 = sizeof(T) == 4;
+  static constexpr int G = D / 32;                     // groups of a row
+  static constexpr int kParts = f32 ? 3 : 1;
+  static constexpr int kCodes = kChunk * D / 2;        // bytes of a chunk's K or V
+  static constexpr int kScales = kChunk * G * 2;
+  static constexpr int kStage = 2 * (kCodes + kScales);  // K, V, their scales
+  static constexpr int kQBytes = kParts * G * 512;     // fragments of 8 query rows: [part][group][lane] of 16 bytes
+  static constexpr int kTiles = D / 16;
+
+  // Where 16-byte piece x of a position's row lies: exchanged so that the fragment loads of a warp (K: rows 0 1 4 5
+  // .., V: a row of every four) hit different banks.
+  static __device__ __forceinline__ int k_at(int row, int x) {
+    return D == 128 ? row * 64 + x * 16 : (row ^ (row >> 2 & 1) << 1) * 32 + x * 16;
+  }
+  static __device__ __forceinline__ int v_at(int row, int x) {
+    return D == 128 ? (row ^ (row >> 2 & 1)) * 64 + (x ^ (row >> 3 & 1) << 1) * 16 : (row ^ (row >> 2 & 3)) * 32 + x * 16;
+  }
+  // A warp's copies of a chunk.
+  static __device__ __forceinline__ void load(uint32_t to, const char *k, const char *v, const char *ks, const char *vs, int lane) {
+#pragma unroll
+    for (int i = 0; i < kCodes / 512; i++) {
+      const int p = i * 32 + lane, row = p / (D / 32), x = p % (D / 32);
+      copy16(to + k_at(row, x), k + p * 16);
+      copy16(to + kCodes + v_at(row, x), v + p * 16);
+    }
+    constexpr int kPieces = kScales / 16;
+    if (lane < 2 * kPieces) copy16(to + 2 * kCodes + lane * 16, lane < kPieces ? ks + lane * 16 : vs + (lane - kPieces) * 16);
+  }
+
+  // The position of row g of the matrix instruction; row g + 8 has that plus 2.
+  static __device__ __forceinline__ int position(int g) { return 4 * (g >> 1) + (g & 1); }
+
+  // ---- fragments of 8 consecutive dims (a query row's, or a drafted key's): pairs (i, 4 + i)
+  static __device__ __forceinline__ void pairs8(uint32_t (&f)[kParts][4], const T *p) {
+    if (!p) {
+#pragma unroll
+      for (int w = 0; w < kParts; w++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[w][i] = 0u;
+    } else if constexpr (f32) {
+      const float4 a = __ldg((const float4 *)p), b = __ldg((const float4 *)p + 1);
+      const float x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        uint32_t u[3], v[3];
+        split3(x[i], u), split3(y[i], v);
+#pragma unroll
+        for (int w = 0; w < 3; w++) f[w][i] = high_halves(u[w], v[w]);
+      }
+    } else {
+      const uint4 a = __ldg((const uint4 *)p);
+      f[0][0] = low_halves(a.x, a.z), f[0][1] = high_halves(a.x, a.z);
+      f[0][2] = low_halves(a.y, a.w), f[0][3] = high_halves(a.y, a.w);
+    }
+  }
+  static __device__ __forceinline__ float sum8(const T *p) {
+    if (!p) return 0.f;
+    float x[8], s = 0.f;
+    load8(x, p);
+#pragma unroll
+    for (int i = 0; i < 8; i++) s += x[i];
+    return s;
+  }
+
+  // ---- cached keys: s of NT x 8 rows.  q: the fragments' address; qr: they themselves (NT = 1, 16 bits); first: the
+  // accumulators' first values of a lane's two rows, in memory [row][group], or the registers fr.
+  template <int NT, bool REGS>
+  static __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&qr)[REGS ? G : 1][4], const float (&fr)[REGS ? G : 1][2],
+                                                uint32_t q, const float *first, uint32_t st, int lane) {
+    const int g = lane >> 2, t = lane & 3, p0 = position(g);
+    uint32_t k[2][4], ks[2][2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+      const int pos = p0 + 2 * r;
+      const uint32_t at = st + 2 * kCodes + pos * (G * 2);
+      if constexpr (D == 128) {
+        lds4u(k[r], st + k_at(pos, t));
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(ks[r][0]), "=r"(ks[r][1]) : "r"(at));
+      } else {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(k[r][0]), "=r"(k[r][2]) : "r"(st + k_at(pos, t >> 1) + (t & 1) * 8));
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(ks[r][0]) : "r"(at));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[n][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+      const uint32_t x0 = halves(k[0][j >> 1], k[0][2 + (j >> 1)], j & 1), x1 = halves(k[1][j >> 1], k[1][2 + (j >> 1)], j & 1);
+      uint32_t a[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        a[h][0] = lifted<B>(x0, 2 * h), a[h][1] = lifted<B>(x1, 2 * h);
+        a[h][2] = lifted<B>(x0, 2 * h + 1), a[h][3] = lifted<B>(x1, 2 * h + 1);
+        if constexpr (f32) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) a[h][i] = sub2(a[h][i], 0x41c041c0u);  // 24: the codes themselves
+        }
+      }
+      const float s0 = __uint_as_float(j & 1 ? ks[0][j >> 1] & 0xffff0000u : ks[0][j >> 1] << 16);
+      const float s1 = __uint_as_float(j & 1 ? ks[1][j >> 1] & 0xffff0000u : ks[1][j >> 1] << 16);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        float p[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (f32) {
+#pragma unroll
+          for (int w = 2; w >= 0; w--) {
+            uint32_t b[4];
+            lds4u(b, q + n * kQBytes + (w * G + j) * 512 + lane * 16);
+            mma_16<B>(p, a[0], b[0], b[1]);
+            mma_16<B>(p, a[1], b[2], b[3]);
+          }
+        } else {
+          uint32_t b[4];
+          if constexpr (REGS) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) b[i] = qr[j][i];
+            p[0] = p[2] = fr[j][0], p[1] = p[3] = fr[j][1];
+          } else {
+            lds4u(b, q + n * kQBytes + j * 512 + lane * 16);
+            p[0] = p[2] = first[(n * 8 + 2 * t) * G + j], p[1] = p[3] = first[(n * 8 + 2 * t + 1) * G + j];
+          }
+          mma_16<B>(p, a[0], b[0], b[1]);
+          mma_16<B>(p, a[1], b[2], b[3]);
+        }
+        s[n][0] = fmaf(s0, p[0], s[n][0]), s[n][1] = fmaf(s0, p[1], s[n][1]);
+        s[n][2] = fmaf(s1, p[2], s[n][2]), s[n][3] = fmaf(s1, p[3], s[n][3]);
+      }
+    }
+  }
+
+  // ---- drafted keys: rows of T, `valid` of the 16 there
+  template <int NT>
+  static __device__ __forceinline__ void draft_scores(float (&s)[NT][4], uint32_t q, const T *rows, long long stride, int valid, int lane) {
+    const int g = lane >> 2, t = lane & 3, p0 = position(g);
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) s[n][e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+      uint32_t f0[kParts][4], f1[kParts][4];
+      pairs8(f0, p0 < valid ? rows + p0 * stride + 32 * j + 8 * t : nullptr);
+      pairs8(f1, p0 + 2 < valid ? rows + (p0 + 2) * stride + 32 * j + 8 * t : nullptr);
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+        // f32: the products of parts whose places add up to two at most, the small ones first
+#pragma unroll
+        for (int both = kParts - 1; both >= 0; both--)
+#pragma unroll
+          for (int w = 0; w <= both; w++) {
+            uint32_t b[4];
+            lds4u(b, q + n * kQBytes + (w * G + j) * 512 + lane * 16);
+            const int x = both - w;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const uint32_t a[4] = {f0[x][2 * h], f1[x][2 * h], f0[x][2 * h + 1], f1[x][2 * h + 1]};
+              mma_16<B>(s[n], a, b[2 * h], b[2 * h + 1]);
+            }
+          }
+    }
+  }
+
+  // The weights of a chunk (as scores leaves them) as the products' second operand.
+  template <int NT>
+  static __device__ __forceinline__ void weights(uint32_t (&b)[kParts][NT][2], const float (&p)[NT][4]) {
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        if constexpr (f32) {
+          uint32_t u[3], v[3];
+          split3(p[n][2 * r], u), split3(p[n][2 * r + 1], v);
+#pragma unroll
+          for (int w = 0; w < 3; w++) b[w][n][r] = transpose8(high_halves(u[w], v[w]));
+        } else {
+          b[0][n][r] = transpose8(pack2(p[n][2 * r], p[n][2 * r + 1], T()));
+        }
+      }
+  }
+
+  // o += v' p over the chunk; tile 2 j + h of o has dims 32 j + 4 g + 2 h (elements 0, 1) and the next (2, 3).
+  template <int NT>
+  static __device__ __forceinline__ void values(float (&o)[kTiles][NT][4], const uint32_t (&b)[kParts][NT][2], uint32_t st, int valid, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    uint32_t v[4][2], vs[4][2];  // of positions 4 t + i
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if constexpr (D == 128)
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[i][0]), "=r"(v[i][1]) : "r"(st + kCodes + v_at(4 * t + i, g >> 1) + (g & 1) * 8));
+      else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i][0]) : "r"(st + kCodes + v_at(4 * t + i, g >> 2) + (g & 3) * 4));
+    }
+    const uint32_t at = st + 2 * kCodes + kScales + t * (8 * G);
+    uint32_t x[4];
+    lds4u(x, at);
+    if constexpr (D == 128) {
+      vs[0][0] = x[0], vs[0][1] = x[1], vs[1][0] = x[2], vs[1][1] = x[3];
+      lds4u(x, at + 16);
+      vs[2][0] = x[0], vs[2][1] = x[1], vs[3][0] = x[2], vs[3][1] = x[3];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) vs[i][0] = x[i];
+    }
+    if (valid < kChunk) {  // what lies behind the end may hold anything
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int w = 0; w < (G + 1) / 2; w++) vs[i][w] = 4 * t + i < valid ? vs[i][w] : 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+      uint32_t s01 = halves(vs[0][j >> 1], vs[1][j >> 1], j & 1), s23 = halves(vs[2][j >> 1], vs[3][j >> 1], j & 1);
+      if constexpr (std::is_same<B, __half>::value) {
+        s01 = pack2(__uint_as_float(s01 << 16), __uint_as_float(s01 & 0xffff0000u), B());
+        s23 = pack2(__uint_as_float(s23 << 16), __uint_as_float(s23 & 0xffff0000u), B());
+      }
+      constexpr uint32_t minus24 = std::is_same<B, __half>::value ? 0xce00ce00u : 0xc1c0c1c0u;
+      const uint32_t n01 = mul2<B>(s01, minus24), n23 = mul2<B>(s23, minus24);
+      const uint32_t x01 = halves(v[0][j >> 1], v[1][j >> 1], j & 1), x23 = halves(v[2][j >> 1], v[3][j >> 1], j & 1);
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t a[4] = {fma2<B>(lifted<B>(x01, 2 * h), s01, n01), fma2<B>(lifted<B>(x01, 2 * h + 1), s01, n01),
+                               fma2<B>(lifted<B>(x23, 2 * h), s23, n23), fma2<B>(lifted<B>(x23, 2 * h + 1), s23, n23)};
+        product<NT, 1>(o[2 * j + h], &a, b);
+      }
+    }
+  }
+
+  // o of a tile += a of PARTS parts times the weights.  f32: summed apart and added in one rounded addition, since
+  // the matrix instruction's own sums are cut, not rounded, which over thousands of chunks would add up.
+  template <int NT, int PARTS>
+  static __device__ __forceinline__ void product(float (&o)[NT][4], const uint32_t (*a)[4], const uint32_t (&b)[kParts][NT][2]) {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      if constexpr (f32) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int both = 2; both >= 0; both--)
+#pragma unroll
+          for (int w = 0; w <= both; w++)
+            if (both - w < PARTS) mma_16<B>(sum, a[both - w], b[w][n][0], b[w][n][1]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[n][e] += sum[e];
+      } else {
+        mma_16<B>(o[n], a[0], b[0][n][0], b[0][n][1]);
+      }
+    }
+  }
+
+  // The same for drafted values; true if some are not finite: those count as 0 here.
+  template <int NT>
+  static __device__ __forceinline__ bool draft_values(float (&o)[kTiles][NT][4], const uint32_t (&b)[kParts][NT][2], const T *rows,
+                                                      long long stride, int valid, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+      uint32_t f[kParts][4][2];  // [part][dim of 4 g ..][positions 4 t, 4 t + 1; 4 t + 2, 4 t + 3]
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        const int p = 4 * t + 2 * r;
+        const T *at = rows + p * stride + 32 * j + 4 * g;
+        if constexpr (f32) {
+          const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 x4 = p < valid ? __ldg((const float4 *)at) : zero, y4 = p + 1 < valid ? __ldg((const float4 *)(at + stride)) : zero;
+          float x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+          for (int d = 0; d < 4; d++) {
+            if (!isfinite(x[d])) x[d] = 0.f, bad = true;
+            if (!isfinite(y[d])) y[d] = 0.f, bad = true;
+            uint32_t u[3], w[3];
+            split3(x[d], u), split3(y[d], w);
+#pragma unroll
+            for (int i = 0; i < 3; i++) f[i][d][r] = high_halves(u[i], w[i]);
+          }
+        } else {
+          const uint2 zero = make_uint2(0u, 0u);
+          const uint2 x = p < valid ? __ldg((const uint2 *)at) : zero, y = p + 1 < valid ? __ldg((const uint2 *)(at + stride)) : zero;
+          f[0][0][r] = low_halves(x.x, y.x), f[0][1][r] = high_halves(x.x, y.x);
+          f[0][2][r] = low_halves(x.y, y.y), f[0][3][r] = high_halves(x.y, y.y);
+          constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+#pragma unroll
+          for (int d = 0; d < 4; d++) {
+            if ((f[0][d][r] & e) == e) f[0][d][r] &= 0xffff0000u, bad = true;
+            if ((f[0][d][r] >> 16 & e) == e) f[0][d][r] &= 0xffffu, bad = true;
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        uint32_t a[kParts][4];
+#pragma unroll
+        for (int w = 0; w < kParts; w++)
+          a[w][0] = f[w][2 * h][0], a[w][1] = f[w][2 * h + 1][0], a[w][2] = f[w][2 * h][1], a[w][3] = f[w][2 * h + 1][1];
+        product<NT, kParts>(o[2 * j + h], a, b);
+      }
+    }
+    return __any_sync(~0u, bad);
+  }
+};
+
+template <typename T, int D, int NT>
+struct PackShape {
+  using L = PackTile<T, D>;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kBlocks = NT == 1 || (sizeof(T) == 2 && NT == 2) ? 2 : 1;  // an SM
+  static constexpr int kStages = kBlocks == 2 ? 4 : 6;  // chunks of a warp on their way or in use
+  static constexpr int kRing = kTreeWarps * kStages * L::kStage;
+  static constexpr int kJoin = kTreeWarps * 8 * D * 4;  // eight rows of every warp
+  static constexpr int kQ = NT * L::kQBytes;
+  static constexpr bool kQInRegs = NT == 1 && sizeof(T) == 2;
+  static constexpr int kFirst = kRows * L::G * 4;
+  static constexpr int kSmem = kRing + kJoin + kQ + kFirst + kTreeWarps * kRows * 8 + kRows * 8 + 64 + kTreeWarps * 8 * 4 + kRows * 8;
+};
+
+template <typename T, int D, int NT, int CS>
+__global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) k_pack_attn(const TreeArgs a, int row_blocks) {
+  using S = PackShape<T, D, NT>;
+  using L = PackTile<T, D>;
+  constexpr int ROWS = S::kRows, NS = S::kStages, G = L::G;
+  namespace cg = cooperative_groups;
+  extern __shared__ __align__(128) char sm[];
+  char *ring = sm, *q_sm = sm + S::kRing + S::kJoin;
+  float *join = (float *)(sm + S::kRing);
+  char *p = q_sm + S::kQ;
+  float *first_sm = (float *)p;  // [row][group]: -24 times the sum of the group's q
+  p += S::kFirst;
+  float *ml = (float *)p;  // [warp][row][m, l]
+  p += kTreeWarps * ROWS * 8;
+  unsigned long long *seen = (unsigned long long *)p;  // [row]
+  p += ROWS * 8;
+  long long *plan = (long long *)p;
+  p += 64;
+  int *there = (int *)p;  // [warp][stage]: positions of the chunk that exist
+  p += kTreeWarps * 8 * 4;
+  float *part_ml = (float *)p;  // CS > 1: [row][m, l] of this block
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+
+  WarpPiece cur;
+  Walk walk;
+  bool more = true;
+  if constexpr (CS == 0) {
+    const bool any = walk.start(a, ROWS, plan, warp, lane, cur);
+    pdl_launch();
+    if (!any) return;
+    cur.chunks_of(warp, kTileChunks);
+  } else {
+    const int seg = blockIdx.x / CS;
+    cur.rb = seg % row_blocks, cur.head = seg / row_blocks % a.kv_heads, cur.b = seg / row_blocks / a.kv_heads;
+    cur.sg = Segments(a, cur.b, ROWS);
+    if (cur.rb >= cur.sg.blocks) return;  // the whole cluster alike
+    cur.t0 = blockIdx.x % CS, cur.t1 = cur.sg.tiles;
+    cur.chunks_of(warp, kTileChunks * CS);
+  }
+  // how many of the warp's chunks are cached ones; they come before those of drafts
+  auto cached_of = [](const WarpPiece &x) {
+    const int end = min(x.t1 * kTileChunks, x.sg.chunks_c);
+    return x.c0 < end ? (end - x.c0 + x.step - 1) / x.step : 0;
+  };
+
+  const uint32_t my_ring = smem_addr(ring) + warp * (NS * L::kStage), q_at = smem_addr(q_sm);
+  int *my_there = there + warp * 8;
+  int pages = -1;  // lane i: the page of the chunk 32 j + i
+  auto issue = [&](const WarpPiece &x, int nc, int k) {
+    if (k < nc) {
+      const int c = x.c0 + k * x.step, slot = k % NS;
+      if ((k & 31) == 0) {
+        const int mine = c + lane * x.step;
+        const int pg = mine < x.sg.chunks_c ? (mine * kChunk) >> a.c.page_shift : -1;
+        pages = pg >= 0 ? a.c.table[x.b * a.c.table_stride + pg] : -1;
+      }
+      const int pg = __shfl_sync(~0u, pages, k & 31), pos = c * kChunk, in_page = pos & ((1 << a.c.page_shift) - 1);
+      const bool mapped = pg >= 0 && pg < a.c.num_pages;
+      if (mapped) {  // whole chunks: a page has room for them
+        const long long at = pg * a.c.page_bytes + x.head * a.c.head_bytes + (long long)in_page * (D / 2);
+        const long long at_s = pg * a.scale_page + x.head * a.scale_head + (long long)in_page * (G * 2);
+        L::load(my_ring + slot * L::kStage, a.c.k + at, a.c.v + at, a.k_scale + at_s, a.v_scale + at_s, lane);
+      }
+      if (lane == 0) my_there[slot] = mapped ? min(kChunk, x.sg.len - pos) : 0;
+    }
+    copy_commit();
+  };
+  // the query rows of a piece, their sums and the drafts that each sees
+  auto load_query = [&](const WarpPiece &x) {
+    const int rows = min(ROWS, x.sg.count * a.group - x.rb * ROWS);
+    for (int i = tid; i < ROWS * G * 4; i += kTreeThreads) {  // (row, group, quarter)
+      const int row = i / (G * 4), j = i / 4 % G, quarter = i % 4, at = x.rb * ROWS + row;
+      const T *from = row < rows ? (const T *)a.q + (x.sg.first + at / a.group) * a.q_stride +
+                                       (long long)(x.head * a.group + at % a.group) * D + 32 * j + 8 * quarter
+                                 : nullptr;
+      uint32_t f[L::kParts][4];
+      L::pairs8(f, from);
+#pragma unroll
+      for (int w = 0; w < L::kParts; w++)
+        sts4u(q_at + row / 8 * L::kQBytes + (w * G + j) * 512 + (row % 8 * 4 + quarter) * 16, f[w][0], f[w][1], f[w][2], f[w][3]);
+      if constexpr (!L::f32) {
+        float s = L::sum8(from);
+        s += __shfl_xor_sync(~0u, s, 1);
+        s += __shfl_xor_sync(~0u, s, 2);
+        if (quarter == 0) first_sm[row * G + j] = -24.f * s;
+      }
+    }
+    for (int r = tid; r < ROWS; r += kTreeThreads)
+      seen[r] = r < rows ? (unsigned long long)a.mask[x.sg.first + (x.rb * ROWS + r) / a.group] : 0ull;
+  };
+
+  int nc = cached_of(cur);
+#pragma unroll
+  for (int k = 0; k < NS - 1; k++) issue(cur, nc, k);
+  load_query(cur);
+  __syncthreads();
+
+  for (int piece = 0; more; piece++) {
+    uint32_t qr[S::kQInRegs ? G : 1][4];
+    float fr[S::kQInRegs ? G : 1][2];
+    if constexpr (S::kQInRegs) {
+#pragma unroll
+      for (int j = 0; j < G; j++) {
+        lds4u(qr[j], q_at + j * 512 + lane * 16);
+        fr[j][0] = first_sm[2 * t * G + j], fr[j][1] = first_sm[(2 * t + 1) * G + j];
+      }
+    }
+    float o[L::kTiles][NT][4] = {}, ref[NT][2], sum[NT][2] = {}, low[NT][2] = {};  // of rows 8 n + 2 t and + 1
+#pragma unroll
+    for (int n = 0; n < NT; n++) ref[n][0] = ref[n][1] = -INFINITY;
+
+    // scores in units of log2 become weights, against the rows' references
+    auto soften = [&](float (&s)[NT][4]) {
+      bool above = false;
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) above |= s[n][e] > ref[n][e & 1] + kSlack<T>;
+      if (__any_sync(~0u, above)) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float top = fmaxf(s[n][h], s[n][2 + h]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+            const float now = fmaxf(ref[n][h], top - kLift<T>);
+            const float alpha = now == -INFINITY ? 1.f : exp2_(ref[n][h] - now);
+            ref[n][h] = now;
+            sum[n][h] *= alpha, low[n][h] *= alpha;
+#pragma unroll
+            for (int i = 0; i < L::kTiles; i++) o[i][n][h] *= alpha, o[i][n][2 + h] *= alpha;
+          }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float m = ref[n][h] == -INFINITY ? 0.f : ref[n][h];
+          s[n][h] = exp2_(s[n][h] - m), s[n][2 + h] = exp2_(s[n][2 + h] - m);
+          add_exactly(sum[n][h], low[n][h], s[n][h] + s[n][2 + h]);
+        }
+    };
+
+    // drafts first, while the first cached chunks are on their way
+    for (int k = nc; k < cur.nk; k++) {
+      const int j0 = (cur.c0 + k * cur.step - cur.sg.chunks_c) * kChunk, valid = min(kChunk, cur.sg.count - j0);
+      const long long from = (cur.sg.first + j0) * a.kv_stride + (long long)cur.head * D;
+      float s[NT][4];
+      L::template draft_scores<NT>(s, q_at, (const T *)a.dk + from, a.kv_stride, valid, lane);
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int j = L::position(g) + (e >> 1) * 2;
+          const bool see = j < valid && seen[n * 8 + 2 * t + (e & 1)] >> (j0 + j) & 1;
+          s[n][e] = see ? s[n][e] * a.scale : -INFINITY;
+        }
+      soften(s);
+      uint32_t b[L::kParts][NT][2];
+      L::template weights<NT>(b, s);
+      if (L::template draft_values<NT>(o, b, (const T *)a.dv + from, a.kv_stride, valid, lane)) {
+        // values that are not finite: 0 * NaN would have reached rows that do not see them, the others get them here
+        for (int j = 0; j < valid; j++) {
+          const T *row = (const T *)a.dv + from + j * a.kv_stride;
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const float w = __shfl_sync(~0u, j & 2 ? s[n][2 + h] : s[n][h], (2 * (j >> 2) + (j & 1)) * 4 + t);
+              const bool see = seen[n * 8 + 2 * t + h] >> (j0 + j) & 1;
+#pragma unroll
+              for (int i = 0; i < L::kTiles; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                  const float x = to_f(row[(i >> 1) * 32 + 4 * g + (i & 1) * 2 + e]);
+                  if (!isfinite(x) && see) o[i][n][2 * e + h] += w * x;
+                }
+            }
+        }
+      }
+    }
+
+    for (int k = 0; k < nc; k++) {
+      copy_wait<NS - 2>();
+      __syncwarp();  // the stage before is read by all lanes too
+      issue(cur, nc, k + NS - 1);
+      const uint32_t st = my_ring + k % NS * L::kStage;
+      const int valid = my_there[k % NS];
+      if (valid == 0) continue;
+      float s[NT][4];
+      L::template scores<NT, S::kQInRegs>(s, qr, fr, q_at, first_sm, st, lane);
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[n][e] *= a.scale;
+      if (valid < kChunk) {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (L::position(g) + (e >> 1) * 2 >= valid) s[n][e] = -INFINITY;
+      }
+      soften(s);
+      uint32_t b[L::kParts][NT][2];
+      L::template weights<NT>(b, s);
+      L::template values<NT>(o, b, st, valid, lane);
+    }
+    // the next piece's first chunks are on their way while this one is joined
+    const WarpPiece done = cur;
+    if constexpr (CS == 0) {
+      if (tid == 0) walk.tell(a, cur, row_blocks, 2 * blockIdx.x + (piece ? 1 : 0));
+      more = walk.next(a, ROWS, cur);
+      if (more) {
+        cur.chunks_of(warp, kTileChunks);
+        nc = cached_of(cur);
+        copy_wait<0>();  // nothing is: the groups left over are empty, and count as the next piece's otherwise
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < NS - 1; k++) issue(cur, nc, k);
+      }
+    } else {
+      more = false;
+    }
+    const int rows = min(ROWS, done.sg.count * a.group - done.rb * ROWS);
+    const bool whole = CS == 0 ? done.t0 == 0 && done.t1 == done.sg.tiles : CS == 1;
+    const long long slot = 2 * (long long)blockIdx.x + (piece ? 1 : 0);
+    float *part = CS > 1 ? (float *)ring : a.part + slot * ROWS * D;
+    float *to_ml = CS > 1 ? part_ml : a.part_ml + slot * ROWS * 2;
+    // dim d of row r: exchanged so that a warp's stores hit different banks
+    auto dim_of = [](int r, int d) { return d ^ (((r >> 1) & 3) << 3); };
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      __syncthreads();  // every warp is done with what the join, or the parts, lie over
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float l = sum[n][h] + low[n][h];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(~0u, l, d);
+        const int r = 2 * t + h, row = n * 8 + r;
+        if (g == 0) ml[(warp * ROWS + row) * 2] = ref[n][h], ml[(warp * ROWS + row) * 2 + 1] = l;
+        float *to = join + (warp * 8 + r) * D;
+#pragma unroll
+        for (int j = 0; j < G; j++)
+          *(float4 *)(to + dim_of(r, j * 32 + 4 * g)) = make_float4(o[2 * j][n][h], o[2 * j][n][2 + h], o[2 * j + 1][n][h], o[2 * j + 1][n][2 + h]);
+      }
+      if (n == NT - 1 && more) load_query(cur);
+      __syncthreads();
+      for (int i = tid; i < min(8, rows - n * 8) * (D / 4); i += kTreeThreads) {
+        const int r = i / (D / 4), d = i % (D / 4), row = n * 8 + r;
+        float top = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kTreeWarps; w++) top = fmaxf(top, ml[(w * ROWS + row) * 2]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kTreeWarps; w++) {
+          const float f = exp2_(ml[(w * ROWS + row) * 2] - base);
+          l = fmaf(f, ml[(w * ROWS + row) * 2 + 1], l);
+          const float4 y = *(const float4 *)(join + (w * 8 + r) * D + dim_of(r, d * 4));
+          x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+        }
+        if (whole) {
+          write_row<T, D>(a, done.sg, done.head, done.rb * ROWS + row, d * 4, x, top, l);
+        } else {
+          *(float4 *)(part + row * D + d * 4) = x;
+          if (d == 0) *(float2 *)(to_ml + row * 2) = make_float2(top, l);
+        }
+      }
+    }
+    if constexpr (CS > 1) {
+      cg::cluster_group cluster = cg::this_cluster();
+      cluster.sync();
+      for (int i = (int)cluster.block_rank() * kTreeThreads + tid; i < rows * (D / 4); i += CS * kTreeThreads) {
+        const int row = i / (D / 4), d = i % (D / 4);
+        float2 w[CS];
+        float4 y[CS];
+#pragma unroll
+        for (int r = 0; r < CS; r++) {
+          w[r] = *(const float2 *)(cluster.map_shared_rank(part_ml, r) + row * 2);
+          y[r] = *(const float4 *)(cluster.map_shared_rank(part, r) + row * D + d * 4);
+        }
+        float top = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int r = 0; r < CS; r++) top = fmaxf(top, w[r].x);
+        const float base = top == -INFINITY ? 0.f : top;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < CS; r++) {
+          const float f = exp2_(w[r].x - base);
+          l = fmaf(f, w[r].y, l);
+          x.x = fmaf(f, y[r].x, x.x), x.y = fmaf(f, y[r].y, x.y), x.z = fmaf(f, y[r].z, x.z), x.w = fmaf(f, y[r].w, x.w);
+        }
+        write_row<T, D>(a, cur.sg, cur.head, cur.rb * ROWS + row, d * 4, x, top, l);
+      }
+      cluster.sync();  // no block ends while another reads its part
+    }
+    __syncthreads();  // the join is read, the query rows are there
+  }
+}
+
+}  // namespace paged
+}  // namespace ocrvl

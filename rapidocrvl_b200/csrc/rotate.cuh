@@ -1,0 +1,143 @@
+// Queries and keys of new tokens: each head's norm, if there is one, and the
+// rotation by positions of several axes, in one pass (ocrvl_op_rotate).
+//
+//   y = x / sqrt(mean x^2 + eps) * w
+//   pair p (dims p and p + pairs, or 2 p and 2 p + 1): angle = pos[axis p] freq[p]
+//   (u, v) -> (u cos - v sin, v cos + u sin);  dims behind 2 pairs stay y
+// A warp a token (or a share of a token's heads): it works out the token's cosines and
+// sines once, two lanes' worth in shared memory, then goes through the heads with a lane
+// for 2 V dims.  The angle is a 64-bit product of turns, whose whole part is dropped before
+// it becomes 32 bits, so far positions keep their last bits.
+#pragma once
+#include "packed.cuh"
+
+namespace ocrvl {
+namespace paged {
+
+constexpr int kRotateWarps = 8;
+constexpr int kRotateMost = 128;  // pairs
+
+struct RotateArgs {
+  const char *q, *k;
+  char *q_out, *k_out;
+  const void *q_weight, *k_weight;
+  const int *pos;
+  long long q_stride, k_stride, q_out_stride, k_out_stride, pos_stride;  // bytes; entries
+  int n_tokens, heads, kv_heads, dim, pairs, neighbours, lanes, share;   // lanes: of a row; share: warps a token
+  float eps;
+  double turns[kRotateMost];  // freq / 2 pi
+  unsigned char axis[kRotateMost];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_v(float (&x)[V], const T *p) {
+  if constexpr (sizeof(T) == 4) {
+    static_assert(V == 4, "");
+    const float4 a = *(const float4 *)p;
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+  } else {
+    uint32_t w[V / 2];
+    if constexpr (V == 8)
+      *(uint4 *)w = *(const uint4 *)p;
+    else
+      *(uint2 *)w = *(const uint2 *)p;
+#pragma unroll
+    for (int i = 0; i < V / 2; i++) {
+      const float2 f = unpack2<T>(w[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T *p, const float (&x)[V]) {
+  if constexpr (sizeof(T) == 4) {
+    *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
+  } else if constexpr (V == 8) {
+    *(uint4 *)p = make_uint4(pack2(x[0], x[1], T()), pack2(x[2], x[3], T()), pack2(x[4], x[5], T()), pack2(x[6], x[7], T()));
+  } else {
+    *(uint2 *)p = make_uint2(pack2(x[0], x[1], T()), pack2(x[2], x[3], T()));
+  }
+}
+
+// NORM: 0 none, 1 weights of T, 2 weights of f32.
+template <typename T, int V, int NORM>
+__global__ void __launch_bounds__(kRotateWarps * 32) k_rotate(const __grid_constant__ RotateArgs a) {
+  __shared__ __align__(16) float trig[kRotateWarps][2][kRotateMost];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long unit = (long long)blockIdx.x * kRotateWarps + warp;
+  const long long token = unit / a.share;
+  if (token >= a.n_tokens) return;  // the whole warp
+  float *cs = trig[warp][0], *sn = trig[warp][1];
+  for (int p = lane; p < a.pairs; p += 32) {
+    const double x = (double)a.pos[token * a.pos_stride + a.axis[p]] * a.turns[p];
+    sincospif(2.f * (float)(x - rint(x)), &sn[p], &cs[p]);
+  }
+  __syncwarp();
+  const int at_once = 32 / a.lanes, sub = lane / a.lanes, v = lane % a.lanes, rotated = a.pairs / V;
+  // the lane's two runs of V dims, and where their pairs are among the cosines
+  int d0, d1;
+  float c[V] = {}, s[V] = {};
+  if (v < rotated) {
+    d0 = a.neighbours ? 2 * V * v : V * v;
+    d1 = a.neighbours ? d0 + V : a.pairs + d0;
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      *(float4 *)(c + e) = *(const float4 *)(cs + V * v + e);
+      *(float4 *)(s + e) = *(const float4 *)(sn + V * v + e);
+    }
+  } else {
+    d0 = 2 * a.pairs + 2 * V * (v - rotated), d1 = d0 + V;
+  }
+  const int rows = a.heads + a.kv_heads, part = (int)(unit % a.share);
+  for (int r0 = part * at_once; r0 < rows; r0 += a.share * at_once) {
+    const int r = r0 + sub;
+    const bool there = sub < at_once && r < rows, is_q = r < a.heads;
+    const int head = is_q ? r : r - a.heads;
+    const T *from = (const T *)((is_q ? a.q : a.k) + token * (is_q ? a.q_stride : a.k_stride)) + (long long)head * a.dim;
+    T *to = (T *)((is_q ? a.q_out : a.k_out) + token * (is_q ? a.q_out_stride : a.k_out_stride)) + (long long)head * a.dim;
+    float x[V] = {}, y[V] = {};
+    if (there) load_v<T, V>(x, from + d0), load_v<T, V>(y, from + d1);
+    if constexpr (NORM > 0) {
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; e++) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
+      // over the row's lanes, whatever their number: the first one collects, all ask it
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        const float other = __shfl_down_sync(~0u, sum, d);
+        if (v < d && v + d < a.lanes) sum += other;
+      }
+      sum = __shfl_sync(~0u, sum, lane - v);
+      const float inv = rsqrtf(sum / a.dim + a.eps);
+      float w0[V], w1[V];
+      if constexpr (NORM == 1) {
+        const T *w = (const T *)(is_q ? a.q_weight : a.k_weight);
+        load_v<T, V>(w0, w + d0), load_v<T, V>(w1, w + d1);
+      } else {
+        const float *w = (const float *)(is_q ? a.q_weight : a.k_weight);
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *(float4 *)(w0 + e) = *(const float4 *)(w + d0 + e), *(float4 *)(w1 + e) = *(const float4 *)(w + d1 + e);
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) x[e] *= inv * w0[e], y[e] *= inv * w1[e];
+    }
+    float z0[V], z1[V];
+    if (v >= rotated) {
+#pragma unroll
+      for (int e = 0; e < V; e++) z0[e] = x[e], z1[e] = y[e];
+    } else if (!a.neighbours) {
+#pragma unroll
+      for (int e = 0; e < V; e++) z0[e] = x[e] * c[e] - y[e] * s[e], z1[e] = y[e] * c[e] + x[e] * s[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        z0[e] = x[e] * c[e / 2] - x[e + 1] * s[e / 2], z0[e + 1] = x[e + 1] * c[e / 2] + x[e] * s[e / 2];
+        z1[e] = y[e] * c[V / 2 + e / 2] - y[e + 1] * s[V / 2 + e / 2], z1[e + 1] = y[e + 1] * c[V / 2 + e / 2] + y[e] * s[V / 2 + e / 2];
+      }
+    }
+    if (there) store_v<T, V>(to + d0, z0), store_v<T, V>(to + d1, z1);
+  }
+}
+
+}  // namespace paged
+}  // namespace ocrvl

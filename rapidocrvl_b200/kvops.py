@@ -5,10 +5,16 @@ over the cache in one pass, and the cache cut to a budget.
                    cache and one another; one token a sequence is the
                    ordinary decode step
   append           accepted drafts (or a prompt) written behind the cache
+  rotate           queries and keys of new tokens, normed and rotated by positions
+                   of one or several axes
+  read             positions of a packed cache as numbers again
   attention_mass   the attention weight that cached positions received,
                    added to a running sum
   evict            keeps the first, the last and the most attended positions
                    (select, then compact)
+
+A cache holds f32, f16 or bf16 (:class:`PagedCache`), or 4 bits (:class:`PackedCache`, for
+append and read).
 
 All run on the tensors' device and torch's current stream, read lengths on the
 device and wait for nothing, so they can be captured in a CUDA graph.  They call
@@ -20,7 +26,8 @@ requires a gradient is refused unless gradients are off.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple
+import math
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -87,6 +94,92 @@ class PagedCache:
         n = C.c_int64()
         _lib.check(_lib.load().ocrvl_op_tree_attn_workspace(C.byref(self.desc), heads, max_draft, C.byref(n)))
         return n.value
+
+
+class PackedCache:
+    """A paged cache in 4 bits: ``k`` and ``v`` are [pages, layers, kv heads, page_size, head_dim / 2] uint8 tensors,
+    ``k_scale`` and ``v_scale`` [pages, layers, kv heads, page_size, head_dim / 32] bfloat16 ones (each pair of the same
+    strides, the last two dimensions contiguous), ``table`` as in :class:`PagedCache`.  32 dims of a position share a
+    scale s and are whole numbers of -7 .. 7 times s: see ``ocrvl_packed_cache`` in the header.  ``append`` quantises into
+    it, ``tree_attention`` attends it, ``read`` gives it back; :meth:`empty` makes one."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, table: torch.Tensor):
+        for name, x, y, dtype in (("k and v", k, v, torch.uint8), ("k_scale and v_scale", k_scale, v_scale, torch.bfloat16)):
+            if x.dim() != 5 or x.shape != y.shape or x.stride() != y.stride() or x.dtype is not dtype or y.dtype is not dtype:
+                raise ValueError(f"{name} must be five-dimensional {dtype} tensors of one shape and one set of strides")
+            if not x.is_cuda or x.device != k.device or y.device != k.device:
+                raise ValueError("k, v and their scales must be on one CUDA device")
+            if x.stride(4) != 1 or x.stride(3) != x.shape[4]:
+                raise ValueError(f"the positions of a page of {name} must be contiguous")
+        pages, layers, heads, page, half = k.shape
+        if half not in (32, 64) or k_scale.shape != (pages, layers, heads, page, half // 16):
+            raise ValueError("k must be [pages, layers, kv heads, page_size, head_dim / 2] with head_dim 64 or 128, its scales one for 32 dims")
+        if table.dim() != 2 or table.dtype is not torch.int32 or table.device != k.device or table.stride(1) != 1:
+            raise ValueError(f"table must be a [batch, max_pages] int32 tensor on {k.device}")
+        if table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+            raise ValueError("the table's rows must not overlap (an expanded row needs a copy: .contiguous())")
+        self.k, self.v, self.k_scale, self.v_scale, self.table, self.device = k, v, k_scale, v_scale, table, k.device
+        self.desc = _lib.PackedCache(2 * half, heads, layers, page, pages, table.shape[0], table.shape[1], 0, *k.stride()[:3],
+                                     *k_scale.stride()[:3], table.stride(0) if table.shape[0] > 1 else table.shape[1],
+                                     k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), table.data_ptr())
+        self._ref = (C.addressof(self.desc), self.device.index, k, v, k_scale, v_scale)  # for the native side
+        self.head_dim, self.kv_heads, self.layers, self.batch = 2 * half, heads, layers, table.shape[0]
+        self.capacity = table.shape[1] * page
+
+    @classmethod
+    def empty(cls, pages: int, layers: int, kv_heads: int, head_dim: int, table: torch.Tensor, *, page_size: int = 16) -> "PackedCache":
+        """A cache of ``pages`` pages on the table's device (every number in it 0)."""
+        if head_dim not in (64, 128):
+            raise ValueError("head_dim must be 64 or 128")
+        k, v = torch.full((2, pages, layers, kv_heads, page_size, head_dim // 2), 0x88, dtype=torch.uint8, device=table.device)
+        ks, vs = torch.zeros(2, pages, layers, kv_heads, page_size, head_dim // 32, dtype=torch.bfloat16, device=table.device)
+        return cls(k, v, ks, vs, table)
+
+
+class Rotary:
+    """Rotary positions: which dims of a head turn by which of a token's positions, and how fast.
+
+    ``pairs`` (default: half of head_dim) pairs of dims turn, by ``theta ** (-p / pairs)`` radians a position or by
+    ``freq`` [pairs]; the dims behind them stay.  Pair p is dims p and p + pairs, or 2 p and 2 p + 1 with ``neighbours``.
+    Without more a token has one position.  ``sections`` (pairs of each axis, in order: (16, 24, 24) for time, height and width, say)
+    or ``axis`` [pairs] (each pair's, in any order) give it several."""
+
+    def __init__(self, head_dim: int, *, theta: float = 10000.0, pairs: Optional[int] = None, freq: Optional[Sequence[float]] = None,
+                 sections: Optional[Sequence[int]] = None, axis: Optional[Sequence[int]] = None, neighbours: bool = False):
+        pairs = head_dim // 2 if pairs is None else pairs
+        if not 8 <= head_dim <= 256 or head_dim % 8:
+            raise ValueError("head_dim must be a multiple of 8, at most 256")
+        if not 4 <= pairs <= head_dim // 2 or pairs % 4:
+            raise ValueError("pairs must be a multiple of 4, at most half of head_dim")
+        if sections is not None and axis is not None:
+            raise ValueError("sections or axis, not both")
+        if sections is not None:
+            axis = [a for a, n in enumerate(sections) for _ in range(n)]
+        axis = [0] * pairs if axis is None else [int(a) for a in axis]
+        axes = len(sections) if sections is not None else max(axis, default=0) + 1
+        if len(axis) != pairs or not 1 <= axes <= 8 or min(axis) < 0 or (sections is not None and min(sections) < 0):
+            raise ValueError(f"sections (or axis) must say which of at most 8 axes each of the {pairs} pairs has")
+        freq = [float(theta) ** (-p / pairs) for p in range(pairs)] if freq is None else [float(f) for f in freq]
+        if len(freq) != pairs or not all(map(math.isfinite, freq)):
+            raise ValueError(f"freq must be {pairs} finite numbers")
+        self.desc = _lib.Rotary(head_dim, pairs, axes, int(bool(neighbours)), (C.c_double * 128)(*freq), (C.c_uint8 * 128)(*axis))
+        self.head_dim, self.pairs, self.axes = head_dim, pairs, axes
+        self._ref = C.addressof(self.desc)
+
+
+def rotate(q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor, rotary: Rotary, *, q_weight: Optional[torch.Tensor] = None,
+           k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+           k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Queries and keys of new tokens, normed and rotated in one pass.
+
+    q [tokens, heads, head_dim], k [tokens, kv heads, head_dim] (or None), each with a stride of its own between tokens:
+    views of one projection's output, say.  ``pos`` [tokens, axes] int32 ([tokens] with one axis).  With ``q_weight`` and
+    ``k_weight`` [head_dim] (float32 or q's type) each head is first divided by the root of its mean square (plus
+    ``eps``) and multiplied by the weights.  ``q_out`` and ``k_out`` may be q and k themselves.  Angles are worked out in
+    64 bits.  Returns (q, k) turned."""
+    if not isinstance(rotary, Rotary):
+        raise ValueError("rotary must be a Rotary")
+    return _kvops.rotate(rotary._ref, q, k, pos, q_weight, k_weight, eps, q_out, k_out)
 
 
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedCache, lens: torch.Tensor,
@@ -170,13 +263,24 @@ def evict(cache: PagedCache, acc: torch.Tensor, lens: torch.Tensor, *, keep: int
 
 
 
-def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor, indptr: torch.Tensor, *,
+def append(cache: Union[PagedCache, PackedCache], k: torch.Tensor, v: torch.Tensor, lens: torch.Tensor, indptr: torch.Tensor, *,
            path: Optional[torch.Tensor] = None, n_path: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Writes tokens behind the cache, for all layers at once.
 
     k, v [layers, tokens, kv heads, head_dim]; ``indptr`` [batch + 1] int32
     bounds each sequence's tokens.  ``path`` [batch, most] int32 with ``n_path``
     [batch] int32 names the tokens of each sequence to write, in order (the
-    accepted path through its tree); without them all are written.  Returns
-    the new lengths."""
+    accepted path through its tree); without them all are written.  A
+    :class:`PackedCache` gets them quantised, from any of the three types.  Returns the new lengths."""
     return _kvops.append(cache._ref, k, v, lens, indptr, path, n_path)
+
+
+def read(cache: PackedCache, lens: torch.Tensor, indptr: torch.Tensor, tokens: int, *, dtype: torch.dtype = torch.bfloat16,
+         k: Optional[torch.Tensor] = None, v: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Reads positions of a packed cache back, all layers at once: what ``append`` with the same ``lens`` and ``indptr`` wrote.
+
+    ``indptr`` [batch + 1] int32 says how many positions of each sequence, from ``lens`` [batch] int32 on, and where they go;
+    ``tokens`` is the length of that flat axis (indptr's last value, which is on the device).  Returns k and v
+    [layers, tokens, kv heads, head_dim] of ``dtype`` (or the tensors given), 0 where a position has no page; tokens behind
+    indptr's last are not written."""
+    return _kvops.read(cache._ref, lens, indptr, tokens, dtype, k, v)
