@@ -472,6 +472,16 @@ int ocrvl_op_packed_append(const ocrvl_packed_cache *c, int type, int n_tokens, 
 int ocrvl_op_packed_read(const ocrvl_packed_cache *c, int type, int n_tokens, const int32_t *lens, const int32_t *indptr,
                          void *k, void *v, int64_t kv_stride, int64_t kv_layer_stride, void *stream);
 
+/* ocrvl_op_tree_attn over a packed cache: q, k, v and out are of `type`, all else is as there.
+ * f32: codes meet all 24 bits of q and of the softmax weights.  bf16: c s is taken as it is; f16: rounded to
+ * f16 (an infinity past its range), exact from 2^-14 on for caches written from f16.  With more than 16 rows (tokens
+ * times heads a kv head) of a 16-bit type keys are taken like values, with fewer not rounded. */
+int ocrvl_op_packed_attn_workspace(const ocrvl_packed_cache *c, int type, int heads, int max_draft, int64_t *bytes);
+int ocrvl_op_packed_attn(const ocrvl_packed_cache *c, int type, int layer, int heads, int n_tokens, int max_draft,
+                         const int32_t *lens, const int32_t *indptr, const int64_t *mask, const void *q, int64_t q_stride,
+                         const void *k, const void *v, int64_t kv_stride, float scale, void *out, int64_t out_stride, float *lse,
+                         void *work, int64_t work_bytes, void *stream);
+
 /* Rotary positions.  Pair p < pairs is dims p and p + pairs, or 2 p and 2 p + 1
  * (neighbours); its angle is freq[p] times the token's position on axis[p].
  * Dims behind 2 pairs are not rotated. */

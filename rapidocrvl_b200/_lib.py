@@ -139,6 +139,8 @@ SIGNATURES = {
     "ocrvl_op_kv_append": (I, [C.POINTER(KVCache), I, P, P, P, P, I, P, P, I64, I64, P, P]),
     "ocrvl_op_packed_append": (I, [C.POINTER(PackedCache), I, I, P, P, P, P, I, P, P, I64, I64, P, P]),
     "ocrvl_op_packed_read": (I, [C.POINTER(PackedCache), I, I, P, P, P, P, I64, I64, P]),
+    "ocrvl_op_packed_attn_workspace": (I, [C.POINTER(PackedCache), I, I, I, C.POINTER(I64)]),
+    "ocrvl_op_packed_attn": (I, [C.POINTER(PackedCache), I, I, I, I, I, P, P, P, P, I64, P, P, I64, F, P, I64, P, P, I64, P]),
     "ocrvl_op_rotate": (I, [C.POINTER(Rotary), I, I, P, I64, I, P, I64, P, I64, I, P, I64, P, I64, I, P, P, F, P]),
 }
 

@@ -7,7 +7,7 @@
 #include "mass_mma.cuh"
 #include "entry.cuh"
 #include "kv_move.cuh"
-#include "tree_attn.cuh"
+#include "tree_launch.cuh"
 #include "tree_mma.cuh"
 
 using namespace ocrvl;
@@ -68,30 +68,6 @@ int check_tokens(const ocrvl_kv_cache *c, int layer, int heads, int n_tokens, in
 }
 
 // ---- tree attention ----------------------------------------------------------
-
-// The workspace: two parts a block, and 16 bytes a segment in front of them.
-int64_t tree_joint_bytes(int batch, int kv_heads, int rows) { return ((int64_t)batch * kv_heads * ((rows + 7) / 8) * 16 + 127) / 128 * 128; }
-int64_t tree_work_bytes(const ocrvl_kv_cache *c, int sms, int rows) {
-  const int64_t parts = 2ll * sms * (c->type == OCRVL_F32 || rows <= 16 ? 2 * 32 : rows > 128 ? 256 : 128);
-  return tree_joint_bytes(c->batch, c->num_kv_heads, rows) + parts * (c->head_dim + 2) * 4;
-}
-
-// Tiles of the longest cache and of its drafts.
-int tree_tiles(const TreeArgs &a) { return (a.s.capacity + a.s.max_draft + kChunk - 1 + kChunk * kTileChunks - 1) / (kChunk * kTileChunks); }
-
-// What a call whose runs are joined must keep to, asked before its first launch.
-int check_combine(const TreeArgs &a, int blocks) { return (long long)blocks * a.kv_heads > 65535 ? invalid("too many kv heads") : OCRVL_OK; }
-
-// The join of runs' parts: eight rows a block, or fewer while the blocks would not fill
-// the GPU, down to one (then eight warps share a row's parts).
-template <typename T, int D>
-int launch_combine(const TreeArgs &a, int sms, int rows_max, int rows_a_block, cudaStream_t stream) {
-  const int blocks = (rows_max + rows_a_block - 1) / rows_a_block, rows = rows_max < rows_a_block ? rows_max : rows_a_block;
-  int group = 8;
-  while (group > 1 && (long long)((rows + group - 1) / group) * blocks * a.kv_heads * a.s.batch < 2 * sms) group /= 2;
-  return launch("tree attention (join)", k_tree_combine<T, D>, dim3((rows + group - 1) / group, blocks * a.kv_heads, a.s.batch),
-                kCombineWarps * 32, 0, stream, true, 1, a, rows_a_block, blocks, group);
-}
 
 // With blocks of 256 rows or 128, a block a segment or runs and their join.
 template <typename T, int D, bool WIDE, bool SPLIT>
@@ -279,7 +255,7 @@ int ocrvl_op_tree_attn_workspace(const ocrvl_kv_cache *c, int heads, int max_dra
   if (heads < 1 || heads % c->num_kv_heads || max_draft < 1 || max_draft > 64) return invalid("heads must be a multiple of num_kv_heads, max_draft 1..64");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  *bytes = tree_work_bytes(c, sms, heads / c->num_kv_heads * max_draft);
+  *bytes = tree_work_bytes(c->type == OCRVL_F32, c->batch, c->num_kv_heads, c->head_dim, sms, heads / c->num_kv_heads * max_draft);
   return OCRVL_OK;
 }
 
@@ -298,7 +274,7 @@ int ocrvl_op_tree_attn(const ocrvl_kv_cache *c, int layer, int heads, int n_toke
     return invalid("out must be 16-byte aligned rows of heads * head_dim elements");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  if (((uintptr_t)work & 127) || work_bytes < tree_work_bytes(c, sms, heads / c->num_kv_heads * max_draft)) return invalid("work is too small or not 128-byte aligned");
+  if (((uintptr_t)work & 127) || work_bytes < tree_work_bytes(c->type == OCRVL_F32, c->batch, c->num_kv_heads, c->head_dim, sms, heads / c->num_kv_heads * max_draft)) return invalid("work is too small or not 128-byte aligned");
   TreeArgs a;
   a.c = layer_of(c, layer);
   a.s = Seqs{lens, indptr, c->batch, n_tokens, max_draft, c->max_pages * c->page_size};

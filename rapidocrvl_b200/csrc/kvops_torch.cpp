@@ -197,8 +197,9 @@ PyObject *pack(std::initializer_list<at::Tensor> ts) {
 
 // (cache, q, k, v, lens, indptr, mask, layer, max_draft, scale, out, lse, work)
 PyObject *tree_attention(PyObject *const *a) {
-  const Cache c(a[0]);
+  Cache c(a[0], true);
   const at::Tensor &q = tensor(a[1], "q"), &k = tensor(a[2], "k"), &v = tensor(a[3], "v");
+  c.in_type(q.scalar_type(), "q");
   const int64_t q_stride = c.tokens(q, "q", 0), kv_stride = c.tokens(k, "k", c->num_kv_heads);
   const int64_t n = q.size(0), heads = q.size(1);
   if (c.tokens(v, "v", c->num_kv_heads) != kv_stride || k.size(0) != n || v.size(0) != n)
@@ -208,16 +209,23 @@ PyObject *tree_attention(PyObject *const *a) {
   void *stream = c.stream();
   const int max_draft = draft_of(a[8], n);
   int64_t bytes = 0;
-  ok(ocrvl_op_tree_attn_workspace(c.c, narrow(heads, "heads"), max_draft, &bytes));
+  ok(c.packed ? ocrvl_op_packed_attn_workspace(c.packed, type_of(c.dtype), narrow(heads, "heads"), max_draft, &bytes)
+              : ocrvl_op_tree_attn_workspace(c.c, narrow(heads, "heads"), max_draft, &bytes));
   const at::Tensor out = none(a[10]) ? at::empty({n, heads, c->head_dim}, c.options(c.dtype)) : tensor(a[10], "out");
   const int64_t out_stride = c.tokens(out, "out", heads);
   if (out.size(0) != n) throw Wrong{"out must have q's shape"};
   const at::Tensor lse = none(a[11]) ? at::empty({n, heads}, c.options(at::kFloat)) : tensor(a[11], "lse");
   const at::Tensor work = none(a[12]) ? at::empty({bytes}, c.options(at::kByte)) : tensor(a[12], "work");
-  ok(ocrvl_op_tree_attn(c.c, small(a[7], "layer"), narrow(heads, "heads"), narrow(n, "tokens"), max_draft, lens, indptr,
-                        (const int64_t *)mask, q.data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), kv_stride, scale_of(a[9], c),
-                        out.data_ptr(), out_stride, (float *)c.flat(lse, "lse", at::kFloat, n * heads),
-                        c.flat(work, "work", at::kByte, work.numel()), work.numel(), stream));
+  const int layer = small(a[7], "layer"), n_heads = narrow(heads, "heads"), tokens = narrow(n, "tokens");
+  const float scale = scale_of(a[9], c);
+  float *lse_at = (float *)c.flat(lse, "lse", at::kFloat, n * heads);
+  void *work_at = c.flat(work, "work", at::kByte, work.numel());
+  ok(c.packed ? ocrvl_op_packed_attn(c.packed, type_of(c.dtype), layer, n_heads, tokens, max_draft, lens, indptr, (const int64_t *)mask,
+                                     q.data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), kv_stride, scale, out.data_ptr(), out_stride,
+                                     lse_at, work_at, work.numel(), stream)
+              : ocrvl_op_tree_attn(c.c, layer, n_heads, tokens, max_draft, lens, indptr, (const int64_t *)mask, q.data_ptr(), q_stride,
+                                   k.data_ptr(), v.data_ptr(), kv_stride, scale, out.data_ptr(), out_stride, lse_at, work_at,
+                                   work.numel(), stream));
   wrote(out), wrote(lse), wrote(work);
   return pack({out, lse});
 }

@@ -31,10 +31,6 @@ __device__ __forceinline__ uint32_t lifted(uint32_t x, int i) {
   else
     return ((i < 1 ? x << 3 : x >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
 }
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162 *>(&a), *reinterpret_cast<__nv_bfloat162 *>(&b));
-  return *reinterpret_cast<uint32_t *>(&r);
-}
 template <typename B>
 struct Two;
 template <>
@@ -52,11 +48,32 @@ __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
   return *reinterpret_cast<uint32_t *>(&r);
 }
 template <typename B>
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  using V = typename Two<B>::V;
+  V r = __hsub2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b));
+  return *reinterpret_cast<uint32_t *>(&r);
+}
+template <typename B>
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   using V = typename Two<B>::V;
   V r = __hmul2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b));
   return *reinterpret_cast<uint32_t *>(&r);
 }
+// Nibble i of both halfwords of codes as c times their scales: exact.  f16 has no room for 24 s of the largest scales of
+// f16 numbers, so the 24 is taken off before.
+template <typename B>
+struct Scaled {
+  uint32_t s, minus;
+  __device__ __forceinline__ explicit Scaled(uint32_t s_) : s(s_), minus(0) {
+    if constexpr (!std::is_same<B, __half>::value) minus = mul2<B>(s, 0xc1c0c1c0u);  // -24
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t codes, int i) const {
+    if constexpr (std::is_same<B, __half>::value)
+      return mul2<B>(sub2<B>(lifted<B>(codes, i), 0x4e004e00u), s);
+    else
+      return fma2<B>(lifted<B>(codes, i), s, minus);
+  }
+};
 __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
 __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, int high) { return high ? high_halves(a, b) : low_halves(a, b); }
@@ -172,7 +189,7 @@ struct PackTile {
         a[h][2] = lifted<B>(x0, 2 * h + 1), a[h][3] = lifted<B>(x1, 2 * h + 1);
         if constexpr (f32) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) a[h][i] = sub2(a[h][i], 0x41c041c0u);  // 24: the codes themselves
+          for (int i = 0; i < 4; i++) a[h][i] = sub2<B>(a[h][i], 0x41c041c0u);  // 24: the codes themselves
         }
       }
       const float s0 = __uint_as_float(j & 1 ? ks[0][j >> 1] & 0xffff0000u : ks[0][j >> 1] << 16);
@@ -221,8 +238,10 @@ struct PackTile {
       pairs8(f0, p0 < valid ? rows + p0 * stride + 32 * j + 8 * t : nullptr);
       pairs8(f1, p0 + 2 < valid ? rows + (p0 + 2) * stride + 32 * j + 8 * t : nullptr);
 #pragma unroll
-      for (int n = 0; n < NT; n++)
-        // f32: the products of parts whose places add up to two at most, the small ones first
+      for (int n = 0; n < NT; n++) {
+        // A group is summed apart and added in a rounded addition; f32: the products of parts whose places add up to two
+        // at most, the small ones first.
+        float p[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int both = kParts - 1; both >= 0; both--)
 #pragma unroll
@@ -233,9 +252,12 @@ struct PackTile {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
               const uint32_t a[4] = {f0[x][2 * h], f1[x][2 * h], f0[x][2 * h + 1], f1[x][2 * h + 1]};
-              mma_16<B>(s[n], a, b[2 * h], b[2 * h + 1]);
+              mma_16<B>(p, a, b[2 * h], b[2 * h + 1]);
             }
           }
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[n][e] += p[e];
+      }
     }
   }
 
@@ -293,13 +315,11 @@ struct PackTile {
         s01 = pack2(__uint_as_float(s01 << 16), __uint_as_float(s01 & 0xffff0000u), B());
         s23 = pack2(__uint_as_float(s23 << 16), __uint_as_float(s23 & 0xffff0000u), B());
       }
-      constexpr uint32_t minus24 = std::is_same<B, __half>::value ? 0xce00ce00u : 0xc1c0c1c0u;
-      const uint32_t n01 = mul2<B>(s01, minus24), n23 = mul2<B>(s23, minus24);
+      const Scaled<B> by01(s01), by23(s23);
       const uint32_t x01 = halves(v[0][j >> 1], v[1][j >> 1], j & 1), x23 = halves(v[2][j >> 1], v[3][j >> 1], j & 1);
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const uint32_t a[4] = {fma2<B>(lifted<B>(x01, 2 * h), s01, n01), fma2<B>(lifted<B>(x01, 2 * h + 1), s01, n01),
-                               fma2<B>(lifted<B>(x23, 2 * h), s23, n23), fma2<B>(lifted<B>(x23, 2 * h + 1), s23, n23)};
+        const uint32_t a[4] = {by01(x01, 2 * h), by01(x01, 2 * h + 1), by23(x23, 2 * h), by23(x23, 2 * h + 1)};
         product<NT, 1>(o[2 * j + h], &a, b);
       }
     }
@@ -608,8 +628,7 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
       if (more) {
         cur.chunks_of(warp, kTileChunks);
         nc = cached_of(cur);
-        copy_wait<0>();  // nothing is: the groups left over are empty, and count as the next piece's otherwise
-        __syncwarp();
+        __syncwarp();  // all lanes are done with the last stage
 #pragma unroll
         for (int k = 0; k < NS - 1; k++) issue(cur, nc, k);
       }

@@ -65,6 +65,8 @@ struct TreeArgs {
   float *part_ml; // [2 grid][rows][2]
   int4 *joint;    // [sequence][kv head][row block] of runs: the first part's slot (-1: the segment is whole), its run, the last run
   int start_cost; // of a segment's start (filling the rings, joining the warps), in tiles, in the split of runs
+  const char *k_scale, *v_scale;         // a packed cache's (c holds its codes): at the layer,
+  long long scale_page, scale_head;      // bytes
 };
 
 struct Segments {  // what a sequence's segments have in common

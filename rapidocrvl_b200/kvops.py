@@ -14,7 +14,7 @@ over the cache in one pass, and the cache cut to a budget.
                    (select, then compact)
 
 A cache holds f32, f16 or bf16 (:class:`PagedCache`), or 4 bits (:class:`PackedCache`, for
-append and read).
+tree_attention, append and read).
 
 All run on the tensors' device and torch's current stream, read lengths on the
 device and wait for nothing, so they can be captured in a CUDA graph.  They call
@@ -126,6 +126,14 @@ class PackedCache:
         self.head_dim, self.kv_heads, self.layers, self.batch = 2 * half, heads, layers, table.shape[0]
         self.capacity = table.shape[1] * page
 
+    def work_bytes(self, heads: int, max_draft: int = 64, dtype: torch.dtype = torch.float32) -> int:
+        """Bytes of workspace a ``tree_attention`` call with that many query heads of ``dtype`` takes."""
+        if dtype not in _TYPES:
+            raise ValueError("dtype must be float32, float16 or bfloat16")
+        n = C.c_int64()
+        _lib.check(_lib.load().ocrvl_op_packed_attn_workspace(C.byref(self.desc), _TYPES[dtype], heads, max_draft, C.byref(n)))
+        return n.value
+
     @classmethod
     def empty(cls, pages: int, layers: int, kv_heads: int, head_dim: int, table: torch.Tensor, *, page_size: int = 16) -> "PackedCache":
         """A cache of ``pages`` pages on the table's device (every number in it 0)."""
@@ -182,7 +190,7 @@ def rotate(q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor, rotary
     return _kvops.rotate(rotary._ref, q, k, pos, q_weight, k_weight, eps, q_out, k_out)
 
 
-def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedCache, lens: torch.Tensor,
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Union[PagedCache, PackedCache], lens: torch.Tensor,
                    indptr: torch.Tensor, mask: torch.Tensor, *, layer: int = 0, max_draft: Optional[int] = None,
                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                    lse: Optional[torch.Tensor] = None, work: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -52,6 +52,24 @@ def test_bad_moves_are_refused():
     assert read(cache(), n=0, k=None, v=None)[0] == _lib.OK  # nothing to do
 
 
+def test_bad_attention_calls_are_refused():
+    L, c, p = _lib.load(), cache(), K
+
+    def attend(c=c, type=30, layer=0, heads=16, n=1, draft=1, lens=p, indptr=p, mask=p, q=p, qs=2048, k=p, ks=256, scale=0.1, out=p, os=2048, work=p, wb=1 << 30):
+        return L.ocrvl_op_packed_attn(c and C.byref(c), type, layer, heads, n, draft, lens, indptr, mask, q, qs, k, k, ks, scale, out, os, None, work, wb, None)
+
+    for kw in (dict(c=None), dict(type=2), dict(layer=1), dict(layer=-1), dict(heads=0), dict(heads=3), dict(heads=34), dict(n=-1), dict(draft=0), dict(draft=65), dict(lens=None),
+               dict(indptr=None), dict(mask=None), dict(q=None), dict(q=p + 4), dict(qs=2050), dict(qs=1024), dict(k=None), dict(k=p + 8), dict(ks=128), dict(ks=1 << 30),
+               dict(scale=math.nan), dict(out=None), dict(os=100), dict(work=None)):
+        assert attend(**kw) == _lib.E_INVALID, kw
+        assert _lib.last_error()
+    assert attend(n=0) == _lib.OK
+    n = C.c_int64()
+    assert L.ocrvl_op_packed_attn_workspace(C.byref(c), 30, 16, 1, None) == _lib.E_INVALID
+    assert L.ocrvl_op_packed_attn_workspace(C.byref(c), 2, 16, 1, C.byref(n)) == _lib.E_INVALID
+    assert L.ocrvl_op_packed_attn_workspace(C.byref(c), 30, 3, 1, C.byref(n)) == _lib.E_INVALID
+
+
 def rotary(**kw):
     r = _lib.Rotary(head_dim=128, pairs=64, num_axes=3, neighbours=0)
     for p in range(64):
