@@ -23,61 +23,6 @@ namespace paged {
 template <typename T>
 using Product = std::conditional_t<std::is_same<T, __half>::value, __half, __nv_bfloat16>;  // the products' type
 
-// Nibble i of both halfwords as 16 + nibble, two numbers of B.
-template <typename B>
-__device__ __forceinline__ uint32_t lifted(uint32_t x, int i) {
-  if constexpr (std::is_same<B, __half>::value)
-    return ((i < 2 ? x << (6 - 4 * i) : x >> (4 * i - 6)) & 0x03c003c0u) | 0x4c004c00u;
-  else
-    return ((i < 1 ? x << 3 : x >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
-}
-template <typename B>
-struct Two;
-template <>
-struct Two<__half> {
-  using V = __half2;
-};
-template <>
-struct Two<__nv_bfloat16> {
-  using V = __nv_bfloat162;
-};
-template <typename B>
-__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-  using V = typename Two<B>::V;
-  V r = __hfma2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b), *reinterpret_cast<V *>(&c));
-  return *reinterpret_cast<uint32_t *>(&r);
-}
-template <typename B>
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  using V = typename Two<B>::V;
-  V r = __hsub2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b));
-  return *reinterpret_cast<uint32_t *>(&r);
-}
-template <typename B>
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  using V = typename Two<B>::V;
-  V r = __hmul2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b));
-  return *reinterpret_cast<uint32_t *>(&r);
-}
-// Nibble i of both halfwords of codes as c times their scales: exact.  f16 has no room for 24 s of the largest scales of
-// f16 numbers, so the 24 is taken off before.
-template <typename B>
-struct Scaled {
-  uint32_t s, minus;
-  __device__ __forceinline__ explicit Scaled(uint32_t s_) : s(s_), minus(0) {
-    if constexpr (!std::is_same<B, __half>::value) minus = mul2<B>(s, 0xc1c0c1c0u);  // -24
-  }
-  __device__ __forceinline__ uint32_t operator()(uint32_t codes, int i) const {
-    if constexpr (std::is_same<B, __half>::value)
-      return mul2<B>(sub2<B>(lifted<B>(codes, i), 0x4e004e00u), s);
-    else
-      return fma2<B>(lifted<B>(codes, i), s, minus);
-  }
-};
-__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
-__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
-__device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, int high) { return high ? high_halves(a, b) : low_halves(a, b); }
-
 // x as three bf16 numbers, in the upper halves: exact (8 bits each, cut, so that none is rounded up to
 // infinity); what is not finite is the last one's alone, so that it meets nothing but another's first part.
 __device__ __forceinline__ void split3(float x, uint32_t (&p)[3]) {
@@ -150,7 +95,9 @@ struct PackTile {
   static __device__ __forceinline__ float sum8(const T *p) {
     if (!p) return 0.f;
     float x[8], s = 0.f;
-    load8(x, p);
+    Eight<T> e;
+    e.load(p);
+    e.floats(x);
 #pragma unroll
     for (int i = 0; i < 8; i++) s += x[i];
     return s;

@@ -42,11 +42,7 @@ struct PackArgs {
 constexpr int kPackLayers = 3;     // layers a warp takes of a token at once
 constexpr int kPackThreads = 256;
 
-// 8 values as 32-bit floats, and back.
-__device__ __forceinline__ void load8(float (&x)[8], const float *p) {
-  const float4 a = __ldg((const float4 *)p), b = __ldg((const float4 *)p + 1);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
+// 8 values of a row: as they lie in memory, and as 32-bit floats.
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t two);
 template <>
@@ -56,160 +52,255 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t two) {
   return make_float2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u));
 }
 template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T *p) {
-  const uint4 a = __ldg((const uint4 *)p);
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+
+  __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const float2 f = unpack2<T>(w[i]);
-    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = __ldg((const uint4 *)p + i);
   }
+  __device__ __forceinline__ void floats(float (&x)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = __uint_as_float(u[i]);
+    } else {
+      const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float2 f = unpack2<T>(u[i]);
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      }
+    }
+  }
+};
+
+// Lifted nibbles: nibble i of both halfwords as 16 + nibble, two numbers of B (at the top of the mantissa of 16).
+template <typename B>
+__device__ __forceinline__ uint32_t lifted(uint32_t x, int i) {
+  if constexpr (std::is_same<B, __half>::value)
+    return ((i < 2 ? x << (6 - 4 * i) : x >> (4 * i - 6)) & 0x03c003c0u) | 0x4c004c00u;
+  else
+    return ((i < 1 ? x << 3 : x >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
 }
-__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
-  *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
-  *((float4 *)p + 1) = make_float4(x[4], x[5], x[6], x[7]);
+template <typename B>
+struct Two;
+template <>
+struct Two<__half> {
+  using V = __half2;
+};
+template <>
+struct Two<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+};
+template <typename B>
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+  using V = typename Two<B>::V;
+  V r = __hfma2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b), *reinterpret_cast<V *>(&c));
+  return *reinterpret_cast<uint32_t *>(&r);
 }
-template <typename T>
-__device__ __forceinline__ void store8(T *p, const float (&x)[8]) {
-  *(uint4 *)p = make_uint4(pack2(x[0], x[1], T()), pack2(x[2], x[3], T()), pack2(x[4], x[5], T()), pack2(x[6], x[7], T()));
+template <typename B>
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  using V = typename Two<B>::V;
+  V r = __hsub2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b));
+  return *reinterpret_cast<uint32_t *>(&r);
+}
+template <typename B>
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  using V = typename Two<B>::V;
+  V r = __hmul2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b));
+  return *reinterpret_cast<uint32_t *>(&r);
+}
+// Nibble i of both halfwords of codes as c times their scales: exact.  In one fused step where there is room for 24 s;
+// f16 has none for the largest scales of f16 numbers (nor bf16 from 2^-5 of its largest on), so that the 24 is taken off before.
+template <typename B, bool ROOM = !std::is_same<B, __half>::value>
+struct Scaled {
+  uint32_t s, minus;
+  __device__ __forceinline__ explicit Scaled(uint32_t s_) : s(s_), minus(0) {
+    static_assert(!ROOM || !std::is_same<B, __half>::value, "");
+    if constexpr (ROOM) minus = mul2<B>(s, 0xc1c0c1c0u);  // -24
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t codes, int i) const {
+    if constexpr (ROOM)
+      return fma2<B>(lifted<B>(codes, i), s, minus);
+    else
+      return mul2<B>(sub2<B>(lifted<B>(codes, i), std::is_same<B, __half>::value ? 0x4e004e00u : 0x41c041c0u), s);
+  }
+};
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+__device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, int high) { return high ? high_halves(a, b) : low_halves(a, b); }
+
+// x / y correctly rounded, for y's reciprocal correctly rounded and a quotient of ordinary size: the first quotient's
+// rest is exact in one fused step, and what the second adds is off by 2^-47 of the whole.
+__device__ __forceinline__ float quotient(float x, float y, float reciprocal) {
+  const float q = x * reciprocal;
+  return fmaf(fmaf(-q, y, x), reciprocal, q);
 }
 
 // The scale of a group by its largest magnitude: max / 7 rounded to five significant bits, to the even
 // one of two.  (A 32-bit quotient is never rounded onto a border between two such numbers that it does not
 // lie on: those are six-bit m, 7 m is a float, and the next float is 4/7 of a rounding further at least.)
+// Below 63/64 of 2^-126 that is no normal number.
 __device__ __forceinline__ float group_scale(float most) {
-  const uint32_t u = __float_as_uint(__fdiv_rn(most, 7.f));
-  const uint32_t r = (u + 0x3ffffu + (u >> 19 & 1u)) & 0xfff80000u;
-  return r < 0x00800000u ? 0.f : __uint_as_float(r);
+  const float y = quotient(most, 7.f, 1.f / 7.f);
+  const uint32_t u = __float_as_uint(y), r = (u + 0x3ffffu + (u >> 19 & 1u)) & 0xfff80000u;
+  return y < 0x1.f8p-127f ? 0.f : __uint_as_float(r);
 }
 
 // Lane i of a row's D / 8 has dims 8 i .. 8 i + 7: of group j = i / 4, halfwords 2 t and 2 t + 1 of it
-// (t = i % 4).  Packs them; returns the four bytes at `at` of the row's codes, and the scale.
+// (t = i % 4).  Packs them; returns the four bytes at place(i) of the row's codes, and the scale.
 template <int D>
-__device__ __forceinline__ uint32_t pack8(const float (&x)[8], int i, int *at, float *scale) {
-  constexpr int G = D / 32;
+__device__ __forceinline__ int place(int i) {
+  const int j = i / 4, t = i % 4;
+  return (2 * t + (j & 1)) * (D / 16) + (j & ~1) * 2;
+}
+template <int D, typename T>
+__device__ __forceinline__ uint32_t pack8(const Eight<T> &e8, int i, float *scale) {
   // The magnitudes' bits have the order of the numbers, infinities and NaN above all others.
-  uint32_t most = 0;
+  uint32_t most;
+  bool finite;
+  float x[8];
+  e8.floats(x);
+  if constexpr (sizeof(T) == 4) {
+    most = 0;
 #pragma unroll
-  for (int e = 0; e < 8; e++) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
-  most = max(most, __shfl_xor_sync(~0u, most, 1));
-  most = max(most, __shfl_xor_sync(~0u, most, 2));
-  const bool finite = most < 0x7f800000u;
-  const float s = finite ? group_scale(__uint_as_float(most)) : 0.f;
-  uint32_t lo = 0x8888u, hi = 0x8888u;
-  if (s > 0.f) {
-    lo = hi = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      // The quotient is not rounded onto a border k + 1/2 either ((k + 1/2) s has nine bits), so its nearest
-      // whole number is the exact quotient's.
-      const uint32_t c = (uint32_t)((int)rintf(__fdiv_rn(x[e], s)) + 8) << e % 4 * 4;
-      if (e < 4)
-        lo |= c;
-      else
-        hi |= c;
-    }
+    for (int e = 0; e < 8; e++) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+    most = max(most, __shfl_xor_sync(~0u, most, 1));
+    most = max(most, __shfl_xor_sync(~0u, most, 2));
+    finite = most < 0x7f800000u;
+  } else {
+    const uint32_t m = 0x7fff7fffu;
+    uint32_t two = __vmaxu2(__vmaxu2(e8.w[0].x & m, e8.w[0].y & m), __vmaxu2(e8.w[0].z & m, e8.w[0].w & m));
+    two = __vmaxu2(two, __shfl_xor_sync(~0u, two, 1));
+    two = __vmaxu2(two, __shfl_xor_sync(~0u, two, 2));
+    const uint32_t one = max(two & 0xffffu, two >> 16);
+    finite = one < (std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u);
+    most = __float_as_uint(unpack2<T>(one).x);
   }
+  const float s = finite ? group_scale(__uint_as_float(most)) : 0.f;
+  // s has five bits and is no less than 2^-126 or 0: an ordinary reciprocal.
+  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  uint32_t c[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    // The quotient is not rounded onto a border k + 1/2 either ((k + 1/2) s has nine bits), so its nearest
+    // whole number is the exact quotient's.  In 1.5 2^23 + 8 + q the sum's rounding makes it whole (of two the even), and its
+    // last bits are c + 8.
+    c[e] = __float_as_uint(quotient(x[e], s, inv) + 12582920.f);
+  }
+  uint32_t lo = c[0] + (c[1] << 4) + (c[2] << 8) + (c[3] << 12), hi = c[4] + (c[5] << 4) + (c[6] << 8) + (c[7] << 12);
+  if (!finite) lo = hi = 0x8888u;
   *scale = finite ? s : __uint_as_float(0x7fc00000u);
   // two groups' halfwords side by side: the even group's lane takes halfwords 2 t, the odd one's 2 t + 1
-  const int j = i / 4, t = i % 4;
-  const uint32_t other = __shfl_xor_sync(~0u, j & 1 ? lo : hi, 4);
-  *at = (2 * t + (j & 1)) * (2 * G) + (j & ~1) * 2;
-  return j & 1 ? other | hi << 16 : lo | other << 16;
+  const bool odd = i / 4 & 1;
+  const uint32_t other = __shfl_xor_sync(~0u, odd ? lo : hi, 4);
+  return odd ? low_halves(other, hi) : low_halves(lo, other);
 }
 
-// The 8 numbers of lane i (as above) of a row whose codes' four bytes at its place are `word`.
-template <int D>
-__device__ __forceinline__ void unpack8(float (&x)[8], uint32_t word, float scale, int i) {
-  const int j = i / 4;
-  const uint32_t other = __shfl_xor_sync(~0u, j & 1 ? word & 0xffffu : word >> 16, 4);
-  const uint32_t lo = j & 1 ? other : word & 0xffffu, hi = j & 1 ? word >> 16 : other;
+// Stores the 8 numbers of lane i (as above) of a row whose codes' four bytes at its place are `word`, scale twice.
+template <int D, typename T>
+__device__ __forceinline__ void unpack8(T *to, uint32_t word, uint32_t scale, int i, bool there) {
+  using B = __nv_bfloat16;
+  const bool odd = i / 4 & 1;
+  const uint32_t other = __shfl_xor_sync(~0u, odd ? word : word >> 16, 4);
+  const uint32_t codes = odd ? __byte_perm(other, word, 0x7610) : low_halves(word, other);
+  const Scaled<B, false> by(scale);
+  uint32_t x[4], y[4];  // dims (k, 4 + k), then in order
 #pragma unroll
-  for (int e = 0; e < 8; e++) x[e] = (float)((int)((e < 4 ? lo : hi) >> e % 4 * 4 & 15u) - 8) * scale;
+  for (int k = 0; k < 4; k++) x[k] = by(codes, k);
+  y[0] = low_halves(x[0], x[1]), y[1] = low_halves(x[2], x[3]), y[2] = high_halves(x[0], x[1]), y[3] = high_halves(x[2], x[3]);
+  if constexpr (std::is_same<T, B>::value) {
+    if (there) *(uint4 *)to = make_uint4(y[0], y[1], y[2], y[3]);
+  } else {
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float2 z = unpack2<B>(y[k]);
+      f[2 * k] = z.x, f[2 * k + 1] = z.y;
+    }
+    if (!there) return;
+    if constexpr (sizeof(T) == 4) {
+      *(float4 *)to = make_float4(f[0], f[1], f[2], f[3]);
+      *((float4 *)to + 1) = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      *(uint4 *)to = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
+    }
+  }
 }
 
-// A warp an item: K and V of one token in up to kPackLayers layers, all heads; D / 8 lanes a row.
+// A warp takes K and V of one token in up to kPackLayers layers (blockIdx.z), all heads; D / 8 lanes a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(kPackThreads) k_packed_append(const PackArgs a) {
   constexpr int LANES = D / 8, ROWS = 32 / LANES;  // of a row; rows at once
   const int b = blockIdx.y, lane = threadIdx.x & 31, i8 = lane % LANES, sub = lane / LANES;
   const int first = min(max(a.indptr[b], 0), a.n_tokens), count = min(max(a.indptr[b + 1], first), a.n_tokens) - first;
   const int len = min(max(a.lens[b], 0), a.capacity);
-  const int n = a.path ? min(max(a.n_path[b], 0), a.max_path) : count;
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.new_lens[b] = min(len + n, a.capacity);
-  const int groups = (a.layers + kPackLayers - 1) / kPackLayers;
-  const long long items = (long long)n * groups;
-  for (long long it = blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5); it < items; it += gridDim.x * (kPackThreads / 32)) {
-    const int i = (int)(it / groups), layer0 = (int)(it % groups) * kPackLayers;
-    if (i >= a.capacity - len) break;
-    const int pos = len + i;
-    const int node = a.path ? a.path[(long long)b * a.max_path + i] : i;
+  const int n = min(a.path ? min(max(a.n_path[b], 0), a.max_path) : count, a.capacity - len);
+  if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.new_lens[b] = len + n;
+  const int at = place<D>(i8);
+  for (int i = blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5); i < n; i += gridDim.x * (kPackThreads / 32)) {
+    const int pos = len + i, node = a.path ? a.path[(long long)b * a.max_path + i] : i;
     if (node < 0 || node >= count) continue;
-    const int pg = a.c.page_of(b, pos);
-    if (pg < 0) continue;
-    const int in_page = pos & ((1 << a.c.shift) - 1);
-    for (int h0 = 0; h0 < a.kv_heads; h0 += ROWS) {
-      const int h = h0 + sub;
-      const bool there = h < a.kv_heads;
-      const long long from = layer0 * a.layer + (first + node) * a.token + ((long long)(there ? h : 0) * D + i8 * 8) * (int)sizeof(T);
-      const long long to = pg * a.c.page + layer0 * a.c.layer + h * a.c.head + (long long)in_page * (D / 2);
-      const long long to_s = pg * a.c.scale_page + layer0 * a.c.scale_layer + h * a.c.scale_head + (long long)in_page * (D / 16) + i8 / 4 * 2;
-      float x[2 * kPackLayers][8];
+    const int pg = a.c.page_of(b, pos), in_page = pos & ((1 << a.c.shift) - 1);
+    for (int layer0 = blockIdx.z * kPackLayers; layer0 < a.layers; layer0 += gridDim.z * kPackLayers)
+      for (int h0 = 0; h0 < a.kv_heads; h0 += ROWS) {
+        const int h = h0 + sub;
+        const bool there = h < a.kv_heads;
+        const long long from = layer0 * a.layer + (first + node) * a.token + (long long)(((there ? h : 0) * D + i8 * 8) * (int)sizeof(T));
+        Eight<T> x[2 * kPackLayers];  // the loads do not wait for the page
 #pragma unroll
-      for (int r = 0; r < 2 * kPackLayers; r++)
-        if (layer0 + r / 2 < a.layers) load8(x[r], (const T *)((r & 1 ? a.v : a.k) + from + r / 2 * a.layer));
+        for (int r = 0; r < 2 * kPackLayers; r++)
+          if (layer0 + r / 2 < a.layers) x[r].load((const T *)((r & 1 ? a.v : a.k) + from + r / 2 * a.layer));
+        const long long to = pg * a.c.page + layer0 * a.c.layer + h * a.c.head + in_page * (D / 2) + at;
+        const long long to_s = pg * a.c.scale_page + layer0 * a.c.scale_layer + h * a.c.scale_head + in_page * (D / 16) + i8 / 4 * 2;
 #pragma unroll
-      for (int r = 0; r < 2 * kPackLayers; r++) {
-        if (layer0 + r / 2 >= a.layers) break;
-        int at;
-        float s;
-        const uint32_t word = pack8<D>(x[r], i8, &at, &s);
-        if (!there) continue;
-        *(uint32_t *)((r & 1 ? a.c.v : a.c.k) + to + r / 2 * a.c.layer + at) = word;
-        if (i8 % 4 == 0)
-          *(uint16_t *)((r & 1 ? a.c.v_scale : a.c.k_scale) + to_s + r / 2 * a.c.scale_layer) = (uint16_t)(__float_as_uint(s) >> 16);
+        for (int r = 0; r < 2 * kPackLayers; r++) {
+          if (layer0 + r / 2 >= a.layers) break;
+          float s;
+          const uint32_t word = pack8<D>(x[r], i8, &s);
+          if (!there || pg < 0) continue;
+          *(uint32_t *)((r & 1 ? a.c.v : a.c.k) + to + r / 2 * a.c.layer) = word;
+          if (i8 % 4 == 0)
+            *(uint16_t *)((r & 1 ? a.c.v_scale : a.c.k_scale) + to_s + r / 2 * a.c.scale_layer) = (uint16_t)(__float_as_uint(s) >> 16);
+        }
       }
-    }
   }
 }
 
-// The other way, items as above; a token without a page reads as 0.
+// The other way, shared out alike; a token without a page reads as 0.
 template <typename T, int D>
 __global__ void __launch_bounds__(kPackThreads) k_packed_read(const PackArgs a) {
-  constexpr int LANES = D / 8, ROWS = 32 / LANES, G = D / 32;
+  constexpr int LANES = D / 8, ROWS = 32 / LANES;
   const int b = blockIdx.y, lane = threadIdx.x & 31, i8 = lane % LANES, sub = lane / LANES;
   const int first = min(max(a.indptr[b], 0), a.n_tokens), count = min(max(a.indptr[b + 1], first), a.n_tokens) - first;
   const int len = min(max(a.lens[b], 0), a.capacity);
-  const int groups = (a.layers + kPackLayers - 1) / kPackLayers;
-  const int at = (2 * (i8 % 4) + (i8 / 4 & 1)) * (2 * G) + (i8 / 4 & ~1) * 2;
-  const long long items = (long long)count * groups;
-  for (long long it = blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5); it < items; it += gridDim.x * (kPackThreads / 32)) {
-    const int i = (int)(it / groups), layer0 = (int)(it % groups) * kPackLayers;
+  const int at = place<D>(i8);
+  for (int i = blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5); i < count; i += gridDim.x * (kPackThreads / 32)) {
     const int pos = i < a.capacity - len ? len + i : -1;
     const int pg = a.c.page_of(b, pos), in_page = pos & ((1 << a.c.shift) - 1);  // without a page nothing of it is used
-    for (int h0 = 0; h0 < a.kv_heads; h0 += ROWS) {
-      const int h = h0 + sub;
-      const bool there = h < a.kv_heads, mapped = there && pg >= 0;
-      const long long to = layer0 * a.layer + (first + i) * a.token + ((long long)h * D + i8 * 8) * (int)sizeof(T);
-      const long long from = (mapped ? pg : 0) * a.c.page + layer0 * a.c.layer + h * a.c.head + (long long)in_page * (D / 2) + at;
-      const long long from_s = (mapped ? pg : 0) * a.c.scale_page + layer0 * a.c.scale_layer + h * a.c.scale_head + (long long)in_page * (D / 16) + i8 / 4 * 2;
-      uint32_t word[2 * kPackLayers], s[2 * kPackLayers];
+    for (int layer0 = blockIdx.z * kPackLayers; layer0 < a.layers; layer0 += gridDim.z * kPackLayers)
+      for (int h0 = 0; h0 < a.kv_heads; h0 += ROWS) {
+        const int h = h0 + sub;
+        const bool there = h < a.kv_heads, mapped = there && pg >= 0;
+        const long long to = layer0 * a.layer + (first + i) * a.token + (long long)((h * D + i8 * 8) * (int)sizeof(T));
+        const long long from = (mapped ? pg : 0) * a.c.page + layer0 * a.c.layer + h * a.c.head + in_page * (D / 2) + at;
+        const long long from_s = (mapped ? pg : 0) * a.c.scale_page + layer0 * a.c.scale_layer + h * a.c.scale_head + in_page * (D / 16) + i8 / 4 * 2;
+        uint32_t word[2 * kPackLayers], s[2 * kPackLayers];
 #pragma unroll
-      for (int r = 0; r < 2 * kPackLayers; r++) {
-        word[r] = 0x88888888u, s[r] = 0;
-        if (mapped && layer0 + r / 2 < a.layers) {
-          word[r] = __ldg((const uint32_t *)((r & 1 ? a.c.v : a.c.k) + from + r / 2 * a.c.layer));
-          s[r] = __ldg((const uint16_t *)((r & 1 ? a.c.v_scale : a.c.k_scale) + from_s + r / 2 * a.c.scale_layer));
+        for (int r = 0; r < 2 * kPackLayers; r++) {
+          word[r] = 0x88888888u, s[r] = 0;
+          if (mapped && layer0 + r / 2 < a.layers) {
+            word[r] = __ldg((const uint32_t *)((r & 1 ? a.c.v : a.c.k) + from + r / 2 * a.c.layer));
+            s[r] = __ldg((const uint16_t *)((r & 1 ? a.c.v_scale : a.c.k_scale) + from_s + r / 2 * a.c.scale_layer));
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2 * kPackLayers; r++) {
+          if (layer0 + r / 2 >= a.layers) break;
+          unpack8<D>((T *)((r & 1 ? a.v : a.k) + to + r / 2 * a.layer), word[r], __byte_perm(s[r], 0, 0x1010), i8, there);
         }
       }
-#pragma unroll
-      for (int r = 0; r < 2 * kPackLayers; r++) {
-        if (layer0 + r / 2 >= a.layers) break;
-        float x[8];
-        unpack8<D>(x, word[r], __uint_as_float(s[r] << 16), i8);
-        if (there) store8((T *)((r & 1 ? a.v : a.k) + to + r / 2 * a.layer), x);
-      }
-    }
   }
 }
 

@@ -75,9 +75,10 @@ PackArgs pack_args(const ocrvl_packed_cache *c, int type, int n_tokens, const in
 int move_grid(const PackArgs &a, int most_tokens, dim3 *grid) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const long long items = (a.layers + kPackLayers - 1) / kPackLayers * (long long)most_tokens;
-  const long long blocks = (items + kPackThreads / 32 - 1) / (kPackThreads / 32), most = (sms * 16 + a.batch - 1) / a.batch;
-  *grid = dim3((unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most), a.batch);
+  const long long groups = (a.layers + kPackLayers - 1) / kPackLayers, z = groups < 64 ? groups : 64;
+  const long long blocks = ((long long)most_tokens + kPackThreads / 32 - 1) / (kPackThreads / 32);
+  const long long most = (sms * 16 + a.batch * z - 1) / (a.batch * z);
+  *grid = dim3((unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most), a.batch, (unsigned)z);
   return OCRVL_OK;
 }
 
@@ -129,13 +130,16 @@ int launch_pack_dim(const TreeArgs &a, int dim, int sms, int rows_max, char *wor
 
 template <typename T, int V, int NORM>
 int launch_rotate(RotateArgs &a, int sms, cudaStream_t stream) {
-  // Warps a token: one, or as many as its heads keep busy while the GPU is not full.
   a.lanes = a.pairs / V + (a.dim - 2 * a.pairs) / (2 * V);
-  const int at_once = 32 / a.lanes, steps = (a.heads + a.kv_heads + at_once - 1) / at_once;
-  const long long room = (long long)sms * 16;
-  a.share = (int)(room / a.n_tokens < 1 ? 1 : room / a.n_tokens < steps ? room / a.n_tokens : steps);
-  const long long units = (long long)a.n_tokens * a.share, blocks = (units + kRotateWarps - 1) / kRotateWarps;
-  return launch("rotate", k_rotate<T, V, NORM>, dim3((unsigned)blocks), kRotateWarps * 32, 0, stream, false, 1, a);
+  a.at_once = 32 / a.lanes, a.lane_factor = (65536 + a.lanes - 1) / a.lanes, a.one_dim = 1.f / a.dim;
+  // Warps a token: one, or as many as its heads keep busy while the GPU is not full.
+  const int steps = (a.heads + a.at_once - 1) / a.at_once, blocks = (a.n_tokens + kRotateWarps - 1) / kRotateWarps;
+  const int room = sms * 2 / blocks, share = room < 1 ? 1 : room < steps ? room : steps;
+  const dim3 grid(blocks, share);
+  auto go = [&](auto kernel) { return launch("rotate", kernel, grid, kRotateWarps * 32, 0, stream, false, 1, a); };
+  if (a.lanes == 8) return go(k_rotate<T, V, NORM, 8>);
+  if (a.lanes == 16) return go(k_rotate<T, V, NORM, 16>);
+  return go(k_rotate<T, V, NORM, 0>);
 }
 
 template <typename T, int V>

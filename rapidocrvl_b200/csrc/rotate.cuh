@@ -23,8 +23,9 @@ struct RotateArgs {
   const void *q_weight, *k_weight;
   const int *pos;
   long long q_stride, k_stride, q_out_stride, k_out_stride, pos_stride;  // bytes; entries
-  int n_tokens, heads, kv_heads, dim, pairs, neighbours, lanes, share;   // lanes: of a row; share: warps a token
-  float eps;
+  int n_tokens, heads, kv_heads, dim, pairs, neighbours;
+  int lanes, at_once, lane_factor;  // lanes of a row, rows at once, 2^16 / lanes rounded up
+  float eps, one_dim;               // 1 / dim
   double turns[kRotateMost];  // freq / 2 pi
   unsigned char axis[kRotateMost];
 };
@@ -59,13 +60,12 @@ __device__ __forceinline__ void store_v(T *p, const float (&x)[V]) {
   }
 }
 
-// NORM: 0 none, 1 weights of T, 2 weights of f32.
-template <typename T, int V, int NORM>
+// NORM: 0 none, 1 weights of T, 2 weights of f32.  LANES: of a row, 0: any number.
+template <typename T, int V, int NORM, int LANES>
 __global__ void __launch_bounds__(kRotateWarps * 32) k_rotate(const __grid_constant__ RotateArgs a) {
   __shared__ __align__(16) float trig[kRotateWarps][2][kRotateMost];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long unit = (long long)blockIdx.x * kRotateWarps + warp;
-  const long long token = unit / a.share;
+  const int token = blockIdx.x * kRotateWarps + warp;
   if (token >= a.n_tokens) return;  // the whole warp
   float *cs = trig[warp][0], *sn = trig[warp][1];
   for (int p = lane; p < a.pairs; p += 32) {
@@ -73,8 +73,9 @@ __global__ void __launch_bounds__(kRotateWarps * 32) k_rotate(const __grid_const
     sincospif(2.f * (float)(x - rint(x)), &sn[p], &cs[p]);
   }
   __syncwarp();
-  const int at_once = 32 / a.lanes, sub = lane / a.lanes, v = lane % a.lanes, rotated = a.pairs / V;
-  // the lane's two runs of V dims, and where their pairs are among the cosines
+  const int lanes = LANES ? LANES : a.lanes, at_once = LANES ? 32 / (LANES ? LANES : 1) : a.at_once;
+  const int sub = LANES ? lane / (LANES ? LANES : 1) : lane * a.lane_factor >> 16, v = lane - sub * lanes, rotated = a.pairs / V;
+  // the lane's two runs of V dims, and its pairs' cosines and sines
   int d0, d1;
   float c[V] = {}, s[V] = {};
   if (v < rotated) {
@@ -88,55 +89,59 @@ __global__ void __launch_bounds__(kRotateWarps * 32) k_rotate(const __grid_const
   } else {
     d0 = 2 * a.pairs + 2 * V * (v - rotated), d1 = d0 + V;
   }
-  const int rows = a.heads + a.kv_heads, part = (int)(unit % a.share);
-  for (int r0 = part * at_once; r0 < rows; r0 += a.share * at_once) {
-    const int r = r0 + sub;
-    const bool there = sub < at_once && r < rows, is_q = r < a.heads;
-    const int head = is_q ? r : r - a.heads;
-    const T *from = (const T *)((is_q ? a.q : a.k) + token * (is_q ? a.q_stride : a.k_stride)) + (long long)head * a.dim;
-    T *to = (T *)((is_q ? a.q_out : a.k_out) + token * (is_q ? a.q_out_stride : a.k_out_stride)) + (long long)head * a.dim;
-    float x[V] = {}, y[V] = {};
-    if (there) load_v<T, V>(x, from + d0), load_v<T, V>(y, from + d1);
-    if constexpr (NORM > 0) {
-      float sum = 0.f;
+  auto heads = [&](int n, const char *in, char *out, const void *weight) {
+    float w0[V], w1[V];
+    if constexpr (NORM == 1) load_v<T, V>(w0, (const T *)weight + d0), load_v<T, V>(w1, (const T *)weight + d1);
+    if constexpr (NORM == 2) {
 #pragma unroll
-      for (int e = 0; e < V; e++) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
-      // over the row's lanes, whatever their number: the first one collects, all ask it
+      for (int e = 0; e < V; e += 4)
+        *(float4 *)(w0 + e) = *(const float4 *)((const float *)weight + d0 + e), *(float4 *)(w1 + e) = *(const float4 *)((const float *)weight + d1 + e);
+    }
+    const int step = gridDim.y * at_once;
+    for (int r = blockIdx.y * at_once + sub; __any_sync(~0u, r < n); r += step) {
+      const bool there = r < n && sub < at_once;
+      const T *from = (const T *)in + r * a.dim;
+      float x[V] = {}, y[V] = {};
+      if (there) load_v<T, V>(x, from + d0), load_v<T, V>(y, from + d1);
+      if constexpr (NORM > 0) {
+        float sum = 0.f;
 #pragma unroll
-      for (int d = 16; d; d >>= 1) {
-        const float other = __shfl_down_sync(~0u, sum, d);
-        if (v < d && v + d < a.lanes) sum += other;
+        for (int e = 0; e < V; e++) sum = fmaf(x[e], x[e], fmaf(y[e], y[e], sum));
+        if constexpr (LANES > 0) {
+#pragma unroll
+          for (int d = LANES / 2; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        } else {  // the row's first lane collects, all ask it
+#pragma unroll
+          for (int d = 16; d; d >>= 1) {
+            const float other = __shfl_down_sync(~0u, sum, d);
+            if (v < d && v + d < lanes) sum += other;
+          }
+          sum = __shfl_sync(~0u, sum, lane - v);
+        }
+        const float inv = rsqrtf(sum * a.one_dim + a.eps);
+#pragma unroll
+        for (int e = 0; e < V; e++) x[e] *= inv * w0[e], y[e] *= inv * w1[e];
       }
-      sum = __shfl_sync(~0u, sum, lane - v);
-      const float inv = rsqrtf(sum / a.dim + a.eps);
-      float w0[V], w1[V];
-      if constexpr (NORM == 1) {
-        const T *w = (const T *)(is_q ? a.q_weight : a.k_weight);
-        load_v<T, V>(w0, w + d0), load_v<T, V>(w1, w + d1);
+      float z0[V], z1[V];
+      if (v >= rotated) {
+#pragma unroll
+        for (int e = 0; e < V; e++) z0[e] = x[e], z1[e] = y[e];
+      } else if (!a.neighbours) {
+#pragma unroll
+        for (int e = 0; e < V; e++) z0[e] = x[e] * c[e] - y[e] * s[e], z1[e] = y[e] * c[e] + x[e] * s[e];
       } else {
-        const float *w = (const float *)(is_q ? a.q_weight : a.k_weight);
 #pragma unroll
-        for (int e = 0; e < V; e += 4) *(float4 *)(w0 + e) = *(const float4 *)(w + d0 + e), *(float4 *)(w1 + e) = *(const float4 *)(w + d1 + e);
+        for (int e = 0; e < V; e += 2) {
+          z0[e] = x[e] * c[e / 2] - x[e + 1] * s[e / 2], z0[e + 1] = x[e + 1] * c[e / 2] + x[e] * s[e / 2];
+          z1[e] = y[e] * c[V / 2 + e / 2] - y[e + 1] * s[V / 2 + e / 2], z1[e + 1] = y[e + 1] * c[V / 2 + e / 2] + y[e] * s[V / 2 + e / 2];
+        }
       }
-#pragma unroll
-      for (int e = 0; e < V; e++) x[e] *= inv * w0[e], y[e] *= inv * w1[e];
+      T *to = (T *)out + r * a.dim;
+      if (there) store_v<T, V>(to + d0, z0), store_v<T, V>(to + d1, z1);
     }
-    float z0[V], z1[V];
-    if (v >= rotated) {
-#pragma unroll
-      for (int e = 0; e < V; e++) z0[e] = x[e], z1[e] = y[e];
-    } else if (!a.neighbours) {
-#pragma unroll
-      for (int e = 0; e < V; e++) z0[e] = x[e] * c[e] - y[e] * s[e], z1[e] = y[e] * c[e] + x[e] * s[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        z0[e] = x[e] * c[e / 2] - x[e + 1] * s[e / 2], z0[e + 1] = x[e + 1] * c[e / 2] + x[e] * s[e / 2];
-        z1[e] = y[e] * c[V / 2 + e / 2] - y[e + 1] * s[V / 2 + e / 2], z1[e + 1] = y[e + 1] * c[V / 2 + e / 2] + y[e] * s[V / 2 + e / 2];
-      }
-    }
-    if (there) store_v<T, V>(to + d0, z0), store_v<T, V>(to + d1, z1);
-  }
+  };
+  heads(a.heads, a.q + token * a.q_stride, a.q_out + token * a.q_out_stride, a.q_weight);
+  if (a.kv_heads) heads(a.kv_heads, a.k + token * a.k_stride, a.k_out + token * a.k_out_stride, a.k_weight);
 }
 
 }  // namespace paged

@@ -143,6 +143,21 @@ def test_append_of_special_values(kvops, dtype):
     assert bool(v[0, 7, 0, :32].isnan().all()) and not bool(v[0, 7, 0, 32:].isnan().any())
 
 
+def test_scales_next_to_the_smallest_normal_number(kvops):
+    """Five bits of a number below 2^-126 are counted from its own first bit on: 31/32 of it is 0, from 63/64 on it is 2^-126."""
+    s = Store(kvops, "f32", [0], [24], 1, 64, layers=1)
+    s.x = torch.zeros(2, 1, 24, 1, 64)
+    tiny = 2.0 ** -126
+    for i, f in enumerate([0.5, 0.9375, 0.96, 0.96875, 0.975, 0.98, 63 / 64 - 2.0 ** -20, 63 / 64, 63 / 64 + 2.0 ** -20, 0.99, 1, 1.03125, 1.04, 1.1, 1.9, 1.97, 2, 3, 31, 63, 0.1, 1e-6, 0, 0.75]):
+        s.x[0, 0, i, 0, i], s.x[1, 0, i, 0, 63 - i] = 7 * f * tiny, -7 * f * tiny
+        s.x[:, 0, i, 0, 30] = 3 * f * tiny
+    dev = s.x.cuda()
+    kvops.append(s.cache, dev[0], dev[1], s.lens, s.indptr)
+    for i in range(24):
+        s.put(0, i, i)
+    s.check()
+
+
 def test_append_of_paths_bad_nodes_and_full_tables(kvops):
     s = Store(kvops, "bf16", [30, 0, 17, 60], [4, 3, 5, 8], layers=4, most=4)
     s.table_h[2, 1] = -1  # no page for positions 16 ..
