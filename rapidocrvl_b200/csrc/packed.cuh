@@ -39,8 +39,8 @@ struct PackArgs {
   int capacity, layers, batch, kv_heads, n_tokens, max_path;
 };
 
-constexpr int kPackLayers = 3;     // layers a warp takes of a token at once
-constexpr int kPackThreads = 256;
+constexpr int kPackWarps = 8, kPackThreads = kPackWarps * 32;
+constexpr int kPackRows = 4;  // steps whose loads go out together
 
 // 8 values of a row: as they lie in memory, and as 32-bit floats.
 template <typename T>
@@ -229,78 +229,102 @@ __device__ __forceinline__ void unpack8(T *to, uint32_t word, uint32_t scale, in
   }
 }
 
-// A warp takes K and V of one token in up to kPackLayers layers (blockIdx.z), all heads; D / 8 lanes a row.
+// What a warp takes: chunks of 16 positions of one (layer, K or V, head), blockIdx.x and further on of the
+// sequence blockIdx.y's, so that a page is looked up, and addresses are worked out, once for 16 rows.  D / 8 lanes a row,
+// kPackRows rows on their way at once.
+template <int D>
+struct PackItem {
+  static constexpr int LANES = D / 8, ROWS = 32 / LANES, STEPS = kChunk / ROWS;  // of a row; rows at once; steps a chunk
+  int first, count, len;   // of the sequence: tokens, cached positions
+  int layer, v, head;
+
+  __device__ __forceinline__ PackItem(const PackArgs &a, int b) {
+    first = min(max(a.indptr[b], 0), a.n_tokens), count = min(max(a.indptr[b + 1], first), a.n_tokens) - first;
+    len = min(max(a.lens[b], 0), a.capacity);
+  }
+  __device__ __forceinline__ bool at(const PackArgs &a, int c) {
+    if (c >= a.layers * 2 * a.kv_heads) return false;
+    const int lv = c / a.kv_heads;
+    head = c - lv * a.kv_heads, v = lv & 1, layer = lv >> 1;
+    return true;
+  }
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kPackThreads) k_packed_append(const PackArgs a) {
-  constexpr int LANES = D / 8, ROWS = 32 / LANES;  // of a row; rows at once
-  const int b = blockIdx.y, lane = threadIdx.x & 31, i8 = lane % LANES, sub = lane / LANES;
-  const int first = min(max(a.indptr[b], 0), a.n_tokens), count = min(max(a.indptr[b + 1], first), a.n_tokens) - first;
-  const int len = min(max(a.lens[b], 0), a.capacity);
-  const int n = min(a.path ? min(max(a.n_path[b], 0), a.max_path) : count, a.capacity - len);
-  if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.new_lens[b] = len + n;
-  const int at = place<D>(i8);
-  for (int i = blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5); i < n; i += gridDim.x * (kPackThreads / 32)) {
-    const int pos = len + i, node = a.path ? a.path[(long long)b * a.max_path + i] : i;
-    if (node < 0 || node >= count) continue;
-    const int pg = a.c.page_of(b, pos), in_page = pos & ((1 << a.c.shift) - 1);
-    for (int layer0 = blockIdx.z * kPackLayers; layer0 < a.layers; layer0 += gridDim.z * kPackLayers)
-      for (int h0 = 0; h0 < a.kv_heads; h0 += ROWS) {
-        const int h = h0 + sub;
-        const bool there = h < a.kv_heads;
-        const long long from = layer0 * a.layer + (first + node) * a.token + (long long)(((there ? h : 0) * D + i8 * 8) * (int)sizeof(T));
-        Eight<T> x[2 * kPackLayers];  // the loads do not wait for the page
+  using I = PackItem<D>;
+  const int b = blockIdx.y, lane = threadIdx.x & 31, i8 = lane % I::LANES, sub = lane / I::LANES;
+  I x(a, b);
+  const int n = min(a.path ? min(max(a.n_path[b], 0), a.max_path) : x.count, a.capacity - x.len);
+  if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.new_lens[b] = x.len + n;
+  if (n == 0) return;
+  const int end = x.len + n, codes_at = sub * (D / 2) + place<D>(i8), scales_at = sub * (D / 16) + i8 / 4 * 2;
+  for (int c = blockIdx.z * kPackWarps + (threadIdx.x >> 5); x.at(a, c); c += gridDim.z * kPackWarps) {
+    const char *from = (x.v ? a.v : a.k) + x.layer * a.layer + x.first * a.token + (x.head * D + i8 * 8) * (long long)sizeof(T);
+    for (int p0 = (x.len / kChunk + blockIdx.x) * kChunk; p0 < end; p0 += gridDim.x * kChunk) {
+      const int pg = a.c.page_of(b, p0), in_page = p0 & ((1 << a.c.shift) - 1);
+      char *codes = (x.v ? a.c.v : a.c.k) + pg * a.c.page + x.layer * a.c.layer + x.head * a.c.head + in_page * (D / 2) + codes_at;
+      char *scales = (x.v ? a.c.v_scale : a.c.k_scale) + pg * a.c.scale_page + x.layer * a.c.scale_layer + x.head * a.c.scale_head +
+                     in_page * (D / 16) + scales_at;
+#pragma unroll 1
+      for (int s0 = 0; s0 < I::STEPS; s0 += kPackRows) {
+        Eight<T> y[kPackRows];
+        bool there[kPackRows];
 #pragma unroll
-        for (int r = 0; r < 2 * kPackLayers; r++)
-          if (layer0 + r / 2 < a.layers) x[r].load((const T *)((r & 1 ? a.v : a.k) + from + r / 2 * a.layer));
-        const long long to = pg * a.c.page + layer0 * a.c.layer + h * a.c.head + in_page * (D / 2) + at;
-        const long long to_s = pg * a.c.scale_page + layer0 * a.c.scale_layer + h * a.c.scale_head + in_page * (D / 16) + i8 / 4 * 2;
+        for (int r = 0; r < kPackRows; r++) {
+          const int i = p0 - x.len + (s0 + r) * I::ROWS + sub;
+          there[r] = i >= 0 && i < n;
+          const int node = there[r] && a.path ? a.path[(long long)b * a.max_path + i] : i;
+          there[r] = there[r] && node >= 0 && node < x.count;
+          if (there[r]) y[r].load((const T *)(from + node * a.token));  // not waiting for the page
+        }
 #pragma unroll
-        for (int r = 0; r < 2 * kPackLayers; r++) {
-          if (layer0 + r / 2 >= a.layers) break;
+        for (int r = 0; r < kPackRows; r++) {
+          if (!__any_sync(~0u, there[r])) continue;
           float s;
-          const uint32_t word = pack8<D>(x[r], i8, &s);
-          if (!there || pg < 0) continue;
-          *(uint32_t *)((r & 1 ? a.c.v : a.c.k) + to + r / 2 * a.c.layer) = word;
-          if (i8 % 4 == 0)
-            *(uint16_t *)((r & 1 ? a.c.v_scale : a.c.k_scale) + to_s + r / 2 * a.c.scale_layer) = (uint16_t)(__float_as_uint(s) >> 16);
+          const uint32_t word = pack8<D>(y[r], i8, &s);
+          if (!there[r] || pg < 0) continue;
+          *(uint32_t *)(codes + (s0 + r) * (I::ROWS * D / 2)) = word;
+          if (i8 % 4 == 0) *(uint16_t *)(scales + (s0 + r) * (I::ROWS * D / 16)) = (uint16_t)(__float_as_uint(s) >> 16);
         }
       }
+    }
   }
 }
 
-// The other way, shared out alike; a token without a page reads as 0.
+// A token without a page reads as 0.
 template <typename T, int D>
 __global__ void __launch_bounds__(kPackThreads) k_packed_read(const PackArgs a) {
-  constexpr int LANES = D / 8, ROWS = 32 / LANES;
-  const int b = blockIdx.y, lane = threadIdx.x & 31, i8 = lane % LANES, sub = lane / LANES;
-  const int first = min(max(a.indptr[b], 0), a.n_tokens), count = min(max(a.indptr[b + 1], first), a.n_tokens) - first;
-  const int len = min(max(a.lens[b], 0), a.capacity);
-  const int at = place<D>(i8);
-  for (int i = blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5); i < count; i += gridDim.x * (kPackThreads / 32)) {
-    const int pos = i < a.capacity - len ? len + i : -1;
-    const int pg = a.c.page_of(b, pos), in_page = pos & ((1 << a.c.shift) - 1);  // without a page nothing of it is used
-    for (int layer0 = blockIdx.z * kPackLayers; layer0 < a.layers; layer0 += gridDim.z * kPackLayers)
-      for (int h0 = 0; h0 < a.kv_heads; h0 += ROWS) {
-        const int h = h0 + sub;
-        const bool there = h < a.kv_heads, mapped = there && pg >= 0;
-        const long long to = layer0 * a.layer + (first + i) * a.token + (long long)((h * D + i8 * 8) * (int)sizeof(T));
-        const long long from = (mapped ? pg : 0) * a.c.page + layer0 * a.c.layer + h * a.c.head + in_page * (D / 2) + at;
-        const long long from_s = (mapped ? pg : 0) * a.c.scale_page + layer0 * a.c.scale_layer + h * a.c.scale_head + in_page * (D / 16) + i8 / 4 * 2;
-        uint32_t word[2 * kPackLayers], s[2 * kPackLayers];
+  using I = PackItem<D>;
+  const int b = blockIdx.y, lane = threadIdx.x & 31, i8 = lane % I::LANES, sub = lane / I::LANES;
+  I x(a, b);
+  if (x.count == 0) return;
+  const int codes_at = sub * (D / 2) + place<D>(i8), scales_at = sub * (D / 16) + i8 / 4 * 2;
+  for (int c = blockIdx.z * kPackWarps + (threadIdx.x >> 5); x.at(a, c); c += gridDim.z * kPackWarps) {
+    char *to = (x.v ? a.v : a.k) + x.layer * a.layer + x.first * a.token + (x.head * D + i8 * 8) * (long long)sizeof(T);
+    const int skip = x.len % kChunk, chunks = (int)(((long long)skip + x.count + kChunk - 1) / kChunk);
+    for (int ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
+      const long long p0 = (x.len / kChunk + (long long)ch) * kChunk;
+      const int pg = p0 < a.capacity ? a.c.page_of(b, (int)p0) : -1, in_page = (int)p0 & ((1 << a.c.shift) - 1);
+      const char *codes = (x.v ? a.c.v : a.c.k) + pg * a.c.page + x.layer * a.c.layer + x.head * a.c.head + in_page * (D / 2) + codes_at;
+      const char *scales = (x.v ? a.c.v_scale : a.c.k_scale) + pg * a.c.scale_page + x.layer * a.c.scale_layer + x.head * a.c.scale_head +
+                           in_page * (D / 16) + scales_at;
+      const int i0 = (int)((long long)ch * kChunk - skip);
+      uint32_t word[I::STEPS], s[I::STEPS];
 #pragma unroll
-        for (int r = 0; r < 2 * kPackLayers; r++) {
-          word[r] = 0x88888888u, s[r] = 0;
-          if (mapped && layer0 + r / 2 < a.layers) {
-            word[r] = __ldg((const uint32_t *)((r & 1 ? a.c.v : a.c.k) + from + r / 2 * a.c.layer));
-            s[r] = __ldg((const uint16_t *)((r & 1 ? a.c.v_scale : a.c.k_scale) + from_s + r / 2 * a.c.scale_layer));
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < 2 * kPackLayers; r++) {
-          if (layer0 + r / 2 >= a.layers) break;
-          unpack8<D>((T *)((r & 1 ? a.v : a.k) + to + r / 2 * a.layer), word[r], __byte_perm(s[r], 0, 0x1010), i8, there);
+      for (int r = 0; r < I::STEPS; r++) {
+        word[r] = 0x88888888u, s[r] = 0;
+        if (pg >= 0) {  // the page holds the whole chunk
+          word[r] = __ldg((const uint32_t *)(codes + r * (I::ROWS * D / 2)));
+          s[r] = __ldg((const uint16_t *)(scales + r * (I::ROWS * D / 16)));
         }
       }
+#pragma unroll
+      for (int r = 0; r < I::STEPS; r++) {
+        const int i = i0 + r * I::ROWS + sub;
+        unpack8<D>((T *)(to + i * a.token), word[r], __byte_perm(s[r], 0, 0x1010), i8, i >= 0 && i < x.count);
+      }
+    }
   }
 }
 

@@ -71,14 +71,15 @@ PackArgs pack_args(const ocrvl_packed_cache *c, int type, int n_tokens, const in
   return a;
 }
 
-// A warp a token and kPackLayers layers, as many blocks as the longest sequence can use or the GPU holds.
+// A warp 16 positions of a (layer, K or V, head); as many blocks as the longest sequence can use, or some waves of them.
 int move_grid(const PackArgs &a, int most_tokens, dim3 *grid) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  const long long groups = (a.layers + kPackLayers - 1) / kPackLayers, z = groups < 64 ? groups : 64;
-  const long long blocks = ((long long)most_tokens + kPackThreads / 32 - 1) / (kPackThreads / 32);
-  const long long most = (sms * 16 + a.batch * z - 1) / (a.batch * z);
-  *grid = dim3((unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most), a.batch, (unsigned)z);
+  const long long rows = 2ll * a.layers * a.kv_heads;
+  if (rows > 1 << 30) return invalid("too many layers and kv heads");
+  const long long z = (rows + kPackWarps - 1) / kPackWarps < 1024 ? (rows + kPackWarps - 1) / kPackWarps : 1024;
+  const long long chunks = (long long)most_tokens / kChunk + 2, most = (sms * 32 + a.batch * z - 1) / (a.batch * z);
+  *grid = dim3((unsigned)(chunks < most ? chunks : most), a.batch, (unsigned)z);
   return OCRVL_OK;
 }
 

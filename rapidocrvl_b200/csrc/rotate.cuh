@@ -30,25 +30,30 @@ struct RotateArgs {
   unsigned char axis[kRotateMost];
 };
 
+// V values as they lie in memory, and as 32-bit floats.
 template <typename T, int V>
-__device__ __forceinline__ void load_v(float (&x)[V], const T *p) {
-  if constexpr (sizeof(T) == 4) {
-    static_assert(V == 4, "");
-    const float4 a = *(const float4 *)p;
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-  } else {
-    uint32_t w[V / 2];
-    if constexpr (V == 8)
+struct Run {
+  uint32_t w[V * sizeof(T) / 4];
+
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (V * sizeof(T) == 16)
       *(uint4 *)w = *(const uint4 *)p;
     else
       *(uint2 *)w = *(const uint2 *)p;
+  }
+  __device__ __forceinline__ void floats(float (&x)[V]) const {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < V / 2; i++) {
-      const float2 f = unpack2<T>(w[i]);
-      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      for (int i = 0; i < V; i++) x[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; i++) {
+        const float2 f = unpack2<T>(w[i]);
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      }
     }
   }
-}
+};
 template <typename T, int V>
 __device__ __forceinline__ void store_v(T *p, const float (&x)[V]) {
   if constexpr (sizeof(T) == 4) {
@@ -60,49 +65,56 @@ __device__ __forceinline__ void store_v(T *p, const float (&x)[V]) {
   }
 }
 
+constexpr int kRotateSteps = 4;  // of rows whose loads go out together
+
 // NORM: 0 none, 1 weights of T, 2 weights of f32.  LANES: of a row, 0: any number.
 template <typename T, int V, int NORM, int LANES>
-__global__ void __launch_bounds__(kRotateWarps * 32) k_rotate(const __grid_constant__ RotateArgs a) {
+__global__ void __launch_bounds__(kRotateWarps * 32, 2) k_rotate(const __grid_constant__ RotateArgs a) {
   __shared__ __align__(16) float trig[kRotateWarps][2][kRotateMost];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int token = blockIdx.x * kRotateWarps + warp;
   if (token >= a.n_tokens) return;  // the whole warp
+  const int lanes = LANES ? LANES : a.lanes, at_once = LANES ? 32 / (LANES ? LANES : 1) : a.at_once;
+  const int sub = LANES ? lane / (LANES ? LANES : 1) : lane * a.lane_factor >> 16, v = lane - sub * lanes, rotated = a.pairs / V;
+  // the lane's two runs of V dims
+  const int d0 = v >= rotated ? 2 * a.pairs + 2 * V * (v - rotated) : a.neighbours ? 2 * V * v : V * v;
+  const int d1 = v >= rotated || a.neighbours ? d0 + V : a.pairs + d0;
+  const int start = blockIdx.y * at_once + sub, step = gridDim.y * at_once;
+  using Rows = Run<T, V>[kRotateSteps][2];
+  auto load = [&](Rows &x, int r0, int n, const char *in) {
+#pragma unroll
+    for (int i = 0; i < kRotateSteps; i++) {
+      const int r = r0 + i * step;
+      const T *from = (const T *)in + r * a.dim;
+      if (r < n && sub < at_once) x[i][0].load(from + d0), x[i][1].load(from + d1);
+    }
+  };
+  const char *q = a.q + token * a.q_stride, *k = a.k + token * a.k_stride;
+  Rows xq;
+  load(xq, start, a.heads, q);  // on their way during what follows
+
   float *cs = trig[warp][0], *sn = trig[warp][1];
   for (int p = lane; p < a.pairs; p += 32) {
     const double x = (double)a.pos[token * a.pos_stride + a.axis[p]] * a.turns[p];
     sincospif(2.f * (float)(x - rint(x)), &sn[p], &cs[p]);
   }
   __syncwarp();
-  const int lanes = LANES ? LANES : a.lanes, at_once = LANES ? 32 / (LANES ? LANES : 1) : a.at_once;
-  const int sub = LANES ? lane / (LANES ? LANES : 1) : lane * a.lane_factor >> 16, v = lane - sub * lanes, rotated = a.pairs / V;
-  // the lane's two runs of V dims, and its pairs' cosines and sines
-  int d0, d1;
   float c[V] = {}, s[V] = {};
   if (v < rotated) {
-    d0 = a.neighbours ? 2 * V * v : V * v;
-    d1 = a.neighbours ? d0 + V : a.pairs + d0;
 #pragma unroll
     for (int e = 0; e < V; e += 4) {
       *(float4 *)(c + e) = *(const float4 *)(cs + V * v + e);
       *(float4 *)(s + e) = *(const float4 *)(sn + V * v + e);
     }
-  } else {
-    d0 = 2 * a.pairs + 2 * V * (v - rotated), d1 = d0 + V;
   }
-  auto heads = [&](int n, const char *in, char *out, const void *weight) {
-    float w0[V], w1[V];
-    if constexpr (NORM == 1) load_v<T, V>(w0, (const T *)weight + d0), load_v<T, V>(w1, (const T *)weight + d1);
-    if constexpr (NORM == 2) {
+  auto turn = [&](const Rows &raw, int r0, int n, char *out, const float (&w0)[V], const float (&w1)[V]) {
 #pragma unroll
-      for (int e = 0; e < V; e += 4)
-        *(float4 *)(w0 + e) = *(const float4 *)((const float *)weight + d0 + e), *(float4 *)(w1 + e) = *(const float4 *)((const float *)weight + d1 + e);
-    }
-    const int step = gridDim.y * at_once;
-    for (int r = blockIdx.y * at_once + sub; __any_sync(~0u, r < n); r += step) {
+    for (int i = 0; i < kRotateSteps; i++) {
+      const int r = r0 + i * step;
+      if (!__any_sync(~0u, r < n)) break;
       const bool there = r < n && sub < at_once;
-      const T *from = (const T *)in + r * a.dim;
-      float x[V] = {}, y[V] = {};
-      if (there) load_v<T, V>(x, from + d0), load_v<T, V>(y, from + d1);
+      float x[V], y[V];
+      raw[i][0].floats(x), raw[i][1].floats(y);
       if constexpr (NORM > 0) {
         float sum = 0.f;
 #pragma unroll
@@ -140,8 +152,35 @@ __global__ void __launch_bounds__(kRotateWarps * 32) k_rotate(const __grid_const
       if (there) store_v<T, V>(to + d0, z0), store_v<T, V>(to + d1, z1);
     }
   };
-  heads(a.heads, a.q + token * a.q_stride, a.q_out + token * a.q_out_stride, a.q_weight);
-  if (a.kv_heads) heads(a.kv_heads, a.k + token * a.k_stride, a.k_out + token * a.k_out_stride, a.k_weight);
+  auto weights = [&](float (&w0)[V], float (&w1)[V], const void *weight) {
+    if constexpr (NORM == 1) {
+      Run<T, V> x;
+      x.load((const T *)weight + d0), x.floats(w0);
+      x.load((const T *)weight + d1), x.floats(w1);
+    }
+    if constexpr (NORM == 2) {
+#pragma unroll
+      for (int e = 0; e < V; e += 4)
+        *(float4 *)(w0 + e) = *(const float4 *)((const float *)weight + d0 + e), *(float4 *)(w1 + e) = *(const float4 *)((const float *)weight + d1 + e);
+    }
+  };
+  const int all = step * kRotateSteps;
+  float w0[V], w1[V];
+  weights(w0, w1, a.q_weight);
+  Rows xk;
+  if (a.kv_heads) load(xk, start, a.kv_heads, k);
+  turn(xq, start, a.heads, a.q_out + token * a.q_out_stride, w0, w1);
+  for (int r0 = start + all; __any_sync(~0u, r0 < a.heads); r0 += all) {
+    load(xq, r0, a.heads, q);
+    turn(xq, r0, a.heads, a.q_out + token * a.q_out_stride, w0, w1);
+  }
+  if (!a.kv_heads) return;
+  weights(w0, w1, a.k_weight);
+  turn(xk, start, a.kv_heads, a.k_out + token * a.k_out_stride, w0, w1);
+  for (int r0 = start + all; __any_sync(~0u, r0 < a.kv_heads); r0 += all) {
+    load(xk, r0, a.kv_heads, k);
+    turn(xk, r0, a.kv_heads, a.k_out + token * a.k_out_stride, w0, w1);
+  }
 }
 
 }  // namespace paged
