@@ -3,7 +3,7 @@
 sm_100a only.  engine.cu is compiled with -fmad=false, which keeps
 multiply/add pairs unfused so that the explicit __fmaf_rn calls are the only
 fused operations (its kernels restate the reference's CPU rounding step by
-step); the operators of kvops.cu and packops.cu have no such order to keep.
+step); the operators of the other sources have no such order to keep.
 
 The torch side of those operators is a second library, _kvops, which links the
 first: the C ABI itself needs nothing from torch.
@@ -24,7 +24,7 @@ LIB = os.path.join(HERE, "libocrvl_cuda.so")
 TORCH_SOURCE = os.path.join(CSRC, "kvops_torch.cpp")
 TORCH_LIB = os.path.join(HERE, "_kvops.so")
 HEADER = os.path.join(ROOT, "include", "ocrvl_cuda.h")
-SOURCES = {"engine.cu": ["-fmad=false"], "kvops.cu": [], "packops.cu": []}  # and the flags of their own
+SOURCES = {"engine.cu": ["-fmad=false"], "kvops.cu": [], "packops.cu": [], "packattn.cu": []}  # and the flags of their own
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [*ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
