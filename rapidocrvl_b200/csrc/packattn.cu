@@ -41,14 +41,18 @@ int launch_pack(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   return launch_combine<T, D>(a, sms, rows_max, S::kRows, stream);
 }
 
+// Rows a block, as for a plain cache: eight or sixteen where there are no more, or where the call's tiles are so few that
+// the GPU is not filled otherwise; else 32 for f32, and the fifth generation's products for 16 bits.
 template <typename T, int D>
 int launch_pack_rows(const TreeArgs &a, int sms, int rows_max, char *work, cudaStream_t stream) {
-  if (rows_max <= 8) return launch_pack<T, D, 1>(a, sms, rows_max, work, stream);
-  if (rows_max <= 16 || sizeof(T) == 2) return launch_pack<T, D, 2>(a, sms, rows_max, work, stream);
+  const int room = sizeof(T) == 4 ? sms : 2 * sms;  // blocks that run at once
+  auto few = [&](int rows) { return (long long)((rows_max + rows - 1) / rows) * a.kv_heads * a.s.batch * tree_tiles(a) * 2 <= 3 * room; };
+  if (rows_max <= 8 || few(8)) return launch_pack<T, D, 1>(a, sms, rows_max, work, stream);
+  if (rows_max <= 16 || few(16)) return launch_pack<T, D, 2>(a, sms, rows_max, work, stream);
   if constexpr (sizeof(T) == 4)
     return launch_pack<T, D, 4>(a, sms, rows_max, work, stream);
   else
-    return OCRVL_OK;
+    return launch_tree_mma_shape<T, D, true>(a, sms, rows_max, work, stream);
 }
 
 template <typename T>

@@ -21,7 +21,12 @@
 // (S, its softmax by one warp an SM quarter, P, O) that the other one covers in part.
 // 8 sequences of up to 8,448, 16 drafts: 29 us, 1.3 TB/s, four tiles a block: most of it is
 // the start, the end and the join.  16 of 4,000, 64 drafts, a block a segment of 128 rows: 53 us.
+//
+// Over a packed cache (PACKED) warps 8 to 11 turn a chunk's codes into numbers of T on their way to shared memory:
+// 16 bytes of a row are 8 consecutive dims of each of four pieces.  A tile's codes are loaded while the one before
+// it is turned.
 #pragma once
+#include "packed.cuh"
 #include "tree_attn.cuh"
 
 namespace ocrvl {
@@ -184,7 +189,65 @@ struct MmaShape {
   static constexpr int kSmem = kTiles + (4 * kStages + 9 + kMeta) * 8 + kMeta * 8 * 4 + 2 * 128 * 8 + 64 + 32;
 };
 
-template <typename T, int D, bool WIDE, bool SPLIT>
+// What a lane of a copying warp takes of a packed chunk: 16 bytes of codes of rows row(i), pieces of 8 dims
+// which each hold, and the rows' scales.
+template <typename T, int D>
+struct PackedChunk {
+  static constexpr int PER = D / 64;  // 16-byte runs a lane
+  uint4 codes[PER];
+  uint32_t scales[PER][D / 64];
+
+  // Rows and runs so that the eight lanes of a store phase write to eight pieces of 16 bytes that lie in different banks.
+  static __device__ __forceinline__ int run(int lane) { return D == 128 ? lane & 3 : lane & 1; }
+  static __device__ __forceinline__ int row(int lane, int i) {
+    return D == 128 ? (lane >> 3) + (lane >> 2 & 1) * 4 + i * 8 : (lane >> 1 & 1) + (lane >> 2 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 4) * 8;
+  }
+  __device__ __forceinline__ void load(const char *from, const char *from_s, int valid, int lane) {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int r = row(lane, i);
+      codes[i] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int w = 0; w < D / 64; w++) scales[i][w] = 0u;
+      if (r < valid) {
+        codes[i] = __ldg((const uint4 *)(from + r * (D / 2)) + run(lane));
+        if constexpr (D == 128) {
+          const uint2 s = __ldg((const uint2 *)(from_s + r * 8));
+          scales[i][0] = s.x, scales[i][D / 64 - 1] = s.y;
+        } else {
+          scales[i][0] = __ldg((const uint32_t *)(from_s + r * 4));
+        }
+      }
+    }
+  }
+  // To the chunk's rows of a tile.
+  __device__ __forceinline__ void store(uint32_t to, int lane) const {
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int r = row(lane, i), x = run(lane);
+      const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        const int j = D == 128 ? q : q >> 1;  // the group
+        const uint32_t c = D == 128 ? halves(w[q >> 1], w[2 + (q >> 1)], q & 1) : halves(w[2 * (q & 1)], w[2 * (q & 1) + 1], q >> 1);
+        uint32_t s = __byte_perm(scales[i][j >> 1], 0, j & 1 ? 0x3232 : 0x1010);
+        if constexpr (std::is_same<T, __half>::value) {
+          const float f = __uint_as_float(s << 16);
+          s = pack2(f, f, T());
+        }
+        const Scaled<T> by(s);
+        uint32_t y[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) y[k] = by(c, k);
+        const int piece = D == 128 ? (j & 1) * 4 + x : j * 4 + x * 2 + (q & 1);
+        sts4u(to + (D == 128 ? j >> 1 : 0) * 16384 + r * 128 + ((piece ^ (r & 7)) * 16), low_halves(y[0], y[1]), low_halves(y[2], y[3]),
+              high_halves(y[0], y[1]), high_halves(y[2], y[3]));
+      }
+    }
+  }
+};
+
+template <typename T, int D, bool WIDE, bool SPLIT, bool PACKED>
 __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, int row_blocks) {
   using S = MmaShape<D, WIDE>;
   constexpr int NS = S::kStages;
@@ -490,34 +553,62 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
     for (int piece = 0; more && ok; piece++) {
       const int n = cur.t1 - cur.t0, rows = rows_of(cur);
       int pages = -1;  // lane i: the page of the warp's i-th chunk from the last look on
-      for (int i = 0; i < n && ok; i++) {
-        const uint32_t tile = T0 + i, stage = tile % NS, use = tile / NS;
+      auto of = [](const char *x, int h) { return (const char *)__shfl_sync(~0u, (unsigned long long)x, h); };
+      // lane h < CH: where the warp's chunk h of a tile lies; the tiles are asked for in order
+      struct Where {
+        const char *k, *v, *ks, *vs;
+        int row_bytes, valid, what;
+      };
+      auto where = [&](int i) {
         if (i % (32 / CH) == 0) {
           const int c = (cur.t0 + i + lane / CH) * kTileChunks + CH * w + lane % CH;
           pages = c < cur.sg.chunks_c ? a.c.table[cur.b * a.c.table_stride + ((c * kChunk) >> a.c.page_shift)] : -1;
         }
-        // lane h < CH: where the warp's chunk h lies
         const int c = (cur.t0 + i) * kTileChunks + CH * w + lane % CH;
         const int pg = __shfl_sync(~0u, pages, i % (32 / CH) * CH + lane % CH);
-        const char *src_k, *src_v;
-        int row_bytes, valid, what = 0;
+        Where x;
+        x.what = 0, x.ks = x.vs = nullptr;
         if (c < cur.sg.chunks_c) {
           const int pos = c * kChunk;
           const bool mapped = pg >= 0 && pg < a.c.num_pages;
-          valid = mapped ? min(kChunk, cur.sg.len - pos) : 0;
-          row_bytes = a.c.token_bytes;
-          const long long at = (mapped ? pg : 0) * a.c.page_bytes + cur.head * a.c.head_bytes +
-                               (long long)(pos & ((1 << a.c.page_shift) - 1)) * a.c.token_bytes;
-          src_k = a.c.k + at, src_v = a.c.v + at;
+          x.valid = mapped ? min(kChunk, cur.sg.len - pos) : 0;
+          x.row_bytes = a.c.token_bytes;
+          const long long in_page = pos & ((1 << a.c.page_shift) - 1);
+          const long long at = (mapped ? pg : 0) * a.c.page_bytes + cur.head * a.c.head_bytes + in_page * a.c.token_bytes;
+          x.k = a.c.k + at, x.v = a.c.v + at;
+          if constexpr (PACKED) {
+            const long long at_s = (mapped ? pg : 0) * a.scale_page + cur.head * a.scale_head + in_page * (D / 16);
+            x.ks = a.k_scale + at_s, x.vs = a.v_scale + at_s;
+          }
         } else {
           const int j = (c - cur.sg.chunks_c) * kChunk;
-          valid = max(0, min(kChunk, cur.sg.count - j));
-          row_bytes = (int)(a.kv_stride * (long long)sizeof(T));
-          const long long at = (cur.sg.first + (valid ? j : 0)) * a.kv_stride + (long long)cur.head * D;
-          src_k = (const char *)((const T *)a.dk + at), src_v = (const char *)((const T *)a.dv + at);
-          what = valid ? 1 << 8 | j << 16 : 0;
+          x.valid = max(0, min(kChunk, cur.sg.count - j));
+          x.row_bytes = (int)(a.kv_stride * (long long)sizeof(T));
+          const long long at = (cur.sg.first + (x.valid ? j : 0)) * a.kv_stride + (long long)cur.head * D;
+          x.k = (const char *)((const T *)a.dk + at), x.v = (const char *)((const T *)a.dv + at);
+          x.what = x.valid ? 1 << 8 | j << 16 : 0;
         }
-        auto of = [](const char *x, int h) { return (const char *)__shfl_sync(~0u, (unsigned long long)x, h); };
+        return x;
+      };
+      // PACKED: the warp's codes of a tile, the next one's fetched as soon as this one's are turned into numbers
+      PackedChunk<T, D> codes_k[PACKED ? CH : 1], codes_v[PACKED ? CH : 1];
+      auto fetch = [&](PackedChunk<T, D> *to, const Where &x, bool v) {
+#pragma unroll
+        for (int h = 0; h < CH; h++)
+          to[h].load(of(v ? x.v : x.k, h), of(v ? x.vs : x.ks, h), __shfl_sync(~0u, x.what ? 0 : x.valid, h), lane);
+      };
+      Where at = where(0), at_next = at;
+      if constexpr (PACKED) fetch(codes_k, at, false), fetch(codes_v, at, true);
+      for (int i = 0; i < n && ok; i++) {
+        const uint32_t tile = T0 + i, stage = tile % NS, use = tile / NS;
+        if constexpr (PACKED) {
+          at = at_next;
+          if (i + 1 < n) at_next = where(i + 1);
+        } else {
+          if (i) at = where(i);
+        }
+        const char *src_k = at.k, *src_v = at.v;
+        const int row_bytes = at.row_bytes, valid = at.valid, what = at.what;
         unsigned draft = __ballot_sync(~0u, what != 0 && lane < CH), odd = 0;  // chunks of drafts; those with values that are not finite
         for (; draft; draft &= draft - 1) {
           const int h = __ffs(draft) - 1, n_h = __shfl_sync(~0u, valid, h), row = __shfl_sync(~0u, row_bytes, h);
@@ -531,10 +622,17 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
         }
         if (lane < CH) meta[tile % S::kMeta * 8 + CH * w + lane] = valid | what | (odd >> lane & 1 ? 1 << 9 : 0);
         __syncwarp();
-        auto copy = [&](char *to, const char *src) {
+        auto copy = [&](char *to, const char *src, const PackedChunk<T, D> *packed) {
           const uint32_t base = smem_addr(to) + CH * w * kChunk * 128;
+          if constexpr (PACKED) {
+#pragma unroll
+            for (int h = 0; h < CH; h++)
+              if (!__shfl_sync(~0u, what, h)) packed[h].store(base + h * kChunk * 128, lane);
+            if (!__any_sync(~0u, what)) return;
+          }
 #pragma unroll 1
           for (int h = 0; h < CH; h++) {
+            if (PACKED && !__shfl_sync(~0u, what, h)) continue;
             const int n_h = __shfl_sync(~0u, valid, h);
             const long long row_h = __shfl_sync(~0u, row_bytes, h);
             const char *from = of(src, h) + piece16 * 16 + r0 * row_h;
@@ -553,8 +651,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
         ok = __all_sync(~0u, use == 0 || bar_wait(&k_empty[stage], (use - 1) & 1, dead));
         if (!ok) break;
         if (lane == 0) bar_arrive(&meta_full[tile % S::kMeta]);
-        copy(k_sm + stage * S::kBlock, src_k);
-        landed(&k_full[stage]);
+        copy(k_sm + stage * S::kBlock, src_k, codes_k);
+        if constexpr (PACKED) {
+          copy_commit();
+          copy_wait<0>();
+          bar_arrive(&k_full[stage]);
+          if (i + 1 < n) fetch(codes_k, at_next, false);
+        } else {
+          landed(&k_full[stage]);
+        }
         if (i == 0) {  // the query rows, once the piece before has no more use for its own
           ok = __all_sync(~0u, piece == 0 || bar_wait(q_empty, (piece - 1) & 1, dead));
           if (!ok) break;
@@ -576,8 +681,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
         }
         ok = __all_sync(~0u, use == 0 || bar_wait(&v_empty[stage], (use - 1) & 1, dead));
         if (!ok) break;
-        copy(v_sm + stage * S::kBlock, src_v);
-        if (!odd) {
+        copy(v_sm + stage * S::kBlock, src_v, codes_v);
+        if (!PACKED && !odd) {
           landed(&v_full[stage]);
         } else {  // what is not finite becomes 0 here (0 * NaN would reach rows that do not see it) and is added at the end
           copy_commit();
@@ -597,6 +702,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
               sts4u(at, x[0], x[1], x[2], x[3]);
             }
           bar_arrive(&v_full[stage]);
+          if (PACKED && i + 1 < n) fetch(codes_v, at_next, true);
         }
       }
       if (!ok) break;
