@@ -34,6 +34,30 @@ __device__ __forceinline__ void split3(float x, uint32_t (&p)[3]) {
   p[2] = finite ? __float_as_uint(r - __uint_as_float(mid)) : __float_as_uint(x) | ((__float_as_uint(x) & 0x7fffffu) ? 0x400000u : 0u);
 }
 
+// Four values as they lie in memory.
+template <typename T>
+struct Four {
+  uint32_t w[sizeof(T)];
+
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (sizeof(T) == 4) {
+      const uint4 x = *(const uint4 *)p;
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+      const uint2 x = *(const uint2 *)p;
+      w[0] = x.x, w[1] = x.y;
+    }
+  }
+  __device__ __forceinline__ float4 floats() const {
+    if constexpr (sizeof(T) == 4) {
+      return make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]), __uint_as_float(w[3]));
+    } else {
+      const float2 a = unpack2<T>(w[0]), b = unpack2<T>(w[1]);
+      return make_float4(a.x, a.y, b.x, b.y);
+    }
+  }
+};
+
 template <typename T, int D>
 struct PackTile {
   using B = Product<T>;
@@ -69,7 +93,7 @@ struct PackTile {
   // The position of row g of the matrix instruction; row g + 8 has that plus 2.
   static __device__ __forceinline__ int position(int g) { return 4 * (g >> 1) + (g & 1); }
 
-  // ---- fragments of 8 consecutive dims (a query row's, or a drafted key's): pairs (i, 4 + i)
+  // ---- fragments of a query row's 8 consecutive dims: pairs (i, 4 + i)
   static __device__ __forceinline__ void pairs8(uint32_t (&f)[kParts][4], const T *p) {
     if (!p) {
 #pragma unroll
@@ -91,6 +115,21 @@ struct PackTile {
       f[0][0] = low_halves(a.x, a.z), f[0][1] = high_halves(a.x, a.z);
       f[0][2] = low_halves(a.y, a.w), f[0][3] = high_halves(a.y, a.w);
     }
+  }
+  // Dims 32 j + 4 g .. + 3 of row r of 8, from the fragments.
+  static __device__ __forceinline__ float4 four(uint32_t q, int r, int j, int g) {
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kParts; w++) {
+      uint32_t f[4];
+      lds4u(f, q + (w * G + j) * 512 + (r * 4 + (g >> 1)) * 16);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float2 y = unpack2<B>(f[i]);
+        x[i] += g & 1 ? y.y : y.x;
+      }
+    }
+    return make_float4(x[0], x[1], x[2], x[3]);
   }
   static __device__ __forceinline__ float sum8(const T *p) {
     if (!p) return 0.f;
@@ -171,43 +210,6 @@ struct PackTile {
     }
   }
 
-  // ---- drafted keys: rows of T, `valid` of the 16 there
-  template <int NT>
-  static __device__ __forceinline__ void draft_scores(float (&s)[NT][4], uint32_t q, const T *rows, long long stride, int valid, int lane) {
-    const int g = lane >> 2, t = lane & 3, p0 = position(g);
-#pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[n][e] = 0.f;
-#pragma unroll
-    for (int j = 0; j < G; j++) {
-      uint32_t f0[kParts][4], f1[kParts][4];
-      pairs8(f0, p0 < valid ? rows + p0 * stride + 32 * j + 8 * t : nullptr);
-      pairs8(f1, p0 + 2 < valid ? rows + (p0 + 2) * stride + 32 * j + 8 * t : nullptr);
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        // A group is summed apart and added in a rounded addition; f32: the products of parts whose places add up to two
-        // at most, the small ones first.
-        float p[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int both = kParts - 1; both >= 0; both--)
-#pragma unroll
-          for (int w = 0; w <= both; w++) {
-            uint32_t b[4];
-            lds4u(b, q + n * kQBytes + (w * G + j) * 512 + lane * 16);
-            const int x = both - w;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const uint32_t a[4] = {f0[x][2 * h], f1[x][2 * h], f0[x][2 * h + 1], f1[x][2 * h + 1]};
-              mma_16<B>(p, a, b[2 * h], b[2 * h + 1]);
-            }
-          }
-#pragma unroll
-        for (int e = 0; e < 4; e++) s[n][e] += p[e];
-      }
-    }
-  }
-
   // The weights of a chunk (as scores leaves them) as the products' second operand.
   template <int NT>
   static __device__ __forceinline__ void weights(uint32_t (&b)[kParts][NT][2], const float (&p)[NT][4]) {
@@ -267,81 +269,27 @@ struct PackTile {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const uint32_t a[4] = {by01(x01, 2 * h), by01(x01, 2 * h + 1), by23(x23, 2 * h), by23(x23, 2 * h + 1)};
-        product<NT, 1>(o[2 * j + h], &a, b);
+        product<NT>(o[2 * j + h], a, b);
       }
     }
   }
 
-  // o of a tile += a of PARTS parts times the weights.  f32: summed apart and added in one rounded addition, since
+  // o of a tile += a times the weights.  f32: summed apart and added in one rounded addition, since
   // the matrix instruction's own sums are cut, not rounded, which over thousands of chunks would add up.
-  template <int NT, int PARTS>
-  static __device__ __forceinline__ void product(float (&o)[NT][4], const uint32_t (*a)[4], const uint32_t (&b)[kParts][NT][2]) {
+  template <int NT>
+  static __device__ __forceinline__ void product(float (&o)[NT][4], const uint32_t (&a)[4], const uint32_t (&b)[kParts][NT][2]) {
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       if constexpr (f32) {
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int both = 2; both >= 0; both--)
-#pragma unroll
-          for (int w = 0; w <= both; w++)
-            if (both - w < PARTS) mma_16<B>(sum, a[both - w], b[w][n][0], b[w][n][1]);
+        for (int w = 2; w >= 0; w--) mma_16<B>(sum, a, b[w][n][0], b[w][n][1]);
 #pragma unroll
         for (int e = 0; e < 4; e++) o[n][e] += sum[e];
       } else {
-        mma_16<B>(o[n], a[0], b[0][n][0], b[0][n][1]);
+        mma_16<B>(o[n], a, b[0][n][0], b[0][n][1]);
       }
     }
-  }
-
-  // The same for drafted values; true if some are not finite: those count as 0 here.
-  template <int NT>
-  static __device__ __forceinline__ bool draft_values(float (&o)[kTiles][NT][4], const uint32_t (&b)[kParts][NT][2], const T *rows,
-                                                      long long stride, int valid, int lane) {
-    const int g = lane >> 2, t = lane & 3;
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < G; j++) {
-      uint32_t f[kParts][4][2];  // [part][dim of 4 g ..][positions 4 t, 4 t + 1; 4 t + 2, 4 t + 3]
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        const int p = 4 * t + 2 * r;
-        const T *at = rows + p * stride + 32 * j + 4 * g;
-        if constexpr (f32) {
-          const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-          const float4 x4 = p < valid ? __ldg((const float4 *)at) : zero, y4 = p + 1 < valid ? __ldg((const float4 *)(at + stride)) : zero;
-          float x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
-#pragma unroll
-          for (int d = 0; d < 4; d++) {
-            if (!isfinite(x[d])) x[d] = 0.f, bad = true;
-            if (!isfinite(y[d])) y[d] = 0.f, bad = true;
-            uint32_t u[3], w[3];
-            split3(x[d], u), split3(y[d], w);
-#pragma unroll
-            for (int i = 0; i < 3; i++) f[i][d][r] = high_halves(u[i], w[i]);
-          }
-        } else {
-          const uint2 zero = make_uint2(0u, 0u);
-          const uint2 x = p < valid ? __ldg((const uint2 *)at) : zero, y = p + 1 < valid ? __ldg((const uint2 *)(at + stride)) : zero;
-          f[0][0][r] = low_halves(x.x, y.x), f[0][1][r] = high_halves(x.x, y.x);
-          f[0][2][r] = low_halves(x.y, y.y), f[0][3][r] = high_halves(x.y, y.y);
-          constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-#pragma unroll
-          for (int d = 0; d < 4; d++) {
-            if ((f[0][d][r] & e) == e) f[0][d][r] &= 0xffff0000u, bad = true;
-            if ((f[0][d][r] >> 16 & e) == e) f[0][d][r] &= 0xffffu, bad = true;
-          }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        uint32_t a[kParts][4];
-#pragma unroll
-        for (int w = 0; w < kParts; w++)
-          a[w][0] = f[w][2 * h][0], a[w][1] = f[w][2 * h + 1][0], a[w][2] = f[w][2 * h][1], a[w][3] = f[w][2 * h + 1][1];
-        product<NT, kParts>(o[2 * j + h], a, b);
-      }
-    }
-    return __any_sync(~0u, bad);
   }
 };
 
@@ -450,9 +398,25 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
       seen[r] = r < rows ? (unsigned long long)a.mask[x.sg.first + (x.rb * ROWS + r) / a.group] : 0ull;
   };
 
+  // The drafts of a piece that this warp takes, and the first one's key and value.
+  int draft0, draft1;
+  const int draft_step = CS > 1 ? kTreeWarps * CS : kTreeWarps;
+  Four<T> key[G], value[G];
+  auto load_draft = [&](const WarpPiece &x, int j) {
+    const long long at = (x.sg.first + j) * a.kv_stride + (long long)x.head * D + 4 * g;
+#pragma unroll
+    for (int i = 0; i < G; i++) key[i].load((const T *)a.dk + at + 32 * i), value[i].load((const T *)a.dv + at + 32 * i);
+  };
+  auto drafts_of = [&](const WarpPiece &x) {
+    const int c0 = CS > 0 ? 0 : x.t0 * kTileChunks - x.sg.chunks_c, c1 = x.t1 * kTileChunks - x.sg.chunks_c;
+    draft0 = max(0, c0) * kChunk + warp + (CS > 1 ? blockIdx.x % CS * kTreeWarps : 0), draft1 = min(x.sg.count, c1 * kChunk);
+    if (draft0 < draft1) load_draft(x, draft0);
+  };
+
   int nc = cached_of(cur);
 #pragma unroll
   for (int k = 0; k < NS - 1; k++) issue(cur, nc, k);
+  drafts_of(cur);
   load_query(cur);
   __syncthreads();
 
@@ -503,43 +467,42 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
         }
     };
 
-    // drafts first, while the first cached chunks are on their way
-    for (int k = nc; k < cur.nk; k++) {
-      const int j0 = (cur.c0 + k * cur.step - cur.sg.chunks_c) * kChunk, valid = min(kChunk, cur.sg.count - j0);
-      const long long from = (cur.sg.first + j0) * a.kv_stride + (long long)cur.head * D;
-      float s[NT][4];
-      L::template draft_scores<NT>(s, q_at, (const T *)a.dk + from, a.kv_stride, valid, lane);
+    // Drafts first, while the first cached chunks are on their way: position by position, shared out over all warps, in 32
+    // bits without the matrix instruction.  A lane has dims 32 j + 4 g .. + 3 of the key, the value and o.
+    for (int j = draft0; j < draft1; j += draft_step) {
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int j = L::position(g) + (e >> 1) * 2;
-          const bool see = j < valid && seen[n * 8 + 2 * t + (e & 1)] >> (j0 + j) & 1;
-          s[n][e] = see ? s[n][e] * a.scale : -INFINITY;
+        for (int h = 0; h < 2; h++) {
+          const int row = n * 8 + 2 * t + h;
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < G; i++) {
+            const float4 q4 = L::four(q_at + n * L::kQBytes, 2 * t + h, i, g);
+            const float4 k4 = key[i].floats();
+            x = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, x))));
+          }
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(~0u, x, d);
+          if (!(seen[row] >> j & 1)) continue;  // what a draft holds that is not seen stays out
+          x *= a.scale;
+          if (x > ref[n][h] + kSlack<T>) {
+            const float now = x - kLift<T>, alpha = exp2_(ref[n][h] - now);
+            ref[n][h] = now;
+            sum[n][h] *= alpha, low[n][h] *= alpha;
+#pragma unroll
+            for (int i = 0; i < L::kTiles; i++) o[i][n][h] *= alpha, o[i][n][2 + h] *= alpha;
+          }
+          const float w = exp2_(x - (ref[n][h] == -INFINITY ? 0.f : ref[n][h]));
+          if (g == 0) add_exactly(sum[n][h], low[n][h], w);
+#pragma unroll
+          for (int i = 0; i < G; i++) {
+            const float4 v4 = value[i].floats();
+            o[2 * i][n][h] = fmaf(w, v4.x, o[2 * i][n][h]), o[2 * i][n][2 + h] = fmaf(w, v4.y, o[2 * i][n][2 + h]);
+            o[2 * i + 1][n][h] = fmaf(w, v4.z, o[2 * i + 1][n][h]), o[2 * i + 1][n][2 + h] = fmaf(w, v4.w, o[2 * i + 1][n][2 + h]);
+          }
         }
-      soften(s);
-      uint32_t b[L::kParts][NT][2];
-      L::template weights<NT>(b, s);
-      if (L::template draft_values<NT>(o, b, (const T *)a.dv + from, a.kv_stride, valid, lane)) {
-        // values that are not finite: 0 * NaN would have reached rows that do not see them, the others get them here
-        for (int j = 0; j < valid; j++) {
-          const T *row = (const T *)a.dv + from + j * a.kv_stride;
-#pragma unroll
-          for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const float w = __shfl_sync(~0u, j & 2 ? s[n][2 + h] : s[n][h], (2 * (j >> 2) + (j & 1)) * 4 + t);
-              const bool see = seen[n * 8 + 2 * t + h] >> (j0 + j) & 1;
-#pragma unroll
-              for (int i = 0; i < L::kTiles; i++)
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                  const float x = to_f(row[(i >> 1) * 32 + 4 * g + (i & 1) * 2 + e]);
-                  if (!isfinite(x) && see) o[i][n][2 * e + h] += w * x;
-                }
-            }
-        }
-      }
+      if (j + draft_step < draft1) load_draft(cur, j + draft_step);
     }
 
     for (int k = 0; k < nc; k++) {
@@ -578,6 +541,7 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
         __syncwarp();  // all lanes are done with the last stage
 #pragma unroll
         for (int k = 0; k < NS - 1; k++) issue(cur, nc, k);
+        drafts_of(cur);
       }
     } else {
       more = false;

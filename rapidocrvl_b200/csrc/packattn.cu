@@ -18,18 +18,20 @@ int launch_pack(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   const int blocks = (rows_max + S::kRows - 1) / S::kRows;
   const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
   if (segments > 1 << 24) return invalid("too many sequences and kv heads");
-  // A cluster (or, for the shortest, a block) a segment where a block then has at most kFew
-  // tiles of the longest cache and all clusters run at once: saves the second launch.
-  constexpr int kFew = 4;
+  // Blocks (in clusters) a segment, as many as run at once; or equal runs of tiles over all blocks and a second launch
+  // that joins them, where a warp then has so many fewer chunks (of the longest cache, which is all that the host knows) that
+  // it makes up for the search, the parts and the join.
+  constexpr int kRunsCost = 16;  // chunks
   const int tiles = tree_tiles(a);
+  const long long room = (long long)sms * S::kBlocks;
   auto one = [&](auto kernel, int cs) {
     return launch("packed attention", kernel, dim3((unsigned)(segments * cs)), kTreeThreads, S::kSmem, stream, false, cs, a, blocks);
   };
-  const int clustered = cluster_room(sms) * S::kBlocks;
-  if (tiles > 2 && tiles <= 4 * kFew && segments * 4 <= clustered)
-    return tiles > 4 && segments * 8 <= clustered ? one(k_pack_attn<T, D, NT, 8>, 8) : one(k_pack_attn<T, D, NT, 4>, 4);
-  if (tiles > kFew && tiles <= 8 * kFew && segments * 8 <= clustered) return one(k_pack_attn<T, D, NT, 8>, 8);
-  if (tiles <= kFew) return one(k_pack_attn<T, D, NT, 1>, 1);
+  int cs = 1;
+  while (cs < 8 && cs < tiles && segments * cs * 2 <= (cs == 1 ? room : (long long)cluster_room(sms) * S::kBlocks)) cs *= 2;
+  const double whole = (double)((tiles + cs - 1) / cs) * ((segments * cs + room - 1) / room), runs = (double)segments * tiles / room;
+  if (whole <= runs + kRunsCost)
+    return cs == 8 ? one(k_pack_attn<T, D, NT, 8>, 8) : cs == 4 ? one(k_pack_attn<T, D, NT, 4>, 4) : cs == 2 ? one(k_pack_attn<T, D, NT, 2>, 2) : one(k_pack_attn<T, D, NT, 1>, 1);
 
   if (int rc = check_combine(a, blocks)) return rc;
   const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
