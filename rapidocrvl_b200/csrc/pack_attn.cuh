@@ -3,13 +3,11 @@
 //
 // The mathematics, segments and runs are tree_attn.cuh's; only the cache is read in another way.
 // The 16 positions of a chunk are the rows of the matrix instruction, 8 query rows its
-// columns.  Codes become 16-bit numbers in registers: a nibble at the top of the mantissa of 16
-// is 16 + (c + 8), so
-//   K   q . (16 + c + 8) - 24 sum q, the sum as the accumulator's first value, a group of 32 dims at a time, then
-//       times the group's scale in 32 bits (f32: the 24 taken off the codes, so that nothing cancels)
-//   V   (24 + c) s - 24 s in one fused step, exact: c s and 24 s are bf16 numbers
-// f32 queries and weights are three bf16 parts (all 24 bits), so their products with codes are
-// exact and only sums are rounded.  A lane finds all that it needs of a row in one piece: of K, dims
+// columns.  Codes become 16-bit numbers in registers:
+//   K   whole numbers in f16, against f16 queries: a row's power of two brings its largest value below 2^14, f32 rows are two
+//       f16 parts (22 bits); a group of 32 dims is summed, then times its scale in 32 bits
+//   V   c s in T (f32: in bf16, which holds it exactly, against weights of three bf16 parts)
+// so products are exact and only sums are rounded.  A lane finds all that it needs of a row in one piece: of K, dims
 // 32 j + 8 t .. + 7 of each group j, of V, dims 32 j + 4 g .. + 3 (g = lane / 4, t = lane % 4).  The chunk's
 // positions are the instruction's rows in the order 0 1 4 5 8 9 12 13, 2 3 6 7 10 11 14 15, so that a
 // lane's four positions of V, and their scales, are neighbours.
@@ -21,7 +19,15 @@ namespace ocrvl {
 namespace paged {
 
 template <typename T>
-using Product = std::conditional_t<std::is_same<T, __half>::value, __half, __nv_bfloat16>;  // the products' type
+using Product = std::conditional_t<std::is_same<T, __half>::value, __half, __nv_bfloat16>;  // the type of V's products
+
+// The four pairs of nibbles of two halfwords as whole numbers c in f16: (1024 + u) - 1032 and (1024 + 16 u) / 16 - 72, all
+// exact.  One shift for four pairs: with one for each (lifted) a chunk's integer instructions took a third longer.
+__device__ __forceinline__ void whole4(uint32_t (&c)[4], uint32_t x) {
+  const uint32_t y = x >> 8, minus = 0xe408e408u, low = 0x2c002c00u, minus72 = 0xd480d480u;
+  c[0] = add2((x & 0x000f000fu) | 0x64006400u, minus), c[1] = fma2<__half>((x & 0x00f000f0u) | 0x64006400u, low, minus72);
+  c[2] = add2((y & 0x000f000fu) | 0x64006400u, minus), c[3] = fma2<__half>((y & 0x00f000f0u) | 0x64006400u, low, minus72);
+}
 
 // x as three bf16 numbers, in the upper halves: exact (8 bits each, cut, so that none is rounded up to
 // infinity); what is not finite is the last one's alone, so that it meets nothing but another's first part.
@@ -63,11 +69,12 @@ struct PackTile {
   using B = Product<T>;
   static constexpr bool f32 = sizeof(T) == 4;
   static constexpr int G = D / 32;                     // groups of a row
-  static constexpr int kParts = f32 ? 3 : 1;
+  static constexpr int kParts = f32 ? 3 : 1;           // of a weight
+  static constexpr int kQParts = f32 ? 2 : 1;          // of a query
   static constexpr int kCodes = kChunk * D / 2;        // bytes of a chunk's K or V
   static constexpr int kScales = kChunk * G * 2;
   static constexpr int kStage = 2 * (kCodes + kScales);  // K, V, their scales
-  static constexpr int kQBytes = kParts * G * 512;     // fragments of 8 query rows: [part][group][lane] of 16 bytes
+  static constexpr int kQBytes = kQParts * G * 512;     // fragments of 8 query rows: [part][group][lane] of 16 bytes
   static constexpr int kTiles = D / 16;
 
   // Where 16-byte piece x of a position's row lies: exchanged so that the fragment loads of a warp (K: rows 0 1 4 5
@@ -78,75 +85,51 @@ struct PackTile {
   static __device__ __forceinline__ int v_at(int row, int x) {
     return D == 128 ? (row ^ (row >> 2 & 1)) * 64 + (x ^ (row >> 3 & 1) << 1) * 16 : (row ^ (row >> 2 & 3)) * 32 + x * 16;
   }
-  // A warp's copies of a chunk.
-  static __device__ __forceinline__ void load(uint32_t to, const char *k, const char *v, const char *ks, const char *vs, int lane) {
+  // A warp's copies of a chunk: k, v, s are the lane's own.
+  static __device__ __forceinline__ void load(uint32_t to, const char *k, const char *v, const char *s, int lane) {
 #pragma unroll
     for (int i = 0; i < kCodes / 512; i++) {
       const int p = i * 32 + lane, row = p / (D / 32), x = p % (D / 32);
-      copy16(to + k_at(row, x), k + p * 16);
-      copy16(to + kCodes + v_at(row, x), v + p * 16);
+      copy16(to + k_at(row, x), k + i * 512);
+      copy16(to + kCodes + v_at(row, x), v + i * 512);
     }
-    constexpr int kPieces = kScales / 16;
-    if (lane < 2 * kPieces) copy16(to + 2 * kCodes + lane * 16, lane < kPieces ? ks + lane * 16 : vs + (lane - kPieces) * 16);
+    if (lane < 2 * (kScales / 16)) copy16(to + 2 * kCodes + lane * 16, s);
   }
 
   // The position of row g of the matrix instruction; row g + 8 has that plus 2.
   static __device__ __forceinline__ int position(int g) { return 4 * (g >> 1) + (g & 1); }
 
-  // ---- fragments of a query row's 8 consecutive dims: pairs (i, 4 + i)
-  static __device__ __forceinline__ void pairs8(uint32_t (&f)[kParts][4], const T *p) {
-    if (!p) {
+  // ---- fragments of a query row's 8 consecutive dims: pairs (i, 4 + i) of f16 parts of up times the row
+  static __device__ __forceinline__ void pairs8(uint32_t (&f)[kQParts][4], const float (&x)[8], float up) {
 #pragma unroll
-      for (int w = 0; w < kParts; w++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) f[w][i] = 0u;
-    } else if constexpr (f32) {
-      const float4 a = __ldg((const float4 *)p), b = __ldg((const float4 *)p + 1);
-      const float x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        uint32_t u[3], v[3];
-        split3(x[i], u), split3(y[i], v);
-#pragma unroll
-        for (int w = 0; w < 3; w++) f[w][i] = high_halves(u[w], v[w]);
+    for (int i = 0; i < 4; i++) {
+      const float a = x[i] * up, b = x[4 + i] * up;
+      f[0][i] = pack2(a, b, __half());
+      if constexpr (f32) {
+        const float2 hi = unpack2<__half>(f[0][i]);
+        f[kQParts - 1][i] = pack2(a - hi.x, b - hi.y, __half());
       }
-    } else {
-      const uint4 a = __ldg((const uint4 *)p);
-      f[0][0] = low_halves(a.x, a.z), f[0][1] = high_halves(a.x, a.z);
-      f[0][2] = low_halves(a.y, a.w), f[0][3] = high_halves(a.y, a.w);
     }
   }
-  // Dims 32 j + 4 g .. + 3 of row r of 8, from the fragments.
+  // Dims 32 j + 4 g .. + 3 of row r of 8, from the fragments: up times them.
   static __device__ __forceinline__ float4 four(uint32_t q, int r, int j, int g) {
     float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kParts; w++) {
+    for (int w = 0; w < kQParts; w++) {
       uint32_t f[4];
       lds4u(f, q + (w * G + j) * 512 + (r * 4 + (g >> 1)) * 16);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const float2 y = unpack2<B>(f[i]);
+        const float2 y = unpack2<__half>(f[i]);
         x[i] += g & 1 ? y.y : y.x;
       }
     }
     return make_float4(x[0], x[1], x[2], x[3]);
   }
-  static __device__ __forceinline__ float sum8(const T *p) {
-    if (!p) return 0.f;
-    float x[8], s = 0.f;
-    Eight<T> e;
-    e.load(p);
-    e.floats(x);
-#pragma unroll
-    for (int i = 0; i < 8; i++) s += x[i];
-    return s;
-  }
 
-  // ---- cached keys: s of NT x 8 rows.  q: the fragments' address; qr: they themselves (NT = 1, 16 bits); first: the
-  // accumulators' first values of a lane's two rows, in memory [row][group], or the registers fr.
+  // ---- cached keys: s of NT x 8 rows (times their up).  q: the fragments' address; qr: they themselves (NT = 1, 16 bits).
   template <int NT, bool REGS>
-  static __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&qr)[REGS ? G : 1][4], const float (&fr)[REGS ? G : 1][2],
-                                                uint32_t q, const float *first, uint32_t st, int lane) {
+  static __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&qr)[REGS ? G : 1][4], uint32_t q, uint32_t st, int lane) {
     const int g = lane >> 2, t = lane & 3, p0 = position(g);
     uint32_t k[2][4], ks[2][2];
 #pragma unroll
@@ -162,50 +145,29 @@ struct PackTile {
       }
     }
 #pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) s[n][e] = 0.f;
-#pragma unroll
     for (int j = 0; j < G; j++) {
-      const uint32_t x0 = halves(k[0][j >> 1], k[0][2 + (j >> 1)], j & 1), x1 = halves(k[1][j >> 1], k[1][2 + (j >> 1)], j & 1);
-      uint32_t a[2][4];
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        a[h][0] = lifted<B>(x0, 2 * h), a[h][1] = lifted<B>(x1, 2 * h);
-        a[h][2] = lifted<B>(x0, 2 * h + 1), a[h][3] = lifted<B>(x1, 2 * h + 1);
-        if constexpr (f32) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) a[h][i] = sub2<B>(a[h][i], 0x41c041c0u);  // 24: the codes themselves
-        }
-      }
+      uint32_t c0[4], c1[4];
+      whole4(c0, halves(k[0][j >> 1], k[0][2 + (j >> 1)], j & 1)), whole4(c1, halves(k[1][j >> 1], k[1][2 + (j >> 1)], j & 1));
+      const uint32_t a0[4] = {c0[0], c1[0], c0[1], c1[1]}, a1[4] = {c0[2], c1[2], c0[3], c1[3]};
       const float s0 = __uint_as_float(j & 1 ? ks[0][j >> 1] & 0xffff0000u : ks[0][j >> 1] << 16);
       const float s1 = __uint_as_float(j & 1 ? ks[1][j >> 1] & 0xffff0000u : ks[1][j >> 1] << 16);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         float p[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (f32) {
 #pragma unroll
-          for (int w = 2; w >= 0; w--) {
-            uint32_t b[4];
-            lds4u(b, q + n * kQBytes + (w * G + j) * 512 + lane * 16);
-            mma_16<B>(p, a[0], b[0], b[1]);
-            mma_16<B>(p, a[1], b[2], b[3]);
-          }
-        } else {
+        for (int w = kQParts - 1; w >= 0; w--) {  // the small part first
           uint32_t b[4];
           if constexpr (REGS) {
 #pragma unroll
             for (int i = 0; i < 4; i++) b[i] = qr[j][i];
-            p[0] = p[2] = fr[j][0], p[1] = p[3] = fr[j][1];
           } else {
-            lds4u(b, q + n * kQBytes + j * 512 + lane * 16);
-            p[0] = p[2] = first[(n * 8 + 2 * t) * G + j], p[1] = p[3] = first[(n * 8 + 2 * t + 1) * G + j];
+            lds4u(b, q + n * kQBytes + (w * G + j) * 512 + lane * 16);
           }
-          mma_16<B>(p, a[0], b[0], b[1]);
-          mma_16<B>(p, a[1], b[2], b[3]);
+          mma_16<__half>(p, a0, b[0], b[1]);
+          mma_16<__half>(p, a1, b[2], b[3]);
         }
-        s[n][0] = fmaf(s0, p[0], s[n][0]), s[n][1] = fmaf(s0, p[1], s[n][1]);
-        s[n][2] = fmaf(s1, p[2], s[n][2]), s[n][3] = fmaf(s1, p[3], s[n][3]);
+        s[n][0] = j ? fmaf(s0, p[0], s[n][0]) : s0 * p[0], s[n][1] = j ? fmaf(s0, p[1], s[n][1]) : s0 * p[1];
+        s[n][2] = j ? fmaf(s1, p[2], s[n][2]) : s1 * p[2], s[n][3] = j ? fmaf(s1, p[3], s[n][3]) : s1 * p[3];
       }
     }
   }
@@ -264,11 +226,20 @@ struct PackTile {
         s01 = pack2(__uint_as_float(s01 << 16), __uint_as_float(s01 & 0xffff0000u), B());
         s23 = pack2(__uint_as_float(s23 << 16), __uint_as_float(s23 & 0xffff0000u), B());
       }
-      const Scaled<B> by01(s01), by23(s23);
       const uint32_t x01 = halves(v[0][j >> 1], v[1][j >> 1], j & 1), x23 = halves(v[2][j >> 1], v[3][j >> 1], j & 1);
+      uint32_t y01[4], y23[4];
+      if constexpr (std::is_same<B, __half>::value) {
+        whole4(y01, x01), whole4(y23, x23);
+#pragma unroll
+        for (int i = 0; i < 4; i++) y01[i] = mul2<B>(y01[i], s01), y23[i] = mul2<B>(y23[i], s23);
+      } else {
+        const Scaled<B> by01(s01), by23(s23);
+#pragma unroll
+        for (int i = 0; i < 4; i++) y01[i] = by01(x01, i), y23[i] = by23(x23, i);
+      }
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const uint32_t a[4] = {by01(x01, 2 * h), by01(x01, 2 * h + 1), by23(x23, 2 * h), by23(x23, 2 * h + 1)};
+        const uint32_t a[4] = {y01[2 * h], y01[2 * h + 1], y23[2 * h], y23[2 * h + 1]};
         product<NT>(o[2 * j + h], a, b);
       }
     }
@@ -303,8 +274,8 @@ struct PackShape {
   static constexpr int kJoin = kTreeWarps * 8 * D * 4;  // eight rows of every warp
   static constexpr int kQ = NT * L::kQBytes;
   static constexpr bool kQInRegs = NT == 1 && sizeof(T) == 2;
-  static constexpr int kFirst = kRows * L::G * 4;
-  static constexpr int kSmem = kRing + kJoin + kQ + kFirst + kTreeWarps * kRows * 8 + kRows * 8 + 64 + kTreeWarps * 8 * 4 + kRows * 8;
+  static constexpr int kFactors = kRows * 4;
+  static constexpr int kSmem = kRing + kJoin + kQ + kFactors + kTreeWarps * kRows * 8 + kRows * 8 + 64 + kTreeWarps * 8 * 4 + kRows * 8;
 };
 
 template <typename T, int D, int NT, int CS>
@@ -317,8 +288,8 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   char *ring = sm, *q_sm = sm + S::kRing + S::kJoin;
   float *join = (float *)(sm + S::kRing);
   char *p = q_sm + S::kQ;
-  float *first_sm = (float *)p;  // [row][group]: -24 times the sum of the group's q
-  p += S::kFirst;
+  float *down_sm = (float *)p;  // [row]: 1 / up
+  p += S::kFactors;
   float *ml = (float *)p;  // [warp][row][m, l]
   p += kTreeWarps * ROWS * 8;
   unsigned long long *seen = (unsigned long long *)p;  // [row]
@@ -355,6 +326,14 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   const uint32_t my_ring = smem_addr(ring) + warp * (NS * L::kStage), q_at = smem_addr(q_sm);
   int *my_there = there + warp * 8;
   int pages = -1;  // lane i: the page of the chunk 32 j + i
+  const int page_mask = (1 << a.c.page_shift) - 1;
+  const char *from_k, *from_v, *from_s;  // of the piece's head: what the lane copies of a page
+  auto head_of = [&](const WarpPiece &x) {
+    const long long at = x.head * a.c.head_bytes + lane * 16, at_s = x.head * a.scale_head;
+    from_k = a.c.k + at, from_v = a.c.v + at;
+    from_s = (lane < L::kScales / 16 ? a.k_scale + lane * 16 : a.v_scale + (lane - L::kScales / 16) * 16) + at_s;
+  };
+  head_of(cur);
   auto issue = [&](const WarpPiece &x, int nc, int k) {
     if (k < nc) {
       const int c = x.c0 + k * x.step, slot = k % NS;
@@ -363,12 +342,11 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
         const int pg = mine < x.sg.chunks_c ? (mine * kChunk) >> a.c.page_shift : -1;
         pages = pg >= 0 ? a.c.table[x.b * a.c.table_stride + pg] : -1;
       }
-      const int pg = __shfl_sync(~0u, pages, k & 31), pos = c * kChunk, in_page = pos & ((1 << a.c.page_shift) - 1);
-      const bool mapped = pg >= 0 && pg < a.c.num_pages;
+      const int pg = __shfl_sync(~0u, pages, k & 31), pos = c * kChunk, in_page = pos & page_mask;
+      const bool mapped = (unsigned)pg < (unsigned)a.c.num_pages;
       if (mapped) {  // whole chunks: a page has room for them
-        const long long at = pg * a.c.page_bytes + x.head * a.c.head_bytes + (long long)in_page * (D / 2);
-        const long long at_s = pg * a.scale_page + x.head * a.scale_head + (long long)in_page * (G * 2);
-        L::load(my_ring + slot * L::kStage, a.c.k + at, a.c.v + at, a.k_scale + at_s, a.v_scale + at_s, lane);
+        const long long at = pg * a.c.page_bytes + in_page * (D / 2), at_s = pg * a.scale_page + in_page * (G * 2);
+        L::load(my_ring + slot * L::kStage, from_k + at, from_v + at, from_s + at_s, lane);
       }
       if (lane == 0) my_there[slot] = mapped ? min(kChunk, x.sg.len - pos) : 0;
     }
@@ -377,22 +355,31 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   // the query rows of a piece, their sums and the drafts that each sees
   auto load_query = [&](const WarpPiece &x) {
     const int rows = min(ROWS, x.sg.count * a.group - x.rb * ROWS);
-    for (int i = tid; i < ROWS * G * 4; i += kTreeThreads) {  // (row, group, quarter)
+    for (int i = tid; i < ROWS * G * 4; i += kTreeThreads) {  // (row, group, quarter): whole warps
       const int row = i / (G * 4), j = i / 4 % G, quarter = i % 4, at = x.rb * ROWS + row;
-      const T *from = row < rows ? (const T *)a.q + (x.sg.first + at / a.group) * a.q_stride +
-                                       (long long)(x.head * a.group + at % a.group) * D + 32 * j + 8 * quarter
-                                 : nullptr;
-      uint32_t f[L::kParts][4];
-      L::pairs8(f, from);
-#pragma unroll
-      for (int w = 0; w < L::kParts; w++)
-        sts4u(q_at + row / 8 * L::kQBytes + (w * G + j) * 512 + (row % 8 * 4 + quarter) * 16, f[w][0], f[w][1], f[w][2], f[w][3]);
-      if constexpr (!L::f32) {
-        float s = L::sum8(from);
-        s += __shfl_xor_sync(~0u, s, 1);
-        s += __shfl_xor_sync(~0u, s, 2);
-        if (quarter == 0) first_sm[row * G + j] = -24.f * s;
+      float y[8] = {};
+      if (row < rows) {
+        Eight<T> e;
+        e.load((const T *)a.q + (x.sg.first + at / a.group) * a.q_stride + (long long)(x.head * a.group + at % a.group) * D + 32 * j + 8 * quarter);
+        e.floats(y);
       }
+      float up = 1.f, down = 1.f;
+      if constexpr (!std::is_same<T, __half>::value) {
+        float most = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) most = fmaxf(most, fabsf(y[k]));
+#pragma unroll
+        for (int d = 1; d < G * 4; d <<= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+        // 2^13 over the largest value's power of two, within what has a reciprocal
+        const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 126);
+        up = __uint_as_float((uint32_t)(127 + 13 - e) << 23), down = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
+      }
+      uint32_t f[L::kQParts][4];
+      L::pairs8(f, y, up);
+#pragma unroll
+      for (int w = 0; w < L::kQParts; w++)
+        sts4u(q_at + row / 8 * L::kQBytes + (w * G + j) * 512 + (row % 8 * 4 + quarter) * 16, f[w][0], f[w][1], f[w][2], f[w][3]);
+      if (j + quarter == 0) down_sm[row] = down;
     }
     for (int r = tid; r < ROWS; r += kTreeThreads)
       seen[r] = r < rows ? (unsigned long long)a.mask[x.sg.first + (x.rb * ROWS + r) / a.group] : 0ull;
@@ -422,17 +409,16 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
 
   for (int piece = 0; more; piece++) {
     uint32_t qr[S::kQInRegs ? G : 1][4];
-    float fr[S::kQInRegs ? G : 1][2];
     if constexpr (S::kQInRegs) {
 #pragma unroll
-      for (int j = 0; j < G; j++) {
-        lds4u(qr[j], q_at + j * 512 + lane * 16);
-        fr[j][0] = first_sm[2 * t * G + j], fr[j][1] = first_sm[(2 * t + 1) * G + j];
-      }
+      for (int j = 0; j < G; j++) lds4u(qr[j], q_at + j * 512 + lane * 16);
     }
-    float o[L::kTiles][NT][4] = {}, ref[NT][2], sum[NT][2] = {}, low[NT][2] = {};  // of rows 8 n + 2 t and + 1
+    // of rows 8 n + 2 t and + 1; factor: what makes scores of the products, in units of log2
+    float o[L::kTiles][NT][4] = {}, ref[NT][2], sum[NT][2] = {}, low[NT][2] = {}, factor[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; n++) ref[n][0] = ref[n][1] = -INFINITY;
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) ref[n][h] = -INFINITY, factor[n][h] = a.scale * down_sm[n * 8 + 2 * t + h];
 
     // scores in units of log2 become weights, against the rows' references
     auto soften = [&](float (&s)[NT][4]) {
@@ -475,12 +461,13 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
 #pragma unroll
         for (int h = 0; h < 2; h++) {
           const int row = n * 8 + 2 * t + h;
+          const float down = down_sm[row];
           float x = 0.f;
 #pragma unroll
           for (int i = 0; i < G; i++) {
             const float4 q4 = L::four(q_at + n * L::kQBytes, 2 * t + h, i, g);
             const float4 k4 = key[i].floats();
-            x = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, x))));
+            x = fmaf(q4.x * down, k4.x, fmaf(q4.y * down, k4.y, fmaf(q4.z * down, k4.z, fmaf(q4.w * down, k4.w, x))));
           }
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(~0u, x, d);
@@ -513,11 +500,11 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
       const int valid = my_there[k % NS];
       if (valid == 0) continue;
       float s[NT][4];
-      L::template scores<NT, S::kQInRegs>(s, qr, fr, q_at, first_sm, st, lane);
+      L::template scores<NT, S::kQInRegs>(s, qr, q_at, st, lane);
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[n][e] *= a.scale;
+        for (int e = 0; e < 4; e++) s[n][e] *= factor[n][e & 1];
       if (valid < kChunk) {
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -539,6 +526,7 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
         cur.chunks_of(warp, kTileChunks);
         nc = cached_of(cur);
         __syncwarp();  // all lanes are done with the last stage
+        head_of(cur);
 #pragma unroll
         for (int k = 0; k < NS - 1; k++) issue(cur, nc, k);
         drafts_of(cur);

@@ -99,6 +99,10 @@ __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
   V r = __hfma2(*reinterpret_cast<V *>(&a), *reinterpret_cast<V *>(&b), *reinterpret_cast<V *>(&c));
   return *reinterpret_cast<uint32_t *>(&r);
 }
+__device__ __forceinline__ uint32_t add2(uint32_t a, uint32_t b) {  // of f16
+  __half2 r = __hadd2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+  return *reinterpret_cast<uint32_t *>(&r);
+}
 template <typename B>
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
   using V = typename Two<B>::V;
