@@ -4,8 +4,9 @@
 // The mathematics, segments and runs are tree_attn.cuh's; only the cache is read in another way.
 // The 16 positions of a chunk are the rows of the matrix instruction, 8 query rows its
 // columns.  Codes become 16-bit numbers in registers:
-//   K   whole numbers in f16, against f16 queries: a row's power of two brings its largest value below 2^14, f32 rows are two
-//       f16 parts (22 bits); a group of 32 dims is summed, then times its scale in 32 bits
+//   K   c + 8 as f16, against f16 queries: a row's power of two brings its largest value below 2^14; a group of 32 dims is
+//       summed from -8 sum q on, then times its scale in 32 bits.  f32: c itself, so that nothing cancels, against two f16
+//       parts of a query (22 bits)
 //   V   c s in T (f32: in bf16, which holds it exactly, against weights of three bf16 parts)
 // so products are exact and only sums are rounded.  A lane finds all that it needs of a row in one piece: of K, dims
 // 32 j + 8 t .. + 7 of each group j, of V, dims 32 j + 4 g .. + 3 (g = lane / 4, t = lane % 4).  The chunk's
@@ -21,12 +22,21 @@ namespace paged {
 template <typename T>
 using Product = std::conditional_t<std::is_same<T, __half>::value, __half, __nv_bfloat16>;  // the type of V's products
 
-// The four pairs of nibbles of two halfwords as whole numbers c in f16: (1024 + u) - 1032 and (1024 + 16 u) / 16 - 72, all
-// exact.  One shift for four pairs: with one for each (lifted) a chunk's integer instructions took a third longer.
-__device__ __forceinline__ void whole4(uint32_t (&c)[4], uint32_t x) {
-  const uint32_t y = x >> 8, minus = 0xe408e408u, low = 0x2c002c00u, minus72 = 0xd480d480u;
-  c[0] = add2((x & 0x000f000fu) | 0x64006400u, minus), c[1] = fma2<__half>((x & 0x00f000f0u) | 0x64006400u, low, minus72);
-  c[2] = add2((y & 0x000f000fu) | 0x64006400u, minus), c[3] = fma2<__half>((y & 0x00f000f0u) | 0x64006400u, low, minus72);
+// The four pairs of nibbles u = c + 8 of two halfwords as f16: a nibble's bits as they lie there, or four places up, are
+// 2^-24 u and 2^-20 u, numbers below the smallest normal one, which the matrix instruction takes like any other.  So a pair
+// costs one mask, and four one shift; the queries of odd dims are a 16th, and 8 of each sum is taken off as the accumulator's
+// first value.
+__device__ __forceinline__ void nibbles4(uint32_t (&u)[4], uint32_t x) {
+  const uint32_t y = x >> 8;
+  u[0] = x & 0x000f000fu, u[1] = x & 0x00f000f0u, u[2] = y & 0x000f000fu, u[3] = y & 0x00f000f0u;
+}
+// As whole numbers c: (1024 + u) - 1032 and (1024 + 16 u) / 16 - 72, all exact.  base: 1024 twice, from a register (as
+// a constant it costs an instruction a pair).
+__device__ __forceinline__ void whole4(uint32_t (&c)[4], uint32_t x, uint32_t base) {
+  const uint32_t minus = 0xe408e408u, low = 0x2c002c00u, minus72 = 0xd480d480u;
+  nibbles4(c, x);
+  c[0] = add2(c[0] | base, minus), c[1] = fma2<__half>(c[1] | base, low, minus72);
+  c[2] = add2(c[2] | base, minus), c[3] = fma2<__half>(c[3] | base, low, minus72);
 }
 
 // x as three bf16 numbers, in the upper halves: exact (8 bits each, cut, so that none is rounded up to
@@ -71,6 +81,8 @@ struct PackTile {
   static constexpr int G = D / 32;                     // groups of a row
   static constexpr int kParts = f32 ? 3 : 1;           // of a weight
   static constexpr int kQParts = f32 ? 2 : 1;          // of a query
+  static constexpr float kOdd = f32 ? 1.f : 16.f;      // how much smaller a query's odd dims are: their codes are that much larger
+  static constexpr float kUnit = f32 ? 1.f : 0x1p24f;  // one over what a code is
   static constexpr int kCodes = kChunk * D / 2;        // bytes of a chunk's K or V
   static constexpr int kScales = kChunk * G * 2;
   static constexpr int kStage = 2 * (kCodes + kScales);  // K, V, their scales
@@ -99,11 +111,11 @@ struct PackTile {
   // The position of row g of the matrix instruction; row g + 8 has that plus 2.
   static __device__ __forceinline__ int position(int g) { return 4 * (g >> 1) + (g & 1); }
 
-  // ---- fragments of a query row's 8 consecutive dims: pairs (i, 4 + i) of f16 parts of up times the row
+  // ---- fragments of a query row's 8 consecutive dims: pairs (i, 4 + i) of f16 parts of up times the row (odd ones a 16th)
   static __device__ __forceinline__ void pairs8(uint32_t (&f)[kQParts][4], const float (&x)[8], float up) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const float a = x[i] * up, b = x[4 + i] * up;
+      const float z = i & 1 ? up / kOdd : up, a = x[i] * z, b = x[4 + i] * z;
       f[0][i] = pack2(a, b, __half());
       if constexpr (f32) {
         const float2 hi = unpack2<__half>(f[0][i]);
@@ -124,12 +136,14 @@ struct PackTile {
         x[i] += g & 1 ? y.y : y.x;
       }
     }
-    return make_float4(x[0], x[1], x[2], x[3]);
+    return make_float4(x[0], kOdd * x[1], x[2], kOdd * x[3]);
   }
 
-  // ---- cached keys: s of NT x 8 rows (times their up).  q: the fragments' address; qr: they themselves (NT = 1, 16 bits).
+  // ---- cached keys: s of NT x 8 rows (times 2^-24 their up).  q: the fragments' address; qr: they themselves (NT = 1, 16
+  // bits); first: -8 times the sums of q, [row][group], and fr a lane's own.
   template <int NT, bool REGS>
-  static __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&qr)[REGS ? G : 1][4], uint32_t q, uint32_t st, int lane) {
+  static __device__ __forceinline__ void scores(float (&s)[NT][4], const uint32_t (&qr)[REGS ? G : 1][4], const float (&fr)[REGS ? G : 1][2],
+                                                uint32_t q, const float *first, uint32_t st, int lane) {
     const int g = lane >> 2, t = lane & 3, p0 = position(g);
     uint32_t k[2][4], ks[2][2];
 #pragma unroll
@@ -147,13 +161,23 @@ struct PackTile {
 #pragma unroll
     for (int j = 0; j < G; j++) {
       uint32_t c0[4], c1[4];
-      whole4(c0, halves(k[0][j >> 1], k[0][2 + (j >> 1)], j & 1)), whole4(c1, halves(k[1][j >> 1], k[1][2 + (j >> 1)], j & 1));
+      const uint32_t x0 = halves(k[0][j >> 1], k[0][2 + (j >> 1)], j & 1), x1 = halves(k[1][j >> 1], k[1][2 + (j >> 1)], j & 1);
+      if constexpr (f32)
+        whole4(c0, x0, 0x64006400u), whole4(c1, x1, 0x64006400u);
+      else
+        nibbles4(c0, x0), nibbles4(c1, x1);
       const uint32_t a0[4] = {c0[0], c1[0], c0[1], c1[1]}, a1[4] = {c0[2], c1[2], c0[3], c1[3]};
       const float s0 = __uint_as_float(j & 1 ? ks[0][j >> 1] & 0xffff0000u : ks[0][j >> 1] << 16);
       const float s1 = __uint_as_float(j & 1 ? ks[1][j >> 1] & 0xffff0000u : ks[1][j >> 1] << 16);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        float p[4] = {0.f, 0.f, 0.f, 0.f};
+        float p[4];
+        if constexpr (f32)
+          p[0] = p[1] = p[2] = p[3] = 0.f;
+        else if constexpr (REGS)
+          p[0] = p[2] = fr[j][0], p[1] = p[3] = fr[j][1];
+        else
+          p[0] = p[2] = first[(n * 8 + 2 * t) * G + j], p[1] = p[3] = first[(n * 8 + 2 * t + 1) * G + j];
 #pragma unroll
         for (int w = kQParts - 1; w >= 0; w--) {  // the small part first
           uint32_t b[4];
@@ -192,7 +216,8 @@ struct PackTile {
 
   // o += v' p over the chunk; tile 2 j + h of o has dims 32 j + 4 g + 2 h (elements 0, 1) and the next (2, 3).
   template <int NT>
-  static __device__ __forceinline__ void values(float (&o)[kTiles][NT][4], const uint32_t (&b)[kParts][NT][2], uint32_t st, int valid, int lane) {
+  static __device__ __forceinline__ void values(float (&o)[kTiles][NT][4], const uint32_t (&b)[kParts][NT][2], uint32_t st, int valid, int lane,
+                                                uint32_t base) {
     const int g = lane >> 2, t = lane & 3;
     uint32_t v[4][2], vs[4][2];  // of positions 4 t + i
 #pragma unroll
@@ -229,13 +254,13 @@ struct PackTile {
       const uint32_t x01 = halves(v[0][j >> 1], v[1][j >> 1], j & 1), x23 = halves(v[2][j >> 1], v[3][j >> 1], j & 1);
       uint32_t y01[4], y23[4];
       if constexpr (std::is_same<B, __half>::value) {
-        whole4(y01, x01), whole4(y23, x23);
+        whole4(y01, x01, base), whole4(y23, x23, base);
 #pragma unroll
         for (int i = 0; i < 4; i++) y01[i] = mul2<B>(y01[i], s01), y23[i] = mul2<B>(y23[i], s23);
       } else {
         const Scaled<B> by01(s01), by23(s23);
 #pragma unroll
-        for (int i = 0; i < 4; i++) y01[i] = by01(x01, i), y23[i] = by23(x23, i);
+        for (int i = 0; i < 4; i++) y01[i] = by01(x01, i, base), y23[i] = by23(x23, i, base);
       }
 #pragma unroll
       for (int h = 0; h < 2; h++) {
@@ -274,8 +299,8 @@ struct PackShape {
   static constexpr int kJoin = kTreeWarps * 8 * D * 4;  // eight rows of every warp
   static constexpr int kQ = NT * L::kQBytes;
   static constexpr bool kQInRegs = NT == 1 && sizeof(T) == 2;
-  static constexpr int kFactors = kRows * 4;
-  static constexpr int kSmem = kRing + kJoin + kQ + kFactors + kTreeWarps * kRows * 8 + kRows * 8 + 64 + kTreeWarps * 8 * 4 + kRows * 8;
+  static constexpr int kFactors = kRows * 4 * (1 + L::G);
+  static constexpr int kSmem = kRing + kJoin + kQ + kFactors + kTreeWarps * kRows * 8 + kRows * 8 + 64 + kTreeWarps * 64 * 4 + kRows * 8;
 };
 
 template <typename T, int D, int NT, int CS>
@@ -288,7 +313,7 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   char *ring = sm, *q_sm = sm + S::kRing + S::kJoin;
   float *join = (float *)(sm + S::kRing);
   char *p = q_sm + S::kQ;
-  float *down_sm = (float *)p;  // [row]: 1 / up
+  float *down_sm = (float *)p, *first_sm = down_sm + ROWS;  // [row]: 1 / up; [row][group]: 2^-24 * -8 times the sum of up q
   p += S::kFactors;
   float *ml = (float *)p;  // [warp][row][m, l]
   p += kTreeWarps * ROWS * 8;
@@ -296,10 +321,12 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   p += ROWS * 8;
   long long *plan = (long long *)p;
   p += 64;
-  int *there = (int *)p;  // [warp][stage]: positions of the chunk that exist
-  p += kTreeWarps * 8 * 4;
+  int *there = (int *)p;  // [warp][chunk % 64]: its positions that exist
+  p += kTreeWarps * 64 * 4;
   float *part_ml = (float *)p;  // CS > 1: [row][m, l] of this block
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint32_t base = lifted_base<typename L::B>();
+  asm("" : "+r"(base));  // stays in a register
 
   WarpPiece cur;
   Walk walk;
@@ -324,10 +351,10 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   };
 
   const uint32_t my_ring = smem_addr(ring) + warp * (NS * L::kStage), q_at = smem_addr(q_sm);
-  int *my_there = there + warp * 8;
-  int pages = -1;  // lane i: the page of the chunk 32 j + i
-  const int page_mask = (1 << a.c.page_shift) - 1;
-  const char *from_k, *from_v, *from_s;  // of the piece's head: what the lane copies of a page
+  int *my_there = there + warp * 64;
+  // Lane i: where the chunk 32 j + i lies, codes and scales, negative without a page.
+  long long codes_at = -1, scales_at = -1;
+  const char *from_k, *from_v, *from_s;  // of the piece's head: what the lane copies
   auto head_of = [&](const WarpPiece &x) {
     const long long at = x.head * a.c.head_bytes + lane * 16, at_s = x.head * a.scale_head;
     from_k = a.c.k + at, from_v = a.c.v + at;
@@ -336,19 +363,17 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   head_of(cur);
   auto issue = [&](const WarpPiece &x, int nc, int k) {
     if (k < nc) {
-      const int c = x.c0 + k * x.step, slot = k % NS;
       if ((k & 31) == 0) {
-        const int mine = c + lane * x.step;
-        const int pg = mine < x.sg.chunks_c ? (mine * kChunk) >> a.c.page_shift : -1;
-        pages = pg >= 0 ? a.c.table[x.b * a.c.table_stride + pg] : -1;
+        const int c = x.c0 + (k + lane) * x.step, pos = c * kChunk, in_page = pos & ((1 << a.c.page_shift) - 1);
+        const int pg = c < x.sg.chunks_c ? a.c.table[x.b * a.c.table_stride + (pos >> a.c.page_shift)] : -1;
+        const bool mapped = pg >= 0 && pg < a.c.num_pages;
+        codes_at = mapped ? pg * a.c.page_bytes + in_page * (D / 2) : -1;
+        scales_at = pg * a.scale_page + in_page * (G * 2);
+        my_there[(k + lane) & 63] = mapped ? min(kChunk, x.sg.len - pos) : 0;
       }
-      const int pg = __shfl_sync(~0u, pages, k & 31), pos = c * kChunk, in_page = pos & page_mask;
-      const bool mapped = (unsigned)pg < (unsigned)a.c.num_pages;
-      if (mapped) {  // whole chunks: a page has room for them
-        const long long at = pg * a.c.page_bytes + in_page * (D / 2), at_s = pg * a.scale_page + in_page * (G * 2);
-        L::load(my_ring + slot * L::kStage, from_k + at, from_v + at, from_s + at_s, lane);
-      }
-      if (lane == 0) my_there[slot] = mapped ? min(kChunk, x.sg.len - pos) : 0;
+      const long long at = __shfl_sync(~0u, codes_at, k & 31), at_s = __shfl_sync(~0u, scales_at, k & 31);
+      // whole chunks: a page has room for them
+      if (at >= 0) L::load(my_ring + k % NS * L::kStage, from_k + at, from_v + at, from_s + at_s, lane);
     }
     copy_commit();
   };
@@ -363,22 +388,30 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
         e.load((const T *)a.q + (x.sg.first + at / a.group) * a.q_stride + (long long)(x.head * a.group + at % a.group) * D + 32 * j + 8 * quarter);
         e.floats(y);
       }
-      float up = 1.f, down = 1.f;
-      if constexpr (!std::is_same<T, __half>::value) {
-        float most = 0.f;
+      float most = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; k++) most = fmaxf(most, fabsf(y[k]));
+      for (int k = 0; k < 8; k++) most = fmaxf(most, fabsf(y[k]));
 #pragma unroll
-        for (int d = 1; d < G * 4; d <<= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
-        // 2^13 over the largest value's power of two, within what has a reciprocal
-        const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 126);
-        up = __uint_as_float((uint32_t)(127 + 13 - e) << 23), down = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
-      }
+      for (int d = 1; d < G * 4; d <<= 1) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+      // 2^13 over the largest value's power of two, within what has a reciprocal
+      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 126);
+      const float up = __uint_as_float((uint32_t)(127 + 13 - e) << 23), down = __uint_as_float((uint32_t)(127 - 13 + e) << 23);
       uint32_t f[L::kQParts][4];
       L::pairs8(f, y, up);
 #pragma unroll
       for (int w = 0; w < L::kQParts; w++)
         sts4u(q_at + row / 8 * L::kQBytes + (w * G + j) * 512 + (row % 8 * 4 + quarter) * 16, f[w][0], f[w][1], f[w][2], f[w][3]);
+      if constexpr (!L::f32) {
+        float q8 = 0.f;  // of the fragments, which may be rounded
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float2 z = unpack2<__half>(f[0][k]);
+          q8 = fmaf(k & 1 ? L::kOdd : 1.f, z.x + z.y, q8);
+        }
+        q8 += __shfl_xor_sync(~0u, q8, 1);
+        q8 += __shfl_xor_sync(~0u, q8, 2);
+        if (quarter == 0) first_sm[row * G + j] = -8.f / L::kUnit * q8;
+      }
       if (j + quarter == 0) down_sm[row] = down;
     }
     for (int r = tid; r < ROWS; r += kTreeThreads)
@@ -409,16 +442,20 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
 
   for (int piece = 0; more; piece++) {
     uint32_t qr[S::kQInRegs ? G : 1][4];
+    float fr[S::kQInRegs ? G : 1][2];
     if constexpr (S::kQInRegs) {
 #pragma unroll
-      for (int j = 0; j < G; j++) lds4u(qr[j], q_at + j * 512 + lane * 16);
+      for (int j = 0; j < G; j++) {
+        lds4u(qr[j], q_at + j * 512 + lane * 16);
+        fr[j][0] = first_sm[2 * t * G + j], fr[j][1] = first_sm[(2 * t + 1) * G + j];
+      }
     }
     // of rows 8 n + 2 t and + 1; factor: what makes scores of the products, in units of log2
     float o[L::kTiles][NT][4] = {}, ref[NT][2], sum[NT][2] = {}, low[NT][2] = {}, factor[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int h = 0; h < 2; h++) ref[n][h] = -INFINITY, factor[n][h] = a.scale * down_sm[n * 8 + 2 * t + h];
+      for (int h = 0; h < 2; h++) ref[n][h] = -INFINITY, factor[n][h] = a.scale * L::kUnit * down_sm[n * 8 + 2 * t + h];
 
     // scores in units of log2 become weights, against the rows' references
     auto soften = [&](float (&s)[NT][4]) {
@@ -497,10 +534,10 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
       __syncwarp();  // the stage before is read by all lanes too
       issue(cur, nc, k + NS - 1);
       const uint32_t st = my_ring + k % NS * L::kStage;
-      const int valid = my_there[k % NS];
+      const int valid = my_there[k & 63];
       if (valid == 0) continue;
       float s[NT][4];
-      L::template scores<NT, S::kQInRegs>(s, qr, q_at, st, lane);
+      L::template scores<NT, S::kQInRegs>(s, qr, fr, q_at, first_sm, st, lane);
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -515,7 +552,7 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
       soften(s);
       uint32_t b[L::kParts][NT][2];
       L::template weights<NT>(b, s);
-      L::template values<NT>(o, b, st, valid, lane);
+      L::template values<NT>(o, b, st, valid, lane, base);
     }
     // the next piece's first chunks are on their way while this one is joined
     const WarpPiece done = cur;

@@ -75,13 +75,18 @@ struct Eight {
   }
 };
 
-// Lifted nibbles: nibble i of both halfwords as 16 + nibble, two numbers of B (at the top of the mantissa of 16).
+// Lifted nibbles: nibble i of both halfwords as 16 + nibble, two numbers of B (at the top of the mantissa of 16).  The base may
+// come from a register: as a constant it costs another instruction in loops that have no register left.
 template <typename B>
-__device__ __forceinline__ uint32_t lifted(uint32_t x, int i) {
+__device__ __forceinline__ constexpr uint32_t lifted_base() {
+  return std::is_same<B, __half>::value ? 0x64006400u : 0x41804180u;  // f16's, 1024 twice, is for whole numbers of loops
+}
+template <typename B>
+__device__ __forceinline__ uint32_t lifted(uint32_t x, int i, uint32_t base = std::is_same<B, __half>::value ? 0x4c004c00u : 0x41804180u) {
   if constexpr (std::is_same<B, __half>::value)
-    return ((i < 2 ? x << (6 - 4 * i) : x >> (4 * i - 6)) & 0x03c003c0u) | 0x4c004c00u;
+    return ((i < 2 ? x << (6 - 4 * i) : x >> (4 * i - 6)) & 0x03c003c0u) | base;
   else
-    return ((i < 1 ? x << 3 : x >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
+    return ((i < 1 ? x << 3 : x >> (4 * i - 3)) & 0x00780078u) | base;
 }
 template <typename B>
 struct Two;
@@ -123,6 +128,9 @@ struct Scaled {
   __device__ __forceinline__ explicit Scaled(uint32_t s_) : s(s_), minus(0) {
     static_assert(!ROOM || !std::is_same<B, __half>::value, "");
     if constexpr (ROOM) minus = mul2<B>(s, 0xc1c0c1c0u);  // -24
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t codes, int i, uint32_t base) const {  // with room
+    return fma2<B>(lifted<B>(codes, i, base), s, minus);
   }
   __device__ __forceinline__ uint32_t operator()(uint32_t codes, int i) const {
     if constexpr (ROOM)
