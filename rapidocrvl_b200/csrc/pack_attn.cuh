@@ -298,6 +298,7 @@ struct PackShape {
   static constexpr int kRing = kTreeWarps * kStages * L::kStage;
   static constexpr int kJoin = kTreeWarps * 8 * D * 4;  // eight rows of every warp
   static constexpr int kQ = NT * L::kQBytes;
+  static_assert(kQ >= kTreeThreads * 4, "the lengths are ranked there");
   static constexpr bool kQInRegs = NT == 1 && sizeof(T) == 2;
   static constexpr int kFactors = kRows * 4 * (1 + L::G);
   static constexpr int kSmem = kRing + kJoin + kQ + kFactors + kTreeWarps * kRows * 8 + kRows * 8 + 64 + kTreeWarps * 64 * 4 + kRows * 8;
@@ -339,6 +340,21 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   } else {
     const int seg = blockIdx.x / CS;
     cur.rb = seg % row_blocks, cur.head = seg / row_blocks % a.kv_heads, cur.b = seg / row_blocks / a.kv_heads;
+    if (a.longest_first) {
+      // Blocks are handed out in order, one an SM first: the longest sequences' come first, so that an SM's second block is
+      // a short one's.  Every block ranks the lengths (at most one a thread) and takes the sequence of its rank.
+      int *lens = (int *)q_sm;
+      const int mine = tid < a.s.batch ? a.s.len(tid) : 0;
+      if (tid < a.s.batch) lens[tid] = mine;
+      __syncthreads();
+      if (tid < a.s.batch) {
+        int rank = 0;
+        for (int i = 0; i < a.s.batch; i++) rank += lens[i] > mine || (lens[i] == mine && i < tid);
+        if (rank == cur.b) plan[0] = tid;
+      }
+      __syncthreads();
+      cur.b = (int)plan[0];
+    }
     cur.sg = Segments(a, cur.b, ROWS);
     if (cur.rb >= cur.sg.blocks) return;  // the whole cluster alike
     cur.t0 = blockIdx.x % CS, cur.t1 = cur.sg.tiles;
@@ -429,12 +445,13 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   };
   auto drafts_of = [&](const WarpPiece &x) {
     const int c0 = CS > 0 ? 0 : x.t0 * kTileChunks - x.sg.chunks_c, c1 = x.t1 * kTileChunks - x.sg.chunks_c;
-    draft0 = max(0, c0) * kChunk + warp + (CS > 1 ? blockIdx.x % CS * kTreeWarps : 0), draft1 = min(x.sg.count, c1 * kChunk);
+    // from the last warp down, which has the fewest chunks
+    draft0 = max(0, c0) * kChunk + draft_step - 1 - warp - (CS > 1 ? blockIdx.x % CS * kTreeWarps : 0), draft1 = min(x.sg.count, c1 * kChunk);
     if (draft0 < draft1) load_draft(x, draft0);
   };
 
   int nc = cached_of(cur);
-#pragma unroll
+#pragma unroll 1
   for (int k = 0; k < NS - 1; k++) issue(cur, nc, k);
   drafts_of(cur);
   load_query(cur);
@@ -564,7 +581,7 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
         nc = cached_of(cur);
         __syncwarp();  // all lanes are done with the last stage
         head_of(cur);
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < NS - 1; k++) issue(cur, nc, k);
         drafts_of(cur);
       }

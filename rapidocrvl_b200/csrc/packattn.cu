@@ -30,6 +30,7 @@ int launch_pack(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   int cs = 1;
   while (cs < 8 && cs < tiles && segments * cs * 2 <= (cs == 1 ? room : (long long)cluster_room(sms) * S::kBlocks)) cs *= 2;
   const double whole = (double)((tiles + cs - 1) / cs) * ((segments * cs + room - 1) / room), runs = (double)segments * tiles / room;
+  a.longest_first = a.s.batch > 1 && a.s.batch <= kTreeThreads && segments * cs > sms;
   if (whole <= runs + kRunsCost)
     return cs == 8 ? one(k_pack_attn<T, D, NT, 8>, 8) : cs == 4 ? one(k_pack_attn<T, D, NT, 4>, 4) : cs == 2 ? one(k_pack_attn<T, D, NT, 2>, 2) : one(k_pack_attn<T, D, NT, 1>, 1);
 

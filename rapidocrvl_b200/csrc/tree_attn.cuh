@@ -67,6 +67,7 @@ struct TreeArgs {
   int start_cost; // of a segment's start (filling the rings, joining the warps), in tiles, in the split of runs
   const char *k_scale, *v_scale;         // a packed cache's (c holds its codes): at the layer,
   long long scale_page, scale_head;      // bytes
+  bool longest_first;                    // blocks of whole segments in the order of the sequences' lengths
 };
 
 struct Segments {  // what a sequence's segments have in common
