@@ -329,9 +329,11 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   uint32_t base = lifted_base<typename L::B>();
   asm("" : "+r"(base));  // stays in a register
 
+  pdl_wait();
   WarpPiece cur;
   Walk walk;
   bool more = true;
+  if constexpr (CS > 0) pdl_launch();
   if constexpr (CS == 0) {
     const bool any = walk.start(a, ROWS, plan, warp, lane, cur);
     pdl_launch();

@@ -39,7 +39,7 @@ struct PackArgs {
   int capacity, layers, batch, kv_heads, n_tokens, max_path;
 };
 
-constexpr int kPackWarps = 8, kPackThreads = kPackWarps * 32;
+constexpr int kPackWarps = 4, kPackThreads = kPackWarps * 32;
 constexpr int kPackRows = 4;  // steps whose loads go out together
 
 // 8 values of a row: as they lie in memory, and as 32-bit floats.
@@ -266,6 +266,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kPackThreads) k_packed_append(const PackArgs a) {
   using I = PackItem<D>;
   const int b = blockIdx.y, lane = threadIdx.x & 31, i8 = lane % I::LANES, sub = lane / I::LANES;
+  pdl_wait();
+  pdl_launch();
   I x(a, b);
   const int n = min(a.path ? min(max(a.n_path[b], 0), a.max_path) : x.count, a.capacity - x.len);
   if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) a.new_lens[b] = x.len + n;
@@ -309,6 +311,8 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kPackThreads) k_packed_read(const PackArgs a) {
   using I = PackItem<D>;
   const int b = blockIdx.y, lane = threadIdx.x & 31, i8 = lane % I::LANES, sub = lane / I::LANES;
+  pdl_wait();
+  pdl_launch();
   I x(a, b);
   if (x.count == 0) return;
   const int codes_at = sub * (D / 2) + place<D>(i8), scales_at = sub * (D / 16) + i8 / 4 * 2;

@@ -56,7 +56,7 @@ int move_grid(const PackArgs &a, int most_tokens, dim3 *grid) {
   const long long rows = 2ll * a.layers * a.kv_heads;
   if (rows > 1 << 30) return invalid("too many layers and kv heads");
   const long long z = (rows + kPackWarps - 1) / kPackWarps < 1024 ? (rows + kPackWarps - 1) / kPackWarps : 1024;
-  const long long chunks = (long long)most_tokens / kChunk + 2, most = (sms * 32 + a.batch * z - 1) / (a.batch * z);
+  const long long chunks = (long long)most_tokens / kChunk + 2, most = (sms * 64 + a.batch * z - 1) / (a.batch * z);
   *grid = dim3((unsigned)(chunks < most ? chunks : most), a.batch, (unsigned)z);
   return OCRVL_OK;
 }
@@ -74,7 +74,7 @@ int launch_rotate(RotateArgs &a, int sms, cudaStream_t stream) {
   a.q_batches = batches(a.heads), a.batches = a.q_batches + batches(a.kv_heads);
   const int share = room < 1 ? 1 : room < a.batches ? room : a.batches;
   const dim3 grid(blocks < full ? blocks : full, share);
-  auto go = [&](auto kernel) { return launch("rotate", kernel, grid, kRotateWarps * 32, kRotateSmem<T, V>, stream, false, 1, a); };
+  auto go = [&](auto kernel) { return launch("rotate", kernel, grid, kRotateWarps * 32, kRotateSmem<T, V>, stream, true, 1, a); };
   if (a.lanes == 8) return go(k_rotate<T, V, NORM, 8>);
   if (a.lanes == 16) return go(k_rotate<T, V, NORM, 16>);
   return go(k_rotate<T, V, NORM, 0>);
@@ -105,7 +105,7 @@ int ocrvl_op_packed_append(const ocrvl_packed_cache *c, int type, int n_tokens, 
   if (int rc = move_grid(a, path ? max_path : n_tokens, &grid)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto wide, auto narrow) {
-    return launch("append, packed", c->head_dim == 128 ? wide : narrow, grid, kPackThreads, 0, st, false, 1, a);
+    return launch("append, packed", c->head_dim == 128 ? wide : narrow, grid, kPackThreads, 0, st, true, 1, a);
   };
   if (type == OCRVL_F32) return go(k_packed_append<float, 128>, k_packed_append<float, 64>);
   if (type == OCRVL_F16) return go(k_packed_append<__half, 128>, k_packed_append<__half, 64>);
@@ -121,7 +121,7 @@ int ocrvl_op_packed_read(const ocrvl_packed_cache *c, int type, int n_tokens, co
   if (int rc = move_grid(a, n_tokens, &grid)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto wide, auto narrow) {
-    return launch("read, packed", c->head_dim == 128 ? wide : narrow, grid, kPackThreads, 0, st, false, 1, a);
+    return launch("read, packed", c->head_dim == 128 ? wide : narrow, grid, kPackThreads, 0, st, true, 1, a);
   };
   if (type == OCRVL_F32) return go(k_packed_read<float, 128>, k_packed_read<float, 64>);
   if (type == OCRVL_F16) return go(k_packed_read<__half, 128>, k_packed_read<__half, 64>);

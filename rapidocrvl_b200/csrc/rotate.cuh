@@ -112,7 +112,10 @@ __global__ void __launch_bounds__(kRotateWarps * 32, kRotateBlocks) k_rotate(con
   // this warp's tokens, and of each its batches
   long long token = warp * gridDim.x + blockIdx.x;
   const int next = kRotateWarps * gridDim.x;
-  if (token >= a.n_tokens || blockIdx.y >= a.batches) return;  // the whole warp
+  if (token >= a.n_tokens || blockIdx.y >= a.batches) {  // the whole warp
+    pdl_wait();  // on every path: this grid's end is to mean that of the one before it too
+    return;
+  }
   const int lanes = LANES ? LANES : a.lanes, at_once = LANES ? 32 / (LANES ? LANES : 1) : a.at_once;
   const int sub = LANES ? lane / (LANES ? LANES : 1) : lane * a.lane_factor >> 16, v = lane - sub * lanes, rotated = a.pairs / V;
   const int d0 = v >= rotated ? 2 * a.pairs + 2 * V * (v - rotated) : a.neighbours ? 2 * V * v : V * v;  // the lane's two runs of V dims
@@ -137,6 +140,8 @@ __global__ void __launch_bounds__(kRotateWarps * 32, kRotateBlocks) k_rotate(con
     to_stage = to_stage + 1 == NS ? 0 : to_stage + 1;
     copy_commit();
   };
+  pdl_wait();
+  pdl_launch();
 #pragma unroll
   for (int i = 0; i < NS - 1; i++) fetch();
   // The tables through their addresses: as constants, which a warp reads one address at a time, they took 4 us of 31.

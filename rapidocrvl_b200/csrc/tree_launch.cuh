@@ -41,7 +41,7 @@ int launch_tree_mma(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t 
   const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
   if (segments > 1 << 24) return invalid("too many sequences and kv heads");
   if constexpr (!SPLIT) {
-    return launch("tree attention", k_tree_mma<T, D, WIDE, false, PACKED>, dim3((unsigned)segments), kMmaThreads, S::kSmem, stream, false, 1, a, blocks);
+    return launch("tree attention", k_tree_mma<T, D, WIDE, false, PACKED>, dim3((unsigned)segments), kMmaThreads, S::kSmem, stream, PACKED, 1, a, blocks);
   } else {
     if (int rc = check_combine(a, blocks)) return rc;
     const int grid = sms < kMaxRuns ? sms : kMaxRuns;
@@ -49,7 +49,7 @@ int launch_tree_mma(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t 
     a.joint = (int4 *)work;
     a.part = (float *)(work + tree_joint_bytes(a.s.batch, a.kv_heads, rows_max));
     a.part_ml = a.part + (int64_t)grid * 2 * S::kRows * D;
-    if (int rc = launch("tree attention", k_tree_mma<T, D, WIDE, true, PACKED>, dim3(grid), kMmaThreads, S::kSmem, stream, false, 1, a, blocks)) return rc;
+    if (int rc = launch("tree attention", k_tree_mma<T, D, WIDE, true, PACKED>, dim3(grid), kMmaThreads, S::kSmem, stream, PACKED, 1, a, blocks)) return rc;
     return launch_combine<T, D>(a, sms, rows_max, S::kRows, stream);
   }
 }

@@ -281,9 +281,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) k_tree_mma(const TreeArgs a, i
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     tc_before();
   }
+  if constexpr (PACKED) pdl_wait();
   Piece cur;
   Walk walk;
   bool more = true;
+  if constexpr (PACKED && !SPLIT) pdl_launch();
   if constexpr (SPLIT) {
     more = walk.start(a, S::kRows, plan, warp, lane, cur);
     pdl_launch();
