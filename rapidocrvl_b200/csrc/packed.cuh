@@ -40,7 +40,8 @@ struct PackArgs {
 };
 
 constexpr int kPackWarps = 4, kPackThreads = kPackWarps * 32;
-constexpr int kPackRows = 4;  // steps whose loads go out together
+template <typename T>
+constexpr int kPackRows = sizeof(T) == 4 ? 2 : 4;  // steps whose loads go out together
 
 // 8 values of a row: as they lie in memory, and as 32-bit floats.
 template <typename T>
@@ -210,9 +211,10 @@ __device__ __forceinline__ uint32_t pack8(const Eight<T> &e8, int i, float *scal
   return odd ? low_halves(other, hi) : low_halves(lo, other);
 }
 
-// Stores the 8 numbers of lane i (as above) of a row whose codes' four bytes at its place are `word`, scale twice.
+// Stores the 8 numbers of lane i (as above) of a row whose codes' four bytes at its place are `word`, scale twice.  sectors: `to` is
+// 32-byte aligned, so that f32 goes out as whole sectors of memory, not as halves of them (1,497 tokens of 18 layers 18.3 us, 12.5 so).
 template <int D, typename T>
-__device__ __forceinline__ void unpack8(T *to, uint32_t word, uint32_t scale, int i, bool there) {
+__device__ __forceinline__ void unpack8(T *to, uint32_t word, uint32_t scale, int i, bool there, bool sectors) {
   using B = __nv_bfloat16;
   const bool odd = i / 4 & 1;
   const uint32_t other = __shfl_xor_sync(~0u, odd ? word : word >> 16, 4);
@@ -233,8 +235,14 @@ __device__ __forceinline__ void unpack8(T *to, uint32_t word, uint32_t scale, in
     }
     if (!there) return;
     if constexpr (sizeof(T) == 4) {
-      *(float4 *)to = make_float4(f[0], f[1], f[2], f[3]);
-      *((float4 *)to + 1) = make_float4(f[4], f[5], f[6], f[7]);
+      if (sectors) {
+        asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]),
+                     "f"(f[5]), "f"(f[6]), "f"(f[7])
+                     : "memory");
+      } else {
+        *(float4 *)to = make_float4(f[0], f[1], f[2], f[3]);
+        *((float4 *)to + 1) = make_float4(f[4], f[5], f[6], f[7]);
+      }
     } else {
       *(uint4 *)to = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
     }
@@ -280,20 +288,21 @@ __global__ void __launch_bounds__(kPackThreads) k_packed_append(const PackArgs a
       char *codes = (x.v ? a.c.v : a.c.k) + pg * a.c.page + x.layer * a.c.layer + x.head * a.c.head + in_page * (D / 2) + codes_at;
       char *scales = (x.v ? a.c.v_scale : a.c.k_scale) + pg * a.c.scale_page + x.layer * a.c.scale_layer + x.head * a.c.scale_head +
                      in_page * (D / 16) + scales_at;
+      const int first = max(0, x.len - p0) / I::ROWS, last = min(I::STEPS, (end - p0 + I::ROWS - 1) / I::ROWS);  // steps with tokens
 #pragma unroll 1
-      for (int s0 = 0; s0 < I::STEPS; s0 += kPackRows) {
-        Eight<T> y[kPackRows];
-        bool there[kPackRows];
+      for (int s0 = first; s0 < last; s0 += kPackRows<T>) {
+        Eight<T> y[kPackRows<T>];
+        bool there[kPackRows<T>];
 #pragma unroll
-        for (int r = 0; r < kPackRows; r++) {
+        for (int r = 0; r < kPackRows<T>; r++) {
           const int i = p0 - x.len + (s0 + r) * I::ROWS + sub;
-          there[r] = i >= 0 && i < n;
+          there[r] = i >= 0 && i < n && s0 + r < last;
           const int node = there[r] && a.path ? a.path[(long long)b * a.max_path + i] : i;
           there[r] = there[r] && node >= 0 && node < x.count;
           if (there[r]) y[r].load((const T *)(from + node * a.token));  // not waiting for the page
         }
 #pragma unroll
-        for (int r = 0; r < kPackRows; r++) {
+        for (int r = 0; r < kPackRows<T>; r++) {
           if (!__any_sync(~0u, there[r])) continue;
           float s;
           const uint32_t word = pack8<D>(y[r], i8, &s);
@@ -315,30 +324,38 @@ __global__ void __launch_bounds__(kPackThreads) k_packed_read(const PackArgs a) 
   pdl_launch();
   I x(a, b);
   if (x.count == 0) return;
+  const bool sectors = (((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.token | (uintptr_t)a.layer) & 31) == 0;
   const int codes_at = sub * (D / 2) + place<D>(i8), scales_at = sub * (D / 16) + i8 / 4 * 2;
   for (int c = blockIdx.z * kPackWarps + (threadIdx.x >> 5); x.at(a, c); c += gridDim.z * kPackWarps) {
     char *to = (x.v ? a.v : a.k) + x.layer * a.layer + x.first * a.token + (x.head * D + i8 * 8) * (long long)sizeof(T);
     const int skip = x.len % kChunk, chunks = (int)(((long long)skip + x.count + kChunk - 1) / kChunk);
-    for (int ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
+    const char *codes0 = (x.v ? a.c.v : a.c.k) + x.layer * a.c.layer + x.head * a.c.head + codes_at;
+    const char *scales0 = (x.v ? a.c.v_scale : a.c.k_scale) + x.layer * a.c.scale_layer + x.head * a.c.scale_head + scales_at;
+    uint32_t word_next[I::STEPS], s_next[I::STEPS];  // of the chunk after the one that is stored
+    auto fetch = [&](int ch) {
       const long long p0 = (x.len / kChunk + (long long)ch) * kChunk;
       const int pg = p0 < a.capacity ? a.c.page_of(b, (int)p0) : -1, in_page = (int)p0 & ((1 << a.c.shift) - 1);
-      const char *codes = (x.v ? a.c.v : a.c.k) + pg * a.c.page + x.layer * a.c.layer + x.head * a.c.head + in_page * (D / 2) + codes_at;
-      const char *scales = (x.v ? a.c.v_scale : a.c.k_scale) + pg * a.c.scale_page + x.layer * a.c.scale_layer + x.head * a.c.scale_head +
-                           in_page * (D / 16) + scales_at;
-      const int i0 = (int)((long long)ch * kChunk - skip);
-      uint32_t word[I::STEPS], s[I::STEPS];
+      const char *codes = codes0 + pg * a.c.page + in_page * (D / 2), *scales = scales0 + pg * a.c.scale_page + in_page * (D / 16);
 #pragma unroll
       for (int r = 0; r < I::STEPS; r++) {
-        word[r] = 0x88888888u, s[r] = 0;
+        word_next[r] = 0x88888888u, s_next[r] = 0;
         if (pg >= 0) {  // the page holds the whole chunk
-          word[r] = __ldg((const uint32_t *)(codes + r * (I::ROWS * D / 2)));
-          s[r] = __ldg((const uint16_t *)(scales + r * (I::ROWS * D / 16)));
+          word_next[r] = __ldg((const uint32_t *)(codes + r * (I::ROWS * D / 2)));
+          s_next[r] = __ldg((const uint16_t *)(scales + r * (I::ROWS * D / 16)));
         }
       }
+    };
+    if ((int)blockIdx.x < chunks) fetch(blockIdx.x);
+    for (int ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
+      uint32_t word[I::STEPS], s[I::STEPS];
+#pragma unroll
+      for (int r = 0; r < I::STEPS; r++) word[r] = word_next[r], s[r] = s_next[r];
+      if (ch + gridDim.x < chunks) fetch(ch + gridDim.x);
+      const int i0 = (int)((long long)ch * kChunk - skip);
 #pragma unroll
       for (int r = 0; r < I::STEPS; r++) {
         const int i = i0 + r * I::ROWS + sub;
-        unpack8<D>((T *)(to + i * a.token), word[r], __byte_perm(s[r], 0, 0x1010), i8, i >= 0 && i < x.count);
+        unpack8<D>((T *)(to + i * a.token), word[r], __byte_perm(s[r], 0, 0x1010), i8, i >= 0 && i < x.count, sectors);
       }
     }
   }

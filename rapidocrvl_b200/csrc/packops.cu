@@ -49,15 +49,17 @@ PackArgs pack_args(const ocrvl_packed_cache *c, int type, int n_tokens, const in
   return a;
 }
 
-// A warp 16 positions of a (layer, K or V, head); as many blocks as the longest sequence can use, or some waves of them.
-int move_grid(const PackArgs &a, int most_tokens, dim3 *grid) {
+// A warp 16 positions of a (layer, K or V, head) at a time; as many blocks as twice an even share of the tokens can use (a
+// sequence has `most_tokens` at most, all have n_tokens), or the GPU holds `waves` times.
+int move_grid(const PackArgs &a, int most_tokens, int waves, dim3 *grid) {
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const long long rows = 2ll * a.layers * a.kv_heads;
   if (rows > 1 << 30) return invalid("too many layers and kv heads");
   const long long z = (rows + kPackWarps - 1) / kPackWarps < 1024 ? (rows + kPackWarps - 1) / kPackWarps : 1024;
-  const long long chunks = (long long)most_tokens / kChunk + 2, most = (sms * 64 + a.batch * z - 1) / (a.batch * z);
-  *grid = dim3((unsigned)(chunks < most ? chunks : most), a.batch, (unsigned)z);
+  const long long chunks = (long long)most_tokens / kChunk + 2, even = 2 * ((long long)a.n_tokens / a.batch / kChunk + 1);
+  const long long most = (sms * 8 * waves + a.batch * z - 1) / (a.batch * z), x = chunks < even ? chunks : even;
+  *grid = dim3((unsigned)(x < most ? x : most), a.batch, (unsigned)z);
   return OCRVL_OK;
 }
 
@@ -102,7 +104,7 @@ int ocrvl_op_packed_append(const ocrvl_packed_cache *c, int type, int n_tokens, 
   PackArgs a = pack_args(c, type, n_tokens, lens, indptr, k, v, kv_stride, kv_layer_stride);
   a.path = path, a.n_path = n_path, a.max_path = max_path, a.new_lens = new_lens;
   dim3 grid;
-  if (int rc = move_grid(a, path ? max_path : n_tokens, &grid)) return rc;
+  if (int rc = move_grid(a, path ? max_path : n_tokens, 8, &grid)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto wide, auto narrow) {
     return launch("append, packed", c->head_dim == 128 ? wide : narrow, grid, kPackThreads, 0, st, true, 1, a);
@@ -118,7 +120,7 @@ int ocrvl_op_packed_read(const ocrvl_packed_cache *c, int type, int n_tokens, co
   if (n_tokens == 0) return OCRVL_OK;
   const PackArgs a = pack_args(c, type, n_tokens, lens, indptr, k, v, kv_stride, kv_layer_stride);
   dim3 grid;
-  if (int rc = move_grid(a, n_tokens, &grid)) return rc;
+  if (int rc = move_grid(a, n_tokens, 4, &grid)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto wide, auto narrow) {
     return launch("read, packed", c->head_dim == 128 ? wide : narrow, grid, kPackThreads, 0, st, true, 1, a);
