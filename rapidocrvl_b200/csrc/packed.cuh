@@ -144,8 +144,8 @@ __device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return 
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
 __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, int high) { return high ? high_halves(a, b) : low_halves(a, b); }
 
-// x / y correctly rounded, for y's reciprocal correctly rounded and a quotient of ordinary size: the first quotient's
-// rest is exact in one fused step, and what the second adds is off by 2^-47 of the whole.
+// x / y correctly rounded but for its last 2^-45, for y's reciprocal to 2^-22 and a quotient of ordinary size: the first
+// quotient's rest is exact in one fused step, and what the second adds is off by 2^-22 of itself.
 __device__ __forceinline__ float quotient(float x, float y, float reciprocal) {
   const float q = x * reciprocal;
   return fmaf(fmaf(-q, y, x), reciprocal, q);
@@ -192,8 +192,10 @@ __device__ __forceinline__ uint32_t pack8(const Eight<T> &e8, int i, float *scal
     most = __float_as_uint(unpack2<T>(one).x);
   }
   const float s = finite ? group_scale(__uint_as_float(most)) : 0.f;
-  // s has five bits and is no less than 2^-126 or 0: an ordinary reciprocal.
-  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  // s is 2^-126 to 2^126, or 0: its reciprocal is an ordinary number
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  inv = s > 0.f ? inv : 0.f;
   uint32_t c[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
