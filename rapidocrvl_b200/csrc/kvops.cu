@@ -111,7 +111,7 @@ int launch_tree_rows(const TreeArgs &a, int sms, int rows_max, char *work, cudaS
   if constexpr (sizeof(T) == 4)
     return launch_tree<T, D, 4>(a, sms, rows_max, work, stream);
   else
-    return launch_tree_mma_shape<T, D, false>(a, sms, rows_max, work, stream);
+    return launch_tree_mma_shape<T, D>(a, sms, rows_max, work, stream);
 }
 
 template <typename T>

@@ -293,7 +293,7 @@ template <typename T, int D, int NT>
 struct PackShape {
   using L = PackTile<T, D>;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kBlocks = NT == 1 || (sizeof(T) == 2 && NT == 2) ? 2 : 1;  // an SM
+  static constexpr int kBlocks = NT == 1 ? 2 : 1;  // an SM
   static constexpr int kStages = kBlocks == 2 ? 4 : 6;  // chunks of a warp on their way or in use
   static constexpr int kRing = kTreeWarps * kStages * L::kStage;
   static constexpr int kJoin = kTreeWarps * 8 * D * 4;  // eight rows of every warp

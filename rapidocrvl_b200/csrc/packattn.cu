@@ -12,30 +12,52 @@ using namespace ocrvl::paged;
 
 namespace {
 
+// What a call would take, in us, by the kernel's shape; all that the host knows of the lengths is the table's width.
+//   8 NT rows a block, clusters of cs blocks a segment: tiles / cs at `tile` each (8 warps, a chunk each; no less than 0.85,
+//     the latency of a chunk), as often as the blocks are waves of the SMs, drafts at `draft` a position of a warp, and 10
+//     for launch, start and join
+//   runs (cs 0): all tiles over all SMs, and 22, with the search for a run's start, the parts and their join
+//   the fifth generation's products, 128 or 256 rows: 2.7 (f16 3.6) or 4.4 a tile, mostly the time of the warps that
+//     unpack it, and 8, or 24 and 45 in runs
+// Measured (bf16, 16 / 2 heads of 128, up to 4,096 positions, 37 sequences of one, two and four tokens; NT 1, 2, 4): 23.6,
+// 35.8 and 60.4 us; 39.3, 27.0 and 45.3; 39.5, 39.2 and 42.0; fifth generation 92.  40 of up to 6,000, 12 tokens (96
+// rows): 119.7, 86.9, 91.7; 135.5.  32 / 8 heads of 64, 103,991 positions, 5 tokens, runs: 74, 76, 60; clusters of eight
+// with NT 1: 100.  f32, 5 of 95 with 50 drafts: 17.4, 19.5, 32.8.
+struct Shape {
+  double us;
+  int nt, cs;
+};
+
 template <typename T, int D, int NT>
-int launch_pack(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stream) {
+Shape shape_of(const TreeArgs &a, int sms, int rows_max) {
+  constexpr double wide = sizeof(T) == 4 ? (NT == 1 ? 1.0 : NT == 2 ? 1.6 : 3.0) : (NT == 1 ? 0.75 : NT == 2 ? 1.0 : 1.9);
+  constexpr double tile = wide * (D == 64 ? 0.55 : 1), alone = tile > 0.85 ? tile : 0.85;
+  constexpr double draft = (sizeof(T) == 4 ? 0.4 : 0.25) * NT;
+  const int blocks_an_sm = PackShape<T, D, NT>::kBlocks, tiles = tree_tiles(a);
+  const double segments = (double)((rows_max + 8 * NT - 1) / (8 * NT)) * a.kv_heads * a.s.batch;
+  int cs = 1;
+  while (cs < 8 && cs < tiles && segments * cs * 2 <= (cs == 1 ? sms : cluster_room(sms)) * blocks_an_sm) cs *= 2;
+  const double drafts = (a.s.max_draft + 8 * cs - 1) / (8 * cs) * draft, waves = segments * cs / sms;
+  const double whole = (waves < 1 ? 1 : waves) * ((tiles + cs - 1) / cs * (waves < 2 ? alone : tile) + drafts) + 10, runs = segments * tiles / sms * tile + drafts + 22;
+  return whole <= runs ? Shape{whole, NT, cs} : Shape{runs, NT, 0};
+}
+
+template <typename T, int D, int NT>
+int launch_pack(TreeArgs a, const Shape &shape, int sms, int rows_max, char *work, cudaStream_t stream) {
   using S = PackShape<T, D, NT>;
   const int blocks = (rows_max + S::kRows - 1) / S::kRows;
   const long long segments = (long long)blocks * a.kv_heads * a.s.batch;
   if (segments > 1 << 24) return invalid("too many sequences and kv heads");
-  // Blocks (in clusters) a segment, as many as run at once; or equal runs of tiles over all blocks and a second launch
-  // that joins them, where a warp then has so many fewer chunks (of the longest cache, which is all that the host knows) that
-  // it makes up for the search, the parts and the join.
-  constexpr int kRunsCost = 16;  // chunks
-  const int tiles = tree_tiles(a);
-  const long long room = (long long)sms * S::kBlocks;
-  auto one = [&](auto kernel, int cs) {
-    return launch("packed attention", kernel, dim3((unsigned)(segments * cs)), kTreeThreads, S::kSmem, stream, !a.longest_first, cs, a, blocks);
-  };
-  int cs = 1;
-  while (cs < 8 && cs < tiles && segments * cs * 2 <= (cs == 1 ? room : (long long)cluster_room(sms) * S::kBlocks)) cs *= 2;
-  const double whole = (double)((tiles + cs - 1) / cs) * ((segments * cs + room - 1) / room), runs = (double)segments * tiles / room;
-  // Where an SM gets more than one block, in the order of lengths; then not ahead of the kernel before (which would hand
-  // blocks out where that one ends first, several of the longest to an SM: 64 bf16 sequences of up to 4,096 27.6 us, 31.4 so).
-  a.longest_first = a.s.batch > 1 && a.s.batch <= kTreeThreads && segments * cs > sms;
-  if (whole <= runs + kRunsCost)
-    return cs == 8 ? one(k_pack_attn<T, D, NT, 8>, 8) : cs == 4 ? one(k_pack_attn<T, D, NT, 4>, 4) : cs == 2 ? one(k_pack_attn<T, D, NT, 2>, 2) : one(k_pack_attn<T, D, NT, 1>, 1);
-
+  const int cs = shape.cs;
+  if (cs) {
+    // Where an SM gets more than one block, in the order of lengths; then not ahead of the kernel before (which would hand
+    // blocks out where that one ends first, several of the longest to an SM: 64 bf16 sequences of up to 4,096 27.6 us, 31.4 so).
+    a.longest_first = a.s.batch > 1 && a.s.batch <= kTreeThreads && segments * cs > sms;
+    auto go = [&](auto kernel) {
+      return launch("packed attention", kernel, dim3((unsigned)(segments * cs)), kTreeThreads, S::kSmem, stream, !a.longest_first, cs, a, blocks);
+    };
+    return cs == 8 ? go(k_pack_attn<T, D, NT, 8>) : cs == 4 ? go(k_pack_attn<T, D, NT, 4>) : cs == 2 ? go(k_pack_attn<T, D, NT, 2>) : go(k_pack_attn<T, D, NT, 1>);
+  }
   if (int rc = check_combine(a, blocks)) return rc;
   const int grid = sms * S::kBlocks < kMaxRuns ? sms * S::kBlocks : kMaxRuns;
   a.start_cost = 1;
@@ -46,18 +68,34 @@ int launch_pack(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t stre
   return launch_combine<T, D>(a, sms, rows_max, S::kRows, stream);
 }
 
-// Rows a block, as for a plain cache: eight or sixteen where there are no more, or where the call's tiles are so few that
-// the GPU is not filled otherwise; else 32 for f32, and the fifth generation's products for 16 bits.
 template <typename T, int D>
 int launch_pack_rows(const TreeArgs &a, int sms, int rows_max, char *work, cudaStream_t stream) {
-  const int room = sizeof(T) == 4 ? sms : 2 * sms;  // blocks that run at once
-  auto few = [&](int rows) { return (long long)((rows_max + rows - 1) / rows) * a.kv_heads * a.s.batch * tree_tiles(a) * 2 <= 3 * room; };
-  if (rows_max <= 8 || few(8)) return launch_pack<T, D, 1>(a, sms, rows_max, work, stream);
-  if (rows_max <= 16 || few(16)) return launch_pack<T, D, 2>(a, sms, rows_max, work, stream);
-  if constexpr (sizeof(T) == 4)
-    return launch_pack<T, D, 4>(a, sms, rows_max, work, stream);
-  else
-    return launch_tree_mma_shape<T, D, true>(a, sms, rows_max, work, stream);
+  Shape best = shape_of<T, D, 1>(a, sms, rows_max);
+  if (rows_max > 8) {
+    const Shape two = shape_of<T, D, 2>(a, sms, rows_max), four = shape_of<T, D, 4>(a, sms, rows_max);
+    if (two.us < best.us) best = two;
+    if (rows_max > 16 && four.us < best.us) best = four;
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (rows_max > 16) {  // the workspace of fewer rows has no room for the parts of these
+      const double tiles = tree_tiles(a), heads = (double)a.kv_heads * a.s.batch, unit = D == 64 ? 0.67 : 1;
+      const double narrow = (rows_max + 127) / 128 * heads, wide = (rows_max + 255) / 256 * heads;  // segments
+      const double few = std::is_same<T, __half>::value ? 3.6 : 2.7;
+      const double t[4] = {std::ceil(narrow / sms) * tiles * few * unit + 8, narrow * tiles / sms * few * unit + 24,
+                           std::ceil(wide / sms) * tiles * 4.4 * unit + 8, wide * tiles / sms * 4.4 * unit + 45};
+      int i = 0;
+      for (int j = 1; j < (rows_max > 128 ? 4 : 2); j++)
+        if (t[j] < t[i]) i = j;
+      if (t[i] < best.us)
+        return i == 0   ? launch_tree_mma<T, D, false, false, true>(a, sms, rows_max, work, stream)
+               : i == 1 ? launch_tree_mma<T, D, false, true, true>(a, sms, rows_max, work, stream)
+               : i == 2 ? launch_tree_mma<T, D, true, false, true>(a, sms, rows_max, work, stream)
+                        : launch_tree_mma<T, D, true, true, true>(a, sms, rows_max, work, stream);
+    }
+  }
+  if (best.nt == 4) return launch_pack<T, D, 4>(a, best, sms, rows_max, work, stream);
+  if (best.nt == 2) return launch_pack<T, D, 2>(a, best, sms, rows_max, work, stream);
+  return launch_pack<T, D, 1>(a, best, sms, rows_max, work, stream);
 }
 
 template <typename T>

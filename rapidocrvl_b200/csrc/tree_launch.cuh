@@ -62,18 +62,18 @@ int launch_tree_mma(TreeArgs a, int sms, int rows_max, char *work, cudaStream_t 
 // memory: 13 and 0.15 a segment, 21 and 0.3 with 256 rows.  16 sequences of 8,000, 64 drafts
 // of 8 heads: 95 us a block a segment of 128 rows, 160 of 256, 130 and 123 in runs; one of
 // 131,072: 1178, 2274, 120 and 108.
-template <typename T, int D, bool PACKED>
+template <typename T, int D>
 int launch_tree_mma_shape(const TreeArgs &a, int sms, int rows_max, char *work, cudaStream_t stream) {
   const double tiles = tree_tiles(a), heads = (double)a.kv_heads * a.s.batch;
   const double narrow = (rows_max + 127) / 128 * heads, wide = (rows_max + 255) / 256 * heads;  // segments
   const double narrow_whole = std::ceil(narrow / sms) * (tiles + 6), wide_whole = std::ceil(wide / sms) * 2 * (tiles + 2);
   const double narrow_runs = narrow * tiles / sms * 4 / 3 + 13 + 0.15 * narrow, wide_runs = wide * tiles / sms * 2 + 21 + 0.3 * wide;
   if (rows_max <= 128)
-    return narrow_whole <= narrow_runs ? launch_tree_mma<T, D, false, false, PACKED>(a, sms, rows_max, work, stream)
-                                       : launch_tree_mma<T, D, false, true, PACKED>(a, sms, rows_max, work, stream);
-  if (narrow_whole <= wide_whole && narrow_whole <= wide_runs) return launch_tree_mma<T, D, false, false, PACKED>(a, sms, rows_max, work, stream);
-  return wide_whole <= wide_runs ? launch_tree_mma<T, D, true, false, PACKED>(a, sms, rows_max, work, stream)
-                                 : launch_tree_mma<T, D, true, true, PACKED>(a, sms, rows_max, work, stream);
+    return narrow_whole <= narrow_runs ? launch_tree_mma<T, D, false, false, false>(a, sms, rows_max, work, stream)
+                                       : launch_tree_mma<T, D, false, true, false>(a, sms, rows_max, work, stream);
+  if (narrow_whole <= wide_whole && narrow_whole <= wide_runs) return launch_tree_mma<T, D, false, false, false>(a, sms, rows_max, work, stream);
+  return wide_whole <= wide_runs ? launch_tree_mma<T, D, true, false, false>(a, sms, rows_max, work, stream)
+                                 : launch_tree_mma<T, D, true, true, false>(a, sms, rows_max, work, stream);
 }
 
 }  // namespace paged
