@@ -473,9 +473,10 @@ int ocrvl_op_packed_read(const ocrvl_packed_cache *c, int type, int n_tokens, co
                          void *k, void *v, int64_t kv_stride, int64_t kv_layer_stride, void *stream);
 
 /* ocrvl_op_tree_attn over a packed cache: q, k, v and out are of `type`, all else is as there.
- * f32: codes meet all 24 bits of q and of the softmax weights.  bf16: c s is taken as it is; f16: rounded to
- * f16 (an infinity past its range), exact from 2^-14 on for caches written from f16.  With more than 16 rows (tokens
- * times heads a kv head) of a 16-bit type keys are taken like values, with fewer not rounded. */
+ * c s is taken as it is by f32 and bf16.  By f16 it is rounded to f16 for values, and for keys too where there are
+ * many rows (no rounding from 2^-14 on for what was written from f16; an infinity past f16's range).  f32 products keep 22 bits
+ * of a query and all of a softmax weight; the drafts' part is plain 32-bit arithmetic where there are few rows.  A scale that is
+ * NaN makes every row NaN that sees the key, or 32 dims of every row that sees the value. */
 int ocrvl_op_packed_attn_workspace(const ocrvl_packed_cache *c, int type, int heads, int max_draft, int64_t *bytes);
 int ocrvl_op_packed_attn(const ocrvl_packed_cache *c, int type, int layer, int heads, int n_tokens, int max_draft,
                          const int32_t *lens, const int32_t *indptr, const int64_t *mask, const void *q, int64_t q_stride,

@@ -14,15 +14,16 @@ namespace {
 
 // What a call would take, in us, by the kernel's shape; all that the host knows of the lengths is the table's width.
 //   8 NT rows a block, clusters of cs blocks a segment: tiles / cs at `tile` each (8 warps, a chunk each; no less than 0.85,
-//     the latency of a chunk), as often as the blocks are waves of the SMs, drafts at `draft` a position of a warp, and 10
+//     the latency of a chunk), as often as the blocks are waves of the SMs (of mean length), drafts at `draft` a position of a warp, and 10
 //     for launch, start and join
 //   runs (cs 0): all tiles over all SMs, and 22, with the search for a run's start, the parts and their join
-//   the fifth generation's products, 128 or 256 rows: 2.7 (f16 3.6) or 4.4 a tile, mostly the time of the warps that
-//     unpack it, and 8, or 24 and 45 in runs
+//   the fifth generation's products, 128 or 256 rows: 2.7 (3.6 in runs) or 4.4 a tile, mostly the time of the warps that
+//     unpack it, and 8, or 24 and 55 in runs
 // Measured (bf16, 16 / 2 heads of 128, up to 4,096 positions, 37 sequences of one, two and four tokens; NT 1, 2, 4): 23.6,
 // 35.8 and 60.4 us; 39.3, 27.0 and 45.3; 39.5, 39.2 and 42.0; fifth generation 92.  40 of up to 6,000, 12 tokens (96
 // rows): 119.7, 86.9, 91.7; 135.5.  32 / 8 heads of 64, 103,991 positions, 5 tokens, runs: 74, 76, 60; clusters of eight
 // with NT 1: 100.  f32, 5 of 95 with 50 drafts: 17.4, 19.5, 32.8.
+constexpr double kMean = 0.75;  // of the lengths, over the longest: between equal and evenly spread ones
 struct Shape {
   double us;
   int nt, cs;
@@ -38,7 +39,8 @@ Shape shape_of(const TreeArgs &a, int sms, int rows_max) {
   int cs = 1;
   while (cs < 8 && cs < tiles && segments * cs * 2 <= (cs == 1 ? sms : cluster_room(sms)) * blocks_an_sm) cs *= 2;
   const double drafts = (a.s.max_draft + 8 * cs - 1) / (8 * cs) * draft, waves = segments * cs / sms;
-  const double whole = (waves < 1 ? 1 : waves) * ((tiles + cs - 1) / cs * (waves < 2 ? alone : tile) + drafts) + 10, runs = segments * tiles / sms * tile + drafts + 22;
+  const double whole = std::fmax(1, waves * kMean) * ((tiles + cs - 1) / cs * (waves < 2 ? alone : tile) + drafts) + 10;
+  const double runs = segments * tiles / sms * tile * kMean + drafts + 22;
   return whole <= runs ? Shape{whole, NT, cs} : Shape{runs, NT, 0};
 }
 
@@ -80,9 +82,9 @@ int launch_pack_rows(const TreeArgs &a, int sms, int rows_max, char *work, cudaS
     if (rows_max > 16) {  // the workspace of fewer rows has no room for the parts of these
       const double tiles = tree_tiles(a), heads = (double)a.kv_heads * a.s.batch, unit = D == 64 ? 0.67 : 1;
       const double narrow = (rows_max + 127) / 128 * heads, wide = (rows_max + 255) / 256 * heads;  // segments
-      const double few = std::is_same<T, __half>::value ? 3.6 : 2.7;
-      const double t[4] = {std::ceil(narrow / sms) * tiles * few * unit + 8, narrow * tiles / sms * few * unit + 24,
-                           std::ceil(wide / sms) * tiles * 4.4 * unit + 8, wide * tiles / sms * 4.4 * unit + 45};
+      auto waves = [&](double n) { return n <= sms ? 1. : std::fmax(1, (std::ceil(n / sms) + n / sms) / 2 * kMean); };
+      const double t[4] = {waves(narrow) * tiles * 2.7 * unit + 8, narrow * tiles / sms * 3.6 * unit * kMean + 24,
+                           waves(wide) * tiles * 4.4 * unit + 8, wide * tiles / sms * 4.4 * unit * kMean + 55};
       int i = 0;
       for (int j = 1; j < (rows_max > 128 ? 4 : 2); j++)
         if (t[j] < t[i]) i = j;

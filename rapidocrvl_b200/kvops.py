@@ -126,13 +126,15 @@ class PackedCache:
         self.head_dim, self.kv_heads, self.layers, self.batch = 2 * half, heads, layers, table.shape[0]
         self.capacity = table.shape[1] * page
 
-    def work_bytes(self, heads: int, max_draft: int = 64, dtype: torch.dtype = torch.float32) -> int:
-        """Bytes of workspace a ``tree_attention`` call with that many query heads of ``dtype`` takes."""
-        if dtype not in _TYPES:
+    def work_bytes(self, heads: int, max_draft: int = 64, dtype: Optional[torch.dtype] = None) -> int:
+        """Bytes of workspace a ``tree_attention`` call with that many query heads (of ``dtype``, or of any type) takes."""
+        if dtype is not None and dtype not in _TYPES:
             raise ValueError("dtype must be float32, float16 or bfloat16")
-        n = C.c_int64()
-        _lib.check(_lib.load().ocrvl_op_packed_attn_workspace(C.byref(self.desc), _TYPES[dtype], heads, max_draft, C.byref(n)))
-        return n.value
+        n, most = C.c_int64(), 0
+        for t in _TYPES.values() if dtype is None else (_TYPES[dtype],):
+            _lib.check(_lib.load().ocrvl_op_packed_attn_workspace(C.byref(self.desc), t, heads, max_draft, C.byref(n)))
+            most = max(most, n.value)
+        return most
 
     @classmethod
     def empty(cls, pages: int, layers: int, kv_heads: int, head_dim: int, table: torch.Tensor, *, page_size: int = 16) -> "PackedCache":
@@ -167,6 +169,8 @@ class Rotary:
         axes = len(sections) if sections is not None else max(axis, default=0) + 1
         if len(axis) != pairs or not 1 <= axes <= 8 or min(axis) < 0 or (sections is not None and min(sections) < 0):
             raise ValueError(f"sections (or axis) must say which of at most 8 axes each of the {pairs} pairs has")
+        if freq is None and not (theta > 0 and math.isfinite(theta)):
+            raise ValueError("theta must be positive")
         freq = [float(theta) ** (-p / pairs) for p in range(pairs)] if freq is None else [float(f) for f in freq]
         if len(freq) != pairs or not all(map(math.isfinite, freq)):
             raise ValueError(f"freq must be {pairs} finite numbers")

@@ -109,6 +109,57 @@ def test_many_rows(kvops, shape, dtype, dim):
     s.ok(s.run(kvops, max_draft=most))
 
 
+# Rows a kv head 6 to 96, a few short caches to many and long ones: blocks of 8, 16 and 32 rows, one and several a segment, clusters of
+# one to eight, runs, and the fifth generation's products, each with drafts in one block and in several.
+SHAPES = [([300], [3]), ([300] * 5, [2] * 5), ([1500] * 9, [1] * 9), ([700] * 40, [1 + b % 4 for b in range(40)]), ([9000, 20], [4, 4]), ([20000], [2]), ([20000], [3]),
+          ([30, 2900] * 10, [12, 1] * 10), ([2500] * 20, [4] * 20), ([(251 * b) % 1200 for b in range(90)], [b % 3 for b in range(90)]), ([6000] * 3, [12, 7, 0])]
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("f16", 128), ("f32", 128), ("f32", 64)])
+@pytest.mark.parametrize("lens,counts", SHAPES)
+def test_shapes(kvops, lens, counts, dtype, dim):
+    s = Packed(kvops, dtype, lens, counts, dim=dim, seed=33)
+    s.ok(s.run(kvops, max_draft=max(counts)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_calls_behind_one_another_without_a_wait(kvops, dtype):
+    """A launch may begin before the one before it ends: it has to wait for what that one writes, and for what it reads."""
+    t, g = TYPES[dtype], torch.Generator().manual_seed(9)
+    rot = kvops.Rotary(128, sections=(32, 32))
+    x = torch.randn(40, 8 + 2 * 2, 128, generator=g).to(t).cuda()
+    pos = torch.randint(0, 500, (40, 2), generator=g, dtype=torch.int32).cuda()
+    q, k, v = x[:, :8], x[:, 8:10], x[:, 10:]
+    mask, indptr = masks([1 << i | 1 for b in range(4) for i in range(10)]), ints([0, 10, 20, 30, 40])
+
+    def steps(wait):
+        cache = kvops.PackedCache.empty(4 * 30, 1, 2, 128, torch.arange(120, dtype=torch.int32, device="cuda").view(4, 30))
+        lens, out, y = ints([0, 3, 17, 40]), [], x.clone()
+        q, k, v = y[:, :8], y[:, 8:10], y[:, 10:]
+        for i in range(30):
+            kvops.rotate(q, k, pos, rot, q_out=q, k_out=k)
+            if wait:
+                torch.cuda.synchronize()
+            o, lse = kvops.tree_attention(q, k, v, cache, lens, indptr, mask, max_draft=10)
+            if wait:
+                torch.cuda.synchronize()
+            new = kvops.append(cache, k[None], v[None], lens, indptr)
+            if wait:
+                torch.cuda.synchronize()
+            kk, vv = kvops.read(cache, lens, indptr, 40, dtype=t)
+            if wait:
+                torch.cuda.synchronize()
+            k.copy_(kk[0]), v.copy_(o[:, ::4])
+            lens = new
+            out += [o, lse, kk, vv, new]
+        torch.cuda.synchronize()
+        return out
+
+    a = steps(True)
+    for _ in range(3):
+        assert all(torch.equal(m, n) for m, n in zip(a, steps(False)))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_second_layer_strides_and_one_pool(kvops, dtype):
     s = Packed(kvops, dtype, [50, 33], [3, 9], layers=3, seed=8, one_pool=True)
@@ -453,4 +504,4 @@ def test_refusals(kvops):
         kvops.attention_mass(s.q, torch.zeros(3, 16, device="cuda"), s.cache, s.lens, s.indptr)
     with pytest.raises(ValueError):
         s.cache.work_bytes(16, 1, torch.int8)
-    assert s.cache.work_bytes(16, 1, torch.bfloat16) > 0
+    assert s.cache.work_bytes(16, 20) == max(s.cache.work_bytes(16, 20, t) for t in TYPES.values()) > 0

@@ -169,6 +169,7 @@ def test_refusals(kvops):
     for bad in (lambda: kvops.Rotary(100), lambda: kvops.Rotary(264), lambda: kvops.Rotary(64, pairs=36), lambda: kvops.Rotary(64, pairs=6), lambda: kvops.Rotary(64, sections=(16, 24)),
                 lambda: kvops.Rotary(64, sections=(16, 24, -8)), lambda: kvops.Rotary(64, axis=[0] * 31), lambda: kvops.Rotary(64, axis=[-1] * 32), lambda: kvops.Rotary(64, axis=[8] * 32),
                 lambda: kvops.Rotary(64, freq=[1.0]), lambda: kvops.Rotary(64, freq=[math.inf] * 32), lambda: kvops.Rotary(64, sections=(32,), axis=[0] * 32),
+                lambda: kvops.Rotary(64, theta=0), lambda: kvops.Rotary(64, theta=-2.0), lambda: kvops.Rotary(64, theta=math.nan),
                 lambda: kvops.rotate(q, k, pos, None), lambda: kvops.rotate(q.cpu(), k, pos, rot), lambda: kvops.rotate(q, k.cpu(), pos, rot), lambda: kvops.rotate(q, k.float(), pos, rot),
                 lambda: kvops.rotate(q.int(), k, pos, rot), lambda: kvops.rotate(qkv, k, pos, rot), lambda: kvops.rotate(q, k[:3], pos, rot), lambda: kvops.rotate(q, k, pos.long(), rot),
                 lambda: kvops.rotate(q, k, pos[:3], rot), lambda: kvops.rotate(q, k, pos.expand(4, 2), rot), lambda: kvops.rotate(q, k, pos.cpu(), rot),
