@@ -9,6 +9,9 @@
 // with the tokens that follow it.  It works out a token's cosines and sines once, two a lane, then takes a row with a lane
 // for 2 V dims, two numbers an instruction.  The angle is a 64-bit product of turns, whose whole part is dropped before
 // it becomes 32 bits, so far positions keep their last bits.
+//
+// 9,928 bf16 tokens of 16 + 2 heads of 128, normed: 23.9 us, 3.8 TB/s, where a plain copy of them takes 17.5; 1,200 warp
+// instructions a token.  Rows loaded into registers, one number an instruction: 30.5; the ring and pairs of numbers made it 25.1.  4,900 f16 patches of 16 + 16 heads of 72: 13.5 us.  One token: 5.8 us, a launch and two loads.
 #pragma once
 #include "packed.cuh"
 
