@@ -389,7 +389,8 @@ __global__ void __launch_bounds__(kTreeThreads, (PackShape<T, D, NT>::kBlocks)) 
   auto issue = [&](const WarpPiece &x, int nc, int k) {
     if (k < nc) {
       if ((k & 31) == 0) {
-        const int c = x.c0 + (k + lane) * x.step, pos = c * kChunk, in_page = pos & ((1 << a.c.page_shift) - 1);
+        const int c = x.c0 + (k + lane) * x.step, pos = c * kChunk;
+        const long long in_page = pos & ((1 << a.c.page_shift) - 1);
         const int pg = c < x.sg.chunks_c ? a.c.table[x.b * a.c.table_stride + (pos >> a.c.page_shift)] : -1;
         const bool mapped = pg >= 0 && pg < a.c.num_pages;
         codes_at = mapped ? pg * a.c.page_bytes + in_page * (D / 2) : -1;

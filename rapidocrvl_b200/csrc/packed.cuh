@@ -292,7 +292,8 @@ __global__ void __launch_bounds__(kPackThreads) k_packed_append(const PackArgs a
   for (int c = blockIdx.z * kPackWarps + (threadIdx.x >> 5); x.at(a, c); c += gridDim.z * kPackWarps) {
     const char *from = (x.v ? a.v : a.k) + x.layer * a.layer + x.first * a.token + (x.head * D + i8 * 8) * (long long)sizeof(T);
     for (int p0 = (x.len / kChunk + blockIdx.x) * kChunk; p0 < end; p0 += gridDim.x * kChunk) {
-      const int pg = a.c.page_of(b, p0), in_page = p0 & ((1 << a.c.shift) - 1);
+      const int pg = a.c.page_of(b, p0);
+      const long long in_page = p0 & ((1 << a.c.shift) - 1);
       char *codes = (x.v ? a.c.v : a.c.k) + pg * a.c.page + x.layer * a.c.layer + x.head * a.c.head + in_page * (D / 2) + codes_at;
       char *scales = (x.v ? a.c.v_scale : a.c.k_scale) + pg * a.c.scale_page + x.layer * a.c.scale_layer + x.head * a.c.scale_head +
                      in_page * (D / 16) + scales_at;
@@ -342,7 +343,8 @@ __global__ void __launch_bounds__(kPackThreads) k_packed_read(const PackArgs a) 
     uint32_t word_next[I::STEPS], s_next[I::STEPS];  // of the chunk after the one that is stored
     auto fetch = [&](int ch) {
       const long long p0 = (x.len / kChunk + (long long)ch) * kChunk;
-      const int pg = p0 < a.capacity ? a.c.page_of(b, (int)p0) : -1, in_page = (int)p0 & ((1 << a.c.shift) - 1);
+      const int pg = p0 < a.capacity ? a.c.page_of(b, (int)p0) : -1;
+      const long long in_page = p0 & ((1 << a.c.shift) - 1);
       const char *codes = codes0 + pg * a.c.page + in_page * (D / 2), *scales = scales0 + pg * a.c.scale_page + in_page * (D / 16);
 #pragma unroll
       for (int r = 0; r < I::STEPS; r++) {

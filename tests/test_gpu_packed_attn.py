@@ -505,3 +505,38 @@ def test_refusals(kvops):
     with pytest.raises(ValueError):
         s.cache.work_bytes(16, 1, torch.int8)
     assert s.cache.work_bytes(16, 20) == max(s.cache.work_bytes(16, 20, t) for t in TYPES.values()) > 0
+
+
+@pytest.mark.parametrize("name,drafts", [("f32", 1), ("bf16", 1), ("bf16", 64)])
+def test_positions_far_inside_a_page(kvops, name, drafts):
+    """One page of 2^26 positions: its codes' offsets pass 2^31 bytes at position 2^25.  Keys and values are 0 up to the 100 positions
+    there, which are written, read back and attended."""
+    dtype, n, D, border = TYPES[name], 100, 128, 1 << 25
+    g = torch.Generator().manual_seed(3)
+    base = 1.4 * torch.randn(D, generator=g)
+    k = (base + 0.1 * torch.randn(1, n, 1, D, generator=g)).to(dtype)
+    v = torch.randn(1, n, 1, D, generator=g).to(dtype)
+    q = base.to(dtype).expand(drafts, 2, D).contiguous()
+    cache = kvops.PackedCache.empty(1, 1, 1, D, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), page_size=1 << 26)
+    for at in (border - n // 2, (1 << 26) - n):
+        lens, indptr = ints([at]), ints([0, n])
+        assert kvops.append(cache, k.cuda(), v.cuda(), lens, indptr).item() == at + n
+        kr, vr = (x.cpu().double()[0, :, 0] for x in kvops.read(cache, lens, indptr, n, dtype=torch.float32))
+        for x, r in ((k, kr), (v, vr)):  # half a step: 1/7 of a group's largest, rounded to five bits, by 1/2
+            assert ((x.double()[0, :, 0] - r).abs() <= x.double().abs().max() / 7 * (1 + 2 ** -5) / 2 + 1e-6).all()
+        if at > border:
+            break
+        none = torch.zeros(drafts, 1, D, dtype=dtype, device="cuda")
+        out, lse = kvops.tree_attention(q.cuda(), none, none, cache, ints([at + n]), ints([0, drafts]),
+                                        torch.zeros(drafts, dtype=torch.int64, device="cuda"), max_draft=drafts)
+        s = kr @ q[0, 0].double() / math.sqrt(D)
+        rest = at * math.exp(-s.max().item())  # the positions before them have scores of 0 and values of 0
+        w = (s - s.max()).exp()
+        want, want_lse = (w @ vr) / (w.sum() + rest), s.max() + (w.sum() + rest).log()
+        assert rest < w.sum() / 2
+        # f32: a score sums 128 products of |q k| <= 60 in all: 128 2^-24 60 = 5e-4, so a weight's is 1e-3 of it, of values up to 4.5.  bf16:
+        # a weight and the output are off by 2^-8 each, and the scores' sums as above: (2^-7 + 1e-3) 4.5.
+        tol = 5e-3 if name == "f32" else 4e-2
+        assert vr.abs().max() <= 4.5 and (q[0, 0].double().abs() * kr.abs()).sum(1).max() / math.sqrt(D) <= 60
+        assert (out.cpu().double() - want).abs().max() <= tol
+        assert (lse.cpu().double() - want_lse).abs().max() <= 1e-3
