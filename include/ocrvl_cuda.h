@@ -468,7 +468,8 @@ int ocrvl_op_packed_append(const ocrvl_packed_cache *c, int type, int n_tokens, 
  * indptr[b] + i of k and v ([num_layers][n_tokens][num_kv_heads][head_dim] of `type`,
  * strides as in append), for all of the sequence's tokens: what an append of the same lens and
  * indptr wrote.  c s is rounded once for f16 and not at all for the others.  A position without
- * a page, or past the table, reads as 0; tokens of no sequence are left as they were. */
+ * a page, or past the table, reads as 0; tokens of no sequence are left as they were.  k and v, and their
+ * layers, must not share memory. */
 int ocrvl_op_packed_read(const ocrvl_packed_cache *c, int type, int n_tokens, const int32_t *lens, const int32_t *indptr,
                          void *k, void *v, int64_t kv_stride, int64_t kv_layer_stride, void *stream);
 

@@ -118,6 +118,9 @@ int ocrvl_op_packed_read(const ocrvl_packed_cache *c, int type, int n_tokens, co
                          void *k, void *v, int64_t kv_stride, int64_t kv_layer_stride, void *stream) {
   if (int rc = check_move(c, type, n_tokens, lens, indptr, k, v, kv_stride, kv_layer_stride)) return rc;
   if (n_tokens == 0) return OCRVL_OK;
+  const int64_t row = (int64_t)c->num_kv_heads * c->head_dim, tokens = (n_tokens - 1) * kv_stride + row;
+  if (k == v || (c->num_layers > 1 && kv_layer_stride < tokens && (kv_layer_stride < row || kv_stride < (c->num_layers - 1) * kv_layer_stride + row)))
+    return invalid("what is read must not share memory (of K and V, of two layers)");
   const PackArgs a = pack_args(c, type, n_tokens, lens, indptr, k, v, kv_stride, kv_layer_stride);
   dim3 grid;
   if (int rc = move_grid(a, n_tokens, 4, &grid)) return rc;

@@ -103,3 +103,9 @@ def test_bad_rotations_are_refused():
         rc, said = rotate(rotary(), **kw)
         assert rc == _lib.E_INVALID and said, kw
     assert rotate(rotary(), n=0)[0] == _lib.OK
+
+
+def test_reads_into_shared_memory_are_refused():
+    for kw in (dict(v=K), dict(layer=0), dict(n=4, layer=128), dict(n=4, layer=256), dict(n=4, stride=256, layer=768)):
+        rc, said = read(cache(num_layers=2), **{"v": K + 4096, **kw})
+        assert rc == _lib.E_INVALID and "share" in said, kw
