@@ -293,6 +293,6 @@ def read(cache: PackedCache, lens: torch.Tensor, indptr: torch.Tensor, tokens: i
 
     ``indptr`` [batch + 1] int32 says how many positions of each sequence, from ``lens`` [batch] int32 on, and where they go;
     ``tokens`` is the length of that flat axis (indptr's last value, which is on the device).  Returns k and v
-    [layers, tokens, kv heads, head_dim] of ``dtype`` (or the tensors given), 0 where a position has no page; tokens behind
+    [layers, tokens, kv heads, head_dim] of ``dtype`` (or the tensors given, which share no memory), 0 where a position has no page; tokens behind
     indptr's last are not written."""
     return _kvops.read(cache._ref, lens, indptr, tokens, dtype, k, v)
